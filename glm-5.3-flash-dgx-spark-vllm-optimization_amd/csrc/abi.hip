@@ -276,6 +276,69 @@ void carve_fp8(void* ws, int64_t P, int64_t T, int64_t n, int64_t K, int64_t N, 
     f.contrib = c.take<float>((size_t)P * K);
     w.bytes = c.off;
 }
+
+int mxfp4_layer_ok(const mi355moe_mxfp4_layer* L) {
+    if (!L || !L->w13 || !L->w13_scale || !L->w2 || !L->w2_scale) return MI355MOE_EINVAL;
+    if (L->n < 1 || L->n > MAX_EXPERTS) return MI355MOE_ELIMIT;
+    if (L->hidden < 32 || L->hidden % 32 || L->intermediate < 32 || L->intermediate % 32) return MI355MOE_ESHAPE;
+    if (L->hidden > 16384 || L->intermediate > 16384) return MI355MOE_ELIMIT;
+    if (L->w13_scale_stride < L->hidden / 32 || L->w13_scale_stride % 4 || L->w13_scale_stride > 4096 ||
+        L->w2_scale_stride < L->intermediate / 32 || L->w2_scale_stride % 4 || L->w2_scale_stride > 4096)
+        return MI355MOE_ESHAPE;
+    if ((reinterpret_cast<uintptr_t>(L->w13) | reinterpret_cast<uintptr_t>(L->w2)) & 15) return MI355MOE_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(L->w13_scale) | reinterpret_cast<uintptr_t>(L->w2_scale)) & 3) return MI355MOE_EINVAL;
+    return 0;
+}
+
+int64_t scale_pitch(int64_t k) { return (k / 32 + 3) / 4 * 4; }
+
+struct Mxfp4Ws {
+    RouteArgs ra;
+    Mxfp4Args fa;
+    size_t bytes;
+};
+
+// Layout of the MXFP4 path's workspace: route tables, quantised input rows and SwiGLU outputs with their scales, the
+// per-pair fp32 contributions.
+void carve_mxfp4(void* ws, int64_t P, int64_t T, int64_t n, int64_t K, int64_t N, Mxfp4Ws& w) {
+    Carve c(ws);
+    RouteArgs& r = w.ra;
+    Mxfp4Args& f = w.fa;
+    memset(&r, 0, sizeof(r));
+    memset(&f, 0, sizeof(f));
+    f.seg = mxfp4_seg_rows(P, n);
+    f.S_cap = (int)(std::min(P, n) + (P + f.seg - 1) / f.seg);
+    r.tok = c.take<int>(P);
+    r.w16 = c.take<uint16_t>(P);
+    r.w32 = c.take<float>(P);
+    r.pe = c.take<int>(P);
+    r.inv = c.take<int>(P);
+    r.seg_expert = c.take<int>(f.S_cap);
+    r.seg_row0 = c.take<int>(f.S_cap);
+    r.seg_rows = c.take<int>(f.S_cap);
+    r.nseg = c.take<int>(1);
+    r.counts = c.take<int>(n + 1);
+    r.loc = c.take<int>(P);
+    r.blk_cnt = c.take<int>(((P + 1023) / 1024) * (n + 1));
+    r.cnt_out = c.take<int>(n + 1);
+    f.sxp = scale_pitch(K);
+    f.shp = scale_pitch(N);
+    f.qx = c.take<uint8_t>((size_t)T * (K / 2));
+    f.sx = c.take<uint8_t>((size_t)T * f.sxp);
+    f.qh = c.take<uint8_t>((size_t)P * (N / 2));
+    f.sh = c.take<uint8_t>((size_t)P * f.shp);
+    f.contrib = c.take<float>((size_t)P * K);
+    w.bytes = c.off;
+}
+
+// The gated block's operands: 16-bit rows at 16-byte addresses, row strides of whole 16 bytes.
+bool rows16_ok(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; }
+int gated_ok(int dtype, int64_t T, int64_t K, int64_t N) {
+    if (dtype != MI355MOE_F16 && dtype != MI355MOE_BF16) return MI355MOE_EDTYPE;
+    if (T < 0 || K < 8 || K % 8 || N < 8 || N % 8) return MI355MOE_ESHAPE;
+    if (T > (1 << 24) || K > 65536 || N > 16384) return MI355MOE_ELIMIT;
+    return 0;
+}
 int dt_w(int dt) {
     return dt == MI355MOE_F32 ? DT_F32 : dt == MI355MOE_F16 ? DT_F16 : dt == MI355MOE_BF16 ? DT_BF16 : -1;
 }
@@ -1778,6 +1841,217 @@ int mi355moe_fp8_moe_forward_ids(const mi355moe_fp8_layer* layer, const void* x,
     if (stages & MI355MOE_STAGE_DOWN) kernels |= 4;
     if (stages & MI355MOE_STAGE_COMBINE) kernels |= 8;
     return rc_launch(launch_fp8(f, stream, kernels));
+}
+
+int mi355moe_mxfp4_quant_rows(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t x_stride, void* q, void* scale,
+                              hipStream_t stream) {
+    if (dt_w(x_dtype) < 0) return MI355MOE_EDTYPE;
+    if (rows < 0 || K < 1 || (rows > 1 && x_stride < K)) return MI355MOE_ESHAPE;
+    if (K > (1 << 24) || rows > (int64_t(1) << 40) / K) return MI355MOE_ELIMIT;
+    if (rows == 0) return 0;
+    if (!x || !q || !scale) return MI355MOE_EINVAL;
+    return rc_launch(launch_mx_quant(x, dt_w(x_dtype), x_stride, rows, (int)K, static_cast<uint8_t*>(q),
+                                     static_cast<uint8_t*>(scale), (K + 31) / 32, stream));
+}
+
+int mi355moe_mxfp4_dequant_rows(const void* q, const void* scale, int64_t rows, int64_t K, void* out, int out_dtype,
+                                hipStream_t stream) {
+    if (dt_w(out_dtype) < 0) return MI355MOE_EDTYPE;
+    if (rows < 0 || K < 1) return MI355MOE_ESHAPE;
+    if (K > (1 << 24) || rows > (int64_t(1) << 40) / K) return MI355MOE_ELIMIT;
+    if (rows == 0) return 0;
+    if (!q || !scale || !out) return MI355MOE_EINVAL;
+    return rc_launch(launch_mx_dequant(static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), rows, (int)K, out,
+                                       dt_w(out_dtype), stream));
+}
+
+static int mx_matmul_ok(int64_t M, int64_t N, int64_t K) {
+    if (M < 0 || N < 1 || K < 32 || K % 32) return MI355MOE_ESHAPE;
+    if (M > (1 << 20) || N > (1 << 20) || K > 65536) return MI355MOE_ELIMIT;
+    return 0;
+}
+
+int64_t mi355moe_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (mx_matmul_ok(M, N, K)) return -1;
+    const MxMatmulPlan p = plan_mx_matmul(M, N, K);
+    int64_t b = 0;
+    if (K % 128) b += (int64_t)(align_up(M * scale_pitch(K)) + align_up(N * scale_pitch(K)));
+    if (p.splits > 1) b += p.splits * M * N * 4;
+    return b;
+}
+
+int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const void* w, const void* w_scale, int64_t N,
+                          int64_t K, void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                          hipStream_t stream) {
+    if (dt_w(out_dtype) < 0) return MI355MOE_EDTYPE;
+    if (int r = mx_matmul_ok(M, N, K)) return r;
+    if (out_stride < N) return MI355MOE_ESHAPE;
+    if (M == 0) return 0;
+    if (!a || !a_scale || !w || !w_scale || !out) return MI355MOE_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15) return MI355MOE_EINVAL;
+    const bool pad = K % 128 != 0;
+    if (!pad && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3)) return MI355MOE_EINVAL;
+    const int64_t need = mi355moe_mxfp4_matmul_workspace_bytes(M, N, K);
+    if (need > 0 && !workspace) return MI355MOE_EINVAL;
+    if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
+    const MxMatmulPlan p = plan_mx_matmul(M, N, K);
+    MxMatmulArgs m{};
+    m.q = static_cast<const uint8_t*>(a);
+    m.qs = static_cast<const uint8_t*>(a_scale);
+    m.M = M;
+    m.w = static_cast<const uint8_t*>(w);
+    m.ws = static_cast<const uint8_t*>(w_scale);
+    m.N = (int)N;
+    m.K = (int)K;
+    m.sp = scale_pitch(K);
+    m.out = out;
+    m.odt = dt_w(out_dtype);
+    m.out_stride = out_stride;
+    m.splits = p.splits;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (pad) {
+        uint8_t* ap = ws;
+        uint8_t* wp = ap + align_up(M * m.sp);
+        ws = wp + align_up(N * m.sp);
+        if (int r = launch_mx_pad_scales(m.qs, M, ap, m.ws, N, wp, (int)(K / 32), (int)m.sp, stream)) return rc_launch(r);
+        m.qs = ap;
+        m.ws = wp;
+    }
+    m.part = reinterpret_cast<float*>(ws);
+    return rc_launch(launch_mx_matmul(m, p, stream));
+}
+
+int64_t mi355moe_mxfp4_moe_workspace_bytes(const mi355moe_mxfp4_layer* layer, int64_t T, int64_t topk) {
+    if (mxfp4_layer_ok(layer) || T < 0 || topk < 1 || topk > MAX_TOPK || T > MAX_PAIRS) return -1;
+    Mxfp4Ws w;
+    carve_mxfp4(nullptr, std::max<int64_t>(1, T * topk), std::max<int64_t>(1, T), layer->n, layer->hidden,
+                layer->intermediate, w);
+    return (int64_t)w.bytes;
+}
+
+int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void* x, int x_dtype, int64_t x_stride,
+                                   int64_t T, const void* ids, int ids_dtype, const void* weights, int weights_dtype,
+                                   int64_t topk, const int64_t* expert_map, int64_t n_global, float limit, void* out,
+                                   int out_dtype, int64_t out_stride, int options, void* workspace,
+                                   size_t workspace_bytes, hipStream_t stream) {
+    if (int r = mxfp4_layer_ok(layer)) return r;
+    if (!x || !ids || !weights || !out || !workspace) return MI355MOE_EINVAL;
+    if (options & ~MI355MOE_OPT_ACCUMULATE) return MI355MOE_EINVAL;
+    if (dt_w(x_dtype) < 0 || dt_w(weights_dtype) < 0 || dt_w(out_dtype) < 0) return MI355MOE_EDTYPE;
+    if (ids_dtype != MI355MOE_I32 && ids_dtype != MI355MOE_I64) return MI355MOE_EDTYPE;
+    const int64_t K = layer->hidden, N = layer->intermediate, n = layer->n;
+    if (T < 0 || T > MAX_PAIRS || topk < 1 || topk > MAX_TOPK) return MI355MOE_ELIMIT;
+    if (x_stride < K || out_stride < K) return MI355MOE_ESHAPE;
+    if (expert_map && n_global < 0) return MI355MOE_EINVAL;
+    const int64_t P = T * topk;
+    if (P > MAX_PAIRS) return MI355MOE_ELIMIT;
+    if (T == 0) return 0;
+    Mxfp4Ws w;
+    carve_mxfp4(workspace, P, T, n, K, N, w);
+    if (workspace_bytes < w.bytes) return MI355MOE_EWORKSPACE;
+    if (w.fa.S_cap > 65535) return MI355MOE_ELIMIT;
+    RouteArgs& r = w.ra;
+    r.ids = ids;
+    r.ids64 = ids_dtype == MI355MOE_I64;
+    r.w = weights;
+    r.wdt = dt_w(weights_dtype);
+    r.emap = expert_map;
+    r.n_global = expert_map ? n_global : 0;
+    r.P = (int)P;
+    r.topk = (int)topk;
+    r.n = (int)n;
+    r.R = 1 << 30;
+    Mxfp4Args& f = w.fa;
+    r.seg = f.seg;
+    r.S_cap = f.S_cap;
+    f.n = (int)n;
+    f.K = (int)K;
+    f.N = (int)N;
+    f.P = (int)P;
+    f.T = (int)T;
+    f.w13 = static_cast<const uint8_t*>(layer->w13);
+    f.w13s = static_cast<const uint8_t*>(layer->w13_scale);
+    f.w13sp = layer->w13_scale_stride;
+    f.w2 = static_cast<const uint8_t*>(layer->w2);
+    f.w2s = static_cast<const uint8_t*>(layer->w2_scale);
+    f.w2sp = layer->w2_scale_stride;
+    f.x = x;
+    f.xdt = dt_w(x_dtype);
+    f.x_stride = x_stride;
+    f.tok = r.tok;
+    f.w32 = r.w32;
+    f.pe = r.pe;
+    f.inv = r.inv;
+    f.seg_expert = r.seg_expert;
+    f.seg_row0 = r.seg_row0;
+    f.seg_rows = r.seg_rows;
+    f.nseg = r.nseg;
+    f.topk = (int)topk;
+    f.limit = limit;
+    f.out = out;
+    f.odt = dt_w(out_dtype);
+    f.out_stride = out_stride;
+    f.accumulate = options & MI355MOE_OPT_ACCUMULATE ? 1 : 0;
+    if (int rc = launch_route(r, stream)) return rc_launch(rc);
+    return rc_launch(launch_mxfp4(f, stream, 15));
+}
+
+int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, int64_t x_stride, const void* w13,
+                           int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, hipStream_t stream) {
+    if (int r = gated_ok(dtype, T, hidden, intermediate)) return r;
+    if (x_stride < hidden || h_stride < intermediate || x_stride > (1 << 22)) return MI355MOE_ESHAPE;
+    if (T == 0) return 0;
+    if (!x || !w13 || !h) return MI355MOE_EINVAL;
+    if (!rows16_ok(x, x_stride) || !rows16_ok(w13, hidden) || (reinterpret_cast<uintptr_t>(gu) & 15)) return MI355MOE_EINVAL;
+    GatedArgs g{};
+    g.dt = dt_act(dtype);
+    g.T = T;
+    g.K = (int)hidden;
+    g.N = (int)intermediate;
+    g.x = static_cast<const uint16_t*>(x);
+    g.x_stride = x_stride;
+    g.w13 = static_cast<const uint16_t*>(w13);
+    g.limit = limit;
+    g.h = static_cast<uint16_t*>(h);
+    g.h_stride = h_stride;
+    g.gu = gu;
+    return rc_launch(launch_gated_forward(g, stream));
+}
+
+int64_t mi355moe_gated_backward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate) {
+    if (gated_ok(MI355MOE_BF16, T, hidden, intermediate)) return -1;
+    return (int64_t)align_up(T * 2 * intermediate * 2) + 4 * gated_part_floats(T, hidden, intermediate, true, true);
+}
+
+int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, const void* x, int dtype, int64_t T,
+                            int64_t hidden, int64_t x_stride, const void* w13, int64_t intermediate, float limit, void* dx,
+                            void* dw13, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (int r = gated_ok(dtype, T, hidden, intermediate)) return r;
+    if (dh_stride < intermediate || x_stride < hidden || x_stride > (1 << 22)) return MI355MOE_ESHAPE;
+    if (!dx && !dw13) return 0;
+    if (T == 0) return dw13 ? MI355MOE_ESHAPE : 0;
+    if (!dh || !gu || !x || !w13 || !workspace) return MI355MOE_EINVAL;
+    if (!rows16_ok(dh, dh_stride) || !rows16_ok(x, x_stride) || !rows16_ok(w13, hidden) || !rows16_ok(dx, hidden) ||
+        !rows16_ok(dw13, hidden) || !rows16_ok(workspace, 0) || (reinterpret_cast<uintptr_t>(gu) & 15))
+        return MI355MOE_EINVAL;
+    if ((int64_t)workspace_bytes < mi355moe_gated_backward_workspace_bytes(T, hidden, intermediate)) return MI355MOE_EWORKSPACE;
+    GatedArgs g{};
+    g.dt = dt_act(dtype);
+    g.T = T;
+    g.K = (int)hidden;
+    g.N = (int)intermediate;
+    g.x = static_cast<const uint16_t*>(x);
+    g.x_stride = x_stride;
+    g.w13 = static_cast<const uint16_t*>(w13);
+    g.limit = limit;
+    g.gu = const_cast<float*>(gu);
+    g.dh = static_cast<const uint16_t*>(dh);
+    g.dh_stride = dh_stride;
+    g.d = static_cast<uint16_t*>(workspace);
+    g.dx = static_cast<uint16_t*>(dx);
+    g.dw = static_cast<uint16_t*>(dw13);
+    g.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(T * 2 * intermediate * 2));
+    return rc_launch(launch_gated_backward(g, stream));
 }
 
 }  // extern "C"

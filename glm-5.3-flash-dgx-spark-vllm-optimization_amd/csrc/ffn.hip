@@ -1,0 +1,345 @@
+// The gated feed-forward block of a layer's shared expert, and its gradient, on the 16-bit matrix cores.
+//
+//   [g | u] = x W13^T (fp32 sums);  h = silu(min(g, L)) clamp(u, -L, L)  (the limit iff L != 0), rounded once
+//   dg = dh u' s (1 + g' (1 - s)) [g <= L],  du = dh g' s [|u| <= L],  s = sigmoid(g'), from the fp32 g and u that the
+//   forward pass keeps;  dx = [dg | du] W13,  dW13 = [dg | du]^T x  (fp32 sums; [dg | du] is rounded once to the operand
+//   type, which the matrix cores take)
+//
+// Forward multiplies two operands whose contraction is contiguous; dx has one, and dW13 both, with the contraction as the
+// row index (the tiles' COL layout).
+#include <algorithm>
+
+#include "gemm_tile.cuh"
+#include "mi355moe_internal.h"
+
+namespace mi355moe {
+
+template <int DT>
+struct KindOf {
+    static constexpr int value = DT == DT_BF16 ? MM_BF16 : MM_F16;
+};
+template <int DT>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    if constexpr (DT == DT_BF16) return pack_bf16x2(lo, hi);
+    else return h_as_u16((_Float16)lo) | (h_as_u16((_Float16)hi) << 16);
+}
+template <int DT>
+__device__ __forceinline__ float value16(uint32_t b) {
+    if constexpr (DT == DT_BF16) return bf16_to_f32((uint16_t)b);
+    else return (float)u16_as_h(b & 0xFFFFu);
+}
+
+// ------------------------------------------------------------------------------------------------ forward, few rows
+
+template <int DT>
+__device__ __forceinline__ f32x4 few_mma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (DT == DT_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// grid (N / 8, ceil(T / 16)), 1024 threads: 8 gate and the same 8 up columns as one 16-row MFMA operand, for 16 tokens.
+// Lane (c = lane % 16, g = lane / 16) holds 64 consecutive bytes of weight row c (128 of the contraction a wave step);
+// the contraction is cut over the sixteen waves, whose sums join in LDS in wave order.
+template <int DT>
+__global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
+    __shared__ __align__(16) float red[16][256];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 8;
+    const int64_t m0 = (int64_t)blockIdx.y * 16;
+    const int rows = (int)min((int64_t)16, a.T - m0);
+    const int chunks = a.K >> 3;                                     // 16-byte chunks of a row
+    const u32x4* w = reinterpret_cast<const u32x4*>(a.w13 + ((size_t)(c < 8 ? 0 : a.N) + n0 + (c & 7)) * a.K);
+    const u32x4* x = reinterpret_cast<const u32x4*>(a.x + (size_t)(m0 + min(c, rows - 1)) * a.x_stride);
+    f32x4 acc = {};
+    for (int b0 = wv * 16; b0 < chunks; b0 += 256) {
+        const int b = b0 + 4 * g;
+        u32x4 wv4[4], xv4[4];
+        if (b0 + 16 <= chunks) {                                     // (uniform)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wv4[i] = w[b + i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) xv4[i] = x[b + i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool ok = b + i < chunks;
+                wv4[i] = w[min(b + i, chunks - 1)];
+                xv4[i] = x[min(b + i, chunks - 1)];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    wv4[i][j] = ok ? wv4[i][j] : 0u;
+                    xv4[i][j] = ok ? xv4[i][j] : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = few_mma16<DT>(wv4[i], xv4[i], acc);
+    }
+    *reinterpret_cast<f32x4*>(&red[wv][lane * 4]) = acc;
+    __syncthreads();
+    if (tid >= 128) return;
+    const int m = tid >> 3, n = tid & 7;
+    if (m >= rows) return;
+    const int ag = (((n >> 2) << 4) + m) * 4 + (n & 3), au = ag + 128;   // (up: n + 8, two lane groups on)
+    float gs = 0.f, us = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        gs += red[i][ag];
+        us += red[i][au];
+    }
+    const size_t t = (size_t)(m0 + m);
+    a.h[t * a.h_stride + n0 + n] = (uint16_t)pack16<DT>(swiglu(gs, us, a.limit), 0.f);
+    if (a.gu) {
+        a.gu[t * 2 * a.N + n0 + n] = gs;
+        a.gu[t * 2 * a.N + a.N + n0 + n] = us;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ forward, tiles
+
+// Workgroup tiles of BP / 2 columns x BQ tokens; a wave's P rows are its gate columns, then the same up columns.
+template <int DT, int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 1) void gated_kernel(GatedArgs a, int nt, int mt) {
+    using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
+    static_assert(G::TP % 2 == 0, "");
+    extern __shared__ __align__(16) unsigned char lds[];
+    constexpr int HALF = BP / WP / 2;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_order(blockIdx.x, nt * mt);
+    const int n0 = (id % nt) * (BP / 2);
+    const int64_t m0 = (int64_t)(id / nt) * BQ;
+    const int ql = (int)min((int64_t)BQ, a.T - m0) - 1;
+    const uint32_t wp = 2u * a.K, xp = 2u * (uint32_t)a.x_stride;
+    G t;
+    t.p.init_row(a.w13, wv, lane, [&](int r) {
+        const int w = r / (2 * HALF), i = r % (2 * HALF);
+        return (uint32_t)(min(n0 + w * HALF + (i % HALF), a.N - 1) + (i < HALF ? 0 : a.N)) * wp;
+    });
+    t.q.init_row(uniform_ptr(a.x + (size_t)m0 * a.x_stride), wv, lane, [&](int r) { return (uint32_t)min(r, ql) * xp; });
+    const int tail = (a.K & 63) >> 3;
+    t.run(lds, 0, (a.K + 63) >> 6, tail, tail, 0, 0);
+    const int p0 = (wv % WP) * HALF, q0 = (wv / WP) * (BQ / WQ);
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        const int64_t m = m0 + q0 + 32 * j + (lane & 31);
+        if (m >= a.T) continue;
+#pragma unroll
+        for (int i = 0; i < G::TP / 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
+                if (n >= a.N) continue;                              // (N % 8 == 0: four columns exist or none)
+                f32x4 g, u, h;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    g[k] = t.acc[i][j][4 * r + k];
+                    u[k] = t.acc[i + G::TP / 2][j][4 * r + k];
+                    h[k] = swiglu(g[k], u[k], a.limit);
+                }
+                store4(a.h, DT, (size_t)m * a.h_stride + n, 4, h);
+                if (a.gu) {
+                    *reinterpret_cast<f32x4*>(a.gu + (size_t)m * 2 * a.N + n) = g;
+                    *reinterpret_cast<f32x4*>(a.gu + (size_t)m * 2 * a.N + a.N + n) = u;
+                }
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+
+// d = [dg | du], eight columns a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void gated_d_kernel(GatedArgs a) {
+    const int per = a.N / 8;
+    const int64_t items = a.T * per;
+    const float L = a.limit;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per;
+        const int c = (int)(i - t * per) * 8;
+        const f32x4* gp = reinterpret_cast<const f32x4*>(a.gu + (size_t)t * 2 * a.N + c);
+        const f32x4* up = reinterpret_cast<const f32x4*>(a.gu + (size_t)t * 2 * a.N + a.N + c);
+        const u32x4 dv = *reinterpret_cast<const u32x4*>(a.dh + (size_t)t * a.dh_stride + c);
+        const f32x4 g4[2] = {gp[0], gp[1]}, u4[2] = {up[0], up[1]};
+        u32x4 og, ou;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float dg[2], du[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int j = 2 * k + e;
+                const float dh = value16<DT>(dv[k] >> (16 * e));
+                float g = g4[j >> 2][j & 3], u = u4[j >> 2][j & 3];
+                const bool gout = L != 0.0f && g > L, uout = L != 0.0f && fabsf(u) > L;
+                if (L != 0.0f) {
+                    g = gout ? L : g;
+                    u = uout ? (u > 0.f ? L : -L) : u;
+                }
+                const float s = __fdiv_rn(1.0f, 1.0f + __expf(-g));
+                dg[e] = gout ? 0.0f : dh * u * s * (1.0f + g * (1.0f - s));
+                du[e] = uout ? 0.0f : dh * g * s;
+            }
+            og[k] = pack16<DT>(dg[0], dg[1]);
+            ou[k] = pack16<DT>(du[0], du[1]);
+        }
+        *reinterpret_cast<u32x4*>(a.d + (size_t)t * 2 * a.N + c) = og;
+        *reinterpret_cast<u32x4*>(a.d + (size_t)t * 2 * a.N + a.N + c) = ou;
+    }
+}
+
+struct Gemm16Args {
+    const uint16_t* p;      // ROW: [N][ldp], COL: [C][ldp]
+    const uint16_t* q;      // ROW: [M][ldq], COL: [C][ldq]
+    int64_t ldp, ldq;       // elements
+    int64_t M;
+    int N;
+    int64_t C;              // contraction
+    void* out;
+    int64_t out_stride;
+    int splits;
+    float* part;
+};
+
+// out[m][n] = sum over k of P Q, dtype DT, or fp32 partials of the contraction's splits (grid y).
+template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 1) void gemm16_kernel(Gemm16Args a, int nt, int mt) {
+    using G = GemmTile<KindOf<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_order(blockIdx.x, nt * mt);
+    const int n0 = (id % nt) * BP;
+    const int64_t m0 = (int64_t)(id / nt) * BQ;
+    const int stages = (int)((a.C + 63) >> 6), per = (stages + a.splits - 1) / a.splits;
+    const int kb0 = blockIdx.y * per, kb1 = min(stages, kb0 + per);
+    const uint32_t ldp = 2u * (uint32_t)a.ldp, ldq = 2u * (uint32_t)a.ldq;
+    const int pl = min(BP, a.N - n0), ql = (int)min((int64_t)BQ, a.M - m0);
+    G t;
+    if constexpr (PL == LAY_ROW)
+        t.p.init_row(uniform_ptr(a.p + (size_t)n0 * a.ldp + (size_t)kb0 * 64), wv, lane, [&](int r) { return (uint32_t)min(r, pl - 1) * ldp; });
+    else t.p.init_col(uniform_ptr(a.p + (size_t)kb0 * 64 * a.ldp + n0), wv, lane, ldp, pl);
+    if constexpr (QL == LAY_ROW)
+        t.q.init_row(uniform_ptr(a.q + (size_t)m0 * a.ldq + (size_t)kb0 * 64), wv, lane, [&](int r) { return (uint32_t)min(r, ql - 1) * ldq; });
+    else t.q.init_col(uniform_ptr(a.q + (size_t)kb0 * 64 * a.ldq + m0), wv, lane, ldq, ql);
+    const int left = kb1 == stages ? (int)(a.C & 63) : 0;
+    if (kb0 < kb1) t.run(lds, kb0, kb1, PL == LAY_ROW ? left >> 3 : left, QL == LAY_ROW ? left >> 3 : left, ldp, ldq);
+    else
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
+    const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
+    void* out = a.splits > 1 ? static_cast<void*>(a.part + (size_t)blockIdx.y * a.M * a.N) : a.out;
+    const int odt = a.splits > 1 ? (int)DT_F32 : DT;
+    const int64_t stride = a.splits > 1 ? a.N : a.out_stride;
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        const int64_t m = m0 + q0 + 32 * j + (lane & 31);
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
+                if (n < a.N)
+                    store4(out, odt, (size_t)m * stride + n, 4,
+                           f32x4{t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2], t.acc[i][j][4 * r + 3]});
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ launchers
+
+constexpr int64_t GATED_FEW_T = 32;                  // tokens up to which the forward streams the weights
+
+struct Gemm16Plan {
+    int tile, splits;
+};
+static Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
+    Gemm16Plan p{256, 1};
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+    if (big >= 192) return p;
+    p.tile = 128;
+    const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), stages = (C + 63) / 64;
+    while (p.splits < 16 && tiles * p.splits * 2 <= 512 && stages / (p.splits * 2) >= 4) p.splits *= 2;
+    return p;
+}
+
+template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
+static int run_gemm16(const Gemm16Args& a, hipStream_t st) {
+    using G = GemmTile<KindOf<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
+    static const bool ok = allow_lds(gemm16_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>, G::LDS);
+    if (!ok) return -1;
+    const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
+    hipLaunchKernelGGL((gemm16_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
+    return 0;
+}
+template <int DT, int PL, int QL>
+static int gemm16(Gemm16Args a, hipStream_t st) {
+    const Gemm16Plan p = plan_gemm16(a.M, a.N, a.C);
+    a.splits = p.splits;
+    const int r = p.tile == 256 ? run_gemm16<DT, PL, QL, 256, 256, 2, 4, 2>(a, st) : run_gemm16<DT, PL, QL, 128, 128, 2, 2, 2>(a, st);
+    if (r) return r;
+    if (p.splits > 1) return launch_join(a.part, p.splits, a.M, a.N, a.out, DT, a.out_stride, st);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int64_t gated_part_floats(int64_t T, int64_t K, int64_t N, bool dx, bool dw) {
+    const Gemm16Plan px = plan_gemm16(T, K, 2 * N), pw = plan_gemm16(2 * N, K, T);
+    int64_t f = 0;
+    if (dx && px.splits > 1) f = std::max(f, px.splits * T * K);
+    if (dw && pw.splits > 1) f = std::max(f, pw.splits * 2 * N * K);
+    return f;
+}
+
+template <int DT, int BP, int BQ, int WP, int WQ, int ST>
+static int run_gated(const GatedArgs& a, hipStream_t st) {
+    using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
+    static const bool ok = allow_lds(gated_kernel<DT, BP, BQ, WP, WQ, ST>, G::LDS);
+    if (!ok) return -1;
+    const int nt = (a.N + BP / 2 - 1) / (BP / 2), mt = (int)((a.T + BQ - 1) / BQ);
+    hipLaunchKernelGGL((gated_kernel<DT, BP, BQ, WP, WQ, ST>), dim3(nt * mt), dim3(G::THREADS), G::LDS, st, a, nt, mt);
+    return 0;
+}
+
+template <int DT>
+static int gated_forward(const GatedArgs& a, hipStream_t st) {
+    if (a.T <= GATED_FEW_T) {
+        hipLaunchKernelGGL(gated_few_kernel<DT>, dim3(a.N / 8, (unsigned)((a.T + 15) / 16)), dim3(1024), 0, st, a);
+    } else {
+        const int64_t big = ((a.T + 255) / 256) * ((a.N + 127) / 128);
+        const int r = big >= 192 ? run_gated<DT, 256, 256, 2, 4, 2>(a, st) : run_gated<DT, 128, 128, 2, 2, 2>(a, st);
+        if (r) return r;
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+int launch_gated_forward(const GatedArgs& a, hipStream_t st) {
+    return a.dt == DT_BF16 ? gated_forward<DT_BF16>(a, st) : gated_forward<DT_F16>(a, st);
+}
+
+template <int DT>
+static int gated_backward(const GatedArgs& a, hipStream_t st) {
+    const int64_t items = a.T * (a.N / 8);
+    hipLaunchKernelGGL(gated_d_kernel<DT>, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 8192)), dim3(256), 0, st, a);
+    if (hipGetLastError() != hipSuccess) return -1;
+    if (a.dx) {
+        Gemm16Args g{};
+        g.p = a.w13, g.ldp = a.K, g.q = a.d, g.ldq = 2 * a.N;
+        g.M = a.T, g.N = a.K, g.C = 2 * a.N, g.out = a.dx, g.out_stride = a.K, g.part = a.part;
+        if (int r = gemm16<DT, LAY_COL, LAY_ROW>(g, st)) return r;
+    }
+    if (a.dw) {
+        Gemm16Args g{};
+        g.p = a.x, g.ldp = a.x_stride, g.q = a.d, g.ldq = 2 * a.N;
+        g.M = 2 * a.N, g.N = a.K, g.C = a.T, g.out = a.dw, g.out_stride = a.K, g.part = a.part;
+        if (int r = gemm16<DT, LAY_COL, LAY_COL>(g, st)) return r;
+    }
+    return 0;
+}
+int launch_gated_backward(const GatedArgs& a, hipStream_t st) {
+    return a.dt == DT_BF16 ? gated_backward<DT_BF16>(a, st) : gated_backward<DT_F16>(a, st);
+}
+
+}  // namespace mi355moe

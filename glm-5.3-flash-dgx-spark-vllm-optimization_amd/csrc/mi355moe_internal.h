@@ -300,6 +300,102 @@ constexpr int fp8_seg_rows(int64_t tokens) { return tokens <= FP8_FEW_T ? FP8_FE
 int launch_fp8(const Fp8Args& a, hipStream_t st, int kernels);
 int launch_quant_rows(const void* x, int xdt, int64_t stride, int rows, int K, uint8_t* q, float* s, hipStream_t st);
 
+// MXFP4 (mxfp4.hip). Codes two a byte, rows K / 2 bytes apart; scales at the given pitches (multiples of 4, the bytes
+// behind a row's K / 32 scales finite).
+struct Mxfp4Args {
+    int n, K, N, P, T;
+    const uint8_t* w13;     // [n][2N][K/2], gate rows then up rows
+    const uint8_t* w13s;    // [n][2N][w13sp]
+    int64_t w13sp;
+    const uint8_t* w2;      // [n][K][N/2]
+    const uint8_t* w2s;     // [n][K][w2sp]
+    int64_t w2sp;
+    const void* x;
+    int xdt;                // DT_F32, DT_F16 or DT_BF16
+    int64_t x_stride;
+    const int* tok;
+    const float* w32;
+    const int* pe;
+    const int* seg_expert;
+    const int* seg_row0;
+    const int* seg_rows;
+    const int* nseg;
+    int S_cap;
+    int seg;                // rows per segment (MX_FEW or MX_TILE)
+    float limit;
+    uint8_t* qx;            // [T][K/2] quantised input rows
+    uint8_t* sx;            // [T][sxp]
+    int64_t sxp;
+    uint8_t* qh;            // [P][N/2] quantised SwiGLU outputs (sorted position order)
+    uint8_t* sh;            // [P][shp]
+    int64_t shp;
+    float* contrib;         // [P][K] per-pair weighted contributions (sorted position order)
+    const int* inv;         // [P] pair j -> sorted position
+    int topk;
+    void* out;
+    int odt;
+    int64_t out_stride;
+    int accumulate;         // out += the routed sum
+};
+constexpr int MX_FEW = 16, MX_TILE = 64;             // rows per segment: streamed weights, LDS tiles
+// Rows per segment of a call of P pairs over n experts: the weights are streamed for segments of few rows.
+constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : MX_TILE; }
+// kernels: bit 0 quantise inputs, bit 1 gate/up, bit 2 down, bit 3 slot-order combine
+int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels);
+// rows x K values to codes [rows][ceil(K/2)] and scales at pitch sp >= ceil(K/32) (the bytes behind them set to 127)
+int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int64_t sp,
+                    hipStream_t st);
+int launch_mx_dequant(const uint8_t* q, const uint8_t* s, int64_t rows, int K, void* out, int odt, hipStream_t st);
+// scales of two arrays of rows (nb a row, back to back) at a pitch of whole dwords
+int launch_mx_pad_scales(const uint8_t* a, int64_t ra, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb, int pitch,
+                         hipStream_t st);
+struct MxMatmulPlan {
+    int few, tile, splits;
+};
+struct MxMatmulArgs {
+    const uint8_t* q;       // [M][K/2]
+    const uint8_t* qs;      // [M][sp]
+    int64_t M;
+    const uint8_t* w;       // [N][K/2]
+    const uint8_t* ws;      // [N][sp]
+    int N, K;
+    int64_t sp;
+    void* out;
+    int odt;
+    int64_t out_stride;
+    int splits;
+    float* part;            // [splits][M][N] (splits > 1)
+};
+// out [M][stride] (dtype odt) = the sum of fp32 partials [splits][M][N] in order
+int launch_join(const float* part, int splits, int64_t M, int N, void* out, int odt, int64_t stride, hipStream_t st);
+MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K);
+int launch_mx_matmul(const MxMatmulArgs& a, const MxMatmulPlan& p, hipStream_t st);
+
+// The gated feed-forward block (ffn.hip): operands F16 or BF16, contraction rows 16-byte aligned.
+struct GatedArgs {
+    int dt;                 // DT_F16 or DT_BF16
+    int64_t T;
+    int K, N;               // hidden, intermediate
+    const uint16_t* x;
+    int64_t x_stride;
+    const uint16_t* w13;    // [2N][K], gate rows then up rows
+    float limit;
+    uint16_t* h;            // [T][h_stride]
+    int64_t h_stride;
+    float* gu;              // [T][2N] gate and up before the limit (nullptr: not kept)
+    // backward
+    const uint16_t* dh;
+    int64_t dh_stride;
+    uint16_t* d;            // [T][2N] gradients of gate and up
+    uint16_t* dx;           // [T][K]
+    uint16_t* dw;           // [2N][K]
+    float* part;            // split sums (gated_part_floats of them)
+};
+int launch_gated_forward(const GatedArgs& a, hipStream_t st);
+// d from gu and dh; then dx (if set) = d W13 and dw (if set) = d^T x
+int launch_gated_backward(const GatedArgs& a, hipStream_t st);
+int64_t gated_part_floats(int64_t T, int64_t K, int64_t N, bool dx, bool dw);
+
 int launch_router_logits(const uint16_t* x, int64_t x_stride, const uint16_t* w, int T, int K, int E, float* logits,
                          hipStream_t st);
 int launch_router_topk(const float* logits, int T, int E, const float* bias, int topk, float scale, int renorm,

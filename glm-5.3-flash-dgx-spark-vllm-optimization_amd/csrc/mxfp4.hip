@@ -1,0 +1,695 @@
+// Microscaled 4-bit floating point (OCP MXFP4): e2m1 elements, element 2i of a row in the low four bits of byte i, and
+// one e8m0 scale (2^(code - 127), 255 = NaN) per 32 consecutive elements of a row.
+//
+//   quant    per block: E = the exponent field of max|v|, s = max(E - 2, 0), q = e2m1(v 2^(127 - s)), to nearest even,
+//            saturating at 6 (a block's largest element lies in [4, 8) after scaling); a block that holds an infinity or
+//            a NaN gets s = 255 and reads back as NaN
+//   product  out[m][n] = sum over blocks of 2^(sa + sw - 254) (sum of the block's 32 products), on the scaled matrix
+//            instructions: the products are exact (multiples of 1/4 up to 36), and against float64 their sums of 128 came
+//            out within 3e-8 of the sum of magnitudes, whatever the scales' spread
+//   experts  z = q(x) W13^T; h = silu(min(g, L)) clamp(u, -L, L) in fp32, quantised without a rounding to 16 bits;
+//            y = q(h) W2^T; out[token] = the token's w y in slot order (fp32), then the output type
+#include <algorithm>
+
+#include "gemm_tile.cuh"
+#include "mi355moe_internal.h"
+
+namespace mi355moe {
+
+// ------------------------------------------------------------------------------------------------ quantisation
+
+// The scale code of a block whose largest magnitude has these fp32 bits (sign cleared; NaN above infinity).
+__device__ __forceinline__ uint32_t mx_scale_code(uint32_t top) {
+    const uint32_t E = top >> 23;
+    return E == 255u ? 255u : (E > 2u ? E - 2u : 0u);
+}
+// 2^(127 - code); 0 for a NaN block, whose codes are then all zero (inf * 0 and NaN convert to some code: masked)
+__device__ __forceinline__ float mx_inv_scale(uint32_t code) {
+    return __builtin_bit_cast(float, code == 255u ? 0u : (254u - code) << 23);
+}
+// Eight values as eight e2m1 codes (round to nearest even, saturating), value 0 in the low bits.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float inv) {
+    uint32_t d = 0;
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[0] * inv, v[1] * inv, 1.0f, 0);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[2] * inv, v[3] * inv, 1.0f, 1);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[4] * inv, v[5] * inv, 1.0f, 2);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, v[6] * inv, v[7] * inv, 1.0f, 3);
+    return inv == 0.0f ? 0u : d;
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
+
+// Eight consecutive values from an aligned address (16 bytes for 16-bit types, two times 16 for fp32).
+template <int XDT>
+__device__ __forceinline__ void mx_load8(const void* x, size_t i, float (&v)[8]) {
+    if constexpr (XDT == DT_F32) {
+        const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(x) + i);
+        const f32x4 a = p[0], b = p[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+    } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (XDT == DT_BF16) {
+                v[2 * j] = bf16_to_f32((uint16_t)w[j]);
+                v[2 * j + 1] = bf16_to_f32((uint16_t)(w[j] >> 16));
+            } else {
+                v[2 * j] = (float)u16_as_h(w[j] & 0xFFFFu);
+                v[2 * j + 1] = (float)u16_as_h(w[j] >> 16);
+            }
+        }
+    }
+}
+
+// Rows of whole blocks at aligned addresses: four lanes a block, eight values a lane. Item i is 8 values; a row has
+// K / 8 of them. Scales lie at a pitch of sp bytes a row; bytes behind a row's scales are set to 127.
+template <int XDT>
+__global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ x, int64_t stride, int64_t items, int per_row,
+                                                       uint32_t* __restrict__ q, uint8_t* __restrict__ s, int64_t sp) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row;
+        const int c = (int)(i - r * per_row);
+        float v[8];
+        mx_load8<XDT>(x, (size_t)(r * stride + 8 * (int64_t)c), v);
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));       // (items % 4 == 0: a block's lanes are all here)
+        top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+        const uint32_t code = mx_scale_code(top);
+        q[i] = e2m1x8(v, mx_inv_scale(code));
+        if ((c & 3) == 0) {
+            s[r * sp + (c >> 2)] = (uint8_t)code;
+            if (c + 4 == per_row)
+                for (int64_t b = per_row >> 2; b < sp; ++b) s[r * sp + b] = 127;
+        }
+    }
+}
+
+// Any row length and alignment: one thread a block.
+__global__ __launch_bounds__(256) void mx_quant_any_kernel(const void* __restrict__ x, int xdt, int64_t stride, int64_t blocks,
+                                                           int K, uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t sp) {
+    const int nb = (K + 31) / 32, qp = (K + 1) / 2;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < blocks; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / nb;
+        const int b = (int)(i - r * nb), k0 = 32 * b, n = min(32, K - k0);
+        uint32_t top = 0;
+        for (int j = 0; j < n; ++j) top = max(top, abs_bits(load_value(x, xdt, (size_t)(r * stride + k0 + j))));
+        const uint32_t code = mx_scale_code(top);
+        const float inv = mx_inv_scale(code);
+        for (int j = 0; j < n; j += 8) {
+            float v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = j + t < n ? load_value(x, xdt, (size_t)(r * stride + k0 + j + t)) : 0.0f;
+            const uint32_t d = e2m1x8(v, inv);
+            uint8_t* o = q + r * qp + (k0 + j) / 2;
+            for (int t = 0; 2 * t < n - j && t < 4; ++t) o[t] = (uint8_t)(d >> (8 * t));
+        }
+        s[r * sp + b] = (uint8_t)code;
+        if (b + 1 == nb)
+            for (int64_t j = nb; j < sp; ++j) s[r * sp + j] = 127;
+    }
+}
+
+__device__ __forceinline__ float e2m1_value(uint32_t c) {
+    // exponent and mantissa bits of 1.x values moved into an fp32's fields; 0 and 0.5 apart
+    const uint32_t m = c & 7u;
+    const float v = m < 2u ? 0.5f * (float)m : __builtin_bit_cast(float, (126u << 23) + (m << 22));
+    return (c & 8u) ? -v : v;
+}
+__device__ __forceinline__ float mx_scale_value(uint32_t code) {
+    return __builtin_bit_cast(float, code == 255u ? 0x7FC00000u : code ? code << 23 : 0x00400000u);
+}
+
+// One thread per 8 values (VEC: rows of whole such groups, outputs at 16-byte addresses).
+template <bool VEC>
+__global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s,
+                                                         int64_t items, int K, void* __restrict__ out, int odt) {
+    const int per_row = (K + 7) / 8, nb = (K + 31) / 32, qp = (K + 1) / 2;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row;
+        const int c = (int)(i - r * per_row);
+        const float f = mx_scale_value(s[r * nb + (c >> 2)]);
+        const int n = min(8, K - 8 * c);
+        uint32_t d = 0;
+        if constexpr (VEC) d = reinterpret_cast<const uint32_t*>(q)[i];
+        else
+            for (int t = 0; 2 * t < n; ++t) d |= (uint32_t)q[r * qp + 4 * c + t] << (8 * t);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = e2m1_value(d >> (4 * j)) * f;
+        const size_t o = (size_t)(r * K + 8 * (int64_t)c);
+        if constexpr (VEC) {
+            if (odt == DT_F32) {
+                f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(out) + o);
+                p[0] = f32x4{v[0], v[1], v[2], v[3]};
+                p[1] = f32x4{v[4], v[5], v[6], v[7]};
+            } else {
+                u32x4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = odt == DT_BF16 ? pack_bf16x2(v[2 * j], v[2 * j + 1])
+                                          : h_as_u16((_Float16)v[2 * j]) | (h_as_u16((_Float16)v[2 * j + 1]) << 16);
+                *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + o) = w;
+            }
+        } else {
+            for (int j = 0; j < n; ++j) {
+                if (odt == DT_F32) static_cast<float*>(out)[o + j] = v[j];
+                else static_cast<uint16_t*>(out)[o + j] = odt == DT_BF16 ? f32_to_bf16(v[j]) : (uint16_t)h_as_u16((_Float16)v[j]);
+            }
+        }
+    }
+}
+
+// Rows of nb scale codes at a pitch of a whole number of dwords, the bytes behind them 127 (the products read whole
+// dwords). Two arrays in one launch.
+__global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t* __restrict__ a, int64_t ra, uint8_t* __restrict__ ao,
+                                                            const uint8_t* __restrict__ b, int64_t rb, uint8_t* __restrict__ bo,
+                                                            int nb, int pitch) {
+    const int64_t total = (ra + rb) * pitch;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / pitch;
+        const int c = (int)(i - r * pitch);
+        if (r < ra) ao[i] = c < nb ? a[r * nb + c] : 127;
+        else bo[i - ra * pitch] = c < nb ? b[(r - ra) * nb + c] : 127;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+
+// Weights for at most 16 rows are streamed once, straight from memory into MFMA operands: lane (c = lane % 16, g = lane
+// / 16) holds 64 consecutive bytes (four blocks, one a step) of weight row c and the dword of their scales, a wave 16
+// rows x 512 of the contraction. A = weights, so lane l's accumulator holds columns n = 4 (l / 16) .. + 3 of row m = l %
+// 16. The contraction is cut over waves; their sums join in LDS in wave order.
+struct FewRow {
+    const uint8_t* q;
+    const uint8_t* s;
+};
+// the four steps' operand bytes and scales of 512 values from block b0 on (nblk blocks in a row; blocks past them: zero
+// codes for ZERO, else those of the last one, and scales of 2^0)
+template <bool ZERO>
+__device__ __forceinline__ void few_load(const FewRow& r, int b0, int g, int nblk, u32x4 (&v)[4], int& sc) {
+    const int b = b0 + 4 * g;
+    if (b0 + 16 <= nblk) {                                           // (uniform)
+        const u32x4* p = reinterpret_cast<const u32x4*>(r.q + (size_t)b * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p[i];
+        sc = *reinterpret_cast<const int*>(r.s + b);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u32x4 t = *reinterpret_cast<const u32x4*>(r.q + (size_t)min(b + i, nblk - 1) * 16);
+            const bool ok = b + i < nblk || !ZERO;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = ok ? t[j] : 0u;
+        }
+        const int last = (nblk - 1) & ~3;
+        const int t = *reinterpret_cast<const int*>(r.s + min(b, last));
+        sc = b <= last ? t : 0x7F7F7F7F;
+    }
+}
+template <int S>
+__device__ __forceinline__ f32x4 few_mma(u32x4 a, u32x4 b, f32x4 c, int sa, int sb) {
+    const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, S, sa, S, sb);
+}
+template <int T>
+__device__ __forceinline__ void few_product(const FewRow (&w)[T], const FewRow& x, int b0, int g, int nblk, f32x4 (&acc)[T]) {
+    u32x4 wv[T][4], xv[4];
+    int ws[T], xs;
+#pragma unroll
+    for (int t = 0; t < T; ++t) few_load<false>(w[t], b0, g, nblk, wv[t], ws[t]);
+    few_load<true>(x, b0, g, nblk, xv, xs);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        acc[t] = few_mma<0>(wv[t][0], xv[0], acc[t], ws[t], xs);
+        acc[t] = few_mma<1>(wv[t][1], xv[1], acc[t], ws[t], xs);
+        acc[t] = few_mma<2>(wv[t][2], xv[2], acc[t], ws[t], xs);
+        acc[t] = few_mma<3>(wv[t][3], xv[3], acc[t], ws[t], xs);
+    }
+}
+
+// grid (N / 32, segments), 512 threads: 32 columns of gate and up for a segment of at most 16 rows, the contraction over
+// the eight waves, then SwiGLU and the quantisation of the 32 columns (one block) by a half wave a row.
+__global__ __launch_bounds__(512) void mx_gateup_few_kernel(Mxfp4Args a) {
+    __shared__ __align__(16) float red[8][4][256];
+    const int cb = blockIdx.x, s = blockIdx.y;
+    if (s >= a.nseg[0]) return;
+    const int e = a.seg_expert[s], row0 = a.seg_row0[s], rn = a.seg_rows[s];
+    if (rn <= 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nblk = a.K >> 5;
+    FewRow w[4], x;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const size_t r = (size_t)e * 2 * a.N + (t >> 1) * a.N + cb * 32 + (t & 1) * 16 + c;
+        w[t] = {a.w13 + r * (a.K / 2), a.w13s + r * a.w13sp};
+    }
+    const size_t tok = a.tok[row0 + min(c, rn - 1)];
+    x = {a.qx + tok * (a.K / 2), a.sx + tok * a.sxp};
+    f32x4 acc[4] = {};
+    for (int b0 = wv * 16; b0 < nblk; b0 += 128) few_product(w, x, b0, g, nblk, acc);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(&red[wv][t][lane * 4]) = acc[t];
+    __syncthreads();
+    const int m = tid >> 5, n = tid & 31;
+    const int at = ((((n & 15) >> 2) << 4) + m) * 4 + (n & 3), t = n >> 4;
+    float gs = 0.f, us = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        gs += red[i][t][at];
+        us += red[i][2 + t][at];
+    }
+    const float h = swiglu(gs, us, a.limit);
+    uint32_t top = abs_bits(h);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    const uint32_t code = mx_scale_code(top);
+    const float inv = mx_inv_scale(code);
+    const uint32_t nib = code == 255u ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, h * inv, 0.0f, 1.0f, 0) & 15u;
+    uint32_t d = nib << (4 * (n & 7));
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
+    if (m < rn) {
+        const size_t r = (size_t)row0 + m;
+        if ((n & 7) == 0) *reinterpret_cast<uint32_t*>(a.qh + r * (a.N / 2) + cb * 16 + (n >> 1)) = d;
+        if (n == 0) a.sh[r * a.shp + cb] = (uint8_t)code;
+        if (n > 0 && (cb + 1) * 32 == a.N && cb + n < a.shp) a.sh[r * a.shp + cb + n] = 127;   // (at most 3)
+    }
+}
+
+// The eight waves of a workgroup as KS cuts of the contraction x 8 / KS groups of 16 T columns. Store(m, n, four sums of
+// columns n ..): called for columns of this wave's own sums (after the join) and rows m < rows.
+template <int T, int KS, typename Store>
+__device__ __forceinline__ void few_columns(const uint8_t* wq, size_t wqp, const uint8_t* wsc, size_t wsp, int cols, int n0,
+                                            const FewRow& x, int nblk, float* red, const Store& store) {
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ks = wv % KS, grp = wv / KS;
+    const int nw = n0 + grp * 16 * T;
+    FewRow w[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const size_t r = min(nw + 16 * t + c, cols - 1);
+        w[t] = {wq + r * wqp, wsc + r * wsp};
+    }
+    f32x4 acc[T] = {};
+    for (int b0 = ks * 16; b0 < nblk; b0 += 16 * KS) few_product(w, x, b0, g, nblk, acc);
+    if constexpr (KS > 1) {
+#pragma unroll
+        for (int t = 0; t < T; ++t) *reinterpret_cast<f32x4*>(red + ((wv * T + t) * 64 + lane) * 4) = acc[t];
+        __syncthreads();
+        // tile t of a group is summed by the group's wave t % KS
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+            if (t % KS == ks) {
+                f32x4 v = {};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const f32x4 p = *reinterpret_cast<const f32x4*>(red + (((grp * KS + i) * T + t) * 64 + lane) * 4);
+                    v += p;
+                }
+                store(c, nw + 16 * t + 4 * g, v);
+            }
+    } else {
+#pragma unroll
+        for (int t = 0; t < T; ++t) store(c, nw + 16 * t + 4 * g, acc[t]);
+    }
+}
+
+// grid (ceil(K / (16 T 8 / KS)), segments), 512 threads: down projection of a segment of at most 16 rows.
+template <int T, int KS>
+__global__ __launch_bounds__(512) void mx_down_few_kernel(Mxfp4Args a) {
+    __shared__ __align__(16) float red[KS > 1 ? 8 * T * 256 : 4];
+    const int s = blockIdx.y;
+    if (s >= a.nseg[0]) return;
+    const int e = a.seg_expert[s], row0 = a.seg_row0[s], rn = a.seg_rows[s];
+    if (rn <= 0) return;
+    const int c = threadIdx.x & 15;
+    const size_t xr = (size_t)row0 + min(c, rn - 1);
+    const FewRow x = {a.qh + xr * (a.N / 2), a.sh + xr * a.shp};
+    const float rw = a.w32[xr];
+    const int pe = a.pe[xr];
+    few_columns<T, KS>(a.w2 + (size_t)e * a.K * (a.N / 2), a.N / 2, a.w2s + (size_t)e * a.K * a.w2sp, a.w2sp, a.K,
+                       (int)blockIdx.x * (16 * T * 8 / KS), x, a.N >> 5, red, [&](int m, int n, f32x4 v) {
+                           if (m < rn && n < a.K && pe >= 0)
+                               *reinterpret_cast<f32x4*>(a.contrib + xr * a.K + n) = v * f32x4{rw, rw, rw, rw};
+                       });
+}
+
+// grid (ceil(N / (16 T 8 / KS)), ceil(M / 16)), 512 threads: the dense product for few rows.
+template <int T, int KS>
+__global__ __launch_bounds__(512) void mx_matmul_few_kernel(MxMatmulArgs a) {
+    __shared__ __align__(16) float red[KS > 1 ? 8 * T * 256 : 4];
+    const int c = threadIdx.x & 15;
+    const int64_t m0 = (int64_t)blockIdx.y * 16;
+    const int64_t xr = min(m0 + c, a.M - 1);
+    const FewRow x = {a.q + xr * (a.K / 2), a.qs + xr * a.sp};
+    few_columns<T, KS>(a.w, a.K / 2, a.ws, a.sp, a.N, (int)blockIdx.x * (16 * T * 8 / KS), x, a.K >> 5, red,
+                       [&](int m, int n, f32x4 v) {
+                           if (m0 + m < a.M && n < a.N)
+                               store4(a.out, a.odt, (size_t)(m0 + m) * a.out_stride + n, a.N - n, v);
+                       });
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+
+template <int BP, int BQ, int WP, int WQ, int ST>
+using MxTile = GemmTile<MM_MX4, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
+
+__device__ __forceinline__ int mx_stages(int K) { return (K + 255) >> 8; }
+__device__ __forceinline__ int mx_tail(int K) { return (K & 255) >> 5; }
+
+// Dense product: workgroup tiles of BP columns x BQ rows, out or (splits > 1) fp32 partials [split][M][N].
+template <int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 1) void mx_matmul_kernel(MxMatmulArgs a, int nt, int mt) {
+    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = xcd_order(blockIdx.x, nt * mt);
+    const int n0 = (id % nt) * BP;
+    const int64_t m0 = (int64_t)(id / nt) * BQ;
+    const int stages = mx_stages(a.K), per = (stages + a.splits - 1) / a.splits;
+    const int kb0 = blockIdx.y * per, kb1 = min(stages, kb0 + per);
+    const uint32_t pitch = a.K / 2, sp = (uint32_t)a.sp;
+    const int pl = min(BP, a.N - n0) - 1;
+    const int ql = (int)min((int64_t)BQ, a.M - m0) - 1;
+    G t;
+    t.p.init_row(uniform_ptr(a.w + (size_t)n0 * pitch + (size_t)kb0 * 128), wv, lane, [&](int r) { return min(r, pl) * pitch; });
+    t.q.init_row(uniform_ptr(a.q + (size_t)m0 * pitch + (size_t)kb0 * 128), wv, lane, [&](int r) { return min(r, ql) * pitch; });
+    t.xp.init(a.ws + (size_t)n0 * sp, wv, lane, sp / 4, [&](int r) { return min(r, pl) * sp; });
+    t.xq.init(a.qs + (size_t)m0 * sp, wv, lane, sp / 4, [&](int r) { return min(r, ql) * sp; });
+    const int tail = kb1 == stages ? mx_tail(a.K) : 0;
+    if (kb0 < kb1) t.run(lds, kb0, kb1, tail, tail, 0, 0);
+    else
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
+    const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
+    void* out = a.splits > 1 ? static_cast<void*>(a.part + (size_t)blockIdx.y * a.M * a.N) : a.out;
+    const int odt = a.splits > 1 ? (int)DT_F32 : a.odt;
+    const int64_t stride = a.splits > 1 ? a.N : a.out_stride;
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        const int64_t m = m0 + q0 + 32 * j + (lane & 31);
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
+                if (n < a.N)
+                    store4(out, odt, (size_t)m * stride + n, a.N - n,
+                              f32x4{t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2], t.acc[i][j][4 * r + 3]});
+            }
+    }
+}
+
+// out = the splits' partials in order
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t M, int N, void* out, int odt,
+                                                   int64_t stride) {
+    const int64_t total = M * N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += part[(size_t)s * total + i];
+        const int64_t m = i / N;
+        const size_t o = (size_t)m * stride + (i - m * N);
+        if (odt == DT_F32) static_cast<float*>(out)[o] = v;
+        else static_cast<uint16_t*>(out)[o] = odt == DT_BF16 ? f32_to_bf16(v) : (uint16_t)h_as_u16((_Float16)v);
+    }
+}
+
+// Gate/up of a segment: grid (ceil(N / (BP / 2)), segments). A wave's P rows are its gate columns, then the same up
+// columns, so the SwiGLU is local to a lane; a 32-column block of a row lies in lanes l and l ^ 32.
+template <int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 1) void mx_gateup_kernel(Mxfp4Args a) {
+    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    static_assert(G::TP % 2 == 0, "");
+    extern __shared__ __align__(16) unsigned char lds[];
+    constexpr int HALF = BP / WP / 2;                                // gate (and up) columns of a wave
+    const int s = blockIdx.y;
+    if (s >= a.nseg[0]) return;
+    const int e = a.seg_expert[s], row0 = a.seg_row0[s], rn = a.seg_rows[s];
+    if (rn <= 0) return;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * (BP / 2);
+    const uint32_t pitch = a.K / 2;
+    auto wrow = [&](int r) {                                         // tile row -> row of w13[e]
+        const int w = r / (2 * HALF), i = r % (2 * HALF);
+        const int col = min(n0 + w * HALF + (i % HALF), a.N - 1);
+        return (uint32_t)(col + (i < HALF ? 0 : a.N));
+    };
+    auto trow = [&](int r) { return (uint32_t)a.tok[row0 + min(r, rn - 1)]; };
+    G t;
+    t.p.init_row(uniform_ptr(a.w13 + (size_t)e * 2 * a.N * pitch), wv, lane, [&](int r) { return wrow(r) * pitch; });
+    t.q.init_row(a.qx, wv, lane, [&](int r) { return trow(r) * pitch; });
+    t.xp.init(a.w13s + (size_t)e * 2 * a.N * a.w13sp, wv, lane, (a.K + 127) / 128, [&](int r) { return wrow(r) * (uint32_t)a.w13sp; });
+    t.xq.init(a.sx, wv, lane, (a.K + 127) / 128, [&](int r) { return trow(r) * (uint32_t)a.sxp; });
+    t.run(lds, 0, mx_stages(a.K), mx_tail(a.K), mx_tail(a.K), 0, 0);
+    const int p0 = (wv % WP) * HALF, q0 = (wv / WP) * (BQ / WQ), hl = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        const int m = q0 + 32 * j + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < G::TP / 2; ++i) {
+            float h[16];
+            uint32_t top = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                h[r] = swiglu(t.acc[i][j][r], t.acc[i + G::TP / 2][j][r], a.limit);
+                top = max(top, abs_bits(h[r]));
+            }
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+            const uint32_t code = mx_scale_code(top);
+            const float inv = mx_inv_scale(code);
+            // this lane's codes: columns 8 r + 4 hl .. + 3 for r = 0 .. 3, 16 bits each
+            uint32_t d[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float v[8] = {h[8 * k], h[8 * k + 1], h[8 * k + 2], h[8 * k + 3],
+                                    h[8 * k + 4], h[8 * k + 5], h[8 * k + 6], h[8 * k + 7]};
+                d[k] = e2m1x8(v, inv);
+            }
+            // lane l (hl 0) takes bytes 0 .. 7 of the block, lane l ^ 32 bytes 8 .. 15
+            const uint32_t other = (uint32_t)__shfl_xor((int)(hl ? d[0] : d[1]), 32, 64);
+            const uint32_t lo = hl ? other : d[0], hi = hl ? d[1] : other;   // columns 8 r .. + 3 and + 4 .. + 7
+            const uint2 v = make_uint2((lo & 0xFFFFu) | (hi << 16), (lo >> 16) | (hi & 0xFFFF0000u));
+            const int col = n0 + p0 + 32 * i;
+            if (m < rn && col < a.N) {
+                const size_t rr = (size_t)row0 + m;
+                *reinterpret_cast<uint2*>(a.qh + rr * (a.N / 2) + col / 2 + 8 * hl) = v;
+                if (hl == 0) {
+                    a.sh[rr * a.shp + col / 32] = (uint8_t)code;
+                    if (col + 32 == a.N)
+                        for (int b = a.N / 32; b < a.shp; ++b) a.sh[rr * a.shp + b] = 127;
+                }
+            }
+        }
+    }
+}
+
+// Down of a segment: grid (ceil(K / BP), segments), weighted contributions.
+template <int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 1) void mx_down_kernel(Mxfp4Args a) {
+    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int s = blockIdx.y;
+    if (s >= a.nseg[0]) return;
+    const int e = a.seg_expert[s], row0 = a.seg_row0[s], rn = a.seg_rows[s];
+    if (rn <= 0) return;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * BP;
+    const uint32_t pitch = a.N / 2;
+    auto wrow = [&](int r) { return (uint32_t)min(n0 + r, a.K - 1); };
+    auto xrow = [&](int r) { return (uint32_t)min(r, rn - 1); };
+    const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
+    float rw[G::TQ];
+    int ok[G::TQ];
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        const int m = q0 + 32 * j + (lane & 31);
+        const int pos = row0 + min(m, rn - 1);
+        rw[j] = a.w32[pos];
+        ok[j] = m < rn && a.pe[pos] >= 0;
+    }
+    G t;
+    t.p.init_row(uniform_ptr(a.w2 + (size_t)e * a.K * pitch), wv, lane, [&](int r) { return wrow(r) * pitch; });
+    t.q.init_row(uniform_ptr(a.qh + (size_t)row0 * pitch), wv, lane, [&](int r) { return xrow(r) * pitch; });
+    t.xp.init(a.w2s + (size_t)e * a.K * a.w2sp, wv, lane, (a.N + 127) / 128, [&](int r) { return wrow(r) * (uint32_t)a.w2sp; });
+    t.xq.init(a.sh + (size_t)row0 * a.shp, wv, lane, (a.N + 127) / 128, [&](int r) { return xrow(r) * (uint32_t)a.shp; });
+    t.run(lds, 0, mx_stages(a.N), mx_tail(a.N), mx_tail(a.N), 0, 0);
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        if (!ok[j]) continue;
+        float* o = a.contrib + (size_t)(row0 + q0 + 32 * j + (lane & 31)) * a.K;
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
+                if (n < a.K)                                         // (K % 32 == 0)
+                    *reinterpret_cast<f32x4*>(o + n) =
+                        f32x4{rw[j] * t.acc[i][j][4 * r], rw[j] * t.acc[i][j][4 * r + 1], rw[j] * t.acc[i][j][4 * r + 2],
+                               rw[j] * t.acc[i][j][4 * r + 3]};
+            }
+    }
+}
+
+// grid (T, ceil(K / 1024)), 256 threads: four columns a thread, a token's valid pairs in slot order (accumulate: added
+// to out's values, one rounding).
+__global__ __launch_bounds__(256) void mx_combine_kernel(Mxfp4Args a) {
+    const int t = blockIdx.x, col = blockIdx.y * 1024 + 4 * threadIdx.x;
+    if (col >= a.K) return;
+    f32x4 sum = {};
+    for (int k0 = 0; k0 < a.topk; k0 += 4) {
+        f32x4 c[4];
+        bool ok[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int pos = a.inv[t * a.topk + min(k0 + k, a.topk - 1)];
+            ok[k] = k0 + k < a.topk && a.pe[pos] >= 0;
+            c[k] = ok[k] ? *reinterpret_cast<const f32x4*>(a.contrib + (size_t)pos * a.K + col) : f32x4{};
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (ok[k]) sum += c[k];
+    }
+    const size_t o = (size_t)t * a.out_stride + col;
+    if (a.accumulate) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += load_value(a.out, a.odt, o + j);
+    }
+    store4(a.out, a.odt, o, 4, sum);
+}
+
+// ------------------------------------------------------------------------------------------------ launchers
+
+static unsigned grid_for(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, 256 * 32); }
+
+int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int64_t sp,
+                    hipStream_t st) {
+    if (rows <= 0) return 0;
+    const int unit = xdt == DT_F32 ? 4 : 8;                          // elements of a 16-byte load
+    const bool vec = K % 32 == 0 && stride % unit == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
+                     (reinterpret_cast<uintptr_t>(q) & 3) == 0;
+    if (vec) {
+        const int64_t items = rows * (K / 8);
+        const dim3 g(grid_for(items));
+        uint32_t* q32 = reinterpret_cast<uint32_t*>(q);
+        if (xdt == DT_F32) hipLaunchKernelGGL(mx_quant_kernel<DT_F32>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, sp);
+        else if (xdt == DT_F16) hipLaunchKernelGGL(mx_quant_kernel<DT_F16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, sp);
+        else hipLaunchKernelGGL(mx_quant_kernel<DT_BF16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, sp);
+    } else {
+        const int64_t blocks = rows * ((K + 31) / 32);
+        hipLaunchKernelGGL(mx_quant_any_kernel, dim3(grid_for(blocks)), dim3(256), 0, st, x, xdt, stride, blocks, K, q, s, sp);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_mx_dequant(const uint8_t* q, const uint8_t* s, int64_t rows, int K, void* out, int odt, hipStream_t st) {
+    if (rows <= 0) return 0;
+    const int64_t items = rows * ((K + 7) / 8);
+    const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
+    if (vec) hipLaunchKernelGGL(mx_dequant_kernel<true>, dim3(grid_for(items)), dim3(256), 0, st, q, s, items, K, out, odt);
+    else hipLaunchKernelGGL(mx_dequant_kernel<false>, dim3(grid_for(items)), dim3(256), 0, st, q, s, items, K, out, odt);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_join(const float* part, int splits, int64_t M, int N, void* out, int odt, int64_t stride, hipStream_t st) {
+    hipLaunchKernelGGL(join_kernel, dim3(grid_for(M * N)), dim3(256), 0, st, part, splits, M, N, out, odt, stride);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+static constexpr int64_t MX_FEW_M = 64;              // rows of a dense product up to which weights are streamed
+MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
+    MxMatmulPlan p{};
+    p.few = M <= MX_FEW_M;
+    p.splits = 1;
+    if (p.few) return p;
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+    p.tile = big >= 192 ? 256 : 128;
+    if (p.tile == 128) {
+        const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), stages = (K + 255) / 256;
+        while (p.splits < 8 && tiles * p.splits * 2 <= 512 && stages / (p.splits * 2) >= 2) p.splits *= 2;
+    }
+    return p;
+}
+
+template <int BP, int BQ, int WP, int WQ, int ST>
+static int run_mx_matmul(const MxMatmulArgs& a, hipStream_t st) {
+    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    static const bool ok = allow_lds(mx_matmul_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
+    if (!ok) return -1;
+    const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
+    hipLaunchKernelGGL((mx_matmul_kernel<BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
+    return 0;
+}
+
+int launch_mx_matmul(const MxMatmulArgs& a, const MxMatmulPlan& p, hipStream_t st) {
+    if (p.few) {
+        const int nblk = a.K >> 5;
+        const unsigned my = (unsigned)((a.M + 15) / 16);
+        auto grid = [&](int cols) { return dim3((a.N + cols - 1) / cols, my); };
+        if (nblk > 64) hipLaunchKernelGGL((mx_matmul_few_kernel<1, 8>), grid(16), dim3(512), 0, st, a);
+        else if (nblk > 32) hipLaunchKernelGGL((mx_matmul_few_kernel<1, 4>), grid(32), dim3(512), 0, st, a);
+        else if (nblk > 16) hipLaunchKernelGGL((mx_matmul_few_kernel<1, 2>), grid(64), dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((mx_matmul_few_kernel<1, 1>), grid(128), dim3(512), 0, st, a);
+    } else {
+        const int r = p.tile == 256 ? run_mx_matmul<256, 256, 2, 4, 2>(a, st) : run_mx_matmul<128, 128, 2, 2, 2>(a, st);
+        if (r) return r;
+        if (a.splits > 1) launch_join(a.part, a.splits, a.M, a.N, a.out, a.odt, a.out_stride, st);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_mx_pad_scales(const uint8_t* a, int64_t ra, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb, int pitch,
+                         hipStream_t st) {
+    hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid_for((ra + rb) * pitch)), dim3(256), 0, st, a, ra, ao, b, rb, bo, nb, pitch);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int BP, int BQ, int WP, int WQ, int ST>
+static int run_mx_gateup(const Mxfp4Args& a, hipStream_t st) {
+    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    static const bool ok = allow_lds(mx_gateup_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
+    if (!ok) return -1;
+    hipLaunchKernelGGL((mx_gateup_kernel<BP, BQ, WP, WQ, ST>), dim3((a.N + BP / 2 - 1) / (BP / 2), a.S_cap), dim3(G::THREADS), G::LDS, st, a);
+    return 0;
+}
+template <int BP, int BQ, int WP, int WQ, int ST>
+static int run_mx_down(const Mxfp4Args& a, hipStream_t st) {
+    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    static const bool ok = allow_lds(mx_down_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
+    if (!ok) return -1;
+    hipLaunchKernelGGL((mx_down_kernel<BP, BQ, WP, WQ, ST>), dim3((a.K + BP - 1) / BP, a.S_cap), dim3(G::THREADS), G::LDS, st, a);
+    return 0;
+}
+
+int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {
+    if ((kernels & 1) && launch_mx_quant(a.x, a.xdt, a.x_stride, a.T, a.K, a.qx, a.sx, a.sxp, st)) return -1;
+    const bool few = a.seg == MX_FEW;
+    if (kernels & 2) {
+        if (few) hipLaunchKernelGGL(mx_gateup_few_kernel, dim3(a.N / 32, a.S_cap), dim3(512), 0, st, a);
+        else if (run_mx_gateup<128, 64, 2, 2, 3>(a, st)) return -1;
+    }
+    if (kernels & 4) {
+        if (few) {
+            const int nblk = a.N >> 5;
+            auto grid = [&](int cols) { return dim3((a.K + cols - 1) / cols, a.S_cap); };
+            if (nblk > 64) hipLaunchKernelGGL((mx_down_few_kernel<2, 8>), grid(32), dim3(512), 0, st, a);
+            else if (nblk > 32) hipLaunchKernelGGL((mx_down_few_kernel<2, 4>), grid(64), dim3(512), 0, st, a);
+            else if (nblk > 16) hipLaunchKernelGGL((mx_down_few_kernel<2, 2>), grid(128), dim3(512), 0, st, a);
+            else hipLaunchKernelGGL((mx_down_few_kernel<2, 1>), grid(256), dim3(512), 0, st, a);
+        } else if (run_mx_down<128, 64, 2, 2, 3>(a, st)) return -1;
+    }
+    if (kernels & 8) hipLaunchKernelGGL(mx_combine_kernel, dim3(a.T, (a.K + 1023) / 1024), dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace mi355moe

@@ -7,6 +7,7 @@ when a call outgrows it; a replaced workspace is kept alive for the graphs captu
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -20,6 +21,11 @@ _RETIRED: dict = {}      # device -> superseded workspaces, kept alive for graph
 
 def _stream(dev: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _on_device(dev: torch.device):
+    """A context in which `dev` is the current device (kernels are launched on the current one)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _p(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -431,6 +431,74 @@ int mi355moe_e4m3_moe_forward_ids(const mi355moe_exl3_layer* layer, const void* 
                                   int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes,
                                   int stages, hipStream_t stream);
 
+/* ---------------------------------------------------------------- microscaled 4-bit floats (OCP MXFP4)
+ *
+ * A row of K values is ceil(K / 2) bytes of e2m1 codes (value 2i in the low four bits of byte i: sign, two exponent
+ * bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) and ceil(K / 32) e8m0 scale codes, one per 32 consecutive values
+ * (2^(code - 127); 255 is NaN). No counterpart in the reference: the format of MXFP4 checkpoints. */
+
+/* Rows to MXFP4. Per block: E = the fp32 exponent field of max|x|, s = max(E - 2, 0), q = e2m1(x * 2^(127 - s)) to
+ * nearest even, saturating at 6; a block that holds an infinity or a NaN gets s = 255. x: F32, F16 or BF16 [rows][K] with
+ * row stride x_stride, any K and alignment; q uint8 [rows][ceil(K/2)], scale uint8 [rows][ceil(K/32)]. */
+int mi355moe_mxfp4_quant_rows(const void* x, int x_dtype, int64_t rows, int64_t K, int64_t x_stride, void* q, void* scale,
+                              hipStream_t stream);
+/* The values of such rows: out F32, F16 or BF16 [rows][K] (exact in F32 and BF16 within their range). */
+int mi355moe_mxfp4_dequant_rows(const void* q, const void* scale, int64_t rows, int64_t K, void* out, int out_dtype,
+                                hipStream_t stream);
+
+/* out [M][N] (F32, F16 or BF16, row stride out_stride) = A W^T, A [M][K] and W [N][K] in MXFP4 (rows back to back as
+ * mi355moe_mxfp4_quant_rows writes them; codes 16-byte aligned, scales 4-byte aligned if K % 128 == 0). K % 32 == 0,
+ * K <= 65536; M and N up to 2^20. The products are exact, the sums fp32. The workspace (may be NULL if the size query says 0) needs no
+ * initialisation. */
+int64_t mi355moe_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const void* w, const void* w_scale, int64_t N,
+                          int64_t K, void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                          hipStream_t stream);
+
+/* A layer's MXFP4 experts. The scale strides are the bytes from one row's scales to the next's: multiples of 4, at
+ * least K / 32; the bytes behind a row's scales must not be 255 (whole dwords are read). hidden and intermediate are
+ * multiples of 32 up to 16384; w13 and w2 16-byte, the scales 4-byte aligned. */
+typedef struct mi355moe_mxfp4_layer {
+    int64_t n, hidden, intermediate;
+    const void* w13;          /* [n][2*intermediate][hidden/2]: rows 0..I-1 gate, I..2I-1 up */
+    const void* w13_scale;    /* [n][2*intermediate][w13_scale_stride] */
+    int64_t w13_scale_stride;
+    const void* w2;           /* [n][hidden][intermediate/2] */
+    const void* w2_scale;     /* [n][hidden][w2_scale_stride] */
+    int64_t w2_scale_stride;
+} mi355moe_mxfp4_layer;
+
+/* Routed-expert output of an MXFP4 layer from router ids and weights: z = q(x) W13^T, h = silu(min(g, L)) * clamp(u, -L,
+ * L) in fp32 (the limit iff L != 0), y = q(h) W2^T (q: mi355moe_mxfp4_quant_rows' rounding), out[token] = the token's
+ * w * y summed in slot order in fp32 (deterministic). Arguments as mi355moe_fp8_moe_forward_ids; options:
+ * MI355MOE_OPT_ACCUMULATE (out += the sum, one rounding) or 0. Pairs whose id is no local expert are skipped. The
+ * workspace needs no initialisation. T * topk <= 65536. */
+int64_t mi355moe_mxfp4_moe_workspace_bytes(const mi355moe_mxfp4_layer* layer, int64_t T, int64_t topk);
+int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void* x, int x_dtype, int64_t x_stride,
+                                   int64_t T, const void* ids, int ids_dtype, const void* weights, int weights_dtype,
+                                   int64_t topk, const int64_t* expert_map, int64_t n_global, float limit, void* out,
+                                   int out_dtype, int64_t out_stride, int options, void* workspace,
+                                   size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------- the shared expert's gated block */
+
+/* h [T][intermediate] = silu(min(g, L)) * clamp(u, -L, L) (the limit iff L != 0), [g | u] = x W13^T in fp32, rounded
+ * once: both projections, the activation and the product in one kernel (what the model's shared expert computes before
+ * its down projection). x [T][hidden] (row stride x_stride), w13 [2 * intermediate][hidden] (gate rows, then up rows)
+ * and h (row stride h_stride) of one dtype, F16 or BF16; hidden and intermediate multiples of 8; x and w13 16-byte
+ * aligned, x_stride a multiple of 8. gu (optional, fp32 [T][2 * intermediate], 16-byte aligned) receives g and u for
+ * the backward pass. */
+int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, int64_t x_stride, const void* w13,
+                           int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, hipStream_t stream);
+/* Its gradients: with s = sigmoid(g'), g' = min(g, L), u' = clamp(u, -L, L): dg = dh u' s (1 + g' (1 - s)) where g <= L,
+ * du = dh g' s where |u| <= L (else 0), both rounded once to dtype; dx [T][hidden] = [dg | du] W13 and dw13
+ * [2 * intermediate][hidden] = [dg | du]^T x, fp32 sums rounded once, deterministic. dx or dw13 may be NULL (not
+ * computed). T >= 1 if dw13 is asked for. Alignment of dh, dx, dw13 and the workspace as for x. */
+int64_t mi355moe_gated_backward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate);
+int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, const void* x, int dtype, int64_t T,
+                            int64_t hidden, int64_t x_stride, const void* w13, int64_t intermediate, float limit, void* dx,
+                            void* dw13, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
