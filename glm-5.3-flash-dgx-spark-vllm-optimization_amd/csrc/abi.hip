@@ -282,15 +282,16 @@ int mxfp4_layer_ok(const mi355moe_mxfp4_layer* L) {
     if (L->n < 1 || L->n > MAX_EXPERTS) return MI355MOE_ELIMIT;
     if (L->hidden < 32 || L->hidden % 32 || L->intermediate < 32 || L->intermediate % 32) return MI355MOE_ESHAPE;
     if (L->hidden > 16384 || L->intermediate > 16384) return MI355MOE_ELIMIT;
-    if (L->w13_scale_stride < L->hidden / 32 || L->w13_scale_stride % 4 || L->w13_scale_stride > 4096 ||
-        L->w2_scale_stride < L->intermediate / 32 || L->w2_scale_stride % 4 || L->w2_scale_stride > 4096)
-        return MI355MOE_ESHAPE;
+    if (L->arranged != 0 && L->arranged != 1) return MI355MOE_EINVAL;
+    if (!L->arranged && (L->hidden % 128 || L->intermediate % 128)) return MI355MOE_ESHAPE;
     if ((reinterpret_cast<uintptr_t>(L->w13) | reinterpret_cast<uintptr_t>(L->w2)) & 15) return MI355MOE_EINVAL;
-    if ((reinterpret_cast<uintptr_t>(L->w13_scale) | reinterpret_cast<uintptr_t>(L->w2_scale)) & 3) return MI355MOE_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(L->w13_scale) | reinterpret_cast<uintptr_t>(L->w2_scale)) & (L->arranged ? 7 : 3))
+        return MI355MOE_EINVAL;
     return 0;
 }
 
-int64_t scale_pitch(int64_t k) { return (k / 32 + 3) / 4 * 4; }
+// bytes of the scales of rows of k values arranged by steps
+int64_t arranged_bytes(int64_t rows, int64_t k) { return rows * ((k / 32 + 7) / 8 * 8); }
 
 struct Mxfp4Ws {
     RouteArgs ra;
@@ -321,12 +322,10 @@ void carve_mxfp4(void* ws, int64_t P, int64_t T, int64_t n, int64_t K, int64_t N
     r.loc = c.take<int>(P);
     r.blk_cnt = c.take<int>(((P + 1023) / 1024) * (n + 1));
     r.cnt_out = c.take<int>(n + 1);
-    f.sxp = scale_pitch(K);
-    f.shp = scale_pitch(N);
     f.qx = c.take<uint8_t>((size_t)T * (K / 2));
-    f.sx = c.take<uint8_t>((size_t)T * f.sxp);
+    f.sx = c.take<uint8_t>(arranged_bytes(T, K));
     f.qh = c.take<uint8_t>((size_t)P * (N / 2));
-    f.sh = c.take<uint8_t>((size_t)P * f.shp);
+    f.sh = c.take<uint8_t>(arranged_bytes(P, N));
     f.contrib = c.take<float>((size_t)P * K);
     w.bytes = c.off;
 }
@@ -1851,7 +1850,7 @@ int mi355moe_mxfp4_quant_rows(const void* x, int x_dtype, int64_t rows, int64_t 
     if (rows == 0) return 0;
     if (!x || !q || !scale) return MI355MOE_EINVAL;
     return rc_launch(launch_mx_quant(x, dt_w(x_dtype), x_stride, rows, (int)K, static_cast<uint8_t*>(q),
-                                     static_cast<uint8_t*>(scale), (K + 31) / 32, stream));
+                                     static_cast<uint8_t*>(scale), 0, stream));
 }
 
 int mi355moe_mxfp4_dequant_rows(const void* q, const void* scale, int64_t rows, int64_t K, void* out, int out_dtype,
@@ -1875,7 +1874,7 @@ int64_t mi355moe_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (mx_matmul_ok(M, N, K)) return -1;
     const MxMatmulPlan p = plan_mx_matmul(M, N, K);
     int64_t b = 0;
-    if (K % 128) b += (int64_t)(align_up(M * scale_pitch(K)) + align_up(N * scale_pitch(K)));
+    if (p.arrange) b += (int64_t)(align_up(arranged_bytes(M, K)) + align_up(arranged_bytes(N, K)));
     if (p.splits > 1) b += p.splits * M * N * 4;
     return b;
 }
@@ -1889,36 +1888,46 @@ int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const v
     if (M == 0) return 0;
     if (!a || !a_scale || !w || !w_scale || !out) return MI355MOE_EINVAL;
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15) return MI355MOE_EINVAL;
-    const bool pad = K % 128 != 0;
-    if (!pad && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3)) return MI355MOE_EINVAL;
+    const MxMatmulPlan p = plan_mx_matmul(M, N, K);
+    if (!p.arrange && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3)) return MI355MOE_EINVAL;
     const int64_t need = mi355moe_mxfp4_matmul_workspace_bytes(M, N, K);
     if (need > 0 && !workspace) return MI355MOE_EINVAL;
     if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
-    const MxMatmulPlan p = plan_mx_matmul(M, N, K);
     MxMatmulArgs m{};
     m.q = static_cast<const uint8_t*>(a);
-    m.qs = static_cast<const uint8_t*>(a_scale);
+    m.qs = MxScales{static_cast<const uint8_t*>(a_scale), (uint32_t)(K / 32), 8};
     m.M = M;
     m.w = static_cast<const uint8_t*>(w);
-    m.ws = static_cast<const uint8_t*>(w_scale);
+    m.ws = MxScales{static_cast<const uint8_t*>(w_scale), (uint32_t)(K / 32), 8};
     m.N = (int)N;
     m.K = (int)K;
-    m.sp = scale_pitch(K);
     m.out = out;
     m.odt = dt_w(out_dtype);
     m.out_stride = out_stride;
     m.splits = p.splits;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    if (pad) {
+    if (p.arrange) {
         uint8_t* ap = ws;
-        uint8_t* wp = ap + align_up(M * m.sp);
-        ws = wp + align_up(N * m.sp);
-        if (int r = launch_mx_pad_scales(m.qs, M, ap, m.ws, N, wp, (int)(K / 32), (int)m.sp, stream)) return rc_launch(r);
-        m.qs = ap;
-        m.ws = wp;
+        uint8_t* wp = ap + align_up(arranged_bytes(M, K));
+        ws = wp + align_up(arranged_bytes(N, K));
+        if (int r = launch_mx_arrange(m.qs.p, 1, M, ap, m.ws.p, N, wp, (int)(K / 32), stream)) return rc_launch(r);
+        m.qs = MxScales{ap, 8, (uint32_t)(8 * M)};
+        m.ws = MxScales{wp, 8, (uint32_t)(8 * N)};
     }
     m.part = reinterpret_cast<float*>(ws);
     return rc_launch(launch_mx_matmul(m, p, stream));
+}
+
+int64_t mi355moe_mxfp4_arranged_bytes(int64_t mats, int64_t rows, int64_t K) {
+    if (mats < 1 || mats > MAX_EXPERTS || rows < 1 || rows > (1 << 20) || K < 32 || K % 32 || K > 65536) return -1;
+    return mats * arranged_bytes(rows, K);
+}
+
+int mi355moe_mxfp4_arrange_scales(const void* scale, int64_t mats, int64_t rows, int64_t K, void* out, hipStream_t stream) {
+    if (mi355moe_mxfp4_arranged_bytes(mats, rows, K) < 0) return MI355MOE_ESHAPE;
+    if (!scale || !out || (reinterpret_cast<uintptr_t>(out) & 7)) return MI355MOE_EINVAL;
+    return rc_launch(launch_mx_arrange(static_cast<const uint8_t*>(scale), mats, rows, static_cast<uint8_t*>(out), nullptr, 0, nullptr,
+                                       (int)(K / 32), stream));
 }
 
 int64_t mi355moe_mxfp4_moe_workspace_bytes(const mi355moe_mxfp4_layer* layer, int64_t T, int64_t topk) {
@@ -1970,11 +1979,20 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
     f.P = (int)P;
     f.T = (int)T;
     f.w13 = static_cast<const uint8_t*>(layer->w13);
-    f.w13s = static_cast<const uint8_t*>(layer->w13_scale);
-    f.w13sp = layer->w13_scale_stride;
     f.w2 = static_cast<const uint8_t*>(layer->w2);
-    f.w2s = static_cast<const uint8_t*>(layer->w2_scale);
-    f.w2sp = layer->w2_scale_stride;
+    const uint8_t* s13 = static_cast<const uint8_t*>(layer->w13_scale);
+    const uint8_t* s2 = static_cast<const uint8_t*>(layer->w2_scale);
+    if (layer->arranged) {
+        f.w13s = MxScales{s13, 8, (uint32_t)(8 * 2 * N)};
+        f.w13se = arranged_bytes(2 * N, K);
+        f.w2s = MxScales{s2, 8, (uint32_t)(8 * K)};
+        f.w2se = arranged_bytes(K, N);
+    } else {
+        f.w13s = MxScales{s13, (uint32_t)(K / 32), 8};
+        f.w13se = 2 * N * (K / 32);
+        f.w2s = MxScales{s2, (uint32_t)(N / 32), 8};
+        f.w2se = K * (N / 32);
+    }
     f.x = x;
     f.xdt = dt_w(x_dtype);
     f.x_stride = x_stride;
@@ -2002,7 +2020,8 @@ int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, 
     if (x_stride < hidden || h_stride < intermediate || x_stride > (1 << 22)) return MI355MOE_ESHAPE;
     if (T == 0) return 0;
     if (!x || !w13 || !h) return MI355MOE_EINVAL;
-    if (!rows16_ok(x, x_stride) || !rows16_ok(w13, hidden) || (reinterpret_cast<uintptr_t>(gu) & 15)) return MI355MOE_EINVAL;
+    if (!rows16_ok(x, x_stride) || !rows16_ok(w13, hidden) || !rows16_ok(h, h_stride) || (reinterpret_cast<uintptr_t>(gu) & 15))
+        return MI355MOE_EINVAL;
     GatedArgs g{};
     g.dt = dt_act(dtype);
     g.T = T;

@@ -101,16 +101,16 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
 
 // Workgroup tiles of BP / 2 columns x BQ tokens; a wave's P rows are its gate columns, then the same up columns.
 template <int DT, int BP, int BQ, int WP, int WQ, int ST>
-__global__ __launch_bounds__(64 * WP * WQ, 1) void gated_kernel(GatedArgs a, int nt, int mt) {
+__global__ __launch_bounds__(64 * WP * WQ, 2) void gated_kernel(GatedArgs a, int nt, int mt) {
     using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
     static_assert(G::TP % 2 == 0, "");
     extern __shared__ __align__(16) unsigned char lds[];
     constexpr int HALF = BP / WP / 2;
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_order(blockIdx.x, nt * mt);
-    const int n0 = (id % nt) * (BP / 2);
-    const int64_t m0 = (int64_t)(id / nt) * BQ;
+    const int2 tile = tile_order(blockIdx.x, nt, mt);
+    const int n0 = tile.x * (BP / 2);
+    const int64_t m0 = (int64_t)tile.y * BQ;
     const int ql = (int)min((int64_t)BQ, a.T - m0) - 1;
     const uint32_t wp = 2u * a.K, xp = 2u * (uint32_t)a.x_stride;
     G t;
@@ -119,33 +119,36 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void gated_kernel(GatedArgs a, int
         return (uint32_t)(min(n0 + w * HALF + (i % HALF), a.N - 1) + (i < HALF ? 0 : a.N)) * wp;
     });
     t.q.init_row(uniform_ptr(a.x + (size_t)m0 * a.x_stride), wv, lane, [&](int r) { return (uint32_t)min(r, ql) * xp; });
-    const int tail = (a.K & 63) >> 3;
-    t.run(lds, 0, (a.K + 63) >> 6, tail, tail, 0, 0);
+    const int tail = a.K % (SB / 2) / 8;
+    t.run(lds, 0, (a.K + SB / 2 - 1) / (SB / 2), tail, tail, 0, 0);
     const int p0 = (wv % WP) * HALF, q0 = (wv / WP) * (BQ / WQ);
+    // SwiGLU in place of the gate sums, after g and u are kept
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
         const int64_t m = m0 + q0 + 32 * j + (lane & 31);
-        if (m >= a.T) continue;
 #pragma unroll
         for (int i = 0; i < G::TP / 2; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
-                if (n >= a.N) continue;                              // (N % 8 == 0: four columns exist or none)
-                f32x4 g, u, h;
+                f32x4 g, u;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     g[k] = t.acc[i][j][4 * r + k];
                     u[k] = t.acc[i + G::TP / 2][j][4 * r + k];
-                    h[k] = swiglu(g[k], u[k], a.limit);
+                    t.acc[i][j][4 * r + k] = swiglu(g[k], u[k], a.limit);
                 }
-                store4(a.h, DT, (size_t)m * a.h_stride + n, 4, h);
-                if (a.gu) {
+                if (a.gu && m < a.T && n < a.N) {                    // (N % 8 == 0: four columns exist or none)
                     *reinterpret_cast<f32x4*>(a.gu + (size_t)m * 2 * a.N + n) = g;
                     *reinterpret_cast<f32x4*>(a.gu + (size_t)m * 2 * a.N + a.N + n) = u;
                 }
             }
     }
+    t.template store_rows16<G::TP / 2>(lds, a.h + (size_t)(m0 + q0) * a.h_stride + n0 + p0, a.h_stride, a.T - m0 - q0,
+                                       a.N - n0 - p0, [&](int i, int j, int r) {
+                                           return pack4(DT, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
+                                                        t.acc[i][j][4 * r + 3]);
+                                       });
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -204,26 +207,26 @@ struct Gemm16Args {
 
 // out[m][n] = sum over k of P Q, dtype DT, or fp32 partials of the contraction's splits (grid y).
 template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
-__global__ __launch_bounds__(64 * WP * WQ, 1) void gemm16_kernel(Gemm16Args a, int nt, int mt) {
+__global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, int nt, int mt) {
     using G = GemmTile<KindOf<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_order(blockIdx.x, nt * mt);
-    const int n0 = (id % nt) * BP;
-    const int64_t m0 = (int64_t)(id / nt) * BQ;
-    const int stages = (int)((a.C + 63) >> 6), per = (stages + a.splits - 1) / a.splits;
+    const int2 tile = tile_order(blockIdx.x, nt, mt);
+    const int n0 = tile.x * BP;
+    const int64_t m0 = (int64_t)tile.y * BQ;
+    const int stages = (int)((a.C + SB / 2 - 1) / (SB / 2)), per = (stages + a.splits - 1) / a.splits;
     const int kb0 = blockIdx.y * per, kb1 = min(stages, kb0 + per);
     const uint32_t ldp = 2u * (uint32_t)a.ldp, ldq = 2u * (uint32_t)a.ldq;
     const int pl = min(BP, a.N - n0), ql = (int)min((int64_t)BQ, a.M - m0);
     G t;
     if constexpr (PL == LAY_ROW)
-        t.p.init_row(uniform_ptr(a.p + (size_t)n0 * a.ldp + (size_t)kb0 * 64), wv, lane, [&](int r) { return (uint32_t)min(r, pl - 1) * ldp; });
-    else t.p.init_col(uniform_ptr(a.p + (size_t)kb0 * 64 * a.ldp + n0), wv, lane, ldp, pl);
+        t.p.init_row(uniform_ptr(a.p + (size_t)n0 * a.ldp + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, pl - 1) * ldp; });
+    else t.p.init_col(uniform_ptr(a.p + (size_t)kb0 * (SB / 2) * a.ldp + n0), wv, lane, ldp, pl);
     if constexpr (QL == LAY_ROW)
-        t.q.init_row(uniform_ptr(a.q + (size_t)m0 * a.ldq + (size_t)kb0 * 64), wv, lane, [&](int r) { return (uint32_t)min(r, ql - 1) * ldq; });
-    else t.q.init_col(uniform_ptr(a.q + (size_t)kb0 * 64 * a.ldq + m0), wv, lane, ldq, ql);
-    const int left = kb1 == stages ? (int)(a.C & 63) : 0;
+        t.q.init_row(uniform_ptr(a.q + (size_t)m0 * a.ldq + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, ql - 1) * ldq; });
+    else t.q.init_col(uniform_ptr(a.q + (size_t)kb0 * (SB / 2) * a.ldq + m0), wv, lane, ldq, ql);
+    const int left = kb1 == stages ? (int)(a.C % (SB / 2)) : 0;
     if (kb0 < kb1) t.run(lds, kb0, kb1, PL == LAY_ROW ? left >> 3 : left, QL == LAY_ROW ? left >> 3 : left, ldp, ldq);
     else
 #pragma unroll
@@ -231,9 +234,15 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void gemm16_kernel(Gemm16Args a, i
 #pragma unroll
             for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
     const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
-    void* out = a.splits > 1 ? static_cast<void*>(a.part + (size_t)blockIdx.y * a.M * a.N) : a.out;
-    const int odt = a.splits > 1 ? (int)DT_F32 : DT;
-    const int64_t stride = a.splits > 1 ? a.N : a.out_stride;
+    if (a.splits == 1) {                                             // (uniform)
+        t.template store_rows16<G::TP>(lds, static_cast<uint16_t*>(a.out) + (size_t)(m0 + q0) * a.out_stride + n0 + p0, a.out_stride,
+                                       a.M - m0 - q0, a.N - n0 - p0, [&](int i, int j, int r) {
+                                           return pack4(DT, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
+                                                        t.acc[i][j][4 * r + 3]);
+                                       });
+        return;
+    }
+    float* part = a.part + (size_t)blockIdx.y * a.M * a.N;
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
         const int64_t m = m0 + q0 + 32 * j + (lane & 31);
@@ -243,9 +252,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void gemm16_kernel(Gemm16Args a, i
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
-                if (n < a.N)
-                    store4(out, odt, (size_t)m * stride + n, 4,
-                           f32x4{t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2], t.acc[i][j][4 * r + 3]});
+                if (n < a.N)                                         // (N % 8 == 0)
+                    *reinterpret_cast<f32x4*>(part + (size_t)m * a.N + n) =
+                        f32x4{t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2], t.acc[i][j][4 * r + 3]};
             }
     }
 }

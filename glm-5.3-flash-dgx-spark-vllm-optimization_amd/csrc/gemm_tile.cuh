@@ -14,7 +14,8 @@
 // Stages are filled by asynchronous global-to-LDS loads (16 bytes a lane, 1 KB a wave instruction).
 //
 // An operand lies in memory in one of two ways:
-//   ROW  the contraction is contiguous: LDS holds row R's eight 16-byte chunks, chunk g at slot g ^ ((R >> 1) & 7)
+//   ROW  the contraction is contiguous: LDS holds row R's 16-byte chunks, chunk g at slot g ^ row_swz(R): sixteen
+//        consecutive rows' chunk g lie in sixteen different 16-byte columns of the banks
 //   COL  the contraction is the row index (16-bit only): LDS holds 64 rows of R values; a fragment is two
 //        ds_read_b64_tr_b16, each of which hands lane i of 16 column i of a 4 x 16 block. Consecutive rows are whole
 //        bank rounds apart, so the 32-byte segments of row k are rotated (xor) by k's place among the rows that one
@@ -31,6 +32,9 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Keeps the compiler from moving anything across: the loops below are scheduled by hand.
+#define SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
 
 enum MmKind { MM_F16 = 0, MM_BF16 = 1, MM_MX4 = 2 };
 enum { LAY_ROW = 0, LAY_COL = 1 };
@@ -50,24 +54,29 @@ __device__ __forceinline__ f32x16 mma_mx(u32x4 a, u32x4 b, f32x16 c, int sa, int
 }
 
 __device__ __forceinline__ int row_swz(int R) { return (R >> 1) & 7; }
-// the xor of row k's 32-byte segment index (R values a row): distinct over the rows one transposing read touches, as far
-// as the row's segments go
+// the xor of row k's 32-byte segment index (R values a row): distinct over the rows one transposing read touches (k & 3 in
+// both halves of the stage), as far as the row's segments go
 template <int R>
 __device__ __forceinline__ int col_swz(int k) {
     if constexpr (R >= 256) return ((k & 3) | ((k >> 3) & 4)) << 1;
     else if constexpr (R == 128) return (k & 3) << 1;
     else return ((k >> 1) & 1) << 1;
 }
+constexpr int SB = 128;                              // bytes of a row in a stage
 
 // Staging of one operand of R rows (LAY_COL: R columns) by NW waves.
 template <int LAY, int R, int NW>
 struct Stager {
-    static constexpr int INST = R / 8 / NW;          // 1 KB wave instructions per stage and wave
-    static_assert(INST * 8 * NW == R, "rows divide over the waves");
+    static constexpr int CH = SB / 16;               // chunks of a row (ROW)
+    static constexpr int KR = SB / 2;                // rows of a stage (COL)
+    static constexpr int INST = R * SB / 1024 / NW;  // 1 KB wave instructions per stage and wave
+    static_assert(INST * 1024 * NW == R * SB, "the stage divides over the waves");
     const unsigned char* base;                       // wave-uniform
     uint32_t off[INST];                              // this lane's source bytes of each instruction
     int lds;                                         // this wave's first byte of the operand's stage
 
+    // the place (in 16 bytes) that instruction j of this lane fills
+    static __device__ __forceinline__ int place(int wv, int j, int lane) { return (wv * INST + j) * 64 + lane; }
     // ROW: rowoff(R) = byte offset of tile row R from `b`
     template <typename F>
     __device__ __forceinline__ void init_row(const void* b, int wv, int lane, const F& rowoff) {
@@ -76,8 +85,8 @@ struct Stager {
         lds = wv * INST * 1024;
 #pragma unroll
         for (int j = 0; j < INST; ++j) {
-            const int r = (wv * INST + j) * 8 + (lane >> 3);
-            off[j] = rowoff(r) + (((lane & 7) ^ row_swz(r)) << 4);
+            const int r = place(wv, j, lane) / CH;
+            off[j] = rowoff(r) + (((lane & (CH - 1)) ^ row_swz(r)) << 4);
         }
     }
     // COL: row k at ld * k bytes; `cols` values of the row from `b` on may be read (a multiple of 8)
@@ -87,29 +96,29 @@ struct Stager {
         lds = wv * INST * 1024;
 #pragma unroll
         for (int j = 0; j < INST; ++j) {
-            const int p = col_slot(wv, j, lane);
-            const int k = p / (R / 8);
-            const int c = p % (R / 8);
+            const int p = place(wv, j, lane), k = p / (R / 8), c = p % (R / 8);
             const int col = (((c >> 1) ^ col_swz<R>(k)) << 4) + ((c & 1) << 3);
             off[j] = (uint32_t)k * ld + 2u * (uint32_t)min(col, cols - 8);
         }
     }
-    __device__ __forceinline__ int col_slot(int wv, int j, int lane) const { return (wv * INST + j) * 64 + lane; }
+    // part I of N of a stage's loads
+    template <int I, int N>
     __device__ __forceinline__ void issue(unsigned char* st) const {
 #pragma unroll
-        for (int j = 0; j < INST; ++j) dma16_base(base, off[j], st + lds + j * 1024);
+        for (int j = INST * I / N; j < INST * (I + 1) / N; ++j) dma16_base(base, off[j], st + lds + j * 1024);
     }
     // the last stage, of which only `valid` chunks (ROW) or rows (COL, of ld bytes) exist: what lies behind them is
     // loaded from the last one that exists (and cleared in LDS by clear_tail)
+    template <int I, int N>
     __device__ __forceinline__ void issue_tail(unsigned char* st, int wv, int lane, int valid, uint32_t ld) const {
 #pragma unroll
-        for (int j = 0; j < INST; ++j) {
+        for (int j = INST * I / N; j < INST * (I + 1) / N; ++j) {
             uint32_t o = off[j];
             if constexpr (LAY == LAY_ROW) {
-                const int g = (lane & 7) ^ row_swz((wv * INST + j) * 8 + (lane >> 3));
+                const int g = (lane & (CH - 1)) ^ row_swz(place(wv, j, lane) / CH);
                 if (g >= valid) o -= (uint32_t)(g - valid + 1) << 4;
             } else {
-                const int k = col_slot(wv, j, lane) / (R / 8);
+                const int k = place(wv, j, lane) / (R / 8);
                 if (k >= valid) o -= (uint32_t)(k - valid + 1) * ld;
             }
             dma16_base(base, o, st + lds + j * 1024);
@@ -118,12 +127,12 @@ struct Stager {
     static __device__ __forceinline__ void clear_tail(unsigned char* st, int tid, int valid) {
         const u32x4 z = {0, 0, 0, 0};
         if constexpr (LAY == LAY_ROW) {
-            for (int i = tid; i < R * 8; i += NW * 64) {
-                const int r = i >> 3, g = i & 7;
-                if (g >= valid) *reinterpret_cast<u32x4*>(st + r * 128 + ((g ^ row_swz(r)) << 4)) = z;
+            for (int i = tid; i < R * CH; i += NW * 64) {
+                const int r = i / CH, g = i % CH;
+                if (g >= valid) *reinterpret_cast<u32x4*>(st + r * SB + ((g ^ row_swz(r)) << 4)) = z;
             }
         } else {
-            for (int i = valid * (R / 8) + tid; i < 64 * (R / 8); i += NW * 64) *reinterpret_cast<u32x4*>(st + i * 16) = z;
+            for (int i = valid * (R / 8) + tid; i < KR * (R / 8); i += NW * 64) *reinterpret_cast<u32x4*>(st + i * 16) = z;
         }
     }
 };
@@ -131,10 +140,10 @@ struct Stager {
 // The 16 bytes (lane r = lane % 32, half h) of step s of the 32-row tile at row r0.
 template <int LAY, int R>
 __device__ __forceinline__ u32x4 fragment(const unsigned char* st, int r0, int s, int lane) {
-    const int c = 4 * (lane >> 5) + s;
+    const int c = SB / 32 * (lane >> 5) + s;
     if constexpr (LAY == LAY_ROW) {
         const int r = r0 + (lane & 31);
-        return *reinterpret_cast<const u32x4*>(st + r * 128 + ((c ^ row_swz(r)) << 4));
+        return *reinterpret_cast<const u32x4*>(st + r * SB + ((c ^ row_swz(r)) << 4));
     } else {
         const int i = lane & 15;
         const int seg = (r0 >> 4) + ((lane >> 4) & 1);
@@ -150,53 +159,55 @@ __device__ __forceinline__ u32x4 fragment(const unsigned char* st, int r0, int s
     }
 }
 
-// Scale dwords of an MXFP4 operand: a stage holds 8 bytes of each row's scales (the dword of half h at 4h), 256 bytes
-// (32 rows) a wave instruction of 4 bytes a lane.
+// Scale dwords of an MXFP4 operand: a stage holds 8 bytes of each row's scales (the dword of half h at 4h), 256 bytes (32
+// rows) a wave instruction of 4 bytes a lane. Row R's scales of stage kb lie at rowoff(R) + kb * step: back to back for the
+// rows of a tile where the scales were arranged by steps; in rows of K / 32 bytes they touch as many lines as the stage's
+// codes do, for a sixteenth of the bytes (256 x 256 tiles, K 16384: 3390 cycles a stage, 2470 without these loads).
 template <int R, int NW>
 struct ScaleStager {
     static constexpr int INST = (R / 32 + NW - 1) / NW;
     const unsigned char* base;
+    uint32_t step;
     uint32_t off[INST];
-    uint32_t last[INST];                             // the row's last dword
+    uint32_t last[INST];                             // the row's last dword (rows of an odd number of them end in mid-stage)
     int lds[INST];
     template <typename F>
-    __device__ __forceinline__ void init(const void* b, int wv, int lane, int dwords, const F& rowoff) {
-        base = static_cast<const unsigned char*>(b);
+    __device__ __forceinline__ void init(const MxScales& s, size_t row0, int dwords, int wv, int lane, const F& row) {
+        base = s.p + row0 * s.row;
+        step = s.step;
 #pragma unroll
         for (int j = 0; j < INST; ++j) {
             const int blk = min(wv * INST + j, R / 32 - 1);          // (waves past the rows repeat the last block)
-            const int r = blk * 32 + (lane >> 1);
-            off[j] = rowoff(r) + ((lane & 1) << 2);
-            last[j] = rowoff(r) + 4u * (uint32_t)(dwords - 1);
+            const uint32_t r = row(blk * 32 + (lane >> 1)) * s.row;
+            off[j] = r + ((lane & 1) << 2);
+            last[j] = s.step == 8 ? r + 4u * (uint32_t)(dwords - 1) : 0xFFFFFFFFu;
             lds[j] = blk * 256;
         }
     }
-    // stage kb; a row with an odd number of dwords ends in the middle of its last stage: that half reads the last dword
-    // again (its codes are cleared)
     __device__ __forceinline__ void issue(unsigned char* st, int kb) const {
 #pragma unroll
-        for (int j = 0; j < INST; ++j) dma4(base + min(off[j] + 8u * (uint32_t)kb, last[j]), st + lds[j]);
+        for (int j = 0; j < INST; ++j) dma4(base + min(off[j] + step * (uint32_t)kb, last[j]), st + lds[j]);
     }
     static __device__ __forceinline__ int read(const unsigned char* st, int r0, int lane) {
         return *reinterpret_cast<const int*>(st + (r0 + (lane & 31)) * 8 + ((lane >> 5) << 2));
     }
 };
 
-// One workgroup's product. `Cfg`: MM, PL, QL (layouts), BP, BQ, WP, WQ.
+// One workgroup's product.
 template <int MM_, int PL_, int QL_, int BP_, int BQ_, int WP_, int WQ_, int STAGES_>
 struct GemmTile {
     static constexpr int MM = MM_, PL = PL_, QL = QL_, BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STAGES = STAGES_;
     static constexpr int NW = WP * WQ, THREADS = 64 * NW;
     static constexpr int TP = BP / WP / 32, TQ = BQ / WQ / 32;      // 32 x 32 tiles of a wave
     static constexpr bool MX = MM == MM_MX4;
-    static constexpr int STAGE = (BP + BQ) * (MX ? 136 : 128);      // bytes: P rows, Q rows, P scales, Q scales
-    static constexpr int LDS = STAGES * STAGE;
-    static constexpr int SCL = (BP + BQ) * 128;
+    static constexpr int QOFF = BP * SB, SCL = (BP + BQ) * SB;       // a stage's P rows, Q rows, P scales, Q scales
+    static constexpr int STAGE = SCL + (MX ? (BP + BQ) * 8 : 0), LDS = STAGES * STAGE;
+    static constexpr int KSTAGE = MX ? 256 : 64;                     // contraction values of a stage
     using SP = Stager<PL, BP, NW>;
     using SQ = Stager<QL, BQ, NW>;
     using XP = ScaleStager<BP, NW>;
     using XQ = ScaleStager<BQ, NW>;
-    static constexpr int LOADS = SP::INST + SQ::INST + (MX ? XP::INST + XQ::INST : 0);
+    static constexpr int LOADS = SP::INST + SQ::INST + (MX ? XP::INST + XQ::INST : 0);   // of a stage and wave
 
     SP p;
     SQ q;
@@ -204,37 +215,51 @@ struct GemmTile {
     XQ xq;
     f32x16 acc[TP][TQ];
 
-    // Stages kb0 .. kb1 - 1 of the contraction (kb0 < kb1; p.base and q.base at stage kb0). tail: what the last one
-    // holds (8-value chunks for ROW, rows for COL; 0: it is whole). ldp / ldq: row bytes of COL operands.
-    template <int S>
-    __device__ __forceinline__ void step(const unsigned char* st, int p0, int q0, int lane, const int (&sp)[TP],
-                                         const int (&sq)[TQ]) {
+    // What one step of a stage multiplies, held in registers one step ahead.
+    struct Frags {
         u32x4 a[TP], b[TQ];
+    };
+    struct Scales {
+        int p[TP], q[TQ];
+    };
+    template <int S>
+    __device__ __forceinline__ void fetch(const unsigned char* st, int p0, int q0, int lane, Frags& f) const {
 #pragma unroll
-        for (int i = 0; i < TP; ++i) a[i] = fragment<PL, BP>(st, p0 + 32 * i, S, lane);
+        for (int i = 0; i < TP; ++i) f.a[i] = fragment<PL, BP>(st, p0 + 32 * i, S, lane);
 #pragma unroll
-        for (int j = 0; j < TQ; ++j) b[j] = fragment<QL, BQ>(st + BP * 128, q0 + 32 * j, S, lane);
+        for (int j = 0; j < TQ; ++j) f.b[j] = fragment<QL, BQ>(st + QOFF, q0 + 32 * j, S, lane);
+    }
+    __device__ __forceinline__ void fetch_scales(const unsigned char* st, int p0, int q0, int lane, Scales& x) const {
+        if constexpr (MX) {
+#pragma unroll
+            for (int i = 0; i < TP; ++i) x.p[i] = XP::read(st + SCL, p0 + 32 * i, lane);
+#pragma unroll
+            for (int j = 0; j < TQ; ++j) x.q[j] = XQ::read(st + SCL + BP * 8, q0 + 32 * j, lane);
+        }
+    }
+    template <int S>
+    __device__ __forceinline__ void multiply(const Frags& f, const Scales& x) {
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
             for (int j = 0; j < TQ; ++j) {
-                if constexpr (MX) acc[i][j] = mma_mx<S>(a[i], b[j], acc[i][j], sp[i], sq[j]);
-                else acc[i][j] = mma16(std::integral_constant<int, MM>{}, a[i], b[j], acc[i][j]);
+                if constexpr (MX) acc[i][j] = mma_mx<S>(f.a[i], f.b[j], acc[i][j], x.p[i], x.q[j]);
+                else acc[i][j] = mma16(std::integral_constant<int, MM>{}, f.a[i], f.b[j], acc[i][j]);
             }
-    }
-    __device__ __forceinline__ void compute(const unsigned char* st, int p0, int q0, int lane) {
-        int sp[TP], sq[TQ];
-        if constexpr (MX) {
+        // the sums pass through here: otherwise the compiler is free to gather several steps' multiplications in one place
 #pragma unroll
-            for (int i = 0; i < TP; ++i) sp[i] = XP::read(st + SCL, p0 + 32 * i, lane);
+        for (int i = 0; i < TP; ++i)
 #pragma unroll
-            for (int j = 0; j < TQ; ++j) sq[j] = XQ::read(st + SCL + BP * 8, q0 + 32 * j, lane);
-        }
-        step<0>(st, p0, q0, lane, sp, sq);
-        step<1>(st, p0, q0, lane, sp, sq);
-        step<2>(st, p0, q0, lane, sp, sq);
-        step<3>(st, p0, q0, lane, sp, sq);
+            for (int j = 0; j < TQ; ++j) asm volatile("" : "+v"(acc[i][j]));
     }
+    // Stages kb0 .. kb1 - 1 of the contraction (kb0 < kb1; p.base and q.base at stage kb0). tail_p / tail_q: what the
+    // last one holds of each operand (8-value chunks or MXFP4 blocks for ROW, rows for COL; 0: it is whole). ldp / ldq:
+    // row bytes of COL operands. One barrier a stage, before its last step: by then every wave has read the stage's last
+    // fragments, so its buffer can be refilled, and the next stage has landed, so its first fragments are read while the
+    // last step multiplies. The refill is issued in halves with the first two steps: issued at once after the barrier it
+    // holds the waves up at the address pipeline while the matrix cores idle, issued later it lands too late (stages of
+    // 256 x 256 x 64 bf16 values, 2048 cycles of multiplication: 2830 cycles at once, 2370 in these halves, 2740 in
+    // quarters over the whole stage).
     __device__ __forceinline__ void run(unsigned char* lds, int kb0, int kb1, int tail_p, int tail_q, uint32_t ldp,
                                         uint32_t ldq) {
         const int tid = threadIdx.x, lane = tid & 63;
@@ -244,41 +269,110 @@ struct GemmTile {
         for (int i = 0; i < TP; ++i)
 #pragma unroll
             for (int j = 0; j < TQ; ++j) acc[i][j] = f32x16{};
-        const uint64_t advp = PL == LAY_ROW ? 128 : 64 * (uint64_t)ldp, advq = QL == LAY_ROW ? 128 : 64 * (uint64_t)ldq;
-        auto issue = [&](int slot, int kb) {
-            unsigned char* st = lds + slot * STAGE;
-            if (kb == kb1 - 1 && tail_p) {
-                p.issue_tail(st, wv, lane, tail_p, ldp);
-                q.issue_tail(st + BP * 128, wv, lane, tail_q, ldq);
-            } else {
-                p.issue(st);
-                q.issue(st + BP * 128);
-            }
-            if constexpr (MX) {
+        const uint64_t advp = PL == LAY_ROW ? SB : SB / 2 * (uint64_t)ldp, advq = QL == LAY_ROW ? SB : SB / 2 * (uint64_t)ldq;
+        auto issue = [&](auto I, auto N, unsigned char* st, int kb) {
+            constexpr int i = decltype(I)::value, n = decltype(N)::value;
+            if constexpr (MX && i == 0) {
                 xp.issue(st + SCL, kb);
                 xq.issue(st + SCL + BP * 8, kb);
             }
-            p.base += advp;
-            q.base += advq;
+            if (kb == kb1 - 1 && tail_p) {                           // (uniform)
+                p.template issue_tail<i, n>(st, wv, lane, tail_p, ldp);
+                q.template issue_tail<i, n>(st + QOFF, wv, lane, tail_q, ldq);
+            } else {
+                p.template issue<i, n>(st);
+                q.template issue<i, n>(st + QOFF);
+            }
+            if constexpr (i == n - 1) {
+                p.base += advp;
+                q.base += advq;
+            }
         };
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s)
-            if (kb0 + s < kb1) issue(s, kb0 + s);
-        int cur = 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
-            if (STAGES > 2 && kb + 1 < kb1) WAIT_VM((STAGES - 2) * LOADS);
+        // stage kb has landed for every wave, and nobody reads the stage before it any more
+        auto arrive = [&](unsigned char* st, int kb) {
+            if (STAGES > 2 && kb + STAGES - 2 < kb1) WAIT_VM((STAGES - 2) * LOADS);   // (the stages after it are on their way)
             else WAIT_VM(0);
             LDS_BARRIER();
-            const int nxt = cur == 0 ? STAGES - 1 : cur - 1;         // the slot read in the previous step
-            if (kb + STAGES - 1 < kb1) issue(nxt, kb + STAGES - 1);
-            unsigned char* st = lds + cur * STAGE;
             if (kb == kb1 - 1 && tail_p) {                           // (uniform)
                 SP::clear_tail(st, tid, tail_p);
-                SQ::clear_tail(st + BP * 128, tid, tail_q);
+                SQ::clear_tail(st + QOFF, tid, tail_q);
                 __syncthreads();
             }
-            compute(st, p0, q0, lane);
+        };
+        constexpr std::integral_constant<int, 0> first{};
+        constexpr std::integral_constant<int, 1> one{};
+        constexpr std::integral_constant<int, 2> parts{};
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s)
+            if (kb0 + s < kb1) issue(first, one, lds + s * STAGE, kb0 + s);
+        Frags f0, f1;
+        Scales x0, x1;
+        arrive(lds, kb0);
+        int cur = 0, next = kb0 + STAGES - 1;                        // the stage that is being requested
+        unsigned char* fill = lds + (STAGES - 1) * STAGE;            // and where it goes
+        fetch_scales(lds, p0, q0, lane, x0);
+        fetch<0>(lds, p0, q0, lane, f0);
+        // every step but the last: the next one's fragments are read while it multiplies
+        auto first_steps = [&](const unsigned char* st) {
+            auto step = [&](auto S, Frags& now, Frags& then) {
+                constexpr int s = decltype(S)::value;
+                if (s < 2 && next < kb1) issue(std::integral_constant<int, s & 1>{}, parts, fill, next);
+                fetch<s + 1>(st, p0, q0, lane, then);
+                SCHED_FENCE();
+                multiply<s>(now, x0);
+                SCHED_FENCE();
+            };
+            step(first, f0, f1);
+            step(one, f1, f0);
+            step(std::integral_constant<int, 2>{}, f0, f1);
+        };
+        for (int kb = kb0; kb + 1 < kb1; ++kb) {
+            first_steps(lds + cur * STAGE);
+            fill = lds + cur * STAGE;
             cur = cur + 1 == STAGES ? 0 : cur + 1;
+            ++next;
+            unsigned char* nx = lds + cur * STAGE;
+            arrive(nx, kb + 1);
+            fetch_scales(nx, p0, q0, lane, x1);
+            fetch<0>(nx, p0, q0, lane, f0);
+            SCHED_FENCE();
+            multiply<3>(f1, x0);
+            SCHED_FENCE();
+            if constexpr (MX) x0 = x1;
+        }
+        first_steps(lds + cur * STAGE);
+        multiply<3>(f1, x0);
+    }
+
+    // Stores TN x 32 columns of 16-bit values (two a dword: value(i, j, r) = columns 8 r + 4 h .. + 3 of column tile i and
+    // row tile j) in whole rows: through LDS, 32 rows of the wave at a time, 16 bytes a lane and 64 TN bytes a row. `out`
+    // at the wave's first row and column, at 16-byte addresses; rows and cols (a multiple of 8): what exists from there on.
+    // Called by all waves after run(). (8192 x 4096 bf16: 17 us of 8-byte stores straight from the accumulators.)
+    template <int TN, typename V>
+    __device__ __forceinline__ void store_rows16(unsigned char* lds, uint16_t* out, int64_t stride, int64_t rows, int cols,
+                                                 const V& value) const {
+        constexpr int UNITS = TN * 4;                                // 16-byte units of a row
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        unsigned char* mine = lds + wv * (32 * 16 * UNITS);
+        static_assert(NW * 32 * 16 * UNITS <= LDS, "the stages hold the waves' rows");
+        __syncthreads();                                             // no wave reads a stage any more
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) {
+            const int m = lane & 31;
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    *reinterpret_cast<uint2*>(mine + m * (16 * UNITS) + (((4 * i + r) ^ (m & (UNITS - 1))) << 4) + 8 * h) = value(i, j, r);
+            asm volatile("" ::: "memory");                           // (a wave's LDS accesses are performed in order)
+#pragma unroll
+            for (int t = 0; t < UNITS / 2; ++t) {
+                const int at = t * 64 + lane, row = at / UNITS, u = at % UNITS;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(mine + row * (16 * UNITS) + ((u ^ (row & (UNITS - 1))) << 4));
+                if (32 * j + row < rows && 8 * u < cols) *reinterpret_cast<u32x4*>(out + (32 * j + row) * stride + 8 * u) = v;
+            }
+            asm volatile("" ::: "memory");
         }
     }
 };
@@ -291,6 +385,10 @@ __device__ __forceinline__ float load_value(const void* x, int xdt, size_t i) {
     return (float)u16_as_h(reinterpret_cast<const uint16_t*>(x)[i]);
 }
 
+__device__ __forceinline__ uint2 pack4(int odt, float a, float b, float c, float d) {
+    if (odt == DT_BF16) return make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+    return make_uint2(h_as_u16((_Float16)a) | (h_as_u16((_Float16)b) << 16), h_as_u16((_Float16)c) | (h_as_u16((_Float16)d) << 16));
+}
 __device__ __forceinline__ void store4(void* out, int odt, size_t o, int cols, f32x4 v) {
     // cols: how many of the four exist; o: the first one's index
     if (odt == DT_F32) {
@@ -326,11 +424,14 @@ __device__ __forceinline__ float swiglu(float g, float u, float L) {
     return __fdiv_rn(g, 1.0f + __expf(-g)) * u;
 }
 
-// Workgroup order: workgroups go round the 8 XCDs, each with an L2 of its own, so XCD x takes a contiguous run of tiles,
-// in bands of `band` tile rows over all columns.
-__device__ __forceinline__ int xcd_order(int id, int total) {
-    const int x = id & 7, per = total >> 3, rest = total & 7;
-    return x * per + min(x, rest) + (id >> 3);
+// The tile (column n, row m) of a workgroup among nt x mt. Workgroups go round the 8 XCDs, each with an L2 of its own: XCD
+// x takes a contiguous run of tiles, in bands of four tile rows, down each column of a band first, so that what it has in
+// flight is about square and reads the fewest different rows of both operands.
+__device__ __forceinline__ int2 tile_order(int id, int nt, int mt) {
+    const int total = nt * mt, x = id & 7, per = total >> 3, rest = total & 7;
+    const int pos = x * per + min(x, rest) + (id >> 3);
+    const int band = pos / (4 * nt), in = pos - band * 4 * nt, rows = min(4, mt - 4 * band);
+    return make_int2(in / rows, 4 * band + in % rows);
 }
 
 // Dynamic LDS beyond 64 KB has to be allowed once per kernel and device.

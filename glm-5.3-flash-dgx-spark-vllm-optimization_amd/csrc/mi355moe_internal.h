@@ -300,16 +300,21 @@ constexpr int fp8_seg_rows(int64_t tokens) { return tokens <= FP8_FEW_T ? FP8_FE
 int launch_fp8(const Fp8Args& a, hipStream_t st, int kernels);
 int launch_quant_rows(const void* x, int xdt, int64_t stride, int rows, int K, uint8_t* q, float* s, hipStream_t st);
 
-// MXFP4 (mxfp4.hip). Codes two a byte, rows K / 2 bytes apart; scales at the given pitches (multiples of 4, the bytes
-// behind a row's K / 32 scales finite).
+// MXFP4 (mxfp4.hip). Codes two a byte, rows K / 2 bytes apart. Scales: the 8 of steps of 256 values together, those of row
+// r and step k at p + r * row + k * step: rows of K / 32 bytes (row = K / 32, a multiple of 4, step = 8), or arranged by
+// steps (row = 8, step = 8 rows; the steps' bytes behind a row's last scale are 127).
+struct MxScales {
+    const uint8_t* p;
+    uint32_t row, step;
+};
 struct Mxfp4Args {
     int n, K, N, P, T;
     const uint8_t* w13;     // [n][2N][K/2], gate rows then up rows
-    const uint8_t* w13s;    // [n][2N][w13sp]
-    int64_t w13sp;
+    MxScales w13s;          // expert e's at w13se * e bytes
+    int64_t w13se;
     const uint8_t* w2;      // [n][K][N/2]
-    const uint8_t* w2s;     // [n][K][w2sp]
-    int64_t w2sp;
+    MxScales w2s;
+    int64_t w2se;
     const void* x;
     int xdt;                // DT_F32, DT_F16 or DT_BF16
     int64_t x_stride;
@@ -324,11 +329,9 @@ struct Mxfp4Args {
     int seg;                // rows per segment (MX_FEW or MX_TILE)
     float limit;
     uint8_t* qx;            // [T][K/2] quantised input rows
-    uint8_t* sx;            // [T][sxp]
-    int64_t sxp;
+    uint8_t* sx;            // their scales, arranged by steps
     uint8_t* qh;            // [P][N/2] quantised SwiGLU outputs (sorted position order)
-    uint8_t* sh;            // [P][shp]
-    int64_t shp;
+    uint8_t* sh;            // their scales, arranged by steps
     float* contrib;         // [P][K] per-pair weighted contributions (sorted position order)
     const int* inv;         // [P] pair j -> sorted position
     int topk;
@@ -342,29 +345,29 @@ constexpr int MX_FEW = 16, MX_TILE = 64;             // rows per segment: stream
 constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : MX_TILE; }
 // kernels: bit 0 quantise inputs, bit 1 gate/up, bit 2 down, bit 3 slot-order combine
 int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels);
-// rows x K values to codes [rows][ceil(K/2)] and scales at pitch sp >= ceil(K/32) (the bytes behind them set to 127)
-int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int64_t sp,
+// rows x K values to codes [rows][ceil(K/2)] and scales [rows][ceil(K/32)] or (steps) arranged by steps
+int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int steps,
                     hipStream_t st);
 int launch_mx_dequant(const uint8_t* q, const uint8_t* s, int64_t rows, int K, void* out, int odt, hipStream_t st);
-// scales of two arrays of rows (nb a row, back to back) at a pitch of whole dwords
-int launch_mx_pad_scales(const uint8_t* a, int64_t ra, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb, int pitch,
-                         hipStream_t st);
+// scales of `mats` matrices of `rows` rows of nb bytes, each arranged by steps; and of a second matrix (b may be nullptr)
+int launch_mx_arrange(const uint8_t* a, int64_t mats, int64_t rows, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb,
+                      hipStream_t st);
 struct MxMatmulPlan {
-    int few, tile, splits;
+    int few, tile, splits, arrange;
 };
 struct MxMatmulArgs {
     const uint8_t* q;       // [M][K/2]
-    const uint8_t* qs;      // [M][sp]
+    MxScales qs;
     int64_t M;
     const uint8_t* w;       // [N][K/2]
-    const uint8_t* ws;      // [N][sp]
+    MxScales ws;
     int N, K;
-    int64_t sp;
     void* out;
     int odt;
     int64_t out_stride;
     int splits;
     float* part;            // [splits][M][N] (splits > 1)
+    int rows16;             // set by the launcher: 16-bit output rows at 16-byte addresses, N % 8 == 0
 };
 // out [M][stride] (dtype odt) = the sum of fp32 partials [splits][M][N] in order
 int launch_join(const float* part, int splits, int64_t M, int N, void* out, int odt, int64_t stride, hipStream_t st);

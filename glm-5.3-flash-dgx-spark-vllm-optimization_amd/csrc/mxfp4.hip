@@ -61,11 +61,20 @@ __device__ __forceinline__ void mx_load8(const void* x, size_t i, float (&v)[8])
     }
 }
 
+// Where the scale of row r, block b goes among `rows` rows: rows of nb bytes, or arranged by steps of eight blocks.
+__device__ __forceinline__ int64_t scale_place(int64_t r, int b, int nb, int64_t rows, int steps) {
+    return steps ? ((b >> 3) * rows + r) * 8 + (b & 7) : r * nb + b;
+}
+// The bytes behind a row's last scale in its last step.
+__device__ __forceinline__ void scale_pad(uint8_t* s, int64_t r, int nb, int64_t rows) {
+    for (int b = nb; b & 7; ++b) s[scale_place(r, b, nb, rows, 1)] = 127;
+}
+
 // Rows of whole blocks at aligned addresses: four lanes a block, eight values a lane. Item i is 8 values; a row has
-// K / 8 of them. Scales lie at a pitch of sp bytes a row; bytes behind a row's scales are set to 127.
+// K / 8 of them.
 template <int XDT>
 __global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ x, int64_t stride, int64_t items, int per_row,
-                                                       uint32_t* __restrict__ q, uint8_t* __restrict__ s, int64_t sp) {
+                                                       uint32_t* __restrict__ q, uint8_t* __restrict__ s, int64_t rows, int steps) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per_row;
         const int c = (int)(i - r * per_row);
@@ -79,16 +88,16 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ 
         const uint32_t code = mx_scale_code(top);
         q[i] = e2m1x8(v, mx_inv_scale(code));
         if ((c & 3) == 0) {
-            s[r * sp + (c >> 2)] = (uint8_t)code;
-            if (c + 4 == per_row)
-                for (int64_t b = per_row >> 2; b < sp; ++b) s[r * sp + b] = 127;
+            s[scale_place(r, c >> 2, per_row >> 2, rows, steps)] = (uint8_t)code;
+            if (steps && c + 4 == per_row) scale_pad(s, r, per_row >> 2, rows);
         }
     }
 }
 
 // Any row length and alignment: one thread a block.
 __global__ __launch_bounds__(256) void mx_quant_any_kernel(const void* __restrict__ x, int xdt, int64_t stride, int64_t blocks,
-                                                           int K, uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t sp) {
+                                                           int K, uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t rows,
+                                                           int steps) {
     const int nb = (K + 31) / 32, qp = (K + 1) / 2;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < blocks; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / nb;
@@ -105,9 +114,8 @@ __global__ __launch_bounds__(256) void mx_quant_any_kernel(const void* __restric
             uint8_t* o = q + r * qp + (k0 + j) / 2;
             for (int t = 0; 2 * t < n - j && t < 4; ++t) o[t] = (uint8_t)(d >> (8 * t));
         }
-        s[r * sp + b] = (uint8_t)code;
-        if (b + 1 == nb)
-            for (int64_t j = nb; j < sp; ++j) s[r * sp + j] = 127;
+        s[scale_place(r, b, nb, rows, steps)] = (uint8_t)code;
+        if (steps && b + 1 == nb) scale_pad(s, r, nb, rows);
     }
 }
 
@@ -161,17 +169,29 @@ __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restri
     }
 }
 
-// Rows of nb scale codes at a pitch of a whole number of dwords, the bytes behind them 127 (the products read whole
-// dwords). Two arrays in one launch.
-__global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t* __restrict__ a, int64_t ra, uint8_t* __restrict__ ao,
-                                                            const uint8_t* __restrict__ b, int64_t rb, uint8_t* __restrict__ bo,
-                                                            int nb, int pitch) {
-    const int64_t total = (ra + rb) * pitch;
+// Scales of rows of nb bytes arranged by steps, the bytes behind a row's last one 127: `mats` matrices of `rows` rows, and a
+// second matrix of rb rows. One thread a row and step.
+__global__ __launch_bounds__(256) void mx_arrange_kernel(const uint8_t* __restrict__ a, int64_t mats, int64_t rows, uint2* __restrict__ ao,
+                                                         const uint8_t* __restrict__ b, int64_t rb, uint2* __restrict__ bo, int nb) {
+    const int ns = (nb + 7) / 8;
+    const int64_t first = mats * rows * ns, total = first + rb * ns;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / pitch;
-        const int c = (int)(i - r * pitch);
-        if (r < ra) ao[i] = c < nb ? a[r * nb + c] : 127;
-        else bo[i - ra * pitch] = c < nb ? b[(r - ra) * nb + c] : 127;
+        const bool second = i >= first;
+        const int64_t j = second ? i - first : i, nr = second ? rb : rows;
+        // consecutive threads take consecutive steps of a row: they read its bytes together
+        const int64_t r = j / ns, mat = r / nr;
+        const int k = (int)(j - r * ns);
+        const uint8_t* src = (second ? b : a) + r * nb + 8 * k;
+        uint2 v = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
+        if ((nb & 7) == 0 && (reinterpret_cast<uintptr_t>(src) & 7) == 0) v = *reinterpret_cast<const uint2*>(src);
+        else {
+            uint8_t c[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) c[t] = 8 * k + t < nb ? src[t] : 127;
+            v.x = c[0] | c[1] << 8 | c[2] << 16 | (uint32_t)c[3] << 24;
+            v.y = c[4] | c[5] << 8 | c[6] << 16 | (uint32_t)c[7] << 24;
+        }
+        (second ? bo : ao)[(mat * ns + k) * nr + (r - mat * nr)] = v;
     }
 }
 
@@ -184,7 +204,11 @@ __global__ __launch_bounds__(256) void mx_pad_scales_kernel(const uint8_t* __res
 struct FewRow {
     const uint8_t* q;
     const uint8_t* s;
+    uint32_t step;
 };
+__device__ __forceinline__ FewRow few_row(const uint8_t* q, size_t pitch, const MxScales& s, size_t r) {
+    return {q + r * pitch, s.p + r * s.row, s.step};
+}
 // the four steps' operand bytes and scales of 512 values from block b0 on (nblk blocks in a row; blocks past them: zero
 // codes for ZERO, else those of the last one, and scales of 2^0)
 template <bool ZERO>
@@ -194,7 +218,7 @@ __device__ __forceinline__ void few_load(const FewRow& r, int b0, int g, int nbl
         const u32x4* p = reinterpret_cast<const u32x4*>(r.q + (size_t)b * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = p[i];
-        sc = *reinterpret_cast<const int*>(r.s + b);
+        sc = *reinterpret_cast<const int*>(r.s + (size_t)(b >> 3) * r.step + (b & 4));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -204,7 +228,8 @@ __device__ __forceinline__ void few_load(const FewRow& r, int b0, int g, int nbl
             for (int j = 0; j < 4; ++j) v[i][j] = ok ? t[j] : 0u;
         }
         const int last = (nblk - 1) & ~3;
-        const int t = *reinterpret_cast<const int*>(r.s + min(b, last));
+        const int bl = min(b, last);
+        const int t = *reinterpret_cast<const int*>(r.s + (size_t)(bl >> 3) * r.step + (bl & 4));
         sc = b <= last ? t : 0x7F7F7F7F;
     }
 }
@@ -242,13 +267,13 @@ __global__ __launch_bounds__(512) void mx_gateup_few_kernel(Mxfp4Args a) {
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nblk = a.K >> 5;
     FewRow w[4], x;
+    const MxScales ws = {a.w13s.p + (size_t)e * a.w13se, a.w13s.row, a.w13s.step};
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const size_t r = (size_t)e * 2 * a.N + (t >> 1) * a.N + cb * 32 + (t & 1) * 16 + c;
-        w[t] = {a.w13 + r * (a.K / 2), a.w13s + r * a.w13sp};
+        const size_t r = (size_t)(t >> 1) * a.N + cb * 32 + (t & 1) * 16 + c;
+        w[t] = few_row(a.w13 + (size_t)e * 2 * a.N * (a.K / 2), a.K / 2, ws, r);
     }
-    const size_t tok = a.tok[row0 + min(c, rn - 1)];
-    x = {a.qx + tok * (a.K / 2), a.sx + tok * a.sxp};
+    x = few_row(a.qx, a.K / 2, MxScales{a.sx, 8, 8u * a.T}, a.tok[row0 + min(c, rn - 1)]);
     f32x4 acc[4] = {};
     for (int b0 = wv * 16; b0 < nblk; b0 += 128) few_product(w, x, b0, g, nblk, acc);
 #pragma unroll
@@ -275,15 +300,17 @@ __global__ __launch_bounds__(512) void mx_gateup_few_kernel(Mxfp4Args a) {
     if (m < rn) {
         const size_t r = (size_t)row0 + m;
         if ((n & 7) == 0) *reinterpret_cast<uint32_t*>(a.qh + r * (a.N / 2) + cb * 16 + (n >> 1)) = d;
-        if (n == 0) a.sh[r * a.shp + cb] = (uint8_t)code;
-        if (n > 0 && (cb + 1) * 32 == a.N && cb + n < a.shp) a.sh[r * a.shp + cb + n] = 127;   // (at most 3)
+        if (n == 0) {
+            a.sh[scale_place(r, cb, 0, a.P, 1)] = (uint8_t)code;
+            if ((cb + 1) * 32 == a.N) scale_pad(a.sh, r, cb + 1, a.P);
+        }
     }
 }
 
 // The eight waves of a workgroup as KS cuts of the contraction x 8 / KS groups of 16 T columns. Store(m, n, four sums of
 // columns n ..): called for columns of this wave's own sums (after the join) and rows m < rows.
 template <int T, int KS, typename Store>
-__device__ __forceinline__ void few_columns(const uint8_t* wq, size_t wqp, const uint8_t* wsc, size_t wsp, int cols, int n0,
+__device__ __forceinline__ void few_columns(const uint8_t* wq, size_t wqp, const MxScales& ws, int cols, int n0,
                                             const FewRow& x, int nblk, float* red, const Store& store) {
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -293,7 +320,7 @@ __device__ __forceinline__ void few_columns(const uint8_t* wq, size_t wqp, const
 #pragma unroll
     for (int t = 0; t < T; ++t) {
         const size_t r = min(nw + 16 * t + c, cols - 1);
-        w[t] = {wq + r * wqp, wsc + r * wsp};
+        w[t] = few_row(wq, wqp, ws, r);
     }
     f32x4 acc[T] = {};
     for (int b0 = ks * 16; b0 < nblk; b0 += 16 * KS) few_product(w, x, b0, g, nblk, acc);
@@ -329,10 +356,10 @@ __global__ __launch_bounds__(512) void mx_down_few_kernel(Mxfp4Args a) {
     if (rn <= 0) return;
     const int c = threadIdx.x & 15;
     const size_t xr = (size_t)row0 + min(c, rn - 1);
-    const FewRow x = {a.qh + xr * (a.N / 2), a.sh + xr * a.shp};
+    const FewRow x = few_row(a.qh, a.N / 2, MxScales{a.sh, 8, 8u * a.P}, xr);
     const float rw = a.w32[xr];
     const int pe = a.pe[xr];
-    few_columns<T, KS>(a.w2 + (size_t)e * a.K * (a.N / 2), a.N / 2, a.w2s + (size_t)e * a.K * a.w2sp, a.w2sp, a.K,
+    few_columns<T, KS>(a.w2 + (size_t)e * a.K * (a.N / 2), a.N / 2, MxScales{a.w2s.p + (size_t)e * a.w2se, a.w2s.row, a.w2s.step}, a.K,
                        (int)blockIdx.x * (16 * T * 8 / KS), x, a.N >> 5, red, [&](int m, int n, f32x4 v) {
                            if (m < rn && n < a.K && pe >= 0)
                                *reinterpret_cast<f32x4*>(a.contrib + xr * a.K + n) = v * f32x4{rw, rw, rw, rw};
@@ -346,8 +373,8 @@ __global__ __launch_bounds__(512) void mx_matmul_few_kernel(MxMatmulArgs a) {
     const int c = threadIdx.x & 15;
     const int64_t m0 = (int64_t)blockIdx.y * 16;
     const int64_t xr = min(m0 + c, a.M - 1);
-    const FewRow x = {a.q + xr * (a.K / 2), a.qs + xr * a.sp};
-    few_columns<T, KS>(a.w, a.K / 2, a.ws, a.sp, a.N, (int)blockIdx.x * (16 * T * 8 / KS), x, a.K >> 5, red,
+    const FewRow x = few_row(a.q, a.K / 2, a.qs, xr);
+    few_columns<T, KS>(a.w, a.K / 2, a.ws, a.N, (int)blockIdx.x * (16 * T * 8 / KS), x, a.K >> 5, red,
                        [&](int m, int n, f32x4 v) {
                            if (m0 + m < a.M && n < a.N)
                                store4(a.out, a.odt, (size_t)(m0 + m) * a.out_stride + n, a.N - n, v);
@@ -359,29 +386,29 @@ __global__ __launch_bounds__(512) void mx_matmul_few_kernel(MxMatmulArgs a) {
 template <int BP, int BQ, int WP, int WQ, int ST>
 using MxTile = GemmTile<MM_MX4, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
 
-__device__ __forceinline__ int mx_stages(int K) { return (K + 255) >> 8; }
-__device__ __forceinline__ int mx_tail(int K) { return (K & 255) >> 5; }
+__device__ __forceinline__ int mx_stages(int K) { return (K + 2 * SB - 1) / (2 * SB); }
+__device__ __forceinline__ int mx_tail(int K) { return K % (2 * SB) / 32; }
 
 // Dense product: workgroup tiles of BP columns x BQ rows, out or (splits > 1) fp32 partials [split][M][N].
 template <int BP, int BQ, int WP, int WQ, int ST>
-__global__ __launch_bounds__(64 * WP * WQ, 1) void mx_matmul_kernel(MxMatmulArgs a, int nt, int mt) {
+__global__ __launch_bounds__(64 * WP * WQ, 2) void mx_matmul_kernel(MxMatmulArgs a, int nt, int mt) {
     using G = MxTile<BP, BQ, WP, WQ, ST>;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = xcd_order(blockIdx.x, nt * mt);
-    const int n0 = (id % nt) * BP;
-    const int64_t m0 = (int64_t)(id / nt) * BQ;
+    const int2 tile = tile_order(blockIdx.x, nt, mt);
+    const int n0 = tile.x * BP;
+    const int64_t m0 = (int64_t)tile.y * BQ;
     const int stages = mx_stages(a.K), per = (stages + a.splits - 1) / a.splits;
     const int kb0 = blockIdx.y * per, kb1 = min(stages, kb0 + per);
-    const uint32_t pitch = a.K / 2, sp = (uint32_t)a.sp;
+    const uint32_t pitch = a.K / 2;
     const int pl = min(BP, a.N - n0) - 1;
     const int ql = (int)min((int64_t)BQ, a.M - m0) - 1;
     G t;
-    t.p.init_row(uniform_ptr(a.w + (size_t)n0 * pitch + (size_t)kb0 * 128), wv, lane, [&](int r) { return min(r, pl) * pitch; });
-    t.q.init_row(uniform_ptr(a.q + (size_t)m0 * pitch + (size_t)kb0 * 128), wv, lane, [&](int r) { return min(r, ql) * pitch; });
-    t.xp.init(a.ws + (size_t)n0 * sp, wv, lane, sp / 4, [&](int r) { return min(r, pl) * sp; });
-    t.xq.init(a.qs + (size_t)m0 * sp, wv, lane, sp / 4, [&](int r) { return min(r, ql) * sp; });
+    t.p.init_row(uniform_ptr(a.w + (size_t)n0 * pitch + (size_t)kb0 * SB), wv, lane, [&](int r) { return min(r, pl) * pitch; });
+    t.q.init_row(uniform_ptr(a.q + (size_t)m0 * pitch + (size_t)kb0 * SB), wv, lane, [&](int r) { return min(r, ql) * pitch; });
+    t.xp.init(a.ws, n0, (a.K + 127) / 128, wv, lane, [&](int r) { return (uint32_t)min(r, pl); });
+    t.xq.init(a.qs, m0, (a.K + 127) / 128, wv, lane, [&](int r) { return (uint32_t)min(r, ql); });
     const int tail = kb1 == stages ? mx_tail(a.K) : 0;
     if (kb0 < kb1) t.run(lds, kb0, kb1, tail, tail, 0, 0);
     else
@@ -390,6 +417,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void mx_matmul_kernel(MxMatmulArgs
 #pragma unroll
             for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
     const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
+    if (a.rows16) {                                                  // (uniform: 16-bit rows at 16-byte addresses)
+        t.template store_rows16<G::TP>(lds, static_cast<uint16_t*>(a.out) + (size_t)(m0 + q0) * a.out_stride + n0 + p0, a.out_stride,
+                                       a.M - m0 - q0, a.N - n0 - p0, [&](int i, int j, int r) {
+                                           return pack4(a.odt, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
+                                                        t.acc[i][j][4 * r + 3]);
+                                       });
+        return;
+    }
     void* out = a.splits > 1 ? static_cast<void*>(a.part + (size_t)blockIdx.y * a.M * a.N) : a.out;
     const int odt = a.splits > 1 ? (int)DT_F32 : a.odt;
     const int64_t stride = a.splits > 1 ? a.N : a.out_stride;
@@ -426,7 +461,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // Gate/up of a segment: grid (ceil(N / (BP / 2)), segments). A wave's P rows are its gate columns, then the same up
 // columns, so the SwiGLU is local to a lane; a 32-column block of a row lies in lanes l and l ^ 32.
 template <int BP, int BQ, int WP, int WQ, int ST>
-__global__ __launch_bounds__(64 * WP * WQ, 1) void mx_gateup_kernel(Mxfp4Args a) {
+__global__ __launch_bounds__(64 * WP * WQ, 2) void mx_gateup_kernel(Mxfp4Args a) {
     using G = MxTile<BP, BQ, WP, WQ, ST>;
     static_assert(G::TP % 2 == 0, "");
     extern __shared__ __align__(16) unsigned char lds[];
@@ -448,8 +483,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void mx_gateup_kernel(Mxfp4Args a)
     G t;
     t.p.init_row(uniform_ptr(a.w13 + (size_t)e * 2 * a.N * pitch), wv, lane, [&](int r) { return wrow(r) * pitch; });
     t.q.init_row(a.qx, wv, lane, [&](int r) { return trow(r) * pitch; });
-    t.xp.init(a.w13s + (size_t)e * 2 * a.N * a.w13sp, wv, lane, (a.K + 127) / 128, [&](int r) { return wrow(r) * (uint32_t)a.w13sp; });
-    t.xq.init(a.sx, wv, lane, (a.K + 127) / 128, [&](int r) { return trow(r) * (uint32_t)a.sxp; });
+    t.xp.init(MxScales{a.w13s.p + (size_t)e * a.w13se, a.w13s.row, a.w13s.step}, 0, (a.K + 127) / 128, wv, lane, wrow);
+    t.xq.init(MxScales{a.sx, 8, 8u * a.T}, 0, (a.K + 127) / 128, wv, lane, trow);
     t.run(lds, 0, mx_stages(a.K), mx_tail(a.K), mx_tail(a.K), 0, 0);
     const int p0 = (wv % WP) * HALF, q0 = (wv / WP) * (BQ / WQ), hl = lane >> 5;
 #pragma unroll
@@ -484,9 +519,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void mx_gateup_kernel(Mxfp4Args a)
                 const size_t rr = (size_t)row0 + m;
                 *reinterpret_cast<uint2*>(a.qh + rr * (a.N / 2) + col / 2 + 8 * hl) = v;
                 if (hl == 0) {
-                    a.sh[rr * a.shp + col / 32] = (uint8_t)code;
-                    if (col + 32 == a.N)
-                        for (int b = a.N / 32; b < a.shp; ++b) a.sh[rr * a.shp + b] = 127;
+                    a.sh[scale_place(rr, col / 32, 0, a.P, 1)] = (uint8_t)code;
+                    if (col + 32 == a.N) scale_pad(a.sh, rr, a.N / 32, a.P);
                 }
             }
         }
@@ -495,7 +529,7 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void mx_gateup_kernel(Mxfp4Args a)
 
 // Down of a segment: grid (ceil(K / BP), segments), weighted contributions.
 template <int BP, int BQ, int WP, int WQ, int ST>
-__global__ __launch_bounds__(64 * WP * WQ, 1) void mx_down_kernel(Mxfp4Args a) {
+__global__ __launch_bounds__(64 * WP * WQ, 2) void mx_down_kernel(Mxfp4Args a) {
     using G = MxTile<BP, BQ, WP, WQ, ST>;
     extern __shared__ __align__(16) unsigned char lds[];
     const int s = blockIdx.y;
@@ -521,8 +555,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 1) void mx_down_kernel(Mxfp4Args a) {
     G t;
     t.p.init_row(uniform_ptr(a.w2 + (size_t)e * a.K * pitch), wv, lane, [&](int r) { return wrow(r) * pitch; });
     t.q.init_row(uniform_ptr(a.qh + (size_t)row0 * pitch), wv, lane, [&](int r) { return xrow(r) * pitch; });
-    t.xp.init(a.w2s + (size_t)e * a.K * a.w2sp, wv, lane, (a.N + 127) / 128, [&](int r) { return wrow(r) * (uint32_t)a.w2sp; });
-    t.xq.init(a.sh + (size_t)row0 * a.shp, wv, lane, (a.N + 127) / 128, [&](int r) { return xrow(r) * (uint32_t)a.shp; });
+    t.xp.init(MxScales{a.w2s.p + (size_t)e * a.w2se, a.w2s.row, a.w2s.step}, 0, (a.N + 127) / 128, wv, lane, wrow);
+    t.xq.init(MxScales{a.sh, 8, 8u * a.P}, row0, (a.N + 127) / 128, wv, lane, xrow);
     t.run(lds, 0, mx_stages(a.N), mx_tail(a.N), mx_tail(a.N), 0, 0);
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
@@ -572,7 +606,7 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(Mxfp4Args a) {
 
 static unsigned grid_for(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, 256 * 32); }
 
-int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int64_t sp,
+int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int steps,
                     hipStream_t st) {
     if (rows <= 0) return 0;
     const int unit = xdt == DT_F32 ? 4 : 8;                          // elements of a 16-byte load
@@ -582,12 +616,12 @@ int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K,
         const int64_t items = rows * (K / 8);
         const dim3 g(grid_for(items));
         uint32_t* q32 = reinterpret_cast<uint32_t*>(q);
-        if (xdt == DT_F32) hipLaunchKernelGGL(mx_quant_kernel<DT_F32>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, sp);
-        else if (xdt == DT_F16) hipLaunchKernelGGL(mx_quant_kernel<DT_F16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, sp);
-        else hipLaunchKernelGGL(mx_quant_kernel<DT_BF16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, sp);
+        if (xdt == DT_F32) hipLaunchKernelGGL(mx_quant_kernel<DT_F32>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, rows, steps);
+        else if (xdt == DT_F16) hipLaunchKernelGGL(mx_quant_kernel<DT_F16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, rows, steps);
+        else hipLaunchKernelGGL(mx_quant_kernel<DT_BF16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, rows, steps);
     } else {
         const int64_t blocks = rows * ((K + 31) / 32);
-        hipLaunchKernelGGL(mx_quant_any_kernel, dim3(grid_for(blocks)), dim3(256), 0, st, x, xdt, stride, blocks, K, q, s, sp);
+        hipLaunchKernelGGL(mx_quant_any_kernel, dim3(grid_for(blocks)), dim3(256), 0, st, x, xdt, stride, blocks, K, q, s, rows, steps);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
@@ -611,9 +645,11 @@ MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
     MxMatmulPlan p{};
     p.few = M <= MX_FEW_M;
     p.splits = 1;
+    p.arrange = K % 128 != 0;                                        // rows whose scales are no whole dwords
     if (p.few) return p;
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
     p.tile = big >= 192 ? 256 : 128;
+    if (p.tile == 256) p.arrange = 1;
     if (p.tile == 128) {
         const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), stages = (K + 255) / 256;
         while (p.splits < 8 && tiles * p.splits * 2 <= 512 && stages / (p.splits * 2) >= 2) p.splits *= 2;
@@ -622,7 +658,8 @@ MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
 }
 
 template <int BP, int BQ, int WP, int WQ, int ST>
-static int run_mx_matmul(const MxMatmulArgs& a, hipStream_t st) {
+static int run_mx_matmul(MxMatmulArgs a, hipStream_t st) {
+    a.rows16 = a.splits == 1 && a.odt != DT_F32 && a.N % 8 == 0 && a.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     using G = MxTile<BP, BQ, WP, WQ, ST>;
     static const bool ok = allow_lds(mx_matmul_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
     if (!ok) return -1;
@@ -648,9 +685,11 @@ int launch_mx_matmul(const MxMatmulArgs& a, const MxMatmulPlan& p, hipStream_t s
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-int launch_mx_pad_scales(const uint8_t* a, int64_t ra, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb, int pitch,
-                         hipStream_t st) {
-    hipLaunchKernelGGL(mx_pad_scales_kernel, dim3(grid_for((ra + rb) * pitch)), dim3(256), 0, st, a, ra, ao, b, rb, bo, nb, pitch);
+int launch_mx_arrange(const uint8_t* a, int64_t mats, int64_t rows, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb,
+                      hipStream_t st) {
+    const int64_t items = (mats * rows + rb) * ((nb + 7) / 8);
+    hipLaunchKernelGGL(mx_arrange_kernel, dim3(grid_for(items)), dim3(256), 0, st, a, mats, rows, reinterpret_cast<uint2*>(ao), b, rb,
+                       reinterpret_cast<uint2*>(bo), nb);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
@@ -672,7 +711,7 @@ static int run_mx_down(const Mxfp4Args& a, hipStream_t st) {
 }
 
 int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {
-    if ((kernels & 1) && launch_mx_quant(a.x, a.xdt, a.x_stride, a.T, a.K, a.qx, a.sx, a.sxp, st)) return -1;
+    if ((kernels & 1) && launch_mx_quant(a.x, a.xdt, a.x_stride, a.T, a.K, a.qx, a.sx, 1, st)) return -1;
     const bool few = a.seg == MX_FEW;
     if (kernels & 2) {
         if (few) hipLaunchKernelGGL(mx_gateup_few_kernel, dim3(a.N / 32, a.S_cap), dim3(512), 0, st, a);

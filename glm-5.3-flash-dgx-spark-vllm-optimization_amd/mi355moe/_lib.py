@@ -47,7 +47,7 @@ class Fp8LayerDesc(ctypes.Structure):
 class Mxfp4LayerDesc(ctypes.Structure):
     """mi355moe_mxfp4_layer: shape + the MXFP4 codes and scale codes of a layer's experts (device pointers)."""
     _fields_ = [("n", _i64), ("hidden", _i64), ("intermediate", _i64), ("w13", _c_p), ("w13_scale", _c_p),
-                ("w13_scale_stride", _i64), ("w2", _c_p), ("w2_scale", _c_p), ("w2_scale_stride", _i64)]
+                ("w2", _c_p), ("w2_scale", _c_p), ("arranged", _i64)]
 
 
 class MoeError(RuntimeError):
@@ -131,6 +131,8 @@ _SIGS = {
     "mi355moe_mxfp4_dequant_rows": (_int, [_c_p, _c_p, _i64, _i64, _c_p, _int, _c_p]),
     "mi355moe_mxfp4_matmul_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "mi355moe_mxfp4_matmul": (_int, [_c_p, _c_p, _i64, _c_p, _c_p, _i64, _i64, _c_p, _int, _i64, _c_p, _sz, _c_p]),
+    "mi355moe_mxfp4_arranged_bytes": (_i64, [_i64, _i64, _i64]),
+    "mi355moe_mxfp4_arrange_scales": (_int, [_c_p, _i64, _i64, _i64, _c_p, _c_p]),
     "mi355moe_mxfp4_moe_workspace_bytes": (_i64, [ctypes.POINTER(Mxfp4LayerDesc), _i64, _i64]),
     "mi355moe_mxfp4_moe_forward_ids": (_int, [ctypes.POINTER(Mxfp4LayerDesc), _c_p, _int, _i64, _i64, _c_p, _int, _c_p,
                                               _int, _i64, _c_p, _i64, _f, _c_p, _int, _i64, _int, _c_p, _sz, _c_p]),

@@ -23,7 +23,6 @@ from . import _lib
 from .ops import _need_cuda, _on_device, _p, _stream, ids_dtype_code, weight_dtype_code
 
 BLOCK = 32
-SCALE_ONE = 127          # the scale code of 2^0
 SCALE_NAN = 255
 
 
@@ -125,17 +124,25 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     return out
 
 
-def _pitched(scale: torch.Tensor) -> torch.Tensor:
-    """Scales [..., K/32] with rows of whole dwords (what the kernels read): themselves, or a copy padded with 2^0."""
-    pad = -scale.shape[-1] % 4
-    return _aligned(torch.nn.functional.pad(scale, (0, pad), value=SCALE_ONE) if pad else scale, 4)
+def _arranged(scale: torch.Tensor) -> torch.Tensor:
+    """Scales [n, rows, K/32] in the order the expert products read them (steps of 256 columns of neighbouring rows)."""
+    n, rows, K = scale.shape[0], scale.shape[1], scale.shape[2] * BLOCK
+    dev = _need_cuda(scale)
+    L = _lib.lib()
+    out = torch.empty(n, -(-K // 256), rows, 8, dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        _lib.check("mi355moe_mxfp4_arrange_scales",
+                   L.mi355moe_mxfp4_arrange_scales(_p(scale), n, rows, K, _p(out), _stream(dev)))
+    return out
 
 
 class Mxfp4Experts:
-    """A layer's MXFP4 experts plus the C descriptor. The codes stay the caller's tensors; so do the scales, except where
-    a row's scales are no whole dwords (K % 128 != 0): then they are copied once, padded."""
+    """A layer's MXFP4 experts plus the C descriptor. The codes stay the caller's tensors; the scales are copied once into
+    the order the kernels read (a seventeenth of the layer's bytes; arrange=False keeps the caller's, which costs time in
+    every call and needs H and I to be multiples of 128)."""
 
-    def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor):
+    def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
+                 arrange: bool = True):
         for name, t in (("w13", w13), ("w13_scale", w13_scale), ("w2", w2), ("w2_scale", w2_scale)):
             _codes(t, name)
             if t.dim() != 3:
@@ -152,16 +159,19 @@ class Mxfp4Experts:
                                ("w2_scale", w2_scale, (n, H, I // BLOCK))):
             if tuple(t.shape) != shape:
                 raise ValueError(f"{name}: expected {shape}, got {tuple(t.shape)}")
-        for name, t in (("w13", w13), ("w2", w2)):
-            if t.data_ptr() % 16:
-                raise ValueError(f"{name} must lie at a 16-byte address")
-        self.w13, self.w13_scale, self.w2, self.w2_scale = w13, _pitched(w13_scale), w2, _pitched(w2_scale)
+        for name, t, by in (("w13", w13, 16), ("w2", w2, 16), ("w13_scale", w13_scale, 1 if arrange else 4),
+                            ("w2_scale", w2_scale, 1 if arrange else 4)):
+            if t.data_ptr() % by:
+                raise ValueError(f"{name} must lie at a {by}-byte address")
+        if not arrange and (H % 128 or I % 128):
+            raise ValueError(f"scales are used as they are only for H and I that are multiples of 128, got {H} and {I}")
+        self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
         self.n, self.K, self.N = n, H, I
+        self._s13, self._s2 = (_arranged(w13_scale), _arranged(w2_scale)) if arrange else (w13_scale, w2_scale)
         d = _lib.Mxfp4LayerDesc()
-        d.n, d.hidden, d.intermediate = n, H, I
-        d.w13, d.w13_scale = ctypes.c_void_p(w13.data_ptr()), ctypes.c_void_p(self.w13_scale.data_ptr())
-        d.w2, d.w2_scale = ctypes.c_void_p(w2.data_ptr()), ctypes.c_void_p(self.w2_scale.data_ptr())
-        d.w13_scale_stride, d.w2_scale_stride = self.w13_scale.shape[-1], self.w2_scale.shape[-1]
+        d.n, d.hidden, d.intermediate, d.arranged = n, H, I, int(arrange)
+        d.w13, d.w13_scale = ctypes.c_void_p(w13.data_ptr()), ctypes.c_void_p(self._s13.data_ptr())
+        d.w2, d.w2_scale = ctypes.c_void_p(w2.data_ptr()), ctypes.c_void_p(self._s2.data_ptr())
         self.desc = d
 
     @classmethod
@@ -231,8 +241,9 @@ def fused_experts_mxfp4(hidden: torch.Tensor, w13: torch.Tensor, w2: torch.Tenso
                         topk_ids: torch.Tensor, scales: tuple, *, limit: float = 10.0,
                         expert_map: torch.Tensor | None = None) -> torch.Tensor:
     """apply(hidden, w13, w2, topk_weights, topk_ids, scales) for MXFP4 experts: scales = (w13_scale, w2_scale). Hosts
-    that call it often keep an Mxfp4Experts and call moe_forward_ids (where hidden or intermediate is no multiple of 128,
-    this form pads the scales in every call)."""
+    that call it often keep an Mxfp4Experts and call moe_forward_ids: this form reads the scales as they are, and arranges
+    them in every call where hidden or intermediate is no multiple of 128."""
     T = hidden.shape[0]
-    return moe_forward_ids(Mxfp4Experts(w13, scales[0], w2, scales[1]), hidden, topk_ids.reshape(T, -1),
+    whole = (2 * w13.shape[-1]) % 128 == 0 and (2 * w2.shape[-1]) % 128 == 0
+    return moe_forward_ids(Mxfp4Experts(w13, scales[0], w2, scales[1], arrange=not whole), hidden, topk_ids.reshape(T, -1),
                            topk_weights.reshape(T, -1), limit=limit, expert_map=expert_map, out_dtype=hidden.dtype)

@@ -455,17 +455,22 @@ int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const v
                           int64_t K, void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes,
                           hipStream_t stream);
 
-/* A layer's MXFP4 experts. The scale strides are the bytes from one row's scales to the next's: multiples of 4, at
- * least K / 32; the bytes behind a row's scales must not be 255 (whole dwords are read). hidden and intermediate are
- * multiples of 32 up to 16384; w13 and w2 16-byte, the scales 4-byte aligned. */
+/* Scale codes arranged for the expert products: `mats` matrices of `rows` rows of K / 32 codes (K % 32 == 0) to [mats]
+ * [ceil(K / 256)][rows][8], the bytes behind a row's last code 127. Done once when a layer is loaded: the kernels read the
+ * scales of 256 columns of neighbouring rows together. out 8-byte aligned, of mi355moe_mxfp4_arranged_bytes (-1: refused). */
+int64_t mi355moe_mxfp4_arranged_bytes(int64_t mats, int64_t rows, int64_t K);
+int mi355moe_mxfp4_arrange_scales(const void* scale, int64_t mats, int64_t rows, int64_t K, void* out, hipStream_t stream);
+
+/* A layer's MXFP4 experts. Scales as arranged above (arranged = 1), or as they come, [n][rows][K / 32] (arranged = 0:
+ * slower, and hidden and intermediate must be multiples of 128). hidden and intermediate are multiples of 32 up to 16384;
+ * w13 and w2 16-byte aligned, the scales 8-byte (arranged = 0: 4-byte). */
 typedef struct mi355moe_mxfp4_layer {
     int64_t n, hidden, intermediate;
     const void* w13;          /* [n][2*intermediate][hidden/2]: rows 0..I-1 gate, I..2I-1 up */
-    const void* w13_scale;    /* [n][2*intermediate][w13_scale_stride] */
-    int64_t w13_scale_stride;
+    const void* w13_scale;    /* the scales of n matrices of 2*intermediate rows */
     const void* w2;           /* [n][hidden][intermediate/2] */
-    const void* w2_scale;     /* [n][hidden][w2_scale_stride] */
-    int64_t w2_scale_stride;
+    const void* w2_scale;     /* the scales of n matrices of hidden rows */
+    int64_t arranged;
 } mi355moe_mxfp4_layer;
 
 /* Routed-expert output of an MXFP4 layer from router ids and weights: z = q(x) W13^T, h = silu(min(g, L)) * clamp(u, -L,
@@ -485,8 +490,8 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
 /* h [T][intermediate] = silu(min(g, L)) * clamp(u, -L, L) (the limit iff L != 0), [g | u] = x W13^T in fp32, rounded
  * once: both projections, the activation and the product in one kernel (what the model's shared expert computes before
  * its down projection). x [T][hidden] (row stride x_stride), w13 [2 * intermediate][hidden] (gate rows, then up rows)
- * and h (row stride h_stride) of one dtype, F16 or BF16; hidden and intermediate multiples of 8; x and w13 16-byte
- * aligned, x_stride a multiple of 8. gu (optional, fp32 [T][2 * intermediate], 16-byte aligned) receives g and u for
+ * and h (row stride h_stride) of one dtype, F16 or BF16; hidden and intermediate multiples of 8; x, w13 and h
+ * 16-byte aligned, x_stride and h_stride multiples of 8. gu (optional, fp32 [T][2 * intermediate], 16-byte aligned) receives g and u for
  * the backward pass. */
 int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, int64_t x_stride, const void* w13,
                            int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, hipStream_t stream);

@@ -186,8 +186,7 @@ def _layer(n, H, I, seed):
 
 
 def _dense(ex):
-    s13, s2 = _np(ex.w13_scale)[..., :ex.K // 32], _np(ex.w2_scale)[..., :ex.N // 32]
-    return ref.values(_np(ex.w13), s13, ex.K), ref.values(_np(ex.w2), s2, ex.N)
+    return ref.values(_np(ex.w13), _np(ex.w13_scale), ex.K), ref.values(_np(ex.w2), _np(ex.w2_scale), ex.N)
 
 
 def _routing(T, n, topk, seed, bad=False):
@@ -276,15 +275,23 @@ def test_moe_non_finite_rows_stay_apart(cuda):
 
 def test_moe_functional_form_and_views(cuda):
     from mi355moe import fused_experts_mxfp4, mxfp4
-    ex = _layer(4, 160, 96, 7)                             # scales of 5 and 3 bytes a row: padded copies
-    s13, s2 = ex.w13_scale[..., :5].contiguous(), ex.w2_scale[..., :3].contiguous()
-    x = torch.randn(6, 160, device="cuda").half()
-    ids, w = _routing(6, 4, 2, 5)
-    ids, w = torch.from_numpy(ids).cuda(), torch.from_numpy(w).cuda()
-    want = mxfp4.moe_forward_ids(ex, x, ids, w)
-    assert torch.equal(fused_experts_mxfp4(x, ex.w13, ex.w2, w, ids, (s13, s2)), want)
+    for H, I, T in ((160, 96, 6), (384, 128, 6), (384, 128, 90)):   # scales arranged in the call, and used as they are
+        ex = _layer(4, H, I, 7)
+        x = torch.randn(T, H, device="cuda").half()
+        ids, w = _routing(T, 4, 2, 5)
+        ids, w = torch.from_numpy(ids).cuda(), torch.from_numpy(w).cuda()
+        want = mxfp4.moe_forward_ids(ex, x, ids, w)
+        assert torch.equal(fused_experts_mxfp4(x, ex.w13, ex.w2, w, ids, (ex.w13_scale, ex.w2_scale)), want)
     wide = torch.stack([ids, ids], 2)[..., 0]              # ids with a column stride
     assert torch.equal(mxfp4.moe_forward_ids(ex, x, wide, w.half().float()), mxfp4.moe_forward_ids(ex, x, ids, w.half()))
+
+
+def test_arranged_scales(cuda):
+    from mi355moe import mxfp4
+    for n, rows, nb in ((1, 3, 1), (2, 64, 8), (3, 17, 21), (2, 5, 128)):
+        s = torch.randint(0, 256, (n, rows, nb), generator=_gen(nb), device="cuda", dtype=torch.uint8)
+        want = torch.nn.functional.pad(s, (0, -nb % 8), value=127).reshape(n, rows, -1, 8).transpose(1, 2)
+        assert torch.equal(mxfp4._arranged(s), want)
 
 
 def test_empty_calls(cuda):

@@ -63,7 +63,7 @@ def test_matmul_refusals(L):
 def _layer(**kw):
     from mi355moe import _lib
     d = _lib.Mxfp4LayerDesc()
-    d.n, d.hidden, d.intermediate, d.w13_scale_stride, d.w2_scale_stride = 8, 128, 128, 4, 4
+    d.n, d.hidden, d.intermediate, d.arranged = 8, 128, 128, 1
     for k in ("w13", "w13_scale", "w2", "w2_scale"):
         setattr(d, k, P)
     for k, v in kw.items():
@@ -80,8 +80,8 @@ def test_moe_refusals(L):
 
     assert call(_layer(n=0)) == ELIMIT and call(_layer(n=5000)) == ELIMIT
     assert call(_layer(hidden=48)) == ESHAPE and call(_layer(intermediate=0)) == ESHAPE
-    assert call(_layer(hidden=32768, w13_scale_stride=1024)) == ELIMIT
-    assert call(_layer(w13_scale_stride=3)) == ESHAPE and call(_layer(w2_scale_stride=6)) == ESHAPE
+    assert call(_layer(hidden=32768)) == ELIMIT and call(_layer(arranged=2)) == EINVAL
+    assert call(_layer(hidden=96, arranged=0)) == ESHAPE and call(_layer(intermediate=160, arranged=0)) == ESHAPE
     assert call(_layer(w13=NUL)) == EINVAL and call(_layer(w2=ODD)) == EINVAL and call(_layer(w2_scale=ODD)) == EINVAL
     assert call(x=NUL) == EINVAL and call(ws=NUL) == EINVAL and call(opt=2) == EINVAL and call(em=P, ng=-1) == EINVAL
     assert call(dt=I32) == EDTYPE and call(idt=F32) == EDTYPE and call(wdt=I64) == EDTYPE and call(odt=7) == EDTYPE
@@ -91,6 +91,14 @@ def test_moe_refusals(L):
     assert call(nb=size(ctypes.byref(lay), 4, 2) - 1) == EWORKSPACE
     assert size(ctypes.byref(_layer(hidden=48)), 4, 2) == -1 and size(ctypes.byref(lay), 4, 0) == -1
     assert call(T=0) == 0
+
+
+def test_arrange_refusals(L):
+    f, size = L.mi355moe_mxfp4_arrange_scales, L.mi355moe_mxfp4_arranged_bytes
+    assert size(2, 5, 96) == 80 and size(1, 3, 288) == 48
+    for bad in ((0, 5, 96), (2, 0, 96), (2, 5, 40), (2, 5, 0), (2, 5, 1 << 17)):
+        assert size(*bad) == -1 and f(P, *bad, P, NUL) == ESHAPE
+    assert f(NUL, 1, 5, 96, P, NUL) == EINVAL and f(P, 1, 5, 96, NUL, NUL) == EINVAL and f(P, 1, 5, 96, ODD, NUL) == EINVAL
 
 
 def test_gated_refusals(L):
@@ -103,6 +111,7 @@ def test_gated_refusals(L):
     assert call(H=60) == ESHAPE and call(I=12) == ESHAPE and call(T=-1) == ESHAPE and call(xs=56) == ESHAPE and call(hs=8) == ESHAPE
     assert call(T=1 << 25) == ELIMIT and call(H=1 << 17, xs=1 << 17) == ELIMIT
     assert call(x=NUL) == EINVAL and call(w=NUL) == EINVAL and call(h=NUL) == EINVAL
+    assert call(h=ODD) == EINVAL and call(hs=20) == EINVAL
     assert call(x=ODD) == EINVAL and call(w=ODD) == EINVAL and call(xs=68) == EINVAL and call(gu=ODD) == EINVAL
     assert call(T=0, x=NUL) == 0
     b, size = L.mi355moe_gated_backward, L.mi355moe_gated_backward_workspace_bytes
@@ -137,15 +146,19 @@ def test_python_refusals():
         mxfp4.matmul(u8.int(), u8, u8, u8)
     w13, w2 = torch.zeros(2, 64, 32, dtype=torch.uint8), torch.zeros(2, 64, 16, dtype=torch.uint8)
     s13, s2 = torch.zeros(2, 64, 2, dtype=torch.uint8), torch.zeros(2, 64, 1, dtype=torch.uint8)
-    ex = mxfp4.Mxfp4Experts(w13, s13, w2, s2)
-    assert (ex.n, ex.K, ex.N) == (2, 64, 32) and ex.w13_scale.shape == (2, 64, 4)
-    assert (ex.w13_scale[..., 2:] == mxfp4.SCALE_ONE).all()
+    with pytest.raises(ValueError, match="GPU"):
+        mxfp4.Mxfp4Experts(w13, s13, w2, s2)
+    with pytest.raises(ValueError, match="128"):
+        mxfp4.Mxfp4Experts(w13, s13, w2, s2, arrange=False)
+    big = [torch.zeros(s, dtype=torch.uint8) for s in ((2, 256, 128), (2, 256, 8), (2, 256, 64), (2, 256, 4))]
+    ex = mxfp4.Mxfp4Experts(*big, arrange=False)
+    assert (ex.n, ex.K, ex.N, ex.desc.arranged) == (2, 256, 128, 0)
     for bad in ((w13[:, :48], s13, w2, s2), (w13, s13[..., :1].contiguous(), w2, s2), (w13, s13, w2[:, :32].contiguous(), s2),
                 (w13, s13, w2, s2.float()), (w13[..., ::2], s13, w2, s2), (w13[0], s13, w2, s2)):
         with pytest.raises(ValueError):
             mxfp4.Mxfp4Experts(*bad)
     with pytest.raises(ValueError, match="GPU"):
-        mxfp4.moe_forward_ids(ex, torch.zeros(1, 64), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, 2))
+        mxfp4.moe_forward_ids(ex, torch.zeros(1, 256), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, 2))
     with pytest.raises(ValueError, match="GPU"):
         ffn.gated(torch.zeros(2, 64).half(), torch.zeros(32, 64).half())
 
