@@ -2010,6 +2010,13 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
     f.odt = dt_w(out_dtype);
     f.out_stride = out_stride;
     f.accumulate = options & MI355MOE_OPT_ACCUMULATE ? 1 : 0;
+    f.ids = ids;
+    f.ids64 = r.ids64;
+    f.emap = r.emap;
+    f.n_global = r.n_global;
+    f.wts = weights;
+    f.wdt = r.wdt;
+    if (mxfp4_direct(P, T, n)) return rc_launch(launch_mxfp4_direct(f, stream));
     if (int rc = launch_route(r, stream)) return rc_launch(rc);
     return rc_launch(launch_mxfp4(f, stream, 15));
 }

@@ -339,10 +339,21 @@ struct Mxfp4Args {
     int odt;
     int64_t out_stride;
     int accumulate;         // out += the routed sum
+    // the router's picks (calls of few pairs read them themselves)
+    const void* ids;
+    int ids64;
+    const int64_t* emap;
+    int64_t n_global;
+    const void* wts;
+    int wdt;
 };
+constexpr int MX_MAX_TOPK = 32;
 constexpr int MX_FEW = 16, MX_TILE = 64;             // rows per segment: streamed weights, LDS tiles
 // Rows per segment of a call of P pairs over n experts: the weights are streamed for segments of few rows.
 constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : MX_TILE; }
+// Calls of few pairs, hardly any of which share an expert: launch_mxfp4_direct, without a permutation.
+constexpr bool mxfp4_direct(int64_t P, int64_t T, int64_t n) { return T == 1 || (P <= 64 && P <= n / 2); }
+int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st);
 // kernels: bit 0 quantise inputs, bit 1 gate/up, bit 2 down, bit 3 slot-order combine
 int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels);
 // rows x K values to codes [rows][ceil(K/2)] and scales [rows][ceil(K/32)] or (steps) arranged by steps

@@ -38,16 +38,20 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8], float inv) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
 
-// Eight consecutive values from an aligned address (16 bytes for 16-bit types, two times 16 for fp32).
+// Vectors at any address of their element (the hardware takes global accesses at any byte address).
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+
+// Eight consecutive values.
 template <int XDT>
 __device__ __forceinline__ void mx_load8(const void* x, size_t i, float (&v)[8]) {
     if constexpr (XDT == DT_F32) {
-        const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(x) + i);
-        const f32x4 a = p[0], b = p[1];
+        const u32x4_any* p = reinterpret_cast<const u32x4_any*>(static_cast<const float*>(x) + i);
+        const f32x4 a = __builtin_bit_cast(f32x4, (u32x4)p[0]), b = __builtin_bit_cast(f32x4, (u32x4)p[1]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
     } else {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + i);
+        const u32x4 w = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(x) + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (XDT == DT_BF16) {
@@ -67,55 +71,42 @@ __device__ __forceinline__ int64_t scale_place(int64_t r, int b, int nb, int64_t
 }
 // The bytes behind a row's last scale in its last step.
 __device__ __forceinline__ void scale_pad(uint8_t* s, int64_t r, int nb, int64_t rows) {
+#pragma unroll 1
     for (int b = nb; b & 7; ++b) s[scale_place(r, b, nb, rows, 1)] = 127;
 }
 
-// Rows of whole blocks at aligned addresses: four lanes a block, eight values a lane. Item i is 8 values; a row has
-// K / 8 of them.
-template <int XDT>
-__global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ x, int64_t stride, int64_t items, int per_row,
-                                                       uint32_t* __restrict__ q, uint8_t* __restrict__ s, int64_t rows, int steps) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per_row;
-        const int c = (int)(i - r * per_row);
+// Four lanes a block, eight values a lane, the lanes of a wave on consecutive places of a row (rows of 4 nb such groups, the
+// last ones partly or wholly behind the row's end); any row length, stride and address. Ix: 32 bits where the groups of the
+// call fit them (the division by the groups of a row is the kernel's longest instruction sequence).
+template <int XDT, typename Ix>
+__global__ __launch_bounds__(256) void mx_quant_kernel(const void* __restrict__ x, int64_t stride, Ix items, int K,
+                                                       uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t rows, int steps) {
+    const int nb = (K + 31) / 32, qp = (K + 1) / 2;
+    const Ix per_row = (Ix)nb * 4;
+    for (Ix i = (Ix)blockIdx.x * 256 + threadIdx.x; i < items; i += (Ix)gridDim.x * 256) {
+        const Ix r = i / per_row;
+        const int c = (int)(i - r * per_row), n = min(8, K - 8 * c);   // this group's values
+        const size_t at = (size_t)r * (size_t)stride + 8 * (size_t)c;
         float v[8];
-        mx_load8<XDT>(x, (size_t)(r * stride + 8 * (int64_t)c), v);
+        if (n == 8) mx_load8<XDT>(x, at, v);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < n ? load_value(x, XDT, at + j) : 0.0f;
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
         top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));       // (items % 4 == 0: a block's lanes are all here)
         top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
         const uint32_t code = mx_scale_code(top);
-        q[i] = e2m1x8(v, mx_inv_scale(code));
+        const uint32_t d = e2m1x8(v, mx_inv_scale(code));
+        uint8_t* o = q + (size_t)r * qp + 4 * (size_t)c;
+        if (n == 8) *reinterpret_cast<u32_any*>(o) = d;
+        else
+            for (int b = 0; 2 * b < n; ++b) o[b] = (uint8_t)(d >> (8 * b));
         if ((c & 3) == 0) {
-            s[scale_place(r, c >> 2, per_row >> 2, rows, steps)] = (uint8_t)code;
-            if (steps && c + 4 == per_row) scale_pad(s, r, per_row >> 2, rows);
+            s[scale_place(r, c >> 2, nb, rows, steps)] = (uint8_t)code;
+            if (steps && c + 4 == 4 * nb) scale_pad(s, r, nb, rows);
         }
-    }
-}
-
-// Any row length and alignment: one thread a block.
-__global__ __launch_bounds__(256) void mx_quant_any_kernel(const void* __restrict__ x, int xdt, int64_t stride, int64_t blocks,
-                                                           int K, uint8_t* __restrict__ q, uint8_t* __restrict__ s, int64_t rows,
-                                                           int steps) {
-    const int nb = (K + 31) / 32, qp = (K + 1) / 2;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < blocks; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / nb;
-        const int b = (int)(i - r * nb), k0 = 32 * b, n = min(32, K - k0);
-        uint32_t top = 0;
-        for (int j = 0; j < n; ++j) top = max(top, abs_bits(load_value(x, xdt, (size_t)(r * stride + k0 + j))));
-        const uint32_t code = mx_scale_code(top);
-        const float inv = mx_inv_scale(code);
-        for (int j = 0; j < n; j += 8) {
-            float v[8];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) v[t] = j + t < n ? load_value(x, xdt, (size_t)(r * stride + k0 + j + t)) : 0.0f;
-            const uint32_t d = e2m1x8(v, inv);
-            uint8_t* o = q + r * qp + (k0 + j) / 2;
-            for (int t = 0; 2 * t < n - j && t < 4; ++t) o[t] = (uint8_t)(d >> (8 * t));
-        }
-        s[scale_place(r, b, nb, rows, steps)] = (uint8_t)code;
-        if (steps && b + 1 == nb) scale_pad(s, r, nb, rows);
     }
 }
 
@@ -129,42 +120,48 @@ __device__ __forceinline__ float mx_scale_value(uint32_t code) {
     return __builtin_bit_cast(float, code == 255u ? 0x7FC00000u : code ? code << 23 : 0x00400000u);
 }
 
-// One thread per 8 values (VEC: rows of whole such groups, outputs at 16-byte addresses).
-template <bool VEC>
-__global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s,
-                                                         int64_t items, int K, void* __restrict__ out, int odt) {
-    const int per_row = (K + 7) / 8, nb = (K + 31) / 32, qp = (K + 1) / 2;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per_row;
-        const int c = (int)(i - r * per_row);
-        const float f = mx_scale_value(s[r * nb + (c >> 2)]);
-        const int n = min(8, K - 8 * c);
+// Eight values a thread, laid out as for quantisation.
+template <int ODT, typename Ix>
+__global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ s, Ix items, int K,
+                                                         void* __restrict__ out) {
+    const int nb = (K + 31) / 32, qp = (K + 1) / 2, per_row = (K + 7) / 8;
+    for (Ix i = (Ix)blockIdx.x * 256 + threadIdx.x; i < items; i += (Ix)gridDim.x * 256) {
+        const Ix r = i / (Ix)per_row;
+        const int c = (int)(i - r * (Ix)per_row), n = min(8, K - 8 * c);
+        const uint8_t* p = q + (size_t)r * qp + 4 * (size_t)c;
+        const float f = mx_scale_value(s[(size_t)r * nb + (c >> 2)]);
         uint32_t d = 0;
-        if constexpr (VEC) d = reinterpret_cast<const uint32_t*>(q)[i];
+        if (n == 8) d = *reinterpret_cast<const u32_any*>(p);
         else
-            for (int t = 0; 2 * t < n; ++t) d |= (uint32_t)q[r * qp + 4 * c + t] << (8 * t);
+            for (int b = 0; 2 * b < n; ++b) d |= (uint32_t)p[b] << (8 * b);
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = e2m1_value(d >> (4 * j)) * f;
-        const size_t o = (size_t)(r * K + 8 * (int64_t)c);
-        if constexpr (VEC) {
-            if (odt == DT_F32) {
-                f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(out) + o);
-                p[0] = f32x4{v[0], v[1], v[2], v[3]};
-                p[1] = f32x4{v[4], v[5], v[6], v[7]};
-            } else {
-                u32x4 w;
+        const size_t o = (size_t)r * K + 8 * (size_t)c;
+        if constexpr (ODT == DT_F32) {
+            float* w = static_cast<float*>(out) + o;
+            if (n == 8) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    w[j] = odt == DT_BF16 ? pack_bf16x2(v[2 * j], v[2 * j + 1])
-                                          : h_as_u16((_Float16)v[2 * j]) | (h_as_u16((_Float16)v[2 * j + 1]) << 16);
-                *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + o) = w;
-            }
+                for (int k = 0; k < 2; ++k)
+                    reinterpret_cast<u32x4_any*>(w)[k] =
+                        __builtin_bit_cast(u32x4, f32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]});
+            } else
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) w[j] = v[j];
         } else {
-            for (int j = 0; j < n; ++j) {
-                if (odt == DT_F32) static_cast<float*>(out)[o + j] = v[j];
-                else static_cast<uint16_t*>(out)[o + j] = odt == DT_BF16 ? f32_to_bf16(v[j]) : (uint16_t)h_as_u16((_Float16)v[j]);
+            uint16_t* w = static_cast<uint16_t*>(out) + o;
+            u32x4 h;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint2 t = pack4(ODT, v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                h[2 * k] = t.x, h[2 * k + 1] = t.y;
             }
+            if (n == 8) *reinterpret_cast<u32x4_any*>(w) = h;
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) w[j] = (uint16_t)(h[j >> 1] >> (16 * (j & 1)));
         }
     }
 }
@@ -305,6 +302,133 @@ __global__ __launch_bounds__(512) void mx_gateup_few_kernel(Mxfp4Args a) {
             if ((cb + 1) * 32 == a.N) scale_pad(a.sh, r, cb + 1, a.P);
         }
     }
+}
+
+// ------------------------------------------------------------------------------------------------ few pairs
+
+// A call of few pairs (mxfp4_direct) takes two launches and no tables: every pair is a segment of its own, read from the
+// router's ids; gate/up quantises the pair's token itself, and down sums a token's pairs. Pairs that share an expert read
+// its weights each for itself (from the caches, where they run together).
+__device__ __forceinline__ int pair_expert(const Mxfp4Args& a, int j) {
+    int64_t id = a.ids64 ? reinterpret_cast<const int64_t*>(a.ids)[j] : (int64_t)reinterpret_cast<const int32_t*>(a.ids)[j];
+    if (a.emap) id = id >= 0 && id < a.n_global ? a.emap[id] : -1;
+    return id >= 0 && id < a.n ? (int)id : -1;
+}
+
+// grid (N / 32, pairs), 512 threads: mx_gateup_few_kernel for one row, which every wave quantises as far as it multiplies it
+// (512 values a step: eight a lane, four lanes a block, through 272 bytes of LDS into the lanes that hold the blocks).
+template <int XDT>
+__global__ __launch_bounds__(512) void mx_gateup_direct_kernel(Mxfp4Args a) {
+    __shared__ __align__(16) float red[8][4][16];
+    __shared__ __align__(16) uint8_t xq[8][272];
+    const int cb = blockIdx.x, j = blockIdx.y;
+    const int e = __builtin_amdgcn_readfirstlane(pair_expert(a, j));
+    if (e < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nblk = a.K >> 5;
+    FewRow w[4];
+    const MxScales ws = {a.w13s.p + (size_t)e * a.w13se, a.w13s.row, a.w13s.step};
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        w[t] = few_row(a.w13 + (size_t)e * 2 * a.N * (a.K / 2), a.K / 2, ws, (size_t)(t >> 1) * a.N + cb * 32 + (t & 1) * 16 + c);
+    const size_t x0 = (size_t)(j / a.topk) * a.x_stride;
+    f32x4 acc[4] = {};
+    for (int b0 = wv * 16; b0 < nblk; b0 += 128) {
+        u32x4 wv4[4][4];
+        int wsc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) few_load<false>(w[t], b0, g, nblk, wv4[t], wsc[t]);
+        const int b = b0 + (lane >> 2);                              // this lane's block, and its eighth
+        float v[8];
+        if (b < nblk) mx_load8<XDT>(a.x, x0 + 32 * (size_t)b + 8 * (lane & 3), v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[i]));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+        const uint32_t code = mx_scale_code(top);
+        asm volatile("" ::: "memory");                               // (a wave's LDS accesses are performed in order)
+        *reinterpret_cast<uint32_t*>(xq[wv] + 4 * lane) = e2m1x8(v, mx_inv_scale(code));
+        if ((lane & 3) == 0) xq[wv][256 + (lane >> 2)] = b < nblk ? (uint8_t)code : (uint8_t)127;
+        asm volatile("" ::: "memory");
+        u32x4 xv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xv[i] = *reinterpret_cast<const u32x4*>(xq[wv] + 64 * g + 16 * i);
+        const int xs = *reinterpret_cast<const int*>(xq[wv] + 256 + 4 * g);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            acc[t] = few_mma<0>(wv4[t][0], xv[0], acc[t], wsc[t], xs);
+            acc[t] = few_mma<1>(wv4[t][1], xv[1], acc[t], wsc[t], xs);
+            acc[t] = few_mma<2>(wv4[t][2], xv[2], acc[t], wsc[t], xs);
+            acc[t] = few_mma<3>(wv4[t][3], xv[3], acc[t], wsc[t], xs);
+        }
+    }
+    // all sixteen columns of an accumulator are this row's: lane 16 g holds n = 4 g .. + 3
+    if (c == 0)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(&red[wv][t][4 * g]) = acc[t];
+    __syncthreads();
+    if (tid >= 32) return;
+    float gs = 0.f, us = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        gs += red[i][tid >> 4][tid & 15];
+        us += red[i][2 + (tid >> 4)][tid & 15];
+    }
+    const float h = swiglu(gs, us, a.limit);
+    uint32_t top = abs_bits(h);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    const uint32_t code = mx_scale_code(top);
+    const uint32_t nib = code == 255u ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, h * mx_inv_scale(code), 0.0f, 1.0f, 0) & 15u;
+    uint32_t d = nib << (4 * (tid & 7));
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
+    if ((tid & 7) == 0) *reinterpret_cast<uint32_t*>(a.qh + (size_t)j * (a.N / 2) + cb * 16 + (tid >> 1)) = d;
+    if (tid == 0) {
+        a.sh[scale_place(j, cb, 0, a.P, 1)] = (uint8_t)code;
+        if ((cb + 1) * 32 == a.N) scale_pad(a.sh, j, cb + 1, a.P);
+    }
+}
+
+// grid (ceil(K / 16), tokens), 512 threads: 16 columns of one token, a pair a wave at a time, summed in slot order.
+__global__ __launch_bounds__(512) void mx_down_direct_kernel(Mxfp4Args a) {
+    __shared__ __align__(16) float sum[MX_MAX_TOPK][16];
+    const int t = blockIdx.y, n0 = blockIdx.x * 16;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nblk = a.N >> 5;
+    for (int k = wv; k < a.topk; k += 8) {
+        const int j = t * a.topk + k;
+        const int e = __builtin_amdgcn_readfirstlane(pair_expert(a, j));
+        f32x4 acc[1] = {};
+        if (e >= 0) {
+            const FewRow w[1] = {few_row(a.w2 + (size_t)e * a.K * (a.N / 2), a.N / 2,
+                                         MxScales{a.w2s.p + (size_t)e * a.w2se, a.w2s.row, a.w2s.step}, min(n0 + c, a.K - 1))};
+            const FewRow x = few_row(a.qh, a.N / 2, MxScales{a.sh, 8, 8u * a.P}, j);
+#pragma unroll 2
+            for (int b0 = 0; b0 < nblk; b0 += 16) few_product(w, x, b0, g, nblk, acc);
+        }
+        const float rw = e < 0 ? 0.0f : load_value(a.wts, a.wdt, j);
+        if (c == 0) *reinterpret_cast<f32x4*>(&sum[k][4 * g]) = acc[0] * f32x4{rw, rw, rw, rw};
+    }
+    __syncthreads();
+    if (tid >= 4) return;
+    f32x4 v = {};
+    for (int k = 0; k < a.topk; ++k)
+        if (pair_expert(a, t * a.topk + k) >= 0) v += *reinterpret_cast<const f32x4*>(&sum[k][4 * tid]);
+    const int n = n0 + 4 * tid;
+    const size_t o = (size_t)t * a.out_stride + n;
+    if (a.accumulate)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < a.K) v[i] += load_value(a.out, a.odt, o + i);
+    if (n < a.K) store4(a.out, a.odt, o, a.K - n, v);
 }
 
 // The eight waves of a workgroup as KS cuts of the contraction x 8 / KS groups of 16 T columns. Store(m, n, four sums of
@@ -606,32 +730,38 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(Mxfp4Args a) {
 
 static unsigned grid_for(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, 256 * 32); }
 
+template <int XDT>
+static void run_mx_quant(const void* x, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int steps, hipStream_t st) {
+    const int64_t items = rows * 4 * ((K + 31) / 32);
+    const dim3 g(grid_for(items)), d(256);
+    if (items + 256 * 256 * 32 < (int64_t(1) << 32))
+        hipLaunchKernelGGL((mx_quant_kernel<XDT, uint32_t>), g, d, 0, st, x, stride, (uint32_t)items, K, q, s, rows, steps);
+    else hipLaunchKernelGGL((mx_quant_kernel<XDT, int64_t>), g, d, 0, st, x, stride, items, K, q, s, rows, steps);
+}
+
 int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int steps,
                     hipStream_t st) {
     if (rows <= 0) return 0;
-    const int unit = xdt == DT_F32 ? 4 : 8;                          // elements of a 16-byte load
-    const bool vec = K % 32 == 0 && stride % unit == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
-                     (reinterpret_cast<uintptr_t>(q) & 3) == 0;
-    if (vec) {
-        const int64_t items = rows * (K / 8);
-        const dim3 g(grid_for(items));
-        uint32_t* q32 = reinterpret_cast<uint32_t*>(q);
-        if (xdt == DT_F32) hipLaunchKernelGGL(mx_quant_kernel<DT_F32>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, rows, steps);
-        else if (xdt == DT_F16) hipLaunchKernelGGL(mx_quant_kernel<DT_F16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, rows, steps);
-        else hipLaunchKernelGGL(mx_quant_kernel<DT_BF16>, g, dim3(256), 0, st, x, stride, items, K / 8, q32, s, rows, steps);
-    } else {
-        const int64_t blocks = rows * ((K + 31) / 32);
-        hipLaunchKernelGGL(mx_quant_any_kernel, dim3(grid_for(blocks)), dim3(256), 0, st, x, xdt, stride, blocks, K, q, s, rows, steps);
-    }
+    if (xdt == DT_F32) run_mx_quant<DT_F32>(x, stride, rows, K, q, s, steps, st);
+    else if (xdt == DT_F16) run_mx_quant<DT_F16>(x, stride, rows, K, q, s, steps, st);
+    else run_mx_quant<DT_BF16>(x, stride, rows, K, q, s, steps, st);
     return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int ODT>
+static void run_mx_dequant(const uint8_t* q, const uint8_t* s, int64_t rows, int K, void* out, hipStream_t st) {
+    const int64_t items = rows * ((K + 7) / 8);
+    const dim3 g(grid_for(items)), d(256);
+    if (items + 256 * 256 * 32 < (int64_t(1) << 32))
+        hipLaunchKernelGGL((mx_dequant_kernel<ODT, uint32_t>), g, d, 0, st, q, s, (uint32_t)items, K, out);
+    else hipLaunchKernelGGL((mx_dequant_kernel<ODT, int64_t>), g, d, 0, st, q, s, items, K, out);
 }
 
 int launch_mx_dequant(const uint8_t* q, const uint8_t* s, int64_t rows, int K, void* out, int odt, hipStream_t st) {
     if (rows <= 0) return 0;
-    const int64_t items = rows * ((K + 7) / 8);
-    const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0;
-    if (vec) hipLaunchKernelGGL(mx_dequant_kernel<true>, dim3(grid_for(items)), dim3(256), 0, st, q, s, items, K, out, odt);
-    else hipLaunchKernelGGL(mx_dequant_kernel<false>, dim3(grid_for(items)), dim3(256), 0, st, q, s, items, K, out, odt);
+    if (odt == DT_F32) run_mx_dequant<DT_F32>(q, s, rows, K, out, st);
+    else if (odt == DT_F16) run_mx_dequant<DT_F16>(q, s, rows, K, out, st);
+    else run_mx_dequant<DT_BF16>(q, s, rows, K, out, st);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
@@ -708,6 +838,15 @@ static int run_mx_down(const Mxfp4Args& a, hipStream_t st) {
     if (!ok) return -1;
     hipLaunchKernelGGL((mx_down_kernel<BP, BQ, WP, WQ, ST>), dim3((a.K + BP - 1) / BP, a.S_cap), dim3(G::THREADS), G::LDS, st, a);
     return 0;
+}
+
+int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st) {
+    const dim3 g(a.N / 32, a.P), d(512);
+    if (a.xdt == DT_F32) hipLaunchKernelGGL(mx_gateup_direct_kernel<DT_F32>, g, d, 0, st, a);
+    else if (a.xdt == DT_F16) hipLaunchKernelGGL(mx_gateup_direct_kernel<DT_F16>, g, d, 0, st, a);
+    else hipLaunchKernelGGL(mx_gateup_direct_kernel<DT_BF16>, g, d, 0, st, a);
+    hipLaunchKernelGGL(mx_down_direct_kernel, dim3((a.K + 15) / 16, a.T), d, 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {

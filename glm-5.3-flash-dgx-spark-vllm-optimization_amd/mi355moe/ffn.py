@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _capturing, _need_cuda, _on_device, _p, _stream, act_dtype_code
+from .ops import _addr, _capturing, _need_cuda, _on_device, _raw_stream, act_dtype_code
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -28,6 +28,8 @@ def _row_stride(t: torch.Tensor) -> int:
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t [rows, K] itself where its rows lie apart at 16-byte addresses, else a contiguous copy."""
+    if t.is_contiguous() and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
     if t.stride(1) == 1 and (t.shape[0] <= 1 or (t.shape[1] <= t.stride(0) <= 1 << 22 and t.stride(0) % 8 == 0)) and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -50,15 +52,18 @@ def gated_forward(x: torch.Tensor, w13: torch.Tensor, limit: float = 0.0, save: 
     W13^T for gated_backward. No gradient is recorded."""
     dev, code = _check(x, w13)
     I, H = w13.shape[0] // 2, w13.shape[1]
-    x2 = _rows16(x.detach().reshape(-1, H))
-    w = _rows16(w13.detach()) if w13.is_contiguous() else w13.detach().contiguous()
+    if x.requires_grad or w13.requires_grad:
+        x, w13 = x.detach(), w13.detach()
+    x2 = _rows16(x if x.dim() == 2 else x.reshape(-1, H))
+    w = _rows16(w13) if w13.is_contiguous() else w13.contiguous()
     T = x2.shape[0]
     with _on_device(dev):
-        h = torch.empty(T, I, dtype=x.dtype, device=dev)
-        gu = torch.empty(T, 2 * I, dtype=torch.float32, device=dev) if save else None
+        h = x2.new_empty((T, I))
+        gu = x2.new_empty((T, 2 * I), dtype=torch.float32) if save else None
         _lib.check("mi355moe_gated_forward", _lib.lib().mi355moe_gated_forward(
-            _p(x2), code, T, H, _row_stride(x2), _p(w), I, float(limit), _p(h), I, _p(gu), _stream(dev)))
-    h = h.reshape(*x.shape[:-1], I)
+            _addr(x2), code, T, H, _row_stride(x2), _addr(w), I, float(limit), _addr(h), I, _addr(gu), _raw_stream(dev)))
+    if x.dim() != 2:
+        h = h.reshape(*x.shape[:-1], I)
     return (h, gu) if save else h
 
 
@@ -86,8 +91,8 @@ def gated_backward(dh: torch.Tensor, gu: torch.Tensor, x: torch.Tensor, w13: tor
         dw = torch.empty(2 * I, H, dtype=x.dtype, device=dev) if need_dw13 else None
         ws = torch.empty(L.mi355moe_gated_backward_workspace_bytes(T, H, I), dtype=torch.uint8, device=dev)
         _lib.check("mi355moe_gated_backward", L.mi355moe_gated_backward(
-            _p(d2), _row_stride(d2), _p(gu), _p(x2), code, T, H, _row_stride(x2), _p(w), I, float(limit), _p(dx), _p(dw),
-            _p(ws), ws.numel(), _stream(dev)))
+            _addr(d2), _row_stride(d2), _addr(gu), _addr(x2), code, T, H, _row_stride(x2), _addr(w), I, float(limit), _addr(dx), _addr(dw),
+            _addr(ws), ws.numel(), _raw_stream(dev)))
     return (dx.reshape(x.shape) if need_dx else None), dw
 
 

@@ -16,11 +16,12 @@ Every call runs on the current stream of its tensors' device. Scratch comes from
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .ops import _need_cuda, _on_device, _p, _stream, ids_dtype_code, weight_dtype_code
+from .ops import _addr, _need_cuda, _on_device, _raw_stream, ids_dtype_code, weight_dtype_code
 
 BLOCK = 32
 SCALE_NAN = 255
@@ -32,10 +33,6 @@ def _codes(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
-
-
 def _row_stride(t: torch.Tensor) -> int:
     return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
 
@@ -44,6 +41,8 @@ def _rows(x: torch.Tensor, name: str = "x") -> torch.Tensor:
     """x as rows that do not overlap, with unit column stride."""
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"{name} must be [rows, K], got {tuple(x.shape)}")
+    if x.is_contiguous():
+        return x
     if (x.stride(1) != 1 and x.shape[1] > 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         raise ValueError(f"{name} must have unit column stride and rows that do not overlap, got strides {x.stride()}")
     return x
@@ -56,11 +55,11 @@ def quant_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dev = _need_cuda(_rows(x))
     rows, K = x.shape
     dt = weight_dtype_code(x.dtype)
-    q = torch.empty(rows, (K + 1) // 2, dtype=torch.uint8, device=dev)
-    s = torch.empty(rows, (K + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=dev)
+    q = x.new_empty((rows, (K + 1) // 2), dtype=torch.uint8)
+    s = x.new_empty((rows, (K + BLOCK - 1) // BLOCK), dtype=torch.uint8)
     with _on_device(dev):
         _lib.check("mi355moe_mxfp4_quant_rows", _lib.lib().mi355moe_mxfp4_quant_rows(
-            _p(x), dt, rows, K, _row_stride(x), _p(q), _p(s), _stream(dev)))
+            _addr(x), dt, rows, K, _row_stride(x), _addr(q), _addr(s), _raw_stream(dev)))
     return q, s
 
 
@@ -78,11 +77,16 @@ def dequant_rows(q: torch.Tensor, scale: torch.Tensor, K: int | None = None,
                          f"{tuple(q.shape)} and {tuple(scale.shape)}")
     dt = weight_dtype_code(out_dtype)
     q, scale = q.contiguous(), scale.contiguous()
-    out = torch.empty(rows, K, dtype=out_dtype, device=dev)
+    out = q.new_empty((rows, K), dtype=out_dtype)
     with _on_device(dev):
         _lib.check("mi355moe_mxfp4_dequant_rows", _lib.lib().mi355moe_mxfp4_dequant_rows(
-            _p(q), _p(scale), rows, K, _p(out), dt, _stream(dev)))
+            _addr(q), _addr(scale), rows, K, _addr(out), dt, _raw_stream(dev)))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _matmul_bytes(M: int, N: int, K: int) -> int:
+    return _lib.lib().mi355moe_mxfp4_matmul_workspace_bytes(M, N, K)
 
 
 def _aligned(t: torch.Tensor, nbytes: int) -> torch.Tensor:
@@ -104,7 +108,7 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
         if tuple(t.shape) != shape:
             raise ValueError(f"{name}: expected {shape}, got {tuple(t.shape)}")
     if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=dev)
+        out = a.new_empty((M, N), dtype=out_dtype)
     dt = weight_dtype_code(out.dtype)
     if tuple(out.shape) != (M, N):
         raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
@@ -114,13 +118,13 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     a, w = _aligned(a, 16), _aligned(w, 16)
     a_scale, w_scale = _aligned(a_scale, 4), _aligned(w_scale, 4)
     L = _lib.lib()
-    nb = L.mi355moe_mxfp4_matmul_workspace_bytes(M, N, K)
+    nb = _matmul_bytes(M, N, K)
     if nb < 0:
         raise ValueError(f"mi355moe_mxfp4_matmul: unsupported size M {M}, N {N}, K {K}")
     with _on_device(dev):
-        ws = _scratch(nb, dev) if nb else None
+        ws = a.new_empty(nb) if nb else None
         _lib.check("mi355moe_mxfp4_matmul", L.mi355moe_mxfp4_matmul(
-            _p(a), _p(a_scale), M, _p(w), _p(w_scale), N, K, _p(out), dt, _row_stride(out), _p(ws), nb, _stream(dev)))
+            _addr(a), _addr(a_scale), M, _addr(w), _addr(w_scale), N, K, _addr(out), dt, _row_stride(out), _addr(ws), nb, _raw_stream(dev)))
     return out
 
 
@@ -132,7 +136,7 @@ def _arranged(scale: torch.Tensor) -> torch.Tensor:
     out = torch.empty(n, -(-K // 256), rows, 8, dtype=torch.uint8, device=dev)
     with _on_device(dev):
         _lib.check("mi355moe_mxfp4_arrange_scales",
-                   L.mi355moe_mxfp4_arrange_scales(_p(scale), n, rows, K, _p(out), _stream(dev)))
+                   L.mi355moe_mxfp4_arrange_scales(_addr(scale), n, rows, K, _addr(out), _raw_stream(dev)))
     return out
 
 
@@ -167,6 +171,7 @@ class Mxfp4Experts:
             raise ValueError(f"scales are used as they are only for H and I that are multiples of 128, got {H} and {I}")
         self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
         self.n, self.K, self.N = n, H, I
+        self._bytes: dict = {}
         self._s13, self._s2 = (_arranged(w13_scale), _arranged(w2_scale)) if arrange else (w13_scale, w2_scale)
         d = _lib.Mxfp4LayerDesc()
         d.n, d.hidden, d.intermediate, d.arranged = n, H, I, int(arrange)
@@ -189,9 +194,20 @@ class Mxfp4Experts:
     def device(self) -> torch.device:
         return self.w13.device
 
+    def workspace_bytes(self, T: int, topk: int) -> int:
+        """The scratch a call of T tokens takes (-1: more than a call can have)."""
+        nb = self._bytes.get((T, topk))
+        if nb is None:
+            nb = self._bytes[T, topk] = _lib.lib().mi355moe_mxfp4_moe_workspace_bytes(ctypes.byref(self.desc), T, topk)
+        return nb
+
     def expert_bytes(self) -> int:
         """Bytes of one expert's three matrices and their block scales."""
         return 3 * self.K * self.N * 17 // 32
+
+
+def _pairs(t: torch.Tensor, T: int) -> torch.Tensor:
+    return t if t.dim() == 2 and t.is_contiguous() else t.reshape(T, -1).contiguous()
 
 
 def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
@@ -213,27 +229,26 @@ def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tens
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if out is None:
-        out = torch.empty(T, experts.K, dtype=out_dtype or x.dtype, device=dev)
+        out = x.new_empty((T, experts.K), dtype=out_dtype or x.dtype)
     if tuple(out.shape) != (T, experts.K):
         raise ValueError(f"out must be [T, {experts.K}], got {tuple(out.shape)}")
     _rows(out, "out")
     xdt, odt = weight_dtype_code(x.dtype), weight_dtype_code(out.dtype)
     if T == 0:
         return out
-    ids = topk_ids.reshape(T, -1).contiguous()
-    w = topk_weights.reshape(T, -1).contiguous()
+    ids, w = _pairs(topk_ids, T), _pairs(topk_weights, T)
     topk = ids.shape[1]
     L = _lib.lib()
-    nb = L.mi355moe_mxfp4_moe_workspace_bytes(ctypes.byref(experts.desc), T, topk)
+    nb = experts.workspace_bytes(T, topk)
     if nb < 0:
         raise ValueError(f"mi355moe_mxfp4_moe_forward_ids: unsupported size (T {T}, top-{topk})")
     em = None if expert_map is None else expert_map.to(torch.int64).contiguous()
     with _on_device(dev):
-        ws = _scratch(nb, dev)
+        ws = experts.w13.new_empty(nb)
         _lib.check("mi355moe_mxfp4_moe_forward_ids", L.mi355moe_mxfp4_moe_forward_ids(
-            ctypes.byref(experts.desc), _p(x), xdt, _row_stride(x), T, _p(ids), ids_dtype_code(ids.dtype), _p(w),
-            weight_dtype_code(w.dtype), topk, _p(em), 0 if em is None else em.numel(), float(limit), _p(out), odt,
-            _row_stride(out), _lib.OPT_ACCUMULATE if accumulate else 0, _p(ws), ws.numel(), _stream(dev)))
+            ctypes.byref(experts.desc), _addr(x), xdt, _row_stride(x), T, _addr(ids), ids_dtype_code(ids.dtype), _addr(w),
+            weight_dtype_code(w.dtype), topk, _addr(em), 0 if em is None else em.numel(), float(limit), _addr(out), odt,
+            _row_stride(out), _lib.OPT_ACCUMULATE if accumulate else 0, _addr(ws), ws.numel(), _raw_stream(dev)))
     return out
 
 

@@ -23,9 +23,21 @@ def _stream(dev: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on_device(dev: torch.device):
     """A context in which `dev` is the current device (kernels are launched on the current one)."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _raw_stream(dev: torch.device) -> int:
+    """The current stream of `dev` as an address: what _stream gives, without a stream object (2 us less a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _addr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _p(t: torch.Tensor | None) -> ctypes.c_void_p:

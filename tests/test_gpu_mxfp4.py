@@ -202,7 +202,9 @@ def _routing(T, n, topk, seed, bad=False):
 CASES = [(8, 512, 256, 40, 4, 10.0, torch.bfloat16), (16, 1024, 512, 33, 8, 0.0, torch.float16),
          (4, 32, 32, 1, 2, 10.0, torch.float32), (6, 544, 96, 70, 6, 1.0, torch.bfloat16),
          (3, 160, 1056, 5, 3, 2.0, torch.float32), (2, 288, 160, 150, 2, 10.0, torch.float16),
-         (1, 2080, 64, 130, 1, 1.5, torch.bfloat16), (5, 256, 4160, 2, 1, 10.0, torch.bfloat16)]
+         (1, 2080, 64, 130, 1, 1.5, torch.bfloat16), (5, 256, 4160, 2, 1, 10.0, torch.bfloat16),
+         # few pairs over many experts: no permutation
+         (70, 288, 64, 8, 4, 1.0, torch.bfloat16), (40, 4160, 96, 2, 9, 10.0, torch.float16), (3, 160, 1056, 1, 3, 0.0, torch.float32)]
 
 
 @pytest.mark.parametrize("n,H,I,T,topk,limit,dt", CASES)
@@ -246,6 +248,35 @@ def test_moe_duplicate_ids_expert_map_strides_and_accumulate(cuda):
         mxfp4.moe_forward_ids(*args, expert_map=torch.from_numpy(emap).cuda(), out=shared, accumulate=True)
         tol2 = tol + np.abs(base + want) * EPS[odt] / 2 + np.abs(base) * 2.0 ** -22
         assert (np.abs(_f64(shared) - (base + want)) <= tol2).all()
+
+
+def test_moe_few_pairs_expert_map_and_accumulate(cuda):
+    """Calls that take no permutation (few pairs over many experts): expert map, duplicate and foreign ids, int32 and int64
+    ids, rows at odd addresses, fp16 weights and accumulation."""
+    from mi355moe import mxfp4
+    n, H, I, T, k = 48, 256, 128, 4, 5
+    ex = _layer(n, H, I, 3)
+    w13, w2 = _dense(ex)
+    rng = np.random.default_rng(1)
+    emap = np.where(rng.random(60) < 0.6, rng.integers(0, n, 60), -1)
+    gids = rng.integers(0, 60, (T, k))
+    gids[1] = np.flatnonzero(emap >= 0)[0]
+    gids[2, :2] = (-1, 77)
+    gids[3] = np.flatnonzero(emap < 0)[0]
+    w = rng.random((T, k)).astype(np.float16)
+    local = np.where((gids >= 0) & (gids < 60), emap[np.clip(gids, 0, 59)], -1)
+    wide = torch.randn(T, H + 9, generator=_gen(9), device="cuda").bfloat16()
+    for x in (wide[:, :H].contiguous(), wide[:, 3:3 + H]):
+        want, tol = ref.moe(_f64(x), w13, w2, local, w.astype(np.float64), 10.0, 0.0)
+        for it in (torch.int32, torch.int64):
+            args = (ex, x, torch.from_numpy(gids).to("cuda", it), torch.from_numpy(w).cuda())
+            buf = torch.full((T, H + 1), 2.0, dtype=torch.float32, device="cuda")
+            base = _f64(buf[:, 1:])
+            mxfp4.moe_forward_ids(*args, expert_map=torch.from_numpy(emap).cuda(), out=buf[:, 1:], accumulate=True)
+            assert (np.abs(_f64(buf[:, 1:]) - (base + want)) <= tol + np.abs(base + want) * 2.0 ** -22 + 2.0 ** -21).all()
+            assert (buf[:, 0] == 2.0).all() and (buf[3, 1:] == 2.0).all()
+            out = mxfp4.moe_forward_ids(*args, expert_map=torch.from_numpy(emap).cuda())
+            assert (np.abs(_f64(out) - want) <= tol + np.abs(want) * 2.0 ** -8 + TINY[torch.bfloat16]).all()
 
 
 def test_moe_no_local_expert_writes_zero(cuda):
