@@ -351,8 +351,7 @@ constexpr int MX_MAX_TOPK = 32;
 constexpr int MX_FEW = 16, MX_TILE = 64;             // rows per segment: streamed weights, LDS tiles
 // Rows per segment of a call of P pairs over n experts: the weights are streamed for segments of few rows.
 constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : MX_TILE; }
-// Calls of few pairs, hardly any of which share an expert: launch_mxfp4_direct, without a permutation.
-constexpr bool mxfp4_direct(int64_t P, int64_t T, int64_t n) { return T == 1 || (P <= 64 && P <= n / 2); }
+// a call whose pairs hardly share experts, in two launches and without a permutation (a.ids, a.wts)
 int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st);
 // kernels: bit 0 quantise inputs, bit 1 gate/up, bit 2 down, bit 3 slot-order combine
 int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels);

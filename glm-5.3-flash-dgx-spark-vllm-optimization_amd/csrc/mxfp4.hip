@@ -252,10 +252,11 @@ __device__ __forceinline__ void few_product(const FewRow (&w)[T], const FewRow& 
     }
 }
 
-// grid (N / 32, segments), 512 threads: 32 columns of gate and up for a segment of at most 16 rows, the contraction over
-// the eight waves, then SwiGLU and the quantisation of the 32 columns (one block) by a half wave a row.
-__global__ __launch_bounds__(512) void mx_gateup_few_kernel(Mxfp4Args a) {
-    __shared__ __align__(16) float red[8][4][256];
+// grid (N / 32, segments), 64 NW threads: 32 columns of gate and up for a segment of at most 16 rows, the contraction over
+// the waves, then SwiGLU and the quantisation of the 32 columns (one block) by a half wave a row.
+template <int NW>
+__global__ __launch_bounds__(64 * NW, 3) void mx_gateup_few_kernel(Mxfp4Args a) {
+    __shared__ __align__(16) float red[NW][4][256];
     const int cb = blockIdx.x, s = blockIdx.y;
     if (s >= a.nseg[0]) return;
     const int e = a.seg_expert[s], row0 = a.seg_row0[s], rn = a.seg_rows[s];
@@ -272,29 +273,29 @@ __global__ __launch_bounds__(512) void mx_gateup_few_kernel(Mxfp4Args a) {
     }
     x = few_row(a.qx, a.K / 2, MxScales{a.sx, 8, 8u * a.T}, a.tok[row0 + min(c, rn - 1)]);
     f32x4 acc[4] = {};
-    for (int b0 = wv * 16; b0 < nblk; b0 += 128) few_product(w, x, b0, g, nblk, acc);
+    for (int b0 = wv * 16; b0 < nblk; b0 += 16 * NW) few_product(w, x, b0, g, nblk, acc);
 #pragma unroll
     for (int t = 0; t < 4; ++t) *reinterpret_cast<f32x4*>(&red[wv][t][lane * 4]) = acc[t];
     __syncthreads();
-    const int m = tid >> 5, n = tid & 31;
-    const int at = ((((n & 15) >> 2) << 4) + m) * 4 + (n & 3), t = n >> 4;
-    float gs = 0.f, us = 0.f;
+    const int n = tid & 31, t = n >> 4;
+    for (int m = tid >> 5; m < rn; m += 2 * NW) {
+        const int at = ((((n & 15) >> 2) << 4) + m) * 4 + (n & 3);
+        float gs = 0.f, us = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        gs += red[i][t][at];
-        us += red[i][2 + t][at];
-    }
-    const float h = swiglu(gs, us, a.limit);
-    uint32_t top = abs_bits(h);
+        for (int i = 0; i < NW; ++i) {
+            gs += red[i][t][at];
+            us += red[i][2 + t][at];
+        }
+        const float h = swiglu(gs, us, a.limit);
+        uint32_t top = abs_bits(h);
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-    const uint32_t code = mx_scale_code(top);
-    const float inv = mx_inv_scale(code);
-    const uint32_t nib = code == 255u ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, h * inv, 0.0f, 1.0f, 0) & 15u;
-    uint32_t d = nib << (4 * (n & 7));
+        for (int o = 16; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        const uint32_t code = mx_scale_code(top);
+        const uint32_t nib =
+            code == 255u ? 0u : __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, h * mx_inv_scale(code), 0.0f, 1.0f, 0) & 15u;
+        uint32_t d = nib << (4 * (n & 7));
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
-    if (m < rn) {
+        for (int o = 4; o >= 1; o >>= 1) d |= (uint32_t)__shfl_xor((int)d, o, 64);
         const size_t r = (size_t)row0 + m;
         if ((n & 7) == 0) *reinterpret_cast<uint32_t*>(a.qh + r * (a.N / 2) + cb * 16 + (n >> 1)) = d;
         if (n == 0) {
@@ -315,12 +316,12 @@ __device__ __forceinline__ int pair_expert(const Mxfp4Args& a, int j) {
     return id >= 0 && id < a.n ? (int)id : -1;
 }
 
-// grid (N / 32, pairs), 512 threads: mx_gateup_few_kernel for one row, which every wave quantises as far as it multiplies it
+// grid (N / 32, pairs), 64 NW threads: mx_gateup_few_kernel for one row, which every wave quantises as far as it multiplies it
 // (512 values a step: eight a lane, four lanes a block, through 272 bytes of LDS into the lanes that hold the blocks).
-template <int XDT>
-__global__ __launch_bounds__(512) void mx_gateup_direct_kernel(Mxfp4Args a) {
-    __shared__ __align__(16) float red[8][4][16];
-    __shared__ __align__(16) uint8_t xq[8][272];
+template <int XDT, int NW>
+__global__ __launch_bounds__(64 * NW, 3) void mx_gateup_direct_kernel(Mxfp4Args a) {
+    __shared__ __align__(16) float red[NW][4][16];
+    __shared__ __align__(16) uint8_t xq[NW][272];
     const int cb = blockIdx.x, j = blockIdx.y;
     const int e = __builtin_amdgcn_readfirstlane(pair_expert(a, j));
     if (e < 0) return;
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(512) void mx_gateup_direct_kernel(Mxfp4Args a) {
         w[t] = few_row(a.w13 + (size_t)e * 2 * a.N * (a.K / 2), a.K / 2, ws, (size_t)(t >> 1) * a.N + cb * 32 + (t & 1) * 16 + c);
     const size_t x0 = (size_t)(j / a.topk) * a.x_stride;
     f32x4 acc[4] = {};
-    for (int b0 = wv * 16; b0 < nblk; b0 += 128) {
+    for (int b0 = wv * 16; b0 < nblk; b0 += 16 * NW) {
         u32x4 wv4[4][4];
         int wsc[4];
 #pragma unroll
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(512) void mx_gateup_direct_kernel(Mxfp4Args a) {
     if (tid >= 32) return;
     float gs = 0.f, us = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NW; ++i) {
         gs += red[i][tid >> 4][tid & 15];
         us += red[i][2 + (tid >> 4)][tid & 15];
     }
@@ -840,12 +841,16 @@ static int run_mx_down(const Mxfp4Args& a, hipStream_t st) {
     return 0;
 }
 
+template <int NW>
+static void run_mx_gateup_direct(const Mxfp4Args& a, hipStream_t st) {
+    const dim3 g(a.N / 32, a.P), d(64 * NW);
+    if (a.xdt == DT_F32) hipLaunchKernelGGL((mx_gateup_direct_kernel<DT_F32, NW>), g, d, 0, st, a);
+    else if (a.xdt == DT_F16) hipLaunchKernelGGL((mx_gateup_direct_kernel<DT_F16, NW>), g, d, 0, st, a);
+    else hipLaunchKernelGGL((mx_gateup_direct_kernel<DT_BF16, NW>), g, d, 0, st, a);
+}
 int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st) {
-    const dim3 g(a.N / 32, a.P), d(512);
-    if (a.xdt == DT_F32) hipLaunchKernelGGL(mx_gateup_direct_kernel<DT_F32>, g, d, 0, st, a);
-    else if (a.xdt == DT_F16) hipLaunchKernelGGL(mx_gateup_direct_kernel<DT_F16>, g, d, 0, st, a);
-    else hipLaunchKernelGGL(mx_gateup_direct_kernel<DT_BF16>, g, d, 0, st, a);
-    hipLaunchKernelGGL(mx_down_direct_kernel, dim3((a.K + 15) / 16, a.T), d, 0, st, a);
+    run_mx_gateup_direct<4>(a, st);
+    hipLaunchKernelGGL(mx_down_direct_kernel, dim3((a.K + 15) / 16, a.T), dim3(512), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
@@ -853,7 +858,7 @@ int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {
     if ((kernels & 1) && launch_mx_quant(a.x, a.xdt, a.x_stride, a.T, a.K, a.qx, a.sx, 1, st)) return -1;
     const bool few = a.seg == MX_FEW;
     if (kernels & 2) {
-        if (few) hipLaunchKernelGGL(mx_gateup_few_kernel, dim3(a.N / 32, a.S_cap), dim3(512), 0, st, a);
+        if (few) hipLaunchKernelGGL(mx_gateup_few_kernel<4>, dim3(a.N / 32, a.S_cap), dim3(256), 0, st, a);
         else if (run_mx_gateup<128, 64, 2, 2, 3>(a, st)) return -1;
     }
     if (kernels & 4) {
