@@ -299,7 +299,9 @@ struct Mxfp4Ws {
     size_t bytes;
 };
 
-// Layout of the MXFP4 path's workspace: route tables, quantised input rows and SwiGLU outputs with their scales, the
+int mxfp4_segments(int64_t P, int64_t n, int seg) { return (int)(std::min(P, n) + (P + seg - 1) / seg); }
+
+// Layout of the MXFP4 path's workspace: route tables (for the shortest segments), quantised input rows and SwiGLU outputs with their scales, the
 // per-pair fp32 contributions.
 void carve_mxfp4(void* ws, int64_t P, int64_t T, int64_t n, int64_t K, int64_t N, Mxfp4Ws& w) {
     Carve c(ws);
@@ -307,16 +309,15 @@ void carve_mxfp4(void* ws, int64_t P, int64_t T, int64_t n, int64_t K, int64_t N
     Mxfp4Args& f = w.fa;
     memset(&r, 0, sizeof(r));
     memset(&f, 0, sizeof(f));
-    f.seg = mxfp4_seg_rows(P, n);
-    f.S_cap = (int)(std::min(P, n) + (P + f.seg - 1) / f.seg);
+    const int segs = mxfp4_segments(P, n, MX_FEW);
     r.tok = c.take<int>(P);
     r.w16 = c.take<uint16_t>(P);
     r.w32 = c.take<float>(P);
     r.pe = c.take<int>(P);
     r.inv = c.take<int>(P);
-    r.seg_expert = c.take<int>(f.S_cap);
-    r.seg_row0 = c.take<int>(f.S_cap);
-    r.seg_rows = c.take<int>(f.S_cap);
+    r.seg_expert = c.take<int>(segs);
+    r.seg_row0 = c.take<int>(segs);
+    r.seg_rows = c.take<int>(segs);
     r.nseg = c.take<int>(1);
     r.counts = c.take<int>(n + 1);
     r.loc = c.take<int>(P);
@@ -1969,7 +1970,8 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
     Mxfp4Ws w;
     carve_mxfp4(workspace, P, T, n, K, N, w);
     if (workspace_bytes < w.bytes) return MI355MOE_EWORKSPACE;
-    if (w.fa.S_cap > 65535) return MI355MOE_ELIMIT;
+    w.fa.seg = mxfp4_seg_rows(local_pairs(P, n, expert_map, n_global), n);
+    w.fa.S_cap = mxfp4_segments(P, n, w.fa.seg);
     RouteArgs& r = w.ra;
     r.ids = ids;
     r.ids64 = ids_dtype == MI355MOE_I64;

@@ -326,7 +326,7 @@ struct Mxfp4Args {
     const int* seg_rows;
     const int* nseg;
     int S_cap;
-    int seg;                // rows per segment (MX_FEW or MX_TILE)
+    int seg;                // rows per segment (mxfp4_seg_rows)
     float limit;
     uint8_t* qx;            // [T][K/2] quantised input rows
     uint8_t* sx;            // their scales, arranged by steps
@@ -348,9 +348,12 @@ struct Mxfp4Args {
     int wdt;
 };
 constexpr int MX_MAX_TOPK = 32;
-constexpr int MX_FEW = 16, MX_TILE = 64;             // rows per segment: streamed weights, LDS tiles
-// Rows per segment of a call of P pairs over n experts: the weights are streamed for segments of few rows.
-constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : MX_TILE; }
+// Rows per segment for P pairs on n local experts: the weights are streamed for segments of few rows, LDS tiles take the
+// others. us with 64- / 128-row tiles (hidden 4096, intermediate 1024, top-8, T = 2047): 288 experts (57 rows each) 530 / 553,
+// 144 (114) 390 / 369, 96 (171) 357 / 348, 36 (455) 310 / 295, 8 (2047) 289 / 264; 36 experts T = 512 (114) 118 / 119. Of
+// 256 rows: 440 at 144 experts, 263 at 8.
+constexpr int MX_FEW = 16, MX_TILE = 64, MX_WIDE = 128;
+constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : P < 96 * n ? MX_TILE : MX_WIDE; }
 // a call whose pairs hardly share experts, in two launches and without a permutation (a.ids, a.wts)
 int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st);
 // kernels: bit 0 quantise inputs, bit 1 gate/up, bit 2 down, bit 3 slot-order combine
