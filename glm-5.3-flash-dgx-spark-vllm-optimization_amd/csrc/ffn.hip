@@ -268,6 +268,7 @@ struct Gemm16Plan {
 };
 static Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
     Gemm16Plan p{256, 1};
+    if (const char* v = getenv("MXT")) { p.tile = atoi(v); p.splits = atoi(getenv("MXS")); return p; }
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
     if (big >= 192) return p;
     p.tile = 128;
@@ -289,7 +290,12 @@ template <int DT, int PL, int QL>
 static int gemm16(Gemm16Args a, hipStream_t st) {
     const Gemm16Plan p = plan_gemm16(a.M, a.N, a.C);
     a.splits = p.splits;
-    const int r = p.tile == 256 ? run_gemm16<DT, PL, QL, 256, 256, 2, 4, 2>(a, st) : run_gemm16<DT, PL, QL, 128, 128, 2, 2, 2>(a, st);
+    const int r = p.tile == 256   ? run_gemm16<DT, PL, QL, 256, 256, 2, 4, 2>(a, st)
+                  : p.tile == 128 ? run_gemm16<DT, PL, QL, 128, 128, 2, 2, 2>(a, st)
+                  : p.tile == 129 ? run_gemm16<DT, PL, QL, 128, 128, 2, 2, 4>(a, st)
+                  : p.tile == 130 ? run_gemm16<DT, PL, QL, 128, 128, 2, 4, 4>(a, st)
+                  : p.tile == 131 ? run_gemm16<DT, PL, QL, 128, 128, 2, 4, 2>(a, st)
+                                  : run_gemm16<DT, PL, QL, 64, 64, 2, 2, 4>(a, st);
     if (r) return r;
     if (p.splits > 1) return launch_join(a.part, p.splits, a.M, a.N, a.out, DT, a.out_stride, st);
     return hipGetLastError() == hipSuccess ? 0 : -1;
@@ -319,7 +325,16 @@ static int gated_forward(const GatedArgs& a, hipStream_t st) {
         hipLaunchKernelGGL(gated_few_kernel<DT>, dim3(a.N / 8, (unsigned)((a.T + 15) / 16)), dim3(1024), 0, st, a);
     } else {
         const int64_t big = ((a.T + 255) / 256) * ((a.N + 127) / 128);
-        const int r = big >= 192 ? run_gated<DT, 256, 256, 2, 4, 2>(a, st) : run_gated<DT, 128, 128, 2, 2, 2>(a, st);
+        int tile = big >= 192 ? 256 : 128;
+        if (const char* v = getenv("GT")) tile = atoi(v);
+        const int r = tile == 256   ? run_gated<DT, 256, 256, 2, 4, 2>(a, st)
+                      : tile == 128 ? run_gated<DT, 128, 128, 2, 2, 2>(a, st)
+                      : tile == 129 ? run_gated<DT, 128, 128, 2, 2, 4>(a, st)
+                      : tile == 130 ? run_gated<DT, 128, 128, 2, 4, 4>(a, st)
+                      : tile == 131 ? run_gated<DT, 128, 128, 2, 4, 2>(a, st)
+                      : tile == 132 ? run_gated<DT, 128, 256, 2, 4, 2>(a, st)
+                      : tile == 133 ? run_gated<DT, 128, 256, 2, 4, 3>(a, st)
+                                    : run_gated<DT, 128, 64, 2, 2, 4>(a, st);
         if (r) return r;
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;

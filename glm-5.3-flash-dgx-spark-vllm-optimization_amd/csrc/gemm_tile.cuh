@@ -101,27 +101,19 @@ struct Stager {
             off[j] = (uint32_t)k * ld + 2u * (uint32_t)min(col, cols - 8);
         }
     }
-    // part I of N of a stage's loads
-    template <int I, int N>
-    __device__ __forceinline__ void issue(unsigned char* st) const {
+    __device__ __forceinline__ void issue(unsigned char* st, int j) const { dma16_base(base, off[j], st + lds + j * 1024); }
+    // from here on the stage being requested is the last one, of which only `valid` chunks (ROW) or rows (COL, of ld bytes)
+    // exist: what lies behind them is loaded from the last one that exists (and cleared in LDS by clear_tail)
+    __device__ __forceinline__ void to_tail(int wv, int lane, int valid, uint32_t ld) {
 #pragma unroll
-        for (int j = INST * I / N; j < INST * (I + 1) / N; ++j) dma16_base(base, off[j], st + lds + j * 1024);
-    }
-    // the last stage, of which only `valid` chunks (ROW) or rows (COL, of ld bytes) exist: what lies behind them is
-    // loaded from the last one that exists (and cleared in LDS by clear_tail)
-    template <int I, int N>
-    __device__ __forceinline__ void issue_tail(unsigned char* st, int wv, int lane, int valid, uint32_t ld) const {
-#pragma unroll
-        for (int j = INST * I / N; j < INST * (I + 1) / N; ++j) {
-            uint32_t o = off[j];
+        for (int j = 0; j < INST; ++j) {
             if constexpr (LAY == LAY_ROW) {
                 const int g = (lane & (CH - 1)) ^ row_swz(place(wv, j, lane) / CH);
-                if (g >= valid) o -= (uint32_t)(g - valid + 1) << 4;
+                if (g >= valid) off[j] -= (uint32_t)(g - valid + 1) << 4;
             } else {
                 const int k = place(wv, j, lane) / (R / 8);
-                if (k >= valid) o -= (uint32_t)(k - valid + 1) * ld;
+                if (k >= valid) off[j] -= (uint32_t)(k - valid + 1) * ld;
             }
-            dma16_base(base, o, st + lds + j * 1024);
         }
     }
     static __device__ __forceinline__ void clear_tail(unsigned char* st, int tid, int valid) {
@@ -184,9 +176,8 @@ struct ScaleStager {
             lds[j] = blk * 256;
         }
     }
-    __device__ __forceinline__ void issue(unsigned char* st, int kb) const {
-#pragma unroll
-        for (int j = 0; j < INST; ++j) dma4(base + min(off[j] + step * (uint32_t)kb, last[j]), st + lds[j]);
+    __device__ __forceinline__ void issue(unsigned char* st, int kb, int j) const {
+        dma4(base + min(off[j] + step * (uint32_t)kb, last[j]), st + lds[j]);
     }
     static __device__ __forceinline__ int read(const unsigned char* st, int r0, int lane) {
         return *reinterpret_cast<const int*>(st + (r0 + (lane & 31)) * 8 + ((lane >> 5) << 2));
@@ -237,29 +228,34 @@ struct GemmTile {
             for (int j = 0; j < TQ; ++j) x.q[j] = XQ::read(st + SCL + BP * 8, q0 + 32 * j, lane);
         }
     }
-    template <int S>
-    __device__ __forceinline__ void multiply(const Frags& f, const Scales& x) {
+    // after(i): called behind the i-th of the step's TP TQ multiplications, in this order
+    template <int S, typename After>
+    __device__ __forceinline__ void multiply(const Frags& f, const Scales& x, const After& after) {
 #pragma unroll
         for (int i = 0; i < TP; ++i)
 #pragma unroll
             for (int j = 0; j < TQ; ++j) {
                 if constexpr (MX) acc[i][j] = mma_mx<S>(f.a[i], f.b[j], acc[i][j], x.p[i], x.q[j]);
                 else acc[i][j] = mma16(std::integral_constant<int, MM>{}, f.a[i], f.b[j], acc[i][j]);
+                // the sums pass through here: otherwise the compiler is free to gather several steps' multiplications
+                asm volatile("" : "+v"(acc[i][j]));
+                after(i * TQ + j);
             }
-        // the sums pass through here: otherwise the compiler is free to gather several steps' multiplications in one place
-#pragma unroll
-        for (int i = 0; i < TP; ++i)
-#pragma unroll
-            for (int j = 0; j < TQ; ++j) asm volatile("" : "+v"(acc[i][j]));
+    }
+    // Load i of the LOADS that stage kb takes (the scales', then P's, then Q's), to `st`.
+    __device__ __forceinline__ void load(unsigned char* st, int kb, int i) const {
+        constexpr int NX = MX ? XP::INST : 0, NY = MX ? NX + XQ::INST : 0;
+        if (i < NX) xp.issue(st + SCL, kb, i);
+        else if (i < NY) xq.issue(st + SCL + BP * 8, kb, i - NX);
+        else if (i < NY + SP::INST) p.issue(st, i - NY);
+        else q.issue(st + QOFF, i - NY - SP::INST);
     }
     // Stages kb0 .. kb1 - 1 of the contraction (kb0 < kb1; p.base and q.base at stage kb0). tail_p / tail_q: what the
     // last one holds of each operand (8-value chunks or MXFP4 blocks for ROW, rows for COL; 0: it is whole). ldp / ldq:
     // row bytes of COL operands. One barrier a stage, before its last step: by then every wave has read the stage's last
     // fragments, so its buffer can be refilled, and the next stage has landed, so its first fragments are read while the
-    // last step multiplies. The refill is issued in halves with the first two steps: issued at once after the barrier it
-    // holds the waves up at the address pipeline while the matrix cores idle, issued later it lands too late (stages of
-    // 256 x 256 x 64 bf16 values, 2048 cycles of multiplication: 2830 cycles at once, 2370 in these halves, 2740 in
-    // quarters over the whole stage).
+    // last step multiplies. The refill's loads are spread over the multiplications of the next stage's first
+    // two steps: issued together they hold the waves up at the address pipeline while the matrix cores idle.
     __device__ __forceinline__ void run(unsigned char* lds, int kb0, int kb1, int tail_p, int tail_q, uint32_t ldp,
                                         uint32_t ldq) {
         const int tid = threadIdx.x, lane = tid & 63;
@@ -270,23 +266,17 @@ struct GemmTile {
 #pragma unroll
             for (int j = 0; j < TQ; ++j) acc[i][j] = f32x16{};
         const uint64_t advp = PL == LAY_ROW ? SB : SB / 2 * (uint64_t)ldp, advq = QL == LAY_ROW ? SB : SB / 2 * (uint64_t)ldq;
-        auto issue = [&](auto I, auto N, unsigned char* st, int kb) {
-            constexpr int i = decltype(I)::value, n = decltype(N)::value;
-            if constexpr (MX && i == 0) {
-                xp.issue(st + SCL, kb);
-                xq.issue(st + SCL + BP * 8, kb);
+        int next = kb0;                                              // the stage that is being requested
+        auto start = [&]() {                                         // before its first load
+            if (next == kb1 - 1 && tail_p) {                         // (uniform)
+                p.to_tail(wv, lane, tail_p, ldp);
+                q.to_tail(wv, lane, tail_q, ldq);
             }
-            if (kb == kb1 - 1 && tail_p) {                           // (uniform)
-                p.template issue_tail<i, n>(st, wv, lane, tail_p, ldp);
-                q.template issue_tail<i, n>(st + QOFF, wv, lane, tail_q, ldq);
-            } else {
-                p.template issue<i, n>(st);
-                q.template issue<i, n>(st + QOFF);
-            }
-            if constexpr (i == n - 1) {
-                p.base += advp;
-                q.base += advq;
-            }
+        };
+        auto done = [&]() {                                          // behind its last one
+            p.base += advp;
+            q.base += advq;
+            ++next;
         };
         // stage kb has landed for every wave, and nobody reads the stage before it any more
         auto arrive = [&](unsigned char* st, int kb) {
@@ -299,49 +289,66 @@ struct GemmTile {
                 __syncthreads();
             }
         };
-        constexpr std::integral_constant<int, 0> first{};
-        constexpr std::integral_constant<int, 1> one{};
-        constexpr std::integral_constant<int, 2> parts{};
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s)
-            if (kb0 + s < kb1) issue(first, one, lds + s * STAGE, kb0 + s);
+            if (next < kb1) {
+                start();
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) load(lds + s * STAGE, next, i);
+                done();
+            }
         Frags f0, f1;
         Scales x0, x1;
+        int cur = 0;
+        unsigned char* fill = lds + (STAGES - 1) * STAGE;            // where the requested stage goes
         arrive(lds, kb0);
-        int cur = 0, next = kb0 + STAGES - 1;                        // the stage that is being requested
-        unsigned char* fill = lds + (STAGES - 1) * STAGE;            // and where it goes
         fetch_scales(lds, p0, q0, lane, x0);
         fetch<0>(lds, p0, q0, lane, f0);
-        // every step but the last: the next one's fragments are read while it multiplies
-        auto first_steps = [&](const unsigned char* st) {
-            auto step = [&](auto S, Frags& now, Frags& then) {
-                constexpr int s = decltype(S)::value;
-                if (s < 2 && next < kb1) issue(std::integral_constant<int, s & 1>{}, parts, fill, next);
-                fetch<s + 1>(st, p0, q0, lane, then);
-                SCHED_FENCE();
-                multiply<s>(now, x0);
-                SCHED_FENCE();
+        auto nothing = [](int) {};
+        // a stage's steps, the next one's fragments read while each multiplies; REQ: with the loads of stage `next`
+        auto stage = [&](auto REQ, auto LAST, int kb) {
+            constexpr bool req = decltype(REQ)::value, last_stage = decltype(LAST)::value;
+            constexpr int M = TP * TQ;
+            const unsigned char* st = lds + cur * STAGE;
+            // loads [LOADS at / (2 M), LOADS (at + 1) / (2 M)) behind multiplication `at` of the window's 2 M
+            auto loads = [&](int at) {
+                if constexpr (req) {
+#pragma unroll
+                    for (int i = LOADS * at / (2 * M); i < LOADS * (at + 1) / (2 * M); ++i) load(fill, next, i);
+                    SCHED_FENCE();
+                }
             };
-            step(first, f0, f1);
-            step(one, f1, f0);
-            step(std::integral_constant<int, 2>{}, f0, f1);
+            if constexpr (req) start();
+            fetch<1>(st, p0, q0, lane, f1);
+            SCHED_FENCE();
+            multiply<0>(f0, x0, [&](int i) { loads(i); });
+            SCHED_FENCE();
+            fetch<2>(st, p0, q0, lane, f0);
+            SCHED_FENCE();
+            multiply<1>(f1, x0, [&](int i) { loads(M + i); });
+            if constexpr (req) done();
+            SCHED_FENCE();
+            fetch<3>(st, p0, q0, lane, f1);
+            SCHED_FENCE();
+            multiply<2>(f0, x0, nothing);
+            SCHED_FENCE();
+            if constexpr (!last_stage) {
+                fill = lds + cur * STAGE;
+                cur = cur + 1 == STAGES ? 0 : cur + 1;
+                unsigned char* nx = lds + cur * STAGE;
+                arrive(nx, kb + 1);
+                fetch_scales(nx, p0, q0, lane, x1);
+                fetch<0>(nx, p0, q0, lane, f0);
+                SCHED_FENCE();
+            }
+            multiply<3>(f1, x0, nothing);
+            SCHED_FENCE();
+            if constexpr (MX && !last_stage) x0 = x1;
         };
-        for (int kb = kb0; kb + 1 < kb1; ++kb) {
-            first_steps(lds + cur * STAGE);
-            fill = lds + cur * STAGE;
-            cur = cur + 1 == STAGES ? 0 : cur + 1;
-            ++next;
-            unsigned char* nx = lds + cur * STAGE;
-            arrive(nx, kb + 1);
-            fetch_scales(nx, p0, q0, lane, x1);
-            fetch<0>(nx, p0, q0, lane, f0);
-            SCHED_FENCE();
-            multiply<3>(f1, x0);
-            SCHED_FENCE();
-            if constexpr (MX) x0 = x1;
-        }
-        first_steps(lds + cur * STAGE);
-        multiply<3>(f1, x0);
+        int kb = kb0;
+        for (; next < kb1; ++kb) stage(std::true_type{}, std::false_type{}, kb);
+        for (; kb + 1 < kb1; ++kb) stage(std::false_type{}, std::false_type{}, kb);
+        stage(std::false_type{}, std::true_type{}, kb);
     }
 
     // Stores TN x 32 columns of 16-bit values (two a dword: value(i, j, r) = columns 8 r + 4 h .. + 3 of column tile i and

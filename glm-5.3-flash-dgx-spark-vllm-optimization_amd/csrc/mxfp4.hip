@@ -780,6 +780,7 @@ MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
     if (p.few) return p;
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
     p.tile = big >= 192 ? 256 : 128;
+    if (const char* v = getenv("MXT")) { p.tile = atoi(v); p.splits = atoi(getenv("MXS")); p.arrange = p.arrange || p.tile == 256; return p; }
     if (p.tile == 256) p.arrange = 1;
     if (p.tile == 128) {
         const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), stages = (K + 255) / 256;
@@ -809,7 +810,10 @@ int launch_mx_matmul(const MxMatmulArgs& a, const MxMatmulPlan& p, hipStream_t s
         else if (nblk > 16) hipLaunchKernelGGL((mx_matmul_few_kernel<1, 2>), grid(64), dim3(512), 0, st, a);
         else hipLaunchKernelGGL((mx_matmul_few_kernel<1, 1>), grid(128), dim3(512), 0, st, a);
     } else {
-        const int r = p.tile == 256 ? run_mx_matmul<256, 256, 2, 4, 2>(a, st) : run_mx_matmul<128, 128, 2, 2, 2>(a, st);
+        const int r = p.tile == 256   ? run_mx_matmul<256, 256, 2, 4, 2>(a, st)
+                      : p.tile == 128 ? run_mx_matmul<128, 128, 2, 2, 2>(a, st)
+                      : p.tile == 129 ? run_mx_matmul<128, 128, 2, 2, 4>(a, st)
+                                      : run_mx_matmul<64, 64, 2, 2, 4>(a, st);
         if (r) return r;
         if (a.splits > 1) launch_join(a.part, a.splits, a.M, a.N, a.out, a.odt, a.out_stride, st);
     }
