@@ -1901,7 +1901,7 @@ int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const v
     if (!a || !a_scale || !w || !w_scale || !out) return MI355MOE_EINVAL;
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w)) & 15) return MI355MOE_EINVAL;
     const MxMatmulPlan p = plan_mx_matmul(M, N, K);
-    if (!p.arrange && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3)) return MI355MOE_EINVAL;
+    if (K % 128 == 0 && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3)) return MI355MOE_EINVAL;
     const int64_t need = mi355moe_mxfp4_matmul_workspace_bytes(M, N, K);
     if (need > 0 && !workspace) return MI355MOE_EINVAL;
     if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;

@@ -266,14 +266,18 @@ constexpr int64_t GATED_FEW_T = 32;                  // tokens up to which the f
 struct Gemm16Plan {
     int tile, splits;
 };
+// By the rule of plan_mx_matmul. us by kind 256 / 128 / 128 deep / 64, dx of 4096 columns from 2048: T = 128 42 / 29 / 20.7 /
+// 20.4, 512 46 / 32 / 24.0 / 22.5, 1791 51 / 41.8 / 47.7 / 61.7, 4096 71 / 83 / 95 / 120. A long contraction of few tiles (128 x
+// 512 x 8192): 36 us, in 4 parts 21.
 static Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
-    Gemm16Plan p{256, 1};
-    if (const char* v = getenv("MXT")) { p.tile = atoi(v); p.splits = atoi(getenv("MXS")); return p; }
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    if (big >= 192) return p;
-    p.tile = 128;
-    const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), stages = (C + 63) / 64;
-    while (p.splits < 16 && tiles * p.splits * 2 <= 512 && stages / (p.splits * 2) >= 4) p.splits *= 2;
+    Gemm16Plan p{TILE_256, 1};
+    auto tiles = [&](int64_t b) { return ((N + b - 1) / b) * ((M + b - 1) / b); };
+    const int64_t t64 = tiles(64), stages = (C + 63) / 64;
+    if (t64 <= 256) {
+        p.tile = TILE_64;
+        while (t64 * p.splits * 2 <= 256 && stages / (p.splits * 2) >= 24) p.splits *= 2;
+    } else if (tiles(128) <= 256) p.tile = TILE_128_DEEP;
+    else if (tiles(256) < 192) p.tile = TILE_128;
     return p;
 }
 
@@ -290,12 +294,10 @@ template <int DT, int PL, int QL>
 static int gemm16(Gemm16Args a, hipStream_t st) {
     const Gemm16Plan p = plan_gemm16(a.M, a.N, a.C);
     a.splits = p.splits;
-    const int r = p.tile == 256   ? run_gemm16<DT, PL, QL, 256, 256, 2, 4, 2>(a, st)
-                  : p.tile == 128 ? run_gemm16<DT, PL, QL, 128, 128, 2, 2, 2>(a, st)
-                  : p.tile == 129 ? run_gemm16<DT, PL, QL, 128, 128, 2, 2, 4>(a, st)
-                  : p.tile == 130 ? run_gemm16<DT, PL, QL, 128, 128, 2, 4, 4>(a, st)
-                  : p.tile == 131 ? run_gemm16<DT, PL, QL, 128, 128, 2, 4, 2>(a, st)
-                                  : run_gemm16<DT, PL, QL, 64, 64, 2, 2, 4>(a, st);
+    const int r = p.tile == TILE_256        ? run_gemm16<DT, PL, QL, 256, 256, 2, 4, 2>(a, st)
+                  : p.tile == TILE_128      ? run_gemm16<DT, PL, QL, 128, 128, 2, 2, 2>(a, st)
+                  : p.tile == TILE_128_DEEP ? run_gemm16<DT, PL, QL, 128, 128, 2, 4, 4>(a, st)
+                                            : run_gemm16<DT, PL, QL, 64, 64, 2, 2, 4>(a, st);
     if (r) return r;
     if (p.splits > 1) return launch_join(a.part, p.splits, a.M, a.N, a.out, DT, a.out_stride, st);
     return hipGetLastError() == hipSuccess ? 0 : -1;
@@ -324,17 +326,14 @@ static int gated_forward(const GatedArgs& a, hipStream_t st) {
     if (a.T <= GATED_FEW_T) {
         hipLaunchKernelGGL(gated_few_kernel<DT>, dim3(a.N / 8, (unsigned)((a.T + 15) / 16)), dim3(1024), 0, st, a);
     } else {
-        const int64_t big = ((a.T + 255) / 256) * ((a.N + 127) / 128);
-        int tile = big >= 192 ? 256 : 128;
-        if (const char* v = getenv("GT")) tile = atoi(v);
-        const int r = tile == 256   ? run_gated<DT, 256, 256, 2, 4, 2>(a, st)
-                      : tile == 128 ? run_gated<DT, 128, 128, 2, 2, 2>(a, st)
-                      : tile == 129 ? run_gated<DT, 128, 128, 2, 2, 4>(a, st)
-                      : tile == 130 ? run_gated<DT, 128, 128, 2, 4, 4>(a, st)
-                      : tile == 131 ? run_gated<DT, 128, 128, 2, 4, 2>(a, st)
-                      : tile == 132 ? run_gated<DT, 128, 256, 2, 4, 2>(a, st)
-                      : tile == 133 ? run_gated<DT, 128, 256, 2, 4, 3>(a, st)
-                                    : run_gated<DT, 128, 64, 2, 2, 4>(a, st);
+        // tiles of n columns (and as many gate as up rows of W13) x b tokens, by the rule of plan_mx_matmul. us by kind 256 /
+        // 128 / 128 deep / 64 (4096 -> 1024): T = 128 72 / 35 / 28 / 23, 512 85 / 49 / 29 / 23, 1791 87 / 52 / 36 / 50, 4096 95 /
+        // 75 / 85 / 108; 8192 (2048 columns) 235 / 272 / 312 / 395
+        auto tiles = [&](int64_t n, int64_t b) { return ((a.N + n - 1) / n) * ((a.T + b - 1) / b); };
+        const int r = tiles(64, 64) <= 256    ? run_gated<DT, 128, 64, 2, 2, 4>(a, st)
+                      : tiles(64, 128) <= 256 ? run_gated<DT, 128, 128, 2, 4, 4>(a, st)
+                      : tiles(128, 256) < 192 ? run_gated<DT, 128, 128, 2, 2, 2>(a, st)
+                                              : run_gated<DT, 256, 256, 2, 4, 2>(a, st);
         if (r) return r;
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;

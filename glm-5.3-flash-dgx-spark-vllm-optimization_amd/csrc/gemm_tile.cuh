@@ -184,21 +184,23 @@ struct ScaleStager {
     }
 };
 
-// One workgroup's product.
-template <int MM_, int PL_, int QL_, int BP_, int BQ_, int WP_, int WQ_, int STAGES_>
+// One workgroup's product. AHEAD (MXFP4): the caller has put the scales of all stages behind the stages, 8 bytes of each P
+// and Q row a stage, before run().
+template <int MM_, int PL_, int QL_, int BP_, int BQ_, int WP_, int WQ_, int STAGES_, bool AHEAD = false>
 struct GemmTile {
     static constexpr int MM = MM_, PL = PL_, QL = QL_, BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STAGES = STAGES_;
     static constexpr int NW = WP * WQ, THREADS = 64 * NW;
     static constexpr int TP = BP / WP / 32, TQ = BQ / WQ / 32;      // 32 x 32 tiles of a wave
     static constexpr bool MX = MM == MM_MX4;
     static constexpr int QOFF = BP * SB, SCL = (BP + BQ) * SB;       // a stage's P rows, Q rows, P scales, Q scales
-    static constexpr int STAGE = SCL + (MX ? (BP + BQ) * 8 : 0), LDS = STAGES * STAGE;
+    static constexpr int XB = MX ? (BP + BQ) * 8 : 0;                // scale bytes of a stage
+    static constexpr int STAGE = SCL + (AHEAD ? 0 : XB), LDS = STAGES * STAGE;
     static constexpr int KSTAGE = MX ? 256 : 64;                     // contraction values of a stage
     using SP = Stager<PL, BP, NW>;
     using SQ = Stager<QL, BQ, NW>;
     using XP = ScaleStager<BP, NW>;
     using XQ = ScaleStager<BQ, NW>;
-    static constexpr int LOADS = SP::INST + SQ::INST + (MX ? XP::INST + XQ::INST : 0);   // of a stage and wave
+    static constexpr int LOADS = SP::INST + SQ::INST + (MX && !AHEAD ? XP::INST + XQ::INST : 0);   // of a stage and wave
 
     SP p;
     SQ q;
@@ -220,12 +222,15 @@ struct GemmTile {
 #pragma unroll
         for (int j = 0; j < TQ; ++j) f.b[j] = fragment<QL, BQ>(st + QOFF, q0 + 32 * j, S, lane);
     }
-    __device__ __forceinline__ void fetch_scales(const unsigned char* st, int p0, int q0, int lane, Scales& x) const {
+    // (st: the stage, the rel-th of those this workgroup multiplies, whose first lies at lds)
+    __device__ __forceinline__ void fetch_scales(const unsigned char* lds, const unsigned char* st, int rel, int p0, int q0,
+                                                 int lane, Scales& x) const {
         if constexpr (MX) {
+            const unsigned char* sc = AHEAD ? lds + LDS + rel * XB : st + SCL;
 #pragma unroll
-            for (int i = 0; i < TP; ++i) x.p[i] = XP::read(st + SCL, p0 + 32 * i, lane);
+            for (int i = 0; i < TP; ++i) x.p[i] = XP::read(sc, p0 + 32 * i, lane);
 #pragma unroll
-            for (int j = 0; j < TQ; ++j) x.q[j] = XQ::read(st + SCL + BP * 8, q0 + 32 * j, lane);
+            for (int j = 0; j < TQ; ++j) x.q[j] = XQ::read(sc + BP * 8, q0 + 32 * j, lane);
         }
     }
     // after(i): called behind the i-th of the step's TP TQ multiplications, in this order
@@ -244,7 +249,7 @@ struct GemmTile {
     }
     // Load i of the LOADS that stage kb takes (the scales', then P's, then Q's), to `st`.
     __device__ __forceinline__ void load(unsigned char* st, int kb, int i) const {
-        constexpr int NX = MX ? XP::INST : 0, NY = MX ? NX + XQ::INST : 0;
+        constexpr int NX = MX && !AHEAD ? XP::INST : 0, NY = MX && !AHEAD ? NX + XQ::INST : 0;
         if (i < NX) xp.issue(st + SCL, kb, i);
         else if (i < NY) xq.issue(st + SCL + BP * 8, kb, i - NX);
         else if (i < NY + SP::INST) p.issue(st, i - NY);
@@ -302,7 +307,7 @@ struct GemmTile {
         int cur = 0;
         unsigned char* fill = lds + (STAGES - 1) * STAGE;            // where the requested stage goes
         arrive(lds, kb0);
-        fetch_scales(lds, p0, q0, lane, x0);
+        fetch_scales(lds, lds, 0, p0, q0, lane, x0);
         fetch<0>(lds, p0, q0, lane, f0);
         auto nothing = [](int) {};
         // a stage's steps, the next one's fragments read while each multiplies; REQ: with the loads of stage `next`
@@ -337,7 +342,7 @@ struct GemmTile {
                 cur = cur + 1 == STAGES ? 0 : cur + 1;
                 unsigned char* nx = lds + cur * STAGE;
                 arrive(nx, kb + 1);
-                fetch_scales(nx, p0, q0, lane, x1);
+                fetch_scales(lds, nx, kb + 1 - kb0, p0, q0, lane, x1);
                 fetch<0>(nx, p0, q0, lane, f0);
                 SCHED_FENCE();
             }

@@ -365,6 +365,9 @@ int launch_mx_dequant(const uint8_t* q, const uint8_t* s, int64_t rows, int K, v
 // scales of `mats` matrices of `rows` rows of nb bytes, each arranged by steps; and of a second matrix (b may be nullptr)
 int launch_mx_arrange(const uint8_t* a, int64_t mats, int64_t rows, uint8_t* ao, const uint8_t* b, int64_t rb, uint8_t* bo, int nb,
                       hipStream_t st);
+// Kinds of workgroup tiles: the largest, 128 x 128 for two workgroups a CU, and three deeply buffered ones for products of
+// at most a workgroup a CU.
+enum TileKind { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_128_64 = 3, TILE_64 = 4 };
 struct MxMatmulPlan {
     int few, tile, splits, arrange;
 };

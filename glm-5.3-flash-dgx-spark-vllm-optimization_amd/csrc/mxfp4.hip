@@ -215,7 +215,7 @@ __device__ __forceinline__ void few_load(const FewRow& r, int b0, int g, int nbl
         const u32x4* p = reinterpret_cast<const u32x4*>(r.q + (size_t)b * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = p[i];
-        sc = *reinterpret_cast<const int*>(r.s + (size_t)(b >> 3) * r.step + (b & 4));
+        sc = (int)*reinterpret_cast<const u32_any*>(r.s + (size_t)(b >> 3) * r.step + (b & 4));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -224,10 +224,11 @@ __device__ __forceinline__ void few_load(const FewRow& r, int b0, int g, int nbl
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[i][j] = ok ? t[j] : 0u;
         }
-        const int last = (nblk - 1) & ~3;
-        const int bl = min(b, last);
-        const int t = *reinterpret_cast<const int*>(r.s + (size_t)(bl >> 3) * r.step + (bl & 4));
-        sc = b <= last ? t : 0x7F7F7F7F;
+        uint32_t c = 0x7F7F7F7Fu;                                    // (rows end at any byte: the last dword in single ones)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (b + i < nblk) c ^= (uint32_t)(r.s[(size_t)(b >> 3) * r.step + (b & 4) + i] ^ 127) << (8 * i);
+        sc = (int)c;
     }
 }
 template <int S>
@@ -511,13 +512,36 @@ __global__ __launch_bounds__(512) void mx_matmul_few_kernel(MxMatmulArgs a) {
 template <int BP, int BQ, int WP, int WQ, int ST>
 using MxTile = GemmTile<MM_MX4, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
 
+constexpr int MX_SCALES_AHEAD_K = 8192;              // contractions whose scales a 64 x 64 tile takes up front (32 KB)
 __device__ __forceinline__ int mx_stages(int K) { return (K + 2 * SB - 1) / (2 * SB); }
 __device__ __forceinline__ int mx_tail(int K) { return K % (2 * SB) / 32; }
 
+// The scales of a tile's rows (row r: tile row min(r, last) of the matrix from row0 on, nb bytes each, at any address) for
+// stages kb0 .. kb1 - 1, into LDS: 8 bytes of row r for stage k at (k - kb0) * step + 8 r, those behind the row's end 127.
+// Published by the barrier before the first stage.
+__device__ __forceinline__ void scales_ahead(const MxScales& s, int64_t row0, int last, int rows, int nb, int kb0, int kb1,
+                                             unsigned char* lds, int step, int threads) {
+    const int n = kb1 - kb0;
+    for (int i = threadIdx.x; i < rows * n; i += threads) {
+        const int r = i / n, k = i - r * n, b = 8 * (kb0 + k);
+        const uint8_t* p = s.p + (size_t)(row0 + min(r, last)) * s.row + b;
+        uint32_t v[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
+        if (b + 8 <= nb) {
+            v[0] = reinterpret_cast<const u32_any*>(p)[0];
+            v[1] = reinterpret_cast<const u32_any*>(p)[1];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (b + j < nb) v[j >> 2] ^= (uint32_t)(p[j] ^ 127) << (8 * (j & 3));
+        }
+        *reinterpret_cast<uint2*>(lds + k * step + 8 * r) = make_uint2(v[0], v[1]);
+    }
+}
+
 // Dense product: workgroup tiles of BP columns x BQ rows, out or (splits > 1) fp32 partials [split][M][N].
-template <int BP, int BQ, int WP, int WQ, int ST>
+template <int BP, int BQ, int WP, int WQ, int ST, bool AHEAD>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void mx_matmul_kernel(MxMatmulArgs a, int nt, int mt) {
-    using G = MxTile<BP, BQ, WP, WQ, ST>;
+    using G = GemmTile<MM_MX4, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST, AHEAD>;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -532,8 +556,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void mx_matmul_kernel(MxMatmulArgs
     G t;
     t.p.init_row(uniform_ptr(a.w + (size_t)n0 * pitch + (size_t)kb0 * SB), wv, lane, [&](int r) { return min(r, pl) * pitch; });
     t.q.init_row(uniform_ptr(a.q + (size_t)m0 * pitch + (size_t)kb0 * SB), wv, lane, [&](int r) { return min(r, ql) * pitch; });
-    t.xp.init(a.ws, n0, (a.K + 127) / 128, wv, lane, [&](int r) { return (uint32_t)min(r, pl); });
-    t.xq.init(a.qs, m0, (a.K + 127) / 128, wv, lane, [&](int r) { return (uint32_t)min(r, ql); });
+    if constexpr (AHEAD) {
+        const int nb = a.K / 32;
+        scales_ahead(a.ws, n0, pl, BP, nb, kb0, kb1, lds + G::LDS, (BP + BQ) * 8, G::THREADS);
+        scales_ahead(a.qs, m0, ql, BQ, nb, kb0, kb1, lds + G::LDS + BP * 8, (BP + BQ) * 8, G::THREADS);
+    } else {
+        t.xp.init(a.ws, n0, (a.K + 127) / 128, wv, lane, [&](int r) { return (uint32_t)min(r, pl); });
+        t.xq.init(a.qs, m0, (a.K + 127) / 128, wv, lane, [&](int r) { return (uint32_t)min(r, ql); });
+    }
     const int tail = kb1 == stages ? mx_tail(a.K) : 0;
     if (kb0 < kb1) t.run(lds, kb0, kb1, tail, tail, 0, 0);
     else
@@ -772,31 +802,42 @@ int launch_join(const float* part, int splits, int64_t M, int N, void* out, int 
 }
 
 static constexpr int64_t MX_FEW_M = 64;              // rows of a dense product up to which weights are streamed
+// The smallest tile that leaves at most one workgroup a CU (its stages deep enough to keep the memory busy), else 128 x 128
+// with two a CU, else 256 x 256 from 192 of them on. us by kind 256 / 128 / 128 deep / 128 x 64 / 64 (N = K = 4096):
+// M = 200 27 / 16.1 / 13.3 / 11.1 / 10.8, 512 29 / 18.3 / 14.7 / 12.4 / 15.9, 1024 30 / 20.9 / 16.9 / 22.8 / 27.3,
+// 2048 32.7 / 28.0 / 30.3 / 42 / 49, 8192 80 / 108 / 124 / - / 184. Long contractions of few tiles are cut (128 x 512 x
+// 32768, 16 tiles: 47 us, in 4 parts 19.5); a cut of fewer than 16 stages costs more than it gains.
 MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
     MxMatmulPlan p{};
     p.few = M <= MX_FEW_M;
     p.splits = 1;
-    p.arrange = K % 128 != 0;                                        // rows whose scales are no whole dwords
     if (p.few) return p;
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.tile = big >= 192 ? 256 : 128;
-    if (const char* v = getenv("MXT")) { p.tile = atoi(v); p.splits = atoi(getenv("MXS")); p.arrange = p.arrange || p.tile == 256; return p; }
-    if (p.tile == 256) p.arrange = 1;
-    if (p.tile == 128) {
-        const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128), stages = (K + 255) / 256;
-        while (p.splits < 8 && tiles * p.splits * 2 <= 512 && stages / (p.splits * 2) >= 2) p.splits *= 2;
-    }
+    auto tiles = [&](int64_t bp, int64_t bq) { return ((N + bp - 1) / bp) * ((M + bq - 1) / bq); };
+    const int64_t stages = (K + 255) / 256, t64 = tiles(64, 64);
+    if (t64 <= 256) {
+        p.tile = TILE_64;
+        while (t64 * p.splits * 2 <= 256 && stages / (p.splits * 2) >= 16) p.splits *= 2;
+    } else if (tiles(128, 64) <= 256) p.tile = TILE_128_64;
+    else if (tiles(128, 128) <= 256) p.tile = TILE_128_DEEP;
+    else if (tiles(256, 256) < 192) p.tile = TILE_128;
+    else p.tile = TILE_256;
+    // scales in an order of their own: for rows of no whole dwords, except where a workgroup reads a tile's scales up front;
+    // and for the largest tiles, which would touch as many lines for their scales as for their codes
+    p.arrange = p.tile == TILE_256 || (K % 128 != 0 && !(p.tile == TILE_64 && K <= MX_SCALES_AHEAD_K));
     return p;
 }
 
-template <int BP, int BQ, int WP, int WQ, int ST>
+template <int BP, int BQ, int WP, int WQ, int ST, bool AHEAD = false>
 static int run_mx_matmul(MxMatmulArgs a, hipStream_t st) {
     a.rows16 = a.splits == 1 && a.odt != DT_F32 && a.N % 8 == 0 && a.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-    using G = MxTile<BP, BQ, WP, WQ, ST>;
-    static const bool ok = allow_lds(mx_matmul_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
+    using G = GemmTile<MM_MX4, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST, AHEAD>;
+    constexpr int most = G::LDS + (AHEAD ? (BP + BQ) * 8 * (MX_SCALES_AHEAD_K / 256) : 0);
+    static const bool ok = allow_lds(mx_matmul_kernel<BP, BQ, WP, WQ, ST, AHEAD>, most);
     if (!ok) return -1;
     const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
-    hipLaunchKernelGGL((mx_matmul_kernel<BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
+    const int per = ((a.K + 255) / 256 + a.splits - 1) / a.splits;
+    const int bytes = G::LDS + (AHEAD ? (BP + BQ) * 8 * per : 0);
+    hipLaunchKernelGGL((mx_matmul_kernel<BP, BQ, WP, WQ, ST, AHEAD>), dim3(nt * mt, a.splits), dim3(G::THREADS), bytes, st, a, nt, mt);
     return 0;
 }
 
@@ -810,10 +851,12 @@ int launch_mx_matmul(const MxMatmulArgs& a, const MxMatmulPlan& p, hipStream_t s
         else if (nblk > 16) hipLaunchKernelGGL((mx_matmul_few_kernel<1, 2>), grid(64), dim3(512), 0, st, a);
         else hipLaunchKernelGGL((mx_matmul_few_kernel<1, 1>), grid(128), dim3(512), 0, st, a);
     } else {
-        const int r = p.tile == 256   ? run_mx_matmul<256, 256, 2, 4, 2>(a, st)
-                      : p.tile == 128 ? run_mx_matmul<128, 128, 2, 2, 2>(a, st)
-                      : p.tile == 129 ? run_mx_matmul<128, 128, 2, 2, 4>(a, st)
-                                      : run_mx_matmul<64, 64, 2, 2, 4>(a, st);
+        const int r = p.tile == TILE_256        ? run_mx_matmul<256, 256, 2, 4, 2>(a, st)
+                      : p.tile == TILE_128      ? run_mx_matmul<128, 128, 2, 2, 2>(a, st)
+                      : p.tile == TILE_128_DEEP ? run_mx_matmul<128, 128, 2, 2, 4>(a, st)
+                      : p.tile == TILE_128_64   ? run_mx_matmul<128, 64, 2, 2, 4>(a, st)
+                      : a.K <= MX_SCALES_AHEAD_K ? run_mx_matmul<64, 64, 2, 2, 4, true>(a, st)
+                                                 : run_mx_matmul<64, 64, 2, 2, 4>(a, st);
         if (r) return r;
         if (a.splits > 1) launch_join(a.part, a.splits, a.M, a.N, a.out, a.odt, a.out_stride, st);
     }

@@ -55,7 +55,9 @@ def test_matmul_refusals(L):
     for k in ("a", "sa", "w", "sw", "out"):
         assert call(**{k: NUL}) == EINVAL
     assert call(a=ODD) == EINVAL and call(w=ODD) == EINVAL and call(K=128, sa=ODD) == EINVAL
-    assert size(4, 8, 64) > 0 and call(ws=NUL) == EINVAL and call(nb=size(4, 8, 64) - 1) == EWORKSPACE
+    big = dict(M=4096, N=1024, K=160, st=1024)             # scales of no whole dwords, large tiles: arranged in the workspace
+    assert size(4096, 1024, 160) > 0 and call(**big, ws=NUL) == EINVAL and call(**big, nb=size(4096, 1024, 160) - 1) == EWORKSPACE
+    assert size(4, 8, 64) == 0 and size(100, 8, 160) == 0
     assert size(4, 8, 128) == 0
     assert call(M=0, a=NUL, out=NUL) == 0
 
