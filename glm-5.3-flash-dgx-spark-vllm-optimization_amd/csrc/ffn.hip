@@ -122,33 +122,25 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gated_kernel(GatedArgs a, int
     const int tail = a.K % (SB / 2) / 8;
     t.run(lds, 0, (a.K + SB / 2 - 1) / (SB / 2), tail, tail, 0, 0);
     const int p0 = (wv % WP) * HALF, q0 = (wv / WP) * (BQ / WQ);
-    // SwiGLU in place of the gate sums, after g and u are kept
+    constexpr int TN = G::TP / 2;
+    const int64_t m1 = m0 + q0, rows = a.T - m1;
+    const int n1 = n0 + p0, cols = a.N - n1;
+    auto exists = [&](int r) { return r < rows; };
+    if (a.gu) {                                                      // (uniform) g and u before the limit
 #pragma unroll
-    for (int j = 0; j < G::TQ; ++j) {
-        const int64_t m = m0 + q0 + 32 * j + (lane & 31);
-#pragma unroll
-        for (int i = 0; i < G::TP / 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
-                f32x4 g, u;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    g[k] = t.acc[i][j][4 * r + k];
-                    u[k] = t.acc[i + G::TP / 2][j][4 * r + k];
-                    t.acc[i][j][4 * r + k] = swiglu(g[k], u[k], a.limit);
-                }
-                if (a.gu && m < a.T && n < a.N) {                    // (N % 8 == 0: four columns exist or none)
-                    *reinterpret_cast<f32x4*>(a.gu + (size_t)m * 2 * a.N + n) = g;
-                    *reinterpret_cast<f32x4*>(a.gu + (size_t)m * 2 * a.N + a.N + n) = u;
-                }
-            }
+        for (int half = 0; half < 2; ++half)
+            t.template store_rows<TN>(lds, a.gu + (size_t)m1 * 2 * a.N + half * a.N + n1, 2 * (int64_t)a.N, cols, exists,
+                                      [&](int i, int j, int r) {
+                                          const f32x16& v = t.acc[half * TN + i][j];
+                                          return f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
+                                      });
     }
-    t.template store_rows16<G::TP / 2>(lds, a.h + (size_t)(m0 + q0) * a.h_stride + n0 + p0, a.h_stride, a.T - m0 - q0,
-                                       a.N - n0 - p0, [&](int i, int j, int r) {
-                                           return pack4(DT, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
-                                                        t.acc[i][j][4 * r + 3]);
-                                       });
+    t.template store_rows<TN>(lds, a.h + (size_t)m1 * a.h_stride + n1, a.h_stride, cols, exists, [&](int i, int j, int r) {
+        float h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = swiglu(t.acc[i][j][4 * r + k], t.acc[TN + i][j][4 * r + k], a.limit);
+        return pack4(DT, h[0], h[1], h[2], h[3]);
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -235,11 +227,12 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, i
             for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
     const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
     if (a.splits == 1) {                                             // (uniform)
-        t.template store_rows16<G::TP>(lds, static_cast<uint16_t*>(a.out) + (size_t)(m0 + q0) * a.out_stride + n0 + p0, a.out_stride,
-                                       a.M - m0 - q0, a.N - n0 - p0, [&](int i, int j, int r) {
-                                           return pack4(DT, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
-                                                        t.acc[i][j][4 * r + 3]);
-                                       });
+        const int64_t rows = a.M - m0 - q0;
+        t.template store_rows<G::TP>(lds, static_cast<uint16_t*>(a.out) + (size_t)(m0 + q0) * a.out_stride + n0 + p0, a.out_stride,
+                                     a.N - n0 - p0, [&](int r) { return r < rows; }, [&](int i, int j, int r) {
+                                         return pack4(DT, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
+                                                      t.acc[i][j][4 * r + 3]);
+                                     });
         return;
     }
     float* part = a.part + (size_t)blockIdx.y * a.M * a.N;

@@ -356,14 +356,16 @@ struct GemmTile {
         stage(std::false_type{}, std::true_type{}, kb);
     }
 
-    // Stores TN x 32 columns of 16-bit values (two a dword: value(i, j, r) = columns 8 r + 4 h .. + 3 of column tile i and
-    // row tile j) in whole rows: through LDS, 32 rows of the wave at a time, 16 bytes a lane and 64 TN bytes a row. `out`
-    // at the wave's first row and column, at 16-byte addresses; rows and cols (a multiple of 8): what exists from there on.
-    // Called by all waves after run(). (8192 x 4096 bf16: 17 us of 8-byte stores straight from the accumulators.)
-    template <int TN, typename V>
-    __device__ __forceinline__ void store_rows16(unsigned char* lds, uint16_t* out, int64_t stride, int64_t rows, int cols,
-                                                 const V& value) const {
-        constexpr int UNITS = TN * 4;                                // 16-byte units of a row
+    // Stores TN x 32 columns of 16-bit (V gives a uint2) or fp32 values (V gives a f32x4) in whole rows: value(i, j, r) =
+    // columns 8 r + 4 h .. + 3 of column tile i and row tile j. Through LDS, 32 rows of the wave at a time, 16 bytes a lane
+    // and whole lines a row. `out` at the wave's first row and column, at 16-byte addresses; cols (a multiple of 8): the
+    // columns that exist from there on; exists(row): whether the wave's row does. Called by all waves after run(). (8192 x
+    // 4096 bf16: 17 us of 8-byte stores straight from the accumulators.)
+    template <int TN, typename T, typename E, typename V>
+    __device__ __forceinline__ void store_rows(unsigned char* lds, T* out, int64_t stride, int cols, const E& exists,
+                                               const V& value) const {
+        constexpr int ES = sizeof(T), UNITS = TN * 2 * ES;           // 16-byte units of a row
+        static_assert(ES == 2 || ES == 4, "");
         const int lane = threadIdx.x & 63, h = lane >> 5;
         const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         unsigned char* mine = lds + wv * (32 * 16 * UNITS);
@@ -372,17 +374,22 @@ struct GemmTile {
 #pragma unroll
         for (int j = 0; j < TQ; ++j) {
             const int m = lane & 31;
+            unsigned char* row = mine + m * (16 * UNITS);
 #pragma unroll
             for (int i = 0; i < TN; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    *reinterpret_cast<uint2*>(mine + m * (16 * UNITS) + (((4 * i + r) ^ (m & (UNITS - 1))) << 4) + 8 * h) = value(i, j, r);
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (ES == 2)
+                        *reinterpret_cast<uint2*>(row + (((4 * i + r) ^ (m & (UNITS - 1))) << 4) + 8 * h) = value(i, j, r);
+                    else *reinterpret_cast<f32x4*>(row + (((8 * i + 2 * r + h) ^ (m & (UNITS - 1))) << 4)) = value(i, j, r);
+                }
             asm volatile("" ::: "memory");                           // (a wave's LDS accesses are performed in order)
 #pragma unroll
             for (int t = 0; t < UNITS / 2; ++t) {
-                const int at = t * 64 + lane, row = at / UNITS, u = at % UNITS;
-                const u32x4 v = *reinterpret_cast<const u32x4*>(mine + row * (16 * UNITS) + ((u ^ (row & (UNITS - 1))) << 4));
-                if (32 * j + row < rows && 8 * u < cols) *reinterpret_cast<u32x4*>(out + (32 * j + row) * stride + 8 * u) = v;
+                const int at = t * 64 + lane, rr = at / UNITS, u = at % UNITS;
+                const u32x4 v = *reinterpret_cast<const u32x4*>(mine + rr * (16 * UNITS) + ((u ^ (rr & (UNITS - 1))) << 4));
+                if (exists(32 * j + rr) && 16 / ES * u < cols)
+                    *reinterpret_cast<u32x4*>(out + (32 * j + rr) * stride + 16 / ES * u) = v;
             }
             asm volatile("" ::: "memory");
         }

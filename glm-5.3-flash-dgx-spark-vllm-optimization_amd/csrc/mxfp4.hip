@@ -521,20 +521,22 @@ __device__ __forceinline__ int mx_tail(int K) { return K % (2 * SB) / 32; }
 // Published by the barrier before the first stage.
 __device__ __forceinline__ void scales_ahead(const MxScales& s, int64_t row0, int last, int rows, int nb, int kb0, int kb1,
                                              unsigned char* lds, int step, int threads) {
-    const int n = kb1 - kb0;
-    for (int i = threadIdx.x; i < rows * n; i += threads) {
-        const int r = i / n, k = i - r * n, b = 8 * (kb0 + k);
-        const uint8_t* p = s.p + (size_t)(row0 + min(r, last)) * s.row + b;
+    // whole stages first, several loads in flight
+    const int n = kb1 - kb0, whole = min(n, nb / 8 - kb0);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * whole; i += threads) {
+        const int r = i / whole, k = i - r * whole;
+        const u32_any* p = reinterpret_cast<const u32_any*>(s.p + (size_t)(row0 + min(r, last)) * s.row + 8 * (kb0 + k));
+        *reinterpret_cast<uint2*>(lds + k * step + 8 * r) = make_uint2(p[0], p[1]);
+    }
+    if (whole == n) return;                                          // (uniform; else the last stage is a partial one)
+    for (int r = threadIdx.x; r < rows; r += threads) {
+        const uint8_t* p = s.p + (size_t)(row0 + min(r, last)) * s.row;
         uint32_t v[2] = {0x7F7F7F7Fu, 0x7F7F7F7Fu};
-        if (b + 8 <= nb) {
-            v[0] = reinterpret_cast<const u32_any*>(p)[0];
-            v[1] = reinterpret_cast<const u32_any*>(p)[1];
-        } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (b + j < nb) v[j >> 2] ^= (uint32_t)(p[j] ^ 127) << (8 * (j & 3));
-        }
-        *reinterpret_cast<uint2*>(lds + k * step + 8 * r) = make_uint2(v[0], v[1]);
+        for (int j = 0; j < 8; ++j)
+            if (8 * whole + 8 * kb0 + j < nb) v[j >> 2] ^= (uint32_t)(p[8 * (kb0 + whole) + j] ^ 127) << (8 * (j & 3));
+        *reinterpret_cast<uint2*>(lds + whole * step + 8 * r) = make_uint2(v[0], v[1]);
     }
 }
 
@@ -573,11 +575,12 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void mx_matmul_kernel(MxMatmulArgs
             for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
     const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
     if (a.rows16) {                                                  // (uniform: 16-bit rows at 16-byte addresses)
-        t.template store_rows16<G::TP>(lds, static_cast<uint16_t*>(a.out) + (size_t)(m0 + q0) * a.out_stride + n0 + p0, a.out_stride,
-                                       a.M - m0 - q0, a.N - n0 - p0, [&](int i, int j, int r) {
-                                           return pack4(a.odt, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
-                                                        t.acc[i][j][4 * r + 3]);
-                                       });
+        const int64_t rows = a.M - m0 - q0;
+        t.template store_rows<G::TP>(lds, static_cast<uint16_t*>(a.out) + (size_t)(m0 + q0) * a.out_stride + n0 + p0, a.out_stride,
+                                     a.N - n0 - p0, [&](int r) { return r < rows; }, [&](int i, int j, int r) {
+                                         return pack4(a.odt, t.acc[i][j][4 * r], t.acc[i][j][4 * r + 1], t.acc[i][j][4 * r + 2],
+                                                      t.acc[i][j][4 * r + 3]);
+                                     });
         return;
     }
     void* out = a.splits > 1 ? static_cast<void*>(a.part + (size_t)blockIdx.y * a.M * a.N) : a.out;
@@ -698,36 +701,21 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void mx_down_kernel(Mxfp4Args a) {
     auto wrow = [&](int r) { return (uint32_t)min(n0 + r, a.K - 1); };
     auto xrow = [&](int r) { return (uint32_t)min(r, rn - 1); };
     const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
-    float rw[G::TQ];
-    int ok[G::TQ];
+    float rw[G::TQ];                                                 // the weights of this lane's rows
 #pragma unroll
-    for (int j = 0; j < G::TQ; ++j) {
-        const int m = q0 + 32 * j + (lane & 31);
-        const int pos = row0 + min(m, rn - 1);
-        rw[j] = a.w32[pos];
-        ok[j] = m < rn && a.pe[pos] >= 0;
-    }
+    for (int j = 0; j < G::TQ; ++j) rw[j] = a.w32[row0 + min(q0 + 32 * j + (lane & 31), rn - 1)];
     G t;
     t.p.init_row(uniform_ptr(a.w2 + (size_t)e * a.K * pitch), wv, lane, [&](int r) { return wrow(r) * pitch; });
     t.q.init_row(uniform_ptr(a.qh + (size_t)row0 * pitch), wv, lane, [&](int r) { return xrow(r) * pitch; });
     t.xp.init(MxScales{a.w2s.p + (size_t)e * a.w2se, a.w2s.row, a.w2s.step}, 0, (a.N + 127) / 128, wv, lane, wrow);
     t.xq.init(MxScales{a.sh, 8, 8u * a.P}, row0, (a.N + 127) / 128, wv, lane, xrow);
     t.run(lds, 0, mx_stages(a.N), mx_tail(a.N), mx_tail(a.N), 0, 0);
-#pragma unroll
-    for (int j = 0; j < G::TQ; ++j) {
-        if (!ok[j]) continue;
-        float* o = a.contrib + (size_t)(row0 + q0 + 32 * j + (lane & 31)) * a.K;
-#pragma unroll
-        for (int i = 0; i < G::TP; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int n = n0 + p0 + 32 * i + 8 * r + 4 * (lane >> 5);
-                if (n < a.K)                                         // (K % 32 == 0)
-                    *reinterpret_cast<f32x4*>(o + n) =
-                        f32x4{rw[j] * t.acc[i][j][4 * r], rw[j] * t.acc[i][j][4 * r + 1], rw[j] * t.acc[i][j][4 * r + 2],
-                               rw[j] * t.acc[i][j][4 * r + 3]};
-            }
-    }
+    // (rows of no valid pair get a value too, which the combine does not read)
+    t.template store_rows<G::TP>(lds, a.contrib + (size_t)(row0 + q0) * a.K + n0 + p0, a.K, a.K - n0 - p0,
+                                 [&](int r) { return q0 + r < rn; }, [&](int i, int j, int r) {
+                                     const f32x16& v = t.acc[i][j];
+                                     return f32x4{rw[j] * v[4 * r], rw[j] * v[4 * r + 1], rw[j] * v[4 * r + 2], rw[j] * v[4 * r + 3]};
+                                 });
 }
 
 // grid (T, ceil(K / 1024)), 256 threads: four columns a thread, a token's valid pairs in slot order (accumulate: added
