@@ -1903,7 +1903,7 @@ int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const v
     const MxMatmulPlan p = plan_mx_matmul(M, N, K);
     if (K % 128 == 0 && ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(w_scale)) & 3)) return MI355MOE_EINVAL;
     const int64_t need = mi355moe_mxfp4_matmul_workspace_bytes(M, N, K);
-    if (need > 0 && !workspace) return MI355MOE_EINVAL;
+    if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MI355MOE_EINVAL;
     if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
     MxMatmulArgs m{};
     m.q = static_cast<const uint8_t*>(a);
@@ -1958,6 +1958,7 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
     if (int r = mxfp4_layer_ok(layer)) return r;
     if (!x || !ids || !weights || !out || !workspace) return MI355MOE_EINVAL;
     if (options & ~MI355MOE_OPT_ACCUMULATE) return MI355MOE_EINVAL;
+    if (!(limit >= 0.0f) || (reinterpret_cast<uintptr_t>(workspace) & 15)) return MI355MOE_EINVAL;
     if (dt_w(x_dtype) < 0 || dt_w(weights_dtype) < 0 || dt_w(out_dtype) < 0) return MI355MOE_EDTYPE;
     if (ids_dtype != MI355MOE_I32 && ids_dtype != MI355MOE_I64) return MI355MOE_EDTYPE;
     const int64_t K = layer->hidden, N = layer->intermediate, n = layer->n;
@@ -2038,6 +2039,7 @@ int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, 
                            int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, hipStream_t stream) {
     if (int r = gated_ok(dtype, T, hidden, intermediate)) return r;
     if (x_stride < hidden || h_stride < intermediate || x_stride > (1 << 22)) return MI355MOE_ESHAPE;
+    if (!(limit >= 0.0f)) return MI355MOE_EINVAL;
     if (T == 0) return 0;
     if (!x || !w13 || !h) return MI355MOE_EINVAL;
     if (!rows16_ok(x, x_stride) || !rows16_ok(w13, hidden) || !rows16_ok(h, h_stride) || (reinterpret_cast<uintptr_t>(gu) & 15))
@@ -2067,6 +2069,7 @@ int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, 
                             void* dw13, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (int r = gated_ok(dtype, T, hidden, intermediate)) return r;
     if (dh_stride < intermediate || x_stride < hidden || x_stride > (1 << 22)) return MI355MOE_ESHAPE;
+    if (!(limit >= 0.0f)) return MI355MOE_EINVAL;
     if (!dx && !dw13) return 0;
     if (T == 0) return dw13 ? MI355MOE_ESHAPE : 0;
     if (!dh || !gu || !x || !w13 || !workspace) return MI355MOE_EINVAL;

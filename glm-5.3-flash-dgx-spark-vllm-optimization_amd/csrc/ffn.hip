@@ -277,8 +277,7 @@ static Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
 template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
 static int run_gemm16(const Gemm16Args& a, hipStream_t st) {
     using G = GemmTile<KindOf<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
-    static const bool ok = allow_lds(gemm16_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>, G::LDS);
-    if (!ok) return -1;
+    if (!allow_lds<gemm16_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
     const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
     hipLaunchKernelGGL((gemm16_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
     return 0;
@@ -307,8 +306,7 @@ int64_t gated_part_floats(int64_t T, int64_t K, int64_t N, bool dx, bool dw) {
 template <int DT, int BP, int BQ, int WP, int WQ, int ST>
 static int run_gated(const GatedArgs& a, hipStream_t st) {
     using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
-    static const bool ok = allow_lds(gated_kernel<DT, BP, BQ, WP, WQ, ST>, G::LDS);
-    if (!ok) return -1;
+    if (!allow_lds<gated_kernel<DT, BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
     const int nt = (a.N + BP / 2 - 1) / (BP / 2), mt = (int)((a.T + BQ - 1) / BQ);
     hipLaunchKernelGGL((gated_kernel<DT, BP, BQ, WP, WQ, ST>), dim3(nt * mt), dim3(G::THREADS), G::LDS, st, a, nt, mt);
     return 0;

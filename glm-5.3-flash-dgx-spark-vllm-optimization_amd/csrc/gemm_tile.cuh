@@ -22,6 +22,8 @@
 //        read touches.
 // Both swizzles are applied through the load addresses.
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 #include "mi355moe_internal.h"
 
@@ -453,10 +455,18 @@ __device__ __forceinline__ int2 tile_order(int id, int nt, int mt) {
     return make_int2(in / rows, 4 * band + in % rows);
 }
 
-// Dynamic LDS beyond 64 KB has to be allowed once per kernel and device.
-template <typename F>
-static bool allow_lds(F* f, int bytes) {
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+// Dynamic LDS beyond 64 KB has to be allowed once per kernel and device (more than 64 devices: every time).
+template <auto Kernel>
+static bool allow_lds(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+        return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
 }  // namespace mi355moe

@@ -820,8 +820,7 @@ static int run_mx_matmul(MxMatmulArgs a, hipStream_t st) {
     a.rows16 = a.splits == 1 && a.odt != DT_F32 && a.N % 8 == 0 && a.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     using G = GemmTile<MM_MX4, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST, AHEAD>;
     constexpr int most = G::LDS + (AHEAD ? (BP + BQ) * 8 * (MX_SCALES_AHEAD_K / 256) : 0);
-    static const bool ok = allow_lds(mx_matmul_kernel<BP, BQ, WP, WQ, ST, AHEAD>, most);
-    if (!ok) return -1;
+    if (!allow_lds<mx_matmul_kernel<BP, BQ, WP, WQ, ST, AHEAD>>(most)) return -1;
     const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
     const int per = ((a.K + 255) / 256 + a.splits - 1) / a.splits;
     const int bytes = G::LDS + (AHEAD ? (BP + BQ) * 8 * per : 0);
@@ -862,16 +861,14 @@ int launch_mx_arrange(const uint8_t* a, int64_t mats, int64_t rows, uint8_t* ao,
 template <int BP, int BQ, int WP, int WQ, int ST>
 static int run_mx_gateup(const Mxfp4Args& a, hipStream_t st) {
     using G = MxTile<BP, BQ, WP, WQ, ST>;
-    static const bool ok = allow_lds(mx_gateup_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
-    if (!ok) return -1;
+    if (!allow_lds<mx_gateup_kernel<BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
     hipLaunchKernelGGL((mx_gateup_kernel<BP, BQ, WP, WQ, ST>), dim3((a.N + BP / 2 - 1) / (BP / 2), a.S_cap), dim3(G::THREADS), G::LDS, st, a);
     return 0;
 }
 template <int BP, int BQ, int WP, int WQ, int ST>
 static int run_mx_down(const Mxfp4Args& a, hipStream_t st) {
     using G = MxTile<BP, BQ, WP, WQ, ST>;
-    static const bool ok = allow_lds(mx_down_kernel<BP, BQ, WP, WQ, ST>, G::LDS);
-    if (!ok) return -1;
+    if (!allow_lds<mx_down_kernel<BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
     hipLaunchKernelGGL((mx_down_kernel<BP, BQ, WP, WQ, ST>), dim3((a.K + BP - 1) / BP, a.S_cap), dim3(G::THREADS), G::LDS, st, a);
     return 0;
 }
@@ -894,7 +891,7 @@ int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {
     const bool few = a.seg == MX_FEW;
     if (kernels & 2) {
         if (few) hipLaunchKernelGGL(mx_gateup_few_kernel<4>, dim3(a.N / 32, a.S_cap), dim3(256), 0, st, a);
-        else if (a.seg == MX_TILE ? run_mx_gateup<128, 64, 2, 2, 2>(a, st) : run_mx_gateup<128, 128, 2, 2, 2>(a, st)) return -1;
+        else if (a.seg == MX_TILE ? run_mx_gateup<128, 64, 2, 2, 3>(a, st) : run_mx_gateup<128, 128, 2, 2, 2>(a, st)) return -1;
     }
     if (kernels & 4) {
         if (few) {
@@ -904,7 +901,7 @@ int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {
             else if (nblk > 32) hipLaunchKernelGGL((mx_down_few_kernel<2, 4>), grid(64), dim3(512), 0, st, a);
             else if (nblk > 16) hipLaunchKernelGGL((mx_down_few_kernel<2, 2>), grid(128), dim3(512), 0, st, a);
             else hipLaunchKernelGGL((mx_down_few_kernel<2, 1>), grid(256), dim3(512), 0, st, a);
-        } else if (a.seg == MX_TILE ? run_mx_down<128, 64, 2, 2, 2>(a, st) : run_mx_down<128, 128, 2, 2, 2>(a, st)) return -1;
+        } else if (a.seg == MX_TILE ? run_mx_down<128, 64, 2, 2, 3>(a, st) : run_mx_down<128, 128, 2, 2, 2>(a, st)) return -1;
     }
     if (kernels & 8) hipLaunchKernelGGL(mx_combine_kernel, dim3(a.T, (a.K + 1023) / 1024), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;

@@ -258,7 +258,6 @@ def fused_experts_mxfp4(hidden: torch.Tensor, w13: torch.Tensor, w2: torch.Tenso
     """apply(hidden, w13, w2, topk_weights, topk_ids, scales) for MXFP4 experts: scales = (w13_scale, w2_scale). Hosts
     that call it often keep an Mxfp4Experts and call moe_forward_ids: this form reads the scales as they are, and arranges
     them in every call where hidden or intermediate is no multiple of 128."""
-    T = hidden.shape[0]
     whole = (2 * w13.shape[-1]) % 128 == 0 and (2 * w2.shape[-1]) % 128 == 0
-    return moe_forward_ids(Mxfp4Experts(w13, scales[0], w2, scales[1], arrange=not whole), hidden, topk_ids.reshape(T, -1),
-                           topk_weights.reshape(T, -1), limit=limit, expert_map=expert_map, out_dtype=hidden.dtype)
+    return moe_forward_ids(Mxfp4Experts(w13, scales[0], w2, scales[1], arrange=not whole), hidden, topk_ids, topk_weights,
+                           limit=limit, expert_map=expert_map, out_dtype=hidden.dtype)

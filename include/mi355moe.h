@@ -448,8 +448,8 @@ int mi355moe_mxfp4_dequant_rows(const void* q, const void* scale, int64_t rows, 
 
 /* out [M][N] (F32, F16 or BF16, row stride out_stride) = A W^T, A [M][K] and W [N][K] in MXFP4 (rows back to back as
  * mi355moe_mxfp4_quant_rows writes them; codes 16-byte aligned, scales 4-byte aligned if K % 128 == 0). K % 32 == 0,
- * K <= 65536; M and N up to 2^20. The products are exact, the sums fp32. The workspace (may be NULL if the size query says 0) needs no
- * initialisation. */
+ * K <= 65536; M and N up to 2^20. The products are exact, the sums fp32. The workspace (may be NULL if the size query says 0) is 16-byte
+ * aligned and needs no initialisation. */
 int64_t mi355moe_mxfp4_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int mi355moe_mxfp4_matmul(const void* a, const void* a_scale, int64_t M, const void* w, const void* w_scale, int64_t N,
                           int64_t K, void* out, int out_dtype, int64_t out_stride, void* workspace, size_t workspace_bytes,
@@ -476,8 +476,8 @@ typedef struct mi355moe_mxfp4_layer {
 /* Routed-expert output of an MXFP4 layer from router ids and weights: z = q(x) W13^T, h = silu(min(g, L)) * clamp(u, -L,
  * L) in fp32 (the limit iff L != 0), y = q(h) W2^T (q: mi355moe_mxfp4_quant_rows' rounding), out[token] = the token's
  * w * y summed in slot order in fp32 (deterministic). Arguments as mi355moe_fp8_moe_forward_ids; options:
- * MI355MOE_OPT_ACCUMULATE (out += the sum, one rounding) or 0. Pairs whose id is no local expert are skipped. The
- * workspace needs no initialisation. T * topk <= 65536. */
+ * MI355MOE_OPT_ACCUMULATE (out += the sum, one rounding) or 0. Pairs whose id is no local expert are skipped. limit >= 0;
+ * the workspace is 16-byte aligned and needs no initialisation. T * topk <= 65536. */
 int64_t mi355moe_mxfp4_moe_workspace_bytes(const mi355moe_mxfp4_layer* layer, int64_t T, int64_t topk);
 int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void* x, int x_dtype, int64_t x_stride,
                                    int64_t T, const void* ids, int ids_dtype, const void* weights, int weights_dtype,

@@ -327,7 +327,7 @@ def test_arranged_scales(cuda):
 
 
 def test_empty_calls(cuda):
-    from mi355moe import mxfp4
+    from mi355moe import fused_experts_mxfp4, mxfp4
     q, s = mxfp4.quant_rows(torch.empty(0, 64, device="cuda"))
     assert q.shape == (0, 32) and s.shape == (0, 2)
     assert mxfp4.dequant_rows(q, s).shape == (0, 64)
@@ -337,6 +337,9 @@ def test_empty_calls(cuda):
     out = mxfp4.moe_forward_ids(ex, torch.empty(0, 64, device="cuda"), torch.empty(0, 2, dtype=torch.int64, device="cuda"),
                                 torch.empty(0, 2, device="cuda"))
     assert out.shape == (0, 64)
+    none = fused_experts_mxfp4(torch.empty(0, 64, device="cuda"), ex.w13, ex.w2, torch.empty(0, 2, device="cuda"),
+                               torch.empty(0, 2, dtype=torch.int64, device="cuda"), (ex.w13_scale, ex.w2_scale))
+    assert none.shape == (0, 64)
 
 
 def test_two_streams_and_two_graphs(cuda):

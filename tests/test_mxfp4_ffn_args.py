@@ -56,6 +56,7 @@ def test_matmul_refusals(L):
         assert call(**{k: NUL}) == EINVAL
     assert call(a=ODD) == EINVAL and call(w=ODD) == EINVAL and call(K=128, sa=ODD) == EINVAL
     big = dict(M=4096, N=1024, K=160, st=1024)             # scales of no whole dwords, large tiles: arranged in the workspace
+    assert call(**big, ws=ODD) == EINVAL
     assert size(4096, 1024, 160) > 0 and call(**big, ws=NUL) == EINVAL and call(**big, nb=size(4096, 1024, 160) - 1) == EWORKSPACE
     assert size(4, 8, 64) == 0 and size(100, 8, 160) == 0
     assert size(4, 8, 128) == 0
@@ -77,8 +78,8 @@ def test_moe_refusals(L):
     f, size = L.mi355moe_mxfp4_moe_forward_ids, L.mi355moe_mxfp4_moe_workspace_bytes
 
     def call(layer=None, x=P, dt=BF16, xs=128, T=4, idt=I32, wdt=F32, topk=2, odt=BF16, os=128, opt=0, ws=P, nb=1 << 40, ng=0,
-             em=NUL):
-        return f(ctypes.byref(layer or _layer()), x, dt, xs, T, P, idt, P, wdt, topk, em, ng, 10.0, P, odt, os, opt, ws, nb, NUL)
+             em=NUL, lim=10.0):
+        return f(ctypes.byref(layer or _layer()), x, dt, xs, T, P, idt, P, wdt, topk, em, ng, lim, P, odt, os, opt, ws, nb, NUL)
 
     assert call(_layer(n=0)) == ELIMIT and call(_layer(n=5000)) == ELIMIT
     assert call(_layer(hidden=48)) == ESHAPE and call(_layer(intermediate=0)) == ESHAPE
@@ -86,6 +87,7 @@ def test_moe_refusals(L):
     assert call(_layer(hidden=96, arranged=0)) == ESHAPE and call(_layer(intermediate=160, arranged=0)) == ESHAPE
     assert call(_layer(w13=NUL)) == EINVAL and call(_layer(w2=ODD)) == EINVAL and call(_layer(w2_scale=ODD)) == EINVAL
     assert call(x=NUL) == EINVAL and call(ws=NUL) == EINVAL and call(opt=2) == EINVAL and call(em=P, ng=-1) == EINVAL
+    assert call(lim=-1.0) == EINVAL and call(lim=float("nan")) == EINVAL and call(ws=ODD) == EINVAL
     assert call(dt=I32) == EDTYPE and call(idt=F32) == EDTYPE and call(wdt=I64) == EDTYPE and call(odt=7) == EDTYPE
     assert call(xs=127) == ESHAPE and call(os=100) == ESHAPE
     assert call(topk=0) == ELIMIT and call(topk=33) == ELIMIT and call(T=40000) == ELIMIT
@@ -106,10 +108,10 @@ def test_arrange_refusals(L):
 def test_gated_refusals(L):
     f = L.mi355moe_gated_forward
 
-    def call(x=P, dt=BF16, T=4, H=64, xs=64, w=P, I=16, h=P, hs=16, gu=NUL):
-        return f(x, dt, T, H, xs, w, I, 10.0, h, hs, gu, NUL)
+    def call(x=P, dt=BF16, T=4, H=64, xs=64, w=P, I=16, h=P, hs=16, gu=NUL, lim=10.0):
+        return f(x, dt, T, H, xs, w, I, lim, h, hs, gu, NUL)
 
-    assert call(dt=F32) == EDTYPE
+    assert call(dt=F32) == EDTYPE and call(lim=-1.0) == EINVAL and call(lim=float("nan")) == EINVAL
     assert call(H=60) == ESHAPE and call(I=12) == ESHAPE and call(T=-1) == ESHAPE and call(xs=56) == ESHAPE and call(hs=8) == ESHAPE
     assert call(T=1 << 25) == ELIMIT and call(H=1 << 17, xs=1 << 17) == ELIMIT
     assert call(x=NUL) == EINVAL and call(w=NUL) == EINVAL and call(h=NUL) == EINVAL
