@@ -39,8 +39,12 @@ __device__ __forceinline__ f32x4 few_mma16(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 // grid (N / 8, ceil(T / 16)), 1024 threads: 8 gate and the same 8 up columns as one 16-row MFMA operand, for 16 tokens.
-// Lane (c = lane % 16, g = lane / 16) holds 64 consecutive bytes of weight row c (128 of the contraction a wave step);
-// the contraction is cut over the sixteen waves, whose sums join in LDS in wave order.
+// Lane (c = lane % 16, g = lane / 16) holds the chunks g, 4 + g, 8 + g, 12 + g of weight row c and of token c, so that a load
+// takes 64 bytes in a row (128 of the contraction a wave step, in the same order on both sides); the contraction is cut over
+// the sixteen waves, whose sums join in LDS in wave order. Bound: the latency of the two or three loads a wave makes and the
+// join (one token, 4096 -> 1024, 16.8 MB of weights: 7.1 us, 2.4 TB/s; 4096 -> 4096: 13.4 us, 5.0 TB/s); more than one group
+// of tokens reads the weights and the tokens through L2 again, 16.8 us at 512 workgroups, all that the card holds at once.
+// Two or four groups a workgroup, which read the weights once: 13.7 us for 32 tokens (9.9 by two workgroups), 21 for 64 (16.8).
 template <int DT>
 __global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
     __shared__ __align__(16) float red[16][256];
@@ -54,19 +58,19 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
     const u32x4* x = reinterpret_cast<const u32x4*>(a.x + (size_t)(m0 + min(c, rows - 1)) * a.x_stride);
     f32x4 acc = {};
     for (int b0 = wv * 16; b0 < chunks; b0 += 256) {
-        const int b = b0 + 4 * g;
+        const int b = b0 + g;
         u32x4 wv4[4], xv4[4];
         if (b0 + 16 <= chunks) {                                     // (uniform)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) wv4[i] = w[b + i];
+            for (int i = 0; i < 4; ++i) wv4[i] = w[b + 4 * i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) xv4[i] = x[b + i];
+            for (int i = 0; i < 4; ++i) xv4[i] = x[b + 4 * i];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool ok = b + i < chunks;
-                wv4[i] = w[min(b + i, chunks - 1)];
-                xv4[i] = x[min(b + i, chunks - 1)];
+                const bool ok = b + 4 * i < chunks;
+                wv4[i] = w[min(b + 4 * i, chunks - 1)];
+                xv4[i] = x[min(b + 4 * i, chunks - 1)];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     wv4[i][j] = ok ? wv4[i][j] : 0u;
@@ -254,7 +258,10 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, i
 
 // ------------------------------------------------------------------------------------------------ launchers
 
-constexpr int64_t GATED_FEW_T = 32;                  // tokens up to which the forward streams the weights
+// The forward streams the weights for one group of 16 tokens, and for more while their workgroups are at most three a CU. us
+// streamed / by tiles, cold weights: 4096 -> 1024, T = 16 9.7 / 26, 64 16.8 / 30, 96 23.5 / 29, 128 30.5 / 29; 4096 -> 4096, 16
+// 18 / 28, 32 31.7 / 29.5; 4096 -> 12288, 1 34 / 44, 16 50 / 45; 2048 -> 768, 128 13.1 / 16.6.
+static bool gated_streams(int64_t T, int64_t N) { return T <= 16 || (T + 15) / 16 * (N / 8) <= 768; }
 
 struct Gemm16Plan {
     int tile, splits;
@@ -314,7 +321,7 @@ static int run_gated(const GatedArgs& a, hipStream_t st) {
 
 template <int DT>
 static int gated_forward(const GatedArgs& a, hipStream_t st) {
-    if (a.T <= GATED_FEW_T) {
+    if (gated_streams(a.T, a.N)) {
         hipLaunchKernelGGL(gated_few_kernel<DT>, dim3(a.N / 8, (unsigned)((a.T + 15) / 16)), dim3(1024), 0, st, a);
     } else {
         // tiles of n columns (and as many gate as up rows of W13) x b tokens, by the rule of plan_mx_matmul. us by kind 256 /

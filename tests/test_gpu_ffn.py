@@ -35,7 +35,8 @@ def _within(got, want, tol, what):
 
 SIZES = [(1, 8, 8, 0.0), (1, 4096, 64, 10.0), (2, 136, 24, 1.0), (16, 512, 40, 2.0), (17, 264, 8, 10.0), (33, 64, 72, 1.0),
          (40, 1000, 200, 3.0), (129, 328, 136, 0.0), (257, 72, 264, 2.0), (300, 640, 8, 10.0), (64, 8, 128, 1.0),
-         (1000, 200, 1032, 2.0), (1300, 1096, 1032, 10.0), (2100, 72, 520, 0.0), (6000, 120, 24, 1.0)]   # every kind of tile
+         (1000, 200, 1032, 2.0), (1300, 1096, 1032, 10.0), (2100, 72, 520, 0.0), (6000, 120, 24, 1.0), (800, 136, 200, 1.0),
+         (1541, 264, 72, 0.0)]                                             # streamed, and every kind of tile
 
 
 @pytest.mark.parametrize("T,H,I,limit", SIZES)
@@ -171,7 +172,7 @@ def test_empty_rows(cuda):
 
 def test_non_finite_rows_stay_apart(cuda):
     from mi355moe import ffn
-    for T in (6, 200):
+    for T in (6, 200, 2100):
         x, w, dh = _inputs(T, 200, 48, torch.bfloat16, 2)
         clean = ffn.gated(x, w, 10.0)
         x[2, 5], x[4, 199] = float("nan"), float("inf")
@@ -189,7 +190,7 @@ def test_captured_forward_and_backward(cuda):
     """The explicit pair captured and replayed with new inputs, eager work between the replays; the differentiable form is
     refused during capture when it would record a gradient, and the capture survives the refusal."""
     from mi355moe import ffn
-    for T in (8, 260):
+    for T in (8, 260, 1600):
         x, w, dh = _inputs(T, 256, 64, torch.bfloat16, 1)
         eager_leaf = x.clone().requires_grad_()
         alive = ffn.gated(eager_leaf, w.clone(), 10.0)       # an eager graph that lives on (w itself is refilled below)
