@@ -789,15 +789,23 @@ int launch_join(const float* part, int splits, int64_t M, int N, void* out, int 
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-static constexpr int64_t MX_FEW_M = 64;              // rows of a dense product up to which weights are streamed
+// Few rows stream the weights: always up to four, up to 16 while the workgroups (16 columns x 16 rows) are at most three a CU,
+// up to 64 at one a CU, since every group of 16 rows reads the weights and its rows through L2 again. us streamed / by tiles,
+// cold weights, K = 4096: N = 1024, M = 16 4.8 / 8.3, 64 4.9 / 8.4; N = 4096, 16 5.3 / 9.4, 32 7.7 / 9.6, 64 12.1 / 10.0; N =
+// 12288, 8 9.0 / 10.1, 16 10.2 / 10.2, 32 16.7 / 10.3; N = 32768, 1 16.8 / 18.2, 16 23.5 / 18.3; N = 131072, 1 52 / 66, 16 80 / 68;
+// 4096 from 16384, 16 12.7 / 14.0, 32 21.4 / 15.7.
+static bool mx_streams(int64_t M, int64_t N) {
+    return M <= 4 || (M <= 64 && (M + 15) / 16 * ((N + 15) / 16) <= (M <= 16 ? 768 : 256));
+}
 // The smallest tile that leaves at most one workgroup a CU (its stages deep enough to keep the memory busy), else 128 x 128
-// with two a CU, else 256 x 256 from 192 of them on. us by kind 256 / 128 / 128 deep / 128 x 64 / 64 (N = K = 4096):
+// with two a CU, else 256 x 256 from 192 of them on (no tile of mostly absent rows: 131072 columns of 4096 for 16 rows 91 us by
+// the largest tiles, 68 by 128 x 64). us by kind 256 / 128 / 128 deep / 128 x 64 / 64 (N = K = 4096):
 // M = 200 27 / 16.1 / 13.3 / 11.1 / 10.8, 512 29 / 18.3 / 14.7 / 12.4 / 15.9, 1024 30 / 20.9 / 16.9 / 22.8 / 27.3,
 // 2048 32.7 / 28.0 / 30.3 / 42 / 49, 8192 80 / 108 / 124 / - / 184. Long contractions of few tiles are cut (128 x 512 x
 // 32768, 16 tiles: 47 us, in 4 parts 19.5); a cut of fewer than 16 stages costs more than it gains.
 MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
     MxMatmulPlan p{};
-    p.few = M <= MX_FEW_M;
+    p.few = mx_streams(M, N);
     p.splits = 1;
     if (p.few) return p;
     auto tiles = [&](int64_t bp, int64_t bq) { return ((N + bp - 1) / bp) * ((M + bq - 1) / bq); };
@@ -805,9 +813,9 @@ MxMatmulPlan plan_mx_matmul(int64_t M, int64_t N, int64_t K) {
     if (t64 <= 256) {
         p.tile = TILE_64;
         while (t64 * p.splits * 2 <= 256 && stages / (p.splits * 2) >= 16) p.splits *= 2;
-    } else if (tiles(128, 64) <= 256) p.tile = TILE_128_64;
+    } else if (tiles(128, 64) <= 256 || M <= 64) p.tile = TILE_128_64;
     else if (tiles(128, 128) <= 256) p.tile = TILE_128_DEEP;
-    else if (tiles(256, 256) < 192) p.tile = TILE_128;
+    else if (tiles(256, 256) < 192 || M <= 128) p.tile = TILE_128;
     else p.tile = TILE_256;
     // scales in an order of their own: for rows of no whole dwords, except where a workgroup reads a tile's scales up front;
     // and for the largest tiles, which would touch as many lines for their scales as for their codes

@@ -110,7 +110,8 @@ def _check_product(a, sa, w, sw, out, K):
 
 SIZES = [(1, 1, 32), (1, 16, 64), (2, 130, 512), (16, 48, 544), (17, 33, 2048), (64, 300, 1056), (65, 129, 96),
          (128, 128, 256), (200, 257, 288), (333, 2050, 2080), (129, 1, 4096), (300, 40, 1024), (70, 64, 8192),
-         (100, 70, 8224), (66, 40, 32768 + 32), (600, 1030, 416), (515, 2049, 992), (1500, 2050, 160), (1100, 2000, 1184)]   # every kind of tile
+         (100, 70, 8224), (66, 40, 32768 + 32), (600, 1030, 416), (515, 2049, 992), (1500, 2050, 160), (1100, 2000, 1184),
+         (33, 2100, 96), (20, 4200, 160), (64, 33000, 64), (5, 12400, 32), (100, 66000, 96), (40, 1100, 16416)]   # every kind of tile
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
