@@ -351,7 +351,7 @@ constexpr int MX_MAX_TOPK = 32;
 // Rows per segment for P pairs on n local experts: the weights are streamed for segments of few rows, LDS tiles take the
 // others. us with 64- / 128-row tiles (hidden 4096, intermediate 1024, top-8, T = 2047): 288 experts (57 rows each) 530 / 553,
 // 144 (114) 390 / 369, 96 (171) 357 / 348, 36 (455) 310 / 295, 8 (2047) 289 / 264; 36 experts T = 512 (114) 118 / 119. Of
-// 256 rows: 440 at 144 experts, 263 at 8.
+// 256 rows: 440 at 144 experts, 263 at 8. (64-row tiles with two stages in LDS; with the three they have, 519 at 57 rows.)
 constexpr int MX_FEW = 16, MX_TILE = 64, MX_WIDE = 128;
 constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : P < 96 * n ? MX_TILE : MX_WIDE; }
 // a call whose pairs hardly share experts, in two launches and without a permutation (a.ids, a.wts)
