@@ -2035,8 +2035,14 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
     return rc_launch(launch_mxfp4(f, stream, 15));
 }
 
+int64_t mi355moe_gated_forward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate) {
+    if (gated_ok(MI355MOE_BF16, T, hidden, intermediate)) return -1;
+    return 4 * gated_forward_floats(T, hidden, intermediate);
+}
+
 int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, int64_t x_stride, const void* w13,
-                           int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, hipStream_t stream) {
+                           int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream) {
     if (int r = gated_ok(dtype, T, hidden, intermediate)) return r;
     if (x_stride < hidden || h_stride < intermediate || x_stride > (1 << 22)) return MI355MOE_ESHAPE;
     if (!(limit >= 0.0f)) return MI355MOE_EINVAL;
@@ -2044,7 +2050,11 @@ int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, 
     if (!x || !w13 || !h) return MI355MOE_EINVAL;
     if (!rows16_ok(x, x_stride) || !rows16_ok(w13, hidden) || !rows16_ok(h, h_stride) || (reinterpret_cast<uintptr_t>(gu) & 15))
         return MI355MOE_EINVAL;
+    const int64_t need = mi355moe_gated_forward_workspace_bytes(T, hidden, intermediate);
+    if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MI355MOE_EINVAL;
+    if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
     GatedArgs g{};
+    g.part = static_cast<float*>(workspace);
     g.dt = dt_act(dtype);
     g.T = T;
     g.K = (int)hidden;

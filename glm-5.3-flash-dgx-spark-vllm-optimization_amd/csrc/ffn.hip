@@ -106,7 +106,7 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
 // Workgroup tiles of BP / 2 columns x BQ tokens; a wave's P rows are its gate columns, then the same up columns, so the SwiGLU
 // is local to a lane. 8192 tokens, 4096 -> 2048, 275 GFLOP with g and u kept: 267 us, 1.03 PFLOP/s (without them 235 us, 1.17; a
 // library product alone takes 218): the matrix cores' power, then 134 MB of fp32 sums. 1791 tokens -> 1024: 36 us, 0.83 PFLOP/s,
-// 240 tiles for 256 CUs. Few tokens: the latency of a stage, 0.33 us whatever the tile (4096 -> 1024 and 97 to 800 tokens: 23 us).
+// 240 tiles for 256 CUs. Few tokens: the latency of a stage, 0.33 us whatever the tile (4096 -> 1024, 400 to 800 tokens: 24 us).
 template <int DT, int BP, int BQ, int WP, int WQ, int ST>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void gated_kernel(GatedArgs a, int nt, int mt) {
     using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
@@ -148,6 +148,39 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gated_kernel(GatedArgs a, int
         for (int k = 0; k < 4; ++k) h[k] = swiglu(t.acc[i][j][4 * r + k], t.acc[TN + i][j][4 * r + k], a.limit);
         return pack4(DT, h[0], h[1], h[2], h[3]);
     });
+}
+
+// h (and gu) from the sums of the contraction's parts [splits][T][2N], added in order: eight columns a thread. Bound: a launch's
+// latency and memory (the parts come mostly from cache).
+template <int DT>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a, int splits) {
+    const int per = a.N / 8;
+    const int64_t items = a.T * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per;
+        const int c = (int)(i - t * per) * 8;
+        const float* p = a.part + (size_t)t * 2 * a.N + c;
+        f32x4 g[2] = {}, u[2] = {};
+        for (int s = 0; s < splits; ++s, p += (size_t)a.T * 2 * a.N) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                g[k] += reinterpret_cast<const f32x4*>(p)[k];
+                u[k] += reinterpret_cast<const f32x4*>(p + a.N)[k];
+            }
+        }
+        u32x4 h;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            h[k] = pack16<DT>(swiglu(g[k >> 1][2 * (k & 1)], u[k >> 1][2 * (k & 1)], a.limit),
+                              swiglu(g[k >> 1][2 * (k & 1) + 1], u[k >> 1][2 * (k & 1) + 1], a.limit));
+        *reinterpret_cast<u32x4*>(a.h + (size_t)t * a.h_stride + c) = h;
+        if (a.gu) {
+            f32x4* o = reinterpret_cast<f32x4*>(a.gu + (size_t)t * 2 * a.N + c);
+            o[0] = g[0], o[1] = g[1];
+            o = reinterpret_cast<f32x4*>(a.gu + (size_t)t * 2 * a.N + a.N + c);
+            o[0] = u[0], o[1] = u[1];
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -264,10 +297,28 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, i
 
 // ------------------------------------------------------------------------------------------------ launchers
 
-// The forward streams the weights for one group of 16 tokens, and for more while their workgroups are at most three a CU. us
-// streamed / by tiles, cold weights: 4096 -> 1024, T = 16 9.7 / 26, 64 16.8 / 30, 96 23.5 / 29, 128 30.5 / 29; 4096 -> 4096, 16
-// 18 / 28, 32 31.7 / 29.5; 4096 -> 12288, 1 34 / 44, 16 50 / 45; 2048 -> 768, 128 13.1 / 16.6.
-static bool gated_streams(int64_t T, int64_t N) { return T <= 16 || (T + 15) / 16 * (N / 8) <= 768; }
+// Parts of the contraction for few 64 x 64 tiles: at least 16 stages each, of at least 48 (a stage takes 0.33 us, the join and its
+// launch 5). us whole / in parts: 4096 -> 1024, 200 tokens (4 parts) 23.8 / 15.8; 8192 -> 512, 200 (4) 42.5 / 15.5; 4096 ->
+// 2048, 128 (2) 23.5 / 15.0; 2048 -> 768, 200 (2) 13.5 / 15.0.
+static int gated_parts(int64_t T, int64_t K, int64_t N) {
+    const int64_t tiles = (2 * N + 63) / 64 * ((T + 63) / 64), stages = (K + 63) / 64;
+    int s = 1;
+    while (stages >= 48 && tiles * s * 2 <= 256 && stages / (s * 2) >= 16) s *= 2;
+    return s;
+}
+// The forward streams the weights for one group of 16 tokens, and for more while their workgroups are at most three a CU, or, where
+// the contraction would be cut, two of 4096 values. us streamed / by tiles, cold weights: 4096 -> 1024, T = 16 9.7 / 26, 64
+// 16.8 / 30, 96 23.5 / 29 (in parts 15), 128 30.5 / 29; 4096 -> 4096, 16 18 / 28, 32 31.7 / 29.5; 4096 -> 12288, 1 34 / 44, 16
+// 50 / 45; 2048 -> 768, 128 13.1 / 16.6; 8192 -> 512, 64 16.6 / 53 (in parts 15.5), 100 31 / 53 (in parts 15.5).
+static bool gated_streams(int64_t T, int64_t K, int64_t N) {
+    const int64_t wgs = (T + 15) / 16 * (N / 8);
+    return T <= 16 || (wgs <= 768 && (wgs * K <= 512 * 4096 || gated_parts(T, K, N) == 1));
+}
+static int gated_splits(int64_t T, int64_t K, int64_t N) { return gated_streams(T, K, N) ? 1 : gated_parts(T, K, N); }
+int64_t gated_forward_floats(int64_t T, int64_t K, int64_t N) {
+    const int s = T > 0 ? gated_splits(T, K, N) : 1;
+    return s > 1 ? s * T * 2 * N : 0;
+}
 
 struct Gemm16Plan {
     int tile, splits;
@@ -327,8 +378,16 @@ static int run_gated(const GatedArgs& a, hipStream_t st) {
 
 template <int DT>
 static int gated_forward(const GatedArgs& a, hipStream_t st) {
-    if (gated_streams(a.T, a.N)) {
+    if (gated_streams(a.T, a.K, a.N)) {
         hipLaunchKernelGGL(gated_few_kernel<DT>, dim3(a.N / 8, (unsigned)((a.T + 15) / 16)), dim3(1024), 0, st, a);
+    } else if (const int splits = gated_splits(a.T, a.K, a.N); splits > 1) {
+        Gemm16Args g{};
+        g.p = a.w13, g.ldp = a.K, g.q = a.x, g.ldq = a.x_stride;
+        g.M = a.T, g.N = 2 * a.N, g.C = a.K, g.part = a.part, g.splits = splits;
+        if (int r = run_gemm16<DT, LAY_ROW, LAY_ROW, 64, 64, 2, 2, 4>(g, st)) return r;
+        if (hipGetLastError() != hipSuccess) return -1;
+        const int64_t items = a.T * (a.N / 8);
+        hipLaunchKernelGGL(gated_join_kernel<DT>, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 8192)), dim3(256), 0, st, a, splits);
     } else {
         // tiles of n columns (and as many gate as up rows of W13) x b tokens, by the rule of plan_mx_matmul. us by kind 256 /
         // 128 / 128 deep / 64 (4096 -> 1024): T = 128 72 / 35 / 28 / 23, 512 85 / 49 / 29 / 23, 1791 87 / 52 / 36 / 50, 4096 95 /

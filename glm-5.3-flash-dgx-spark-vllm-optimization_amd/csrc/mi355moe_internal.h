@@ -408,8 +408,9 @@ struct GatedArgs {
     uint16_t* d;            // [T][2N] gradients of gate and up
     uint16_t* dx;           // [T][K]
     uint16_t* dw;           // [2N][K]
-    float* part;            // split sums (gated_part_floats of them)
+    float* part;            // split sums (gated_forward_floats, gated_part_floats of them)
 };
+int64_t gated_forward_floats(int64_t T, int64_t K, int64_t N);
 int launch_gated_forward(const GatedArgs& a, hipStream_t st);
 // d from gu and dh; then dx (if set) = d W13 and dw (if set) = d^T x
 int launch_gated_backward(const GatedArgs& a, hipStream_t st);

@@ -136,7 +136,8 @@ _SIGS = {
     "mi355moe_mxfp4_moe_workspace_bytes": (_i64, [ctypes.POINTER(Mxfp4LayerDesc), _i64, _i64]),
     "mi355moe_mxfp4_moe_forward_ids": (_int, [ctypes.POINTER(Mxfp4LayerDesc), _c_p, _int, _i64, _i64, _c_p, _int, _c_p,
                                               _int, _i64, _c_p, _i64, _f, _c_p, _int, _i64, _int, _c_p, _sz, _c_p]),
-    "mi355moe_gated_forward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _f, _c_p, _i64, _c_p, _c_p]),
+    "mi355moe_gated_forward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mi355moe_gated_forward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _f, _c_p, _i64, _c_p, _c_p, _sz, _c_p]),
     "mi355moe_gated_backward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "mi355moe_gated_backward": (_int, [_c_p, _i64, _c_p, _c_p, _int, _i64, _i64, _i64, _c_p, _i64, _f, _c_p, _c_p, _c_p,
                                        _sz, _c_p]),

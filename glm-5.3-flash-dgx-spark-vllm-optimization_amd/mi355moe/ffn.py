@@ -2,7 +2,7 @@
 
     [g | u] = x W13^T;  h = silu(min(g, L)) * clamp(u, -L, L)   (the limit iff L != 0)
 
-in fp16 or bf16 with fp32 sums and one rounding: both projections, the activation and the product in one kernel. The
+in fp16 or bf16 with fp32 sums and one rounding: both projections, the activation and the product. The
 shared expert is h W2^T (a plain library product); its output is what the routed experts' `accumulate` adds to.
 
   gated            h, differentiable in x and w13
@@ -14,6 +14,8 @@ fifth of the time that computing them again would, and the gradients carry one r
 Every call runs on the current stream of its tensors' device; scratch comes from torch's caching allocator.
 """
 from __future__ import annotations
+
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -33,6 +35,11 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     if t.stride(1) == 1 and (t.shape[0] <= 1 or (t.shape[1] <= t.stride(0) <= 1 << 22 and t.stride(0) % 8 == 0)) and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=4096)
+def _forward_bytes(T: int, H: int, I: int) -> int:
+    return _lib.lib().mi355moe_gated_forward_workspace_bytes(T, H, I)
 
 
 def _check(x: torch.Tensor, w13: torch.Tensor) -> tuple[torch.device, int]:
@@ -60,8 +67,11 @@ def gated_forward(x: torch.Tensor, w13: torch.Tensor, limit: float = 0.0, save: 
     with _on_device(dev):
         h = x2.new_empty((T, I))
         gu = x2.new_empty((T, 2 * I), dtype=torch.float32) if save else None
+        nb = _forward_bytes(T, H, I)
+        ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
         _lib.check("mi355moe_gated_forward", _lib.lib().mi355moe_gated_forward(
-            _addr(x2), code, T, H, _row_stride(x2), _addr(w), I, float(limit), _addr(h), I, _addr(gu), _raw_stream(dev)))
+            _addr(x2), code, T, H, _row_stride(x2), _addr(w), I, float(limit), _addr(h), I, _addr(gu), _addr(ws), max(nb, 0),
+            _raw_stream(dev)))
     if x.dim() != 2:
         h = h.reshape(*x.shape[:-1], I)
     return (h, gu) if save else h

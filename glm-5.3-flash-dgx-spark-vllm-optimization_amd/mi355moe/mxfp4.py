@@ -224,7 +224,7 @@ def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tens
         raise ValueError(f"x must be [T, {experts.K}], got {tuple(x.shape)}")
     _rows(x)
     T = x.shape[0]
-    if topk_weights.numel() != topk_ids.numel() or topk_ids.shape[0] != T:
+    if topk_ids.dim() not in (1, 2) or topk_ids.shape[0] != T or topk_weights.shape != topk_ids.shape:
         raise ValueError("topk_ids and topk_weights must be [T, k]")
     if accumulate and out is None:
         raise ValueError("accumulate needs out")

@@ -36,7 +36,8 @@ def _within(got, want, tol, what):
 SIZES = [(1, 8, 8, 0.0), (1, 4096, 64, 10.0), (2, 136, 24, 1.0), (16, 512, 40, 2.0), (17, 264, 8, 10.0), (33, 64, 72, 1.0),
          (40, 1000, 200, 3.0), (129, 328, 136, 0.0), (257, 72, 264, 2.0), (300, 640, 8, 10.0), (64, 8, 128, 1.0),
          (1000, 200, 1032, 2.0), (1300, 1096, 1032, 10.0), (2100, 72, 520, 0.0), (6000, 120, 24, 1.0), (800, 136, 200, 1.0),
-         (1541, 264, 72, 0.0)]                                             # streamed, and every kind of tile
+         (200, 2056, 520, 10.0), (97, 4168, 1032, 1.0), (400, 8200, 136, 2.0), (130, 2048, 776, 0.0),
+         (1541, 264, 72, 0.0)]                                             # streamed, every kind of tile, cut contractions
 
 
 @pytest.mark.parametrize("T,H,I,limit", SIZES)

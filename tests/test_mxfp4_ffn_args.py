@@ -108,8 +108,8 @@ def test_arrange_refusals(L):
 def test_gated_refusals(L):
     f = L.mi355moe_gated_forward
 
-    def call(x=P, dt=BF16, T=4, H=64, xs=64, w=P, I=16, h=P, hs=16, gu=NUL, lim=10.0):
-        return f(x, dt, T, H, xs, w, I, lim, h, hs, gu, NUL)
+    def call(x=P, dt=BF16, T=4, H=64, xs=64, w=P, I=16, h=P, hs=16, gu=NUL, lim=10.0, ws=NUL, nb=0):
+        return f(x, dt, T, H, xs, w, I, lim, h, hs, gu, ws, nb, NUL)
 
     assert call(dt=F32) == EDTYPE and call(lim=-1.0) == EINVAL and call(lim=float("nan")) == EINVAL
     assert call(H=60) == ESHAPE and call(I=12) == ESHAPE and call(T=-1) == ESHAPE and call(xs=56) == ESHAPE and call(hs=8) == ESHAPE
@@ -118,6 +118,11 @@ def test_gated_refusals(L):
     assert call(h=ODD) == EINVAL and call(hs=20) == EINVAL
     assert call(x=ODD) == EINVAL and call(w=ODD) == EINVAL and call(xs=68) == EINVAL and call(gu=ODD) == EINVAL
     assert call(T=0, x=NUL) == 0
+    need = L.mi355moe_gated_forward_workspace_bytes        # a cut contraction: fp32 sums of its parts
+    cut = dict(T=120, H=4096, xs=4096, I=1024, hs=1024)
+    nb = need(120, 4096, 1024)
+    assert need(4, 64, 16) == 0 and need(4, 60, 16) == -1 and nb > 0 and need(8192, 4096, 1024) == 0
+    assert call(**cut) == EINVAL and call(**cut, ws=ODD, nb=nb) == EINVAL and call(**cut, ws=P, nb=nb - 1) == EWORKSPACE
     b, size = L.mi355moe_gated_backward, L.mi355moe_gated_backward_workspace_bytes
 
     def back(dh=P, ds=16, gu=P, x=P, dt=BF16, T=4, H=64, xs=64, w=P, I=16, dx=P, dw=P, ws=P, nb=1 << 40):
