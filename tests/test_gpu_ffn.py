@@ -264,3 +264,21 @@ def test_layer_with_shared_expert(cuda, T):
     routed, tol = ref.moe(_f64(x), d13, d2, ids.cpu().numpy(), _f64(wts), 10.0, 0.0)
     total = _f64(shared) + routed
     _within(out, total, tol + np.abs(total) * EPS[dt] / 2 + np.abs(_f64(shared)) * 2.0 ** -22, "layer")
+
+
+def test_rows_beyond_32_bit_offsets(cuda):
+    """More than 2^31 values of h and of [g | u]: the last rows, and their gradients, against float64."""
+    from mi355moe import ffn
+    T, H, I = 1 << 20, 32, 2064
+    x, w, dh = _inputs(T, H, I, torch.bfloat16, 4)
+    h, gu = ffn.gated_forward(x, w, 2.0, save=True)
+    dx, _ = ffn.gated_backward(dh, gu, x, w, 2.0, True, False)
+    W = _f64(w)
+    for lo in (0, T // 2, T - 300):
+        X = _f64(x[lo:lo + 300])
+        want, tol, z, ez = ref.gated(X, W, 2.0, EPS[torch.bfloat16])
+        _within(h[lo:lo + 300], want, tol + TINY[torch.bfloat16], "h")
+        _within(gu[lo:lo + 300], z, ez, "gu")
+        (rx, tx), _ = ref.gated_grads(_f64(dh[lo:lo + 300]), _f64(gu[lo:lo + 300]), X, W, 2.0, EPS[torch.bfloat16],
+                                      TINY[torch.bfloat16])
+        _within(dx[lo:lo + 300], rx, tx, "dx")

@@ -406,3 +406,20 @@ def test_rows_beyond_32_bit_offsets(cuda):
     ids = torch.zeros(3, 1, dtype=torch.int32, device="cuda")
     w = torch.ones(3, 1, device="cuda")
     assert torch.equal(mxfp4.moe_forward_ids(ex, x, ids, w), mxfp4.moe_forward_ids(ex, x.contiguous(), ids, w))
+
+
+def test_outputs_beyond_32_bit_offsets(cuda):
+    """More than 2^31 output values: the last rows against the same rows on their own."""
+    from mi355moe import mxfp4
+    M, N, K = 1 << 20, 2064, 32
+    a, sa = _mx(M, K, 1)
+    w, sw = _mx(N, K, 2)
+    out = mxfp4.matmul(a, sa, w, sw)
+    for lo in (0, M // 2, M - 100):
+        assert torch.equal(out[lo:lo + 100], mxfp4.matmul(a[lo:lo + 100], sa[lo:lo + 100], w, sw))
+    q, s = mxfp4.quant_rows(out)
+    back = mxfp4.dequant_rows(q, s, N)
+    for lo in (0, M // 2, M - 100):
+        q2, s2 = mxfp4.quant_rows(out[lo:lo + 100])
+        assert torch.equal(q[lo:lo + 100], q2) and torch.equal(s[lo:lo + 100], s2)
+        assert torch.equal(back[lo:lo + 100], mxfp4.dequant_rows(q2, s2, N))
