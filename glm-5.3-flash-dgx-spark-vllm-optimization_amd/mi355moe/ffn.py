@@ -42,6 +42,15 @@ def _forward_bytes(T: int, H: int, I: int) -> int:
     return _lib.lib().mi355moe_gated_forward_workspace_bytes(T, H, I)
 
 
+@functools.lru_cache(maxsize=4096)
+def _backward_bytes(T: int, H: int, I: int) -> int:
+    return _lib.lib().mi355moe_gated_backward_workspace_bytes(T, H, I)
+
+
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    return t.detach() if t.requires_grad else t
+
+
 def _check(x: torch.Tensor, w13: torch.Tensor) -> tuple[torch.device, int]:
     dev = _need_cuda(x, w13)
     code = act_dtype_code(x.dtype)
@@ -59,8 +68,7 @@ def gated_forward(x: torch.Tensor, w13: torch.Tensor, limit: float = 0.0, save: 
     W13^T for gated_backward. No gradient is recorded."""
     dev, code = _check(x, w13)
     I, H = w13.shape[0] // 2, w13.shape[1]
-    if x.requires_grad or w13.requires_grad:
-        x, w13 = x.detach(), w13.detach()
+    x, w13 = _plain(x), _plain(w13)
     x2 = _rows16(x if x.dim() == 2 else x.reshape(-1, H))
     w = _rows16(w13) if w13.is_contiguous() else w13.contiguous()
     T = x2.shape[0]
@@ -84,26 +92,27 @@ def gated_backward(dh: torch.Tensor, gu: torch.Tensor, x: torch.Tensor, w13: tor
     dev, code = _check(x, w13)
     _need_cuda(x, dh, gu)
     I, H = w13.shape[0] // 2, w13.shape[1]
-    if dh.dtype != x.dtype or tuple(dh.shape) != (*x.shape[:-1], I):
+    if dh.dtype != x.dtype or dh.shape[:-1] != x.shape[:-1] or dh.shape[-1] != I:
         raise ValueError(f"dh must be {x.dtype} {(*x.shape[:-1], I)}, got {dh.dtype} {tuple(dh.shape)}")
-    x2 = _rows16(x.detach().reshape(-1, H))
+    x2, d2, w = _plain(x), _plain(dh), _plain(w13)
+    if x.dim() != 2:
+        x2, d2 = x2.reshape(-1, H), d2.reshape(-1, I)
     T = x2.shape[0]
     if gu.dtype != torch.float32 or tuple(gu.shape) != (T, 2 * I) or not gu.is_contiguous():
         raise ValueError(f"gu must be contiguous float32 {(T, 2 * I)}, got {gu.dtype} {tuple(gu.shape)}")
-    d2 = _rows16(dh.detach().reshape(-1, I))
-    w = _rows16(w13.detach()) if w13.is_contiguous() else w13.detach().contiguous()
-    L = _lib.lib()
+    x2, d2 = _rows16(x2), _rows16(d2)
+    w = _rows16(w) if w.is_contiguous() else w.contiguous()
     with _on_device(dev):
-        dx = torch.empty(T, H, dtype=x.dtype, device=dev) if need_dx else None
+        dx = x2.new_empty((T, H)) if need_dx else None
         if T == 0:
-            return (dx.reshape(x.shape) if need_dx else None,
-                    torch.zeros(w13.shape, dtype=x.dtype, device=dev) if need_dw13 else None)
-        dw = torch.empty(2 * I, H, dtype=x.dtype, device=dev) if need_dw13 else None
-        ws = torch.empty(L.mi355moe_gated_backward_workspace_bytes(T, H, I), dtype=torch.uint8, device=dev)
-        _lib.check("mi355moe_gated_backward", L.mi355moe_gated_backward(
+            return (dx.reshape(x.shape) if need_dx else None, w.new_zeros(w13.shape) if need_dw13 else None)
+        dw = x2.new_empty((2 * I, H)) if need_dw13 else None
+        nb = _backward_bytes(T, H, I)
+        ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
+        _lib.check("mi355moe_gated_backward", _lib.lib().mi355moe_gated_backward(
             _addr(d2), _row_stride(d2), _addr(gu), _addr(x2), code, T, H, _row_stride(x2), _addr(w), I, float(limit), _addr(dx), _addr(dw),
-            _addr(ws), ws.numel(), _raw_stream(dev)))
-    return (dx.reshape(x.shape) if need_dx else None), dw
+            _addr(ws), max(nb, 0), _raw_stream(dev)))
+    return (dx if dx is None or x.dim() == 2 else dx.reshape(x.shape)), dw
 
 
 class _Gated(torch.autograd.Function):
