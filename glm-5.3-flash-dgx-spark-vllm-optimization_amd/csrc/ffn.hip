@@ -106,7 +106,7 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
 // Workgroup tiles of BP / 2 columns x BQ tokens; a wave's P rows are its gate columns, then the same up columns, so the SwiGLU
 // is local to a lane. 8192 tokens, 4096 -> 2048, 275 GFLOP with g and u kept: 267 us, 1.03 PFLOP/s (without them 235 us, 1.17; a
 // library product alone takes 218): the matrix cores' power, then 134 MB of fp32 sums. 1791 tokens -> 1024: 36 us, 0.83 PFLOP/s,
-// 240 tiles for 256 CUs. Few tokens: the latency of a stage, 0.33 us whatever the tile (4096 -> 1024, 400 to 800 tokens: 24 us).
+// 240 tiles for 256 CUs. Few tokens: the latency of a stage, 0.33 us whatever the tile (4096 -> 1024, 700 tokens: 24 us).
 template <int DT, int BP, int BQ, int WP, int WQ, int ST>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void gated_kernel(GatedArgs a, int nt, int mt) {
     using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
@@ -299,11 +299,13 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, i
 
 // Parts of the contraction for few 64 x 64 tiles: at least 16 stages each, of at least 48 (a stage takes 0.33 us, the join and its
 // launch 5). us whole / in parts: 4096 -> 1024, 200 tokens (4 parts) 23.8 / 15.8; 8192 -> 512, 200 (4) 42.5 / 15.5; 4096 ->
-// 2048, 128 (2) 23.5 / 15.0; 2048 -> 768, 200 (2) 13.5 / 15.0.
+// 2048, 128 (2) 23.5 / 15.0; 2048 -> 768, 200 (2) 13.5 / 15.0. Two parts also where that makes two workgroups a CU, which wait
+// for their stages by turns: 4096 -> 1024, 512 23.7 / 19.9; 5120 -> 1536, 256 28.1 / 22.6; 4096 -> 2048, 300 23.8 / 23.3 (four or
+// eight instead of two or four to that end: 8192 -> 512, 200 tokens 15.0 / 16.4).
 static int gated_parts(int64_t T, int64_t K, int64_t N) {
     const int64_t tiles = (2 * N + 63) / 64 * ((T + 63) / 64), stages = (K + 63) / 64;
     int s = 1;
-    while (stages >= 48 && tiles * s * 2 <= 256 && stages / (s * 2) >= 16) s *= 2;
+    while (stages >= 48 && tiles * s * 2 <= (s == 1 ? 512 : 256) && stages / (s * 2) >= 16) s *= 2;
     return s;
 }
 // The forward streams the weights for one group of 16 tokens, and for more while their workgroups are at most three a CU, or, where
