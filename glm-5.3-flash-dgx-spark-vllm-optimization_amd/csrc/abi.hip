@@ -2071,7 +2071,8 @@ int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, 
 
 int64_t mi355moe_gated_backward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate) {
     if (gated_ok(MI355MOE_BF16, T, hidden, intermediate)) return -1;
-    return (int64_t)align_up(T * 2 * intermediate * 2) + 4 * gated_part_floats(T, hidden, intermediate, true, true);
+    return (int64_t)(align_up(T * 2 * intermediate * 2) + align_up(4 * (GATED_TOPS + 1))) +
+           4 * gated_part_floats(T, hidden, intermediate, true, true);
 }
 
 int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, const void* x, int dtype, int64_t T,
@@ -2102,7 +2103,9 @@ int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, 
     g.d = static_cast<uint16_t*>(workspace);
     g.dx = static_cast<uint16_t*>(dx);
     g.dw = static_cast<uint16_t*>(dw13);
-    g.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(T * 2 * intermediate * 2));
+    g.tops = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + align_up(T * 2 * intermediate * 2));
+    g.unscale = reinterpret_cast<float*>(g.tops + GATED_TOPS);
+    g.part = reinterpret_cast<float*>(reinterpret_cast<char*>(g.tops) + align_up(4 * (GATED_TOPS + 1)));
     return rc_launch(launch_gated_backward(g, stream));
 }
 

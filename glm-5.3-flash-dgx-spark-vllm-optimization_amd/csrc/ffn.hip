@@ -3,7 +3,7 @@
 //   [g | u] = x W13^T (fp32 sums);  h = silu(min(g, L)) clamp(u, -L, L)  (the limit iff L != 0), rounded once
 //   dg = dh u' s (1 + g' (1 - s)) [g <= L],  du = dh g' s [|u| <= L],  s = sigmoid(g'), from the fp32 g and u that the
 //   forward pass keeps;  dx = [dg | du] W13,  dW13 = [dg | du]^T x  (fp32 sums; [dg | du] is rounded once to the operand
-//   type, which the matrix cores take)
+//   type, which the matrix cores take, in fp16 times a power of two that the call's largest value sets)
 //
 // Forward multiplies two operands whose contraction is contiguous; dx has one, and dW13 both, with the contraction as the
 // row index (the tiles' COL layout).
@@ -185,40 +185,94 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedArgs a, int splits
 
 // ------------------------------------------------------------------------------------------------ backward
 
+// dg and du of eight columns of token t, in fp32.
+template <int DT>
+__device__ __forceinline__ void gate_grads(const GatedArgs& a, int64_t t, int c, float (&dg)[8], float (&du)[8]) {
+    const float L = a.limit;
+    const f32x4* gp = reinterpret_cast<const f32x4*>(a.gu + (size_t)t * 2 * a.N + c);
+    const f32x4* up = reinterpret_cast<const f32x4*>(a.gu + (size_t)t * 2 * a.N + a.N + c);
+    const u32x4 dv = *reinterpret_cast<const u32x4*>(a.dh + (size_t)t * a.dh_stride + c);
+    const f32x4 g4[2] = {gp[0], gp[1]}, u4[2] = {up[0], up[1]};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float dh = value16<DT>(dv[j >> 1] >> (16 * (j & 1)));
+        float g = g4[j >> 2][j & 3], u = u4[j >> 2][j & 3];
+        const bool gout = L != 0.0f && g > L, uout = L != 0.0f && fabsf(u) > L;
+        if (L != 0.0f) {
+            g = gout ? L : g;
+            u = uout ? (u > 0.f ? L : -L) : u;
+        }
+        const float s = __fdiv_rn(1.0f, 1.0f + __expf(-g));
+        dg[j] = gout ? 0.0f : dh * u * s * (1.0f + g * (1.0f - s));
+        du[j] = uout ? 0.0f : dh * g * s;
+    }
+}
+
+// The largest finite magnitude of d, as fp32 bits, of each workgroup's share. fp16 only: at dh = 60000 and the layer's limit d
+// reaches 660000, and where dh is small d lies among fp16's subnormals, while the sums over it are ordinary fp16 numbers; d is
+// therefore held times a power of two that goes by this maximum. Bound: memory and the exponentials; 8192 x 2048, 168 MB: 44 us,
+// 3.8 TB/s (of 590 for both gradients); 64 x 1024: 3.6 us.
+template <int DT>
+__global__ __launch_bounds__(256) void gated_top_kernel(GatedArgs a) {
+    __shared__ uint32_t red[4];
+    const int per = a.N / 8;
+    const int64_t items = a.T * per;
+    uint32_t top = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / per;
+        float d[2][8];
+        gate_grads<DT>(a, t, (int)(i - t * per) * 8, d[0], d[1]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, d[j >> 3][j & 7]) & 0x7FFFFFFFu;
+            top = max(top, b < 0x7F800000u ? b : 0u);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) a.tops[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+// 2^k that brings the largest of `n` maxima into [2^14, 2^15) (k between -113 and 120, 0 where all are zero): every thread of the
+// workgroup gets it. An exact factor: d keeps its bits, apart from what it would lose at the ends of fp16's range.
+__device__ __forceinline__ int gated_shift(const uint32_t* tops, int n) {
+    __shared__ uint32_t red[4];
+    uint32_t top = 0;
+    for (int i = threadIdx.x; i < n; i += 256) top = max(top, tops[i]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = max(max(red[0], red[1]), max(red[2], red[3]));
+    return top ? min(14 - ((int)(top >> 23) - 127), 120) : 0;
+}
+__device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast(float, (uint32_t)(127 + k) << 23); }
+
 // d = [dg | du], eight columns a thread. Bound: memory; 8192 x 2048, 235 MB: 35 us, 6.7 TB/s (part of it from cache). Rounded
 // once to the operand type, which the matrix cores take; unrounded, the two products would be fp32 ones, at a tenth of the rate.
+// fp16: times 2^k by the maxima of gated_top_kernel, and 2^-k left for the products.
 template <int DT>
 __global__ __launch_bounds__(256) void gated_d_kernel(GatedArgs a) {
     const int per = a.N / 8;
     const int64_t items = a.T * per;
-    const float L = a.limit;
+    float f = 1.0f;
+    if constexpr (DT == DT_F16) {
+        const int k = gated_shift(a.tops, a.ntops);
+        f = power_of_two(k);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.unscale = power_of_two(-k);
+    }
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
         const int64_t t = i / per;
         const int c = (int)(i - t * per) * 8;
-        const f32x4* gp = reinterpret_cast<const f32x4*>(a.gu + (size_t)t * 2 * a.N + c);
-        const f32x4* up = reinterpret_cast<const f32x4*>(a.gu + (size_t)t * 2 * a.N + a.N + c);
-        const u32x4 dv = *reinterpret_cast<const u32x4*>(a.dh + (size_t)t * a.dh_stride + c);
-        const f32x4 g4[2] = {gp[0], gp[1]}, u4[2] = {up[0], up[1]};
+        float dg[8], du[8];
+        gate_grads<DT>(a, t, c, dg, du);
         u32x4 og, ou;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float dg[2], du[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int j = 2 * k + e;
-                const float dh = value16<DT>(dv[k] >> (16 * e));
-                float g = g4[j >> 2][j & 3], u = u4[j >> 2][j & 3];
-                const bool gout = L != 0.0f && g > L, uout = L != 0.0f && fabsf(u) > L;
-                if (L != 0.0f) {
-                    g = gout ? L : g;
-                    u = uout ? (u > 0.f ? L : -L) : u;
-                }
-                const float s = __fdiv_rn(1.0f, 1.0f + __expf(-g));
-                dg[e] = gout ? 0.0f : dh * u * s * (1.0f + g * (1.0f - s));
-                du[e] = uout ? 0.0f : dh * g * s;
-            }
-            og[k] = pack16<DT>(dg[0], dg[1]);
-            ou[k] = pack16<DT>(du[0], du[1]);
+            og[k] = pack16<DT>(dg[2 * k] * f, dg[2 * k + 1] * f);
+            ou[k] = pack16<DT>(du[2 * k] * f, du[2 * k + 1] * f);
         }
         *reinterpret_cast<u32x4*>(a.d + (size_t)t * 2 * a.N + c) = og;
         *reinterpret_cast<u32x4*>(a.d + (size_t)t * 2 * a.N + a.N + c) = ou;
@@ -236,6 +290,7 @@ struct Gemm16Args {
     int64_t out_stride;
     int splits;
     float* part;
+    const float* unscale;   // fp16: the factor of the sums (nullptr: none)
 };
 
 // out[m][n] = sum over k of P Q, dtype DT, or fp32 partials of the contraction's splits (grid y). Bound: the matrix cores' power
@@ -268,6 +323,14 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, i
         for (int i = 0; i < G::TP; ++i)
 #pragma unroll
             for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
+    if constexpr (DT == DT_F16)
+        if (a.unscale) {                                             // (uniform)
+            const float f = *a.unscale;
+#pragma unroll
+            for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+                for (int j = 0; j < G::TQ; ++j) t.acc[i][j] *= f;
+        }
     const int p0 = (wv % WP) * (BP / WP), q0 = (wv / WP) * (BQ / WQ);
     if (a.splits == 1) {                                             // (uniform)
         const int64_t rows = a.M - m0 - q0;
@@ -408,18 +471,26 @@ int launch_gated_forward(const GatedArgs& a, hipStream_t st) {
 }
 
 template <int DT>
-static int gated_backward(const GatedArgs& a, hipStream_t st) {
+static int gated_backward(GatedArgs a, hipStream_t st) {
     const int64_t items = a.T * (a.N / 8);
+    if constexpr (DT == DT_F16) {
+        a.ntops = (int)std::min<int64_t>((items + 255) / 256, GATED_TOPS);
+        hipLaunchKernelGGL(gated_top_kernel<DT>, dim3(a.ntops), dim3(256), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return -1;
+    }
     hipLaunchKernelGGL(gated_d_kernel<DT>, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 8192)), dim3(256), 0, st, a);
     if (hipGetLastError() != hipSuccess) return -1;
+    const float* unscale = DT == DT_F16 ? a.unscale : nullptr;
     if (a.dx) {
         Gemm16Args g{};
+        g.unscale = unscale;
         g.p = a.w13, g.ldp = a.K, g.q = a.d, g.ldq = 2 * a.N;
         g.M = a.T, g.N = a.K, g.C = 2 * a.N, g.out = a.dx, g.out_stride = a.K, g.part = a.part;
         if (int r = gemm16<DT, LAY_COL, LAY_ROW>(g, st)) return r;
     }
     if (a.dw) {
         Gemm16Args g{};
+        g.unscale = unscale;
         g.p = a.x, g.ldp = a.x_stride, g.q = a.d, g.ldq = 2 * a.N;
         g.M = 2 * a.N, g.N = a.K, g.C = a.T, g.out = a.dw, g.out_stride = a.K, g.part = a.part;
         if (int r = gemm16<DT, LAY_COL, LAY_COL>(g, st)) return r;

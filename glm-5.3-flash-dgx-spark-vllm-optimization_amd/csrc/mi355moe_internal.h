@@ -409,7 +409,11 @@ struct GatedArgs {
     uint16_t* dx;           // [T][K]
     uint16_t* dw;           // [2N][K]
     float* part;            // split sums (gated_forward_floats, gated_part_floats of them)
+    uint32_t* tops;         // fp16: the largest magnitudes of d, GATED_TOPS of them at most (ntops: set by the launcher)
+    int ntops;
+    float* unscale;         // fp16: 2^-k of the power of two that d is held times
 };
+constexpr int GATED_TOPS = 1024;
 int64_t gated_forward_floats(int64_t T, int64_t K, int64_t N);
 int launch_gated_forward(const GatedArgs& a, hipStream_t st);
 // d from gu and dh; then dx (if set) = d W13 and dw (if set) = d^T x

@@ -498,7 +498,8 @@ int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, 
                            int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, void* workspace,
                            size_t workspace_bytes, hipStream_t stream);
 /* Its gradients: with s = sigmoid(g'), g' = min(g, L), u' = clamp(u, -L, L): dg = dh u' s (1 + g' (1 - s)) where g <= L,
- * du = dh g' s where |u| <= L (else 0), both rounded once to dtype; dx [T][hidden] = [dg | du] W13 and dw13
+ * du = dh g' s where |u| <= L (else 0), both rounded once to dtype (in F16 times a power of two that brings the call's
+ * largest into its range: they neither overflow nor vanish where the sums do not); dx [T][hidden] = [dg | du] W13 and dw13
  * [2 * intermediate][hidden] = [dg | du]^T x, fp32 sums rounded once, deterministic. dx or dw13 may be NULL (not
  * computed). T >= 1 if dw13 is asked for. Alignment of dh, dx, dw13 and the workspace as for x. */
 int64_t mi355moe_gated_backward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate);

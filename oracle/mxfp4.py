@@ -123,10 +123,11 @@ def gated(x, w13, L, eps):
     return h, tol * (1 + eps) + np.abs(h) * eps / 2, z, ez
 
 
-def gated_grads(dh, z, x, w13, L, eps, tiny):
+def gated_grads(dh, z, x, w13, L, eps, tiny, tiny_d=None):
     """((dx, bound), (dw13, bound)) from float64 dh [T, I], the forward's z [T, 2I] as the kernel kept it (so masks and
-    factors start from the same numbers), x and w13. d is rounded once to the operand type (eps; tiny: its smallest
-    step), the sums once more."""
+    factors start from the same numbers), x and w13. d is rounded once to the operand type (eps; tiny_d: the smallest step
+    it has there), the sums once more (tiny: the output type's smallest step, and d's unless tiny_d is given). z is finite."""
+    tiny_d = tiny if tiny_d is None else tiny_d
     I = w13.shape[0] // 2
     g, u = z[:, :I], z[:, I:]
     mg, mu = (g <= L, np.abs(u) <= L) if L else (np.ones_like(g), np.ones_like(u))
@@ -137,7 +138,7 @@ def gated_grads(dh, z, x, w13, L, eps, tiny):
     # fp32 evaluation: s within (|g| + 4) 2^-23 relative; 1 + g (1 - s) within that of 1 + |g|
     e = (np.abs(g) + 10) * 2.0 ** -23
     ed = np.concatenate([np.abs(dh * u * s) * (1 + np.abs(g)) * mg * 2 * e, np.abs(du) * e], -1)
-    ed = ed + (np.abs(d) + ed) * eps / 2 + tiny
+    ed = ed + (np.abs(d) + ed) * eps / 2 + tiny_d
     res = []
     for a, ea, b, K in ((d, ed, w13, 2 * I), (d.T, ed.T, x, x.shape[0])):
         v = a @ b
