@@ -25,11 +25,14 @@ from .ops import _addr, _capturing, _need_cuda, _on_device, _raw_stream, act_dty
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    """Values between two rows of t. One row (or none) has none: its stride(0) can be anything, also in what torch calls
+    contiguous."""
+    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t [rows, K] itself where its rows lie apart at 16-byte addresses, else a contiguous copy."""
+    """t [rows, K] itself where its rows lie apart at 16-byte addresses, at most 2^22 values from one to the next, else a
+    contiguous copy."""
     if t.is_contiguous() and t.shape[1] % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
     if t.stride(1) == 1 and (t.shape[0] <= 1 or (t.shape[1] <= t.stride(0) <= 1 << 22 and t.stride(0) % 8 == 0)) and t.data_ptr() % 16 == 0:
