@@ -21,7 +21,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _addr, _capturing, _need_cuda, _on_device, _raw_stream, act_dtype_code
+from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _raw_stream, act_dtype_code
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -56,6 +56,7 @@ def _plain(t: torch.Tensor) -> torch.Tensor:
 
 def _check(x: torch.Tensor, w13: torch.Tensor) -> tuple[torch.device, int]:
     dev = _need_cuda(x, w13)
+    _no_tangents("the gated block", x, w13)
     code = act_dtype_code(x.dtype)
     if w13.dtype != x.dtype:
         raise ValueError(f"x is {x.dtype}, w13 {w13.dtype}")
@@ -94,6 +95,7 @@ def gated_backward(dh: torch.Tensor, gu: torch.Tensor, x: torch.Tensor, w13: tor
     Each gradient is a fp32 sum over [dg | du] rounded to x's dtype; the sums' order does not vary."""
     dev, code = _check(x, w13)
     _need_cuda(x, dh, gu)
+    _no_tangents("the gated block's backward", dh, gu)
     I, H = w13.shape[0] // 2, w13.shape[1]
     if dh.dtype != x.dtype or dh.shape[:-1] != x.shape[:-1] or dh.shape[-1] != I:
         raise ValueError(f"dh must be {x.dtype} {(*x.shape[:-1], I)}, got {dh.dtype} {tuple(dh.shape)}")
@@ -135,9 +137,10 @@ class _Gated(torch.autograd.Function):
 
 
 def gated(x: torch.Tensor, w13: torch.Tensor, limit: float = 0.0) -> torch.Tensor:
-    """h [..., I] = silu(min(g, L)) * clamp(u, -L, L) of x [..., H] and w13 [2I, H], differentiable once in x and w13.
-    While a graph is captured, a call that would record a gradient is refused: torch's autograd does not keep an eager
-    graph of the same leaves apart from a captured one; capture gated_forward(save=True) and gated_backward instead."""
+    """h [..., I] = silu(min(g, L)) * clamp(u, -L, L) of x [..., H] and w13 [2I, H], differentiable once in x and w13
+    by reverse mode (forward-mode derivatives are refused). While a graph is captured, a call that would record a gradient is
+    refused: torch's autograd does not keep an eager graph of the same leaves apart from a captured one; capture
+    gated_forward(save=True) and gated_backward instead."""
     if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad):
         dev, _ = _check(x, w13)
         if _capturing(dev):

@@ -11,6 +11,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .layer import Exl3Experts
@@ -56,6 +57,16 @@ def _need_cuda(*ts: torch.Tensor) -> torch.device:
         elif t.device != dev:
             raise ValueError(f"mi355moe: tensors on {t.device} and {dev}")
     return dev
+
+
+def _no_tangents(what: str, *ts: torch.Tensor | None) -> None:
+    """Refuses tensors that carry a forward-mode derivative: the kernels read their values alone, and the result would come
+    without its derivative. (Such a tensor has requires_grad False, under torch.no_grad too.)"""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"mi355moe: {what} has no forward-mode derivative; call it on "
+                                   "torch.autograd.forward_ad.unpack_dual(x).primal")
 
 
 def act_dtype_code(dt: torch.dtype) -> int:
