@@ -10,6 +10,9 @@ codes (2^(code - 127); 255 = NaN), the layout of MXFP4 checkpoints.
   moe_forward_ids             routed output from router ids and weights, activations quantised per block of 32
   fused_experts_mxfp4         the functional form apply(hidden, w13, w2, topk_weights, topk_ids, scales)
 
+Nothing here has a gradient. Codes carry none; the routed output of an x or topk_weights that needs one raises in the backward
+pass, and an `out` that autograd would lose track of is refused.
+
 Every call runs on the current stream of its tensors' device. Scratch comes from torch's caching allocator call by call
 (a captured call's from its graph's own pool), so calls on several streams, and graphs replayed side by side, share none.
 """
@@ -19,9 +22,10 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
-from .ops import _addr, _need_cuda, _on_device, _raw_stream, ids_dtype_code, weight_dtype_code
+from .ops import _addr, _need_cuda, _no_tangents, _on_device, _raw_stream, ids_dtype_code, weight_dtype_code
 
 BLOCK = 32
 SCALE_NAN = 255
@@ -46,6 +50,39 @@ def _rows(x: torch.Tensor, name: str = "x") -> torch.Tensor:
     if (x.stride(1) != 1 and x.shape[1] > 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         raise ValueError(f"{name} must have unit column stride and rows that do not overlap, got strides {x.stride()}")
     return x
+
+
+def _may_write(out: torch.Tensor, what: str, adds: bool, *inputs: torch.Tensor) -> None:
+    """Refuses an `out` whose gradient a call that writes through its address would falsify: one that is overwritten or a leaf (or
+    a view of one) where it needs a gradient itself, and any where the inputs do. What is added to an intermediate result leaves its gradient
+    as it is."""
+    _no_tangents(what, out, *inputs)
+    if torch.is_grad_enabled():
+        if any(t.requires_grad for t in inputs):
+            raise RuntimeError(f"mi355moe: {what} with out= has no gradient, but an input needs one; pass detached inputs, or "
+                               "call it under torch.no_grad()")
+        if out.requires_grad and (not adds or (out if out._base is None else out._base).is_leaf):
+            raise RuntimeError(f"mi355moe: {what} writes out, which needs a gradient; pass out.detach(), or call it under "
+                               "torch.no_grad()")
+
+
+class _NoGradient(torch.autograd.Function):
+    """A finished result as an output of inputs that need gradients: the backward pass raises in place of losing them."""
+
+    @staticmethod
+    def forward(ctx, out, what, *inputs):
+        ctx.what = what
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError(f"mi355moe: {ctx.what} has no gradient; pass x.detach() and topk_weights.detach() where that is meant")
+
+
+def _without_gradient(out: torch.Tensor, what: str, *inputs: torch.Tensor) -> torch.Tensor:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+        return _NoGradient.apply(out, what, *inputs)
+    return out
 
 
 def quant_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -107,7 +144,10 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     for name, t, shape in (("a_scale", a_scale, (M, K // BLOCK)), ("w", w, (N, K // 2)), ("w_scale", w_scale, (N, K // BLOCK))):
         if tuple(t.shape) != shape:
             raise ValueError(f"{name}: expected {shape}, got {tuple(t.shape)}")
-    if out is None:
+    given = out is not None
+    if given:
+        _may_write(out, "mxfp4.matmul", False)
+    else:
         out = a.new_empty((M, N), dtype=out_dtype)
     dt = weight_dtype_code(out.dtype)
     if tuple(out.shape) != (M, N):
@@ -125,6 +165,8 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
         ws = a.new_empty(nb) if nb else None
         _lib.check("mi355moe_mxfp4_matmul", L.mi355moe_mxfp4_matmul(
             _addr(a), _addr(a_scale), M, _addr(w), _addr(w_scale), N, K, _addr(out), dt, _row_stride(out), _addr(ws), nb, _raw_stream(dev)))
+    if given:
+        increment_version(out)
     return out
 
 
@@ -216,7 +258,9 @@ def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tens
     """Routed-expert output [T, H] in x's dtype (unless out / out_dtype say otherwise). x: fp32, fp16 or bf16 [T, H];
     topk_ids int32/int64 [T, k] (global ids; expert_map maps them to local ids or -1; pairs of no local expert are
     skipped); topk_weights [T, k] (already scaled by the router). accumulate: out, which then has to be given, += the
-    routed sum with one rounding (out holds the shared expert's output)."""
+    routed sum with one rounding (out holds the shared expert's output, and may be an intermediate result of autograd's: its
+    own gradient passes through). The routed experts have no gradient: where x or topk_weights need one, out is refused and
+    the result's backward raises; pass detached ones."""
     dev = _need_cuda(x, topk_ids, topk_weights, expert_map, out)
     if dev != experts.device:
         raise ValueError(f"activations on {dev}, experts on {experts.device}")
@@ -228,7 +272,11 @@ def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tens
         raise ValueError("topk_ids and topk_weights must be [T, k]")
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
-    if out is None:
+    given = out is not None
+    if given:
+        _may_write(out, "mxfp4.moe_forward_ids", accumulate, x, topk_weights)
+    else:
+        _no_tangents("mxfp4.moe_forward_ids", x, topk_weights)
         out = x.new_empty((T, experts.K), dtype=out_dtype or x.dtype)
     if tuple(out.shape) != (T, experts.K):
         raise ValueError(f"out must be [T, {experts.K}], got {tuple(out.shape)}")
@@ -249,7 +297,10 @@ def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tens
             ctypes.byref(experts.desc), _addr(x), xdt, _row_stride(x), T, _addr(ids), ids_dtype_code(ids.dtype), _addr(w),
             weight_dtype_code(w.dtype), topk, _addr(em), 0 if em is None else em.numel(), float(limit), _addr(out), odt,
             _row_stride(out), _lib.OPT_ACCUMULATE if accumulate else 0, _addr(ws), ws.numel(), _raw_stream(dev)))
-    return out
+    if given:
+        increment_version(out)
+        return out
+    return _without_gradient(out, "mxfp4.moe_forward_ids", x, topk_weights)
 
 
 def fused_experts_mxfp4(hidden: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor,
