@@ -420,8 +420,9 @@ static int gemm16(Gemm16Args a, hipStream_t st) {
                   : p.tile == TILE_128_DEEP ? run_gemm16<DT, PL, QL, 128, 128, 2, 4, 4>(a, st)
                                             : run_gemm16<DT, PL, QL, 64, 64, 2, 2, 4>(a, st);
     if (r) return r;
+    if (hipGetLastError() != hipSuccess) return -1;
     if (p.splits > 1) return launch_join(a.part, p.splits, a.M, a.N, a.out, DT, a.out_stride, st);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return 0;
 }
 
 int64_t gated_part_floats(int64_t T, int64_t K, int64_t N, bool dx, bool dw) {

@@ -869,7 +869,10 @@ int launch_mx_matmul(const MxMatmulArgs& a, const MxMatmulPlan& p, hipStream_t s
                       : a.K <= MX_SCALES_AHEAD_K ? run_mx_matmul<64, 64, 2, 2, 4, true>(a, st)
                                                  : run_mx_matmul<64, 64, 2, 2, 4>(a, st);
         if (r) return r;
-        if (a.splits > 1) launch_join(a.part, a.splits, a.M, a.N, a.out, a.odt, a.out_stride, st);
+        if (a.splits > 1) {
+            if (hipGetLastError() != hipSuccess) return -1;
+            return launch_join(a.part, a.splits, a.M, a.N, a.out, a.odt, a.out_stride, st);
+        }
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
