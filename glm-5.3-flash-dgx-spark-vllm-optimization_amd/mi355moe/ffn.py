@@ -131,6 +131,9 @@ class _Gated(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
+        if _capturing(dh.device):
+            raise RuntimeError("mi355moe: the backward pass of an eagerly recorded ffn.gated cannot be captured; capture "
+                               "ffn.gated_forward(save=True) and ffn.gated_backward")
         x, w13, gu = ctx.saved_tensors
         dx, dw = gated_backward(dh, gu, x, w13, ctx.limit, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dx, dw, None
@@ -140,7 +143,7 @@ def gated(x: torch.Tensor, w13: torch.Tensor, limit: float = 0.0) -> torch.Tenso
     """h [..., I] = silu(min(g, L)) * clamp(u, -L, L) of x [..., H] and w13 [2I, H], differentiable once in x and w13
     by reverse mode (forward-mode derivatives are refused). While a graph is captured, a call that would record a gradient is
     refused: torch's autograd does not keep an eager graph of the same leaves apart from a captured one; capture
-    gated_forward(save=True) and gated_backward instead."""
+    gated_forward(save=True) and gated_backward instead. The backward pass of an eager call is refused during capture too."""
     if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad):
         dev, _ = _check(x, w13)
         if _capturing(dev):
