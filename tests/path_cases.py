@@ -40,7 +40,10 @@ ROUTED = [
     (3, 544, 288, 333, 2, 10.0, [WIDE, DOWN_WIDE]),
     (2, 160, 1120, 700, 1, 0.0, [WIDE, DOWN_WIDE]),
     (5, 96, 32, 2100, 2, 2.0, [WIDE, DOWN_WIDE]),
+    (3, 16384, 64, 263, 2, 10.0, [WIDE, DOWN_WIDE]),
+    (3, 64, 16384, 263, 2, 1.0, [WIDE, DOWN_WIDE]),
     (16, 544, 288, 20, 4, 10.0, DIRECT),
+    (9, 16384, 32, 5, 2, 2.0, DIRECT),
 ]
 # the same with hidden and intermediate that are multiples of 128 but not of 256: scales as they come
 STORED = [

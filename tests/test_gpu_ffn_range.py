@@ -86,3 +86,21 @@ def test_zero_gradient_and_repeats(cuda, dt):
     first = ffn.gated_backward(dh, gu, x, w, 10.0)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, ffn.gated_backward(dh, gu, x, w, 10.0)))
+
+
+def test_captured_gradients_follow_their_inputs(cuda):
+    """Replays with dh of other magnitudes, eager work in between: the power of two is the replay's own."""
+    from mi355moe import ffn
+    x, w, dh = _inputs(300, 264, 72, 1.0, 4.0, 1.0, 4)
+    _, gu = ffn.gated_forward(x, w, 10.0, save=True)
+    ffn.gated_backward(dh, gu, x, w, 10.0)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = ffn.gated_backward(dh, gu, x, w, 10.0)
+    for scale in (1.0, 2.0 ** 14, 2.0 ** -20, 0.0, 3.0):
+        dh.copy_(_inputs(300, 264, 72, 1.0, 4.0, scale, 5)[2])
+        g.replay()
+        want = ffn.gated_backward(dh, gu, x, w, 10.0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))

@@ -228,3 +228,23 @@ def test_nan_blocks_of_weights(cuda, case):
         nan[(tid == e2).any(1), col] = True
         nan[(tid == e13).any(1)] = True
         assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], out[~nan])
+
+
+@pytest.mark.parametrize("T,k", [(65536, 1), (2048, 32), (8191, 8)])
+def test_most_pairs(cuda, T, k):
+    """65536 pairs, the most a call takes, and picks of 32 experts; a sample of the tokens."""
+    from mi355moe import mxfp4
+    n, H, I, limit, dt = 64, 96, 32, 2.0, torch.bfloat16
+    ex = _layer(n, H, I, 9)
+    x = torch.randn(T, H, generator=_gen(T), device="cuda").to(dt)
+    ids, w = _routing(T, n, k, 3)
+    tid, tw = torch.from_numpy(ids).cuda(), torch.from_numpy(w).cuda()
+    out = mxfp4.moe_forward_ids(ex, x, tid, tw, limit=limit)
+    some = np.unique(np.concatenate([[0, 1, 2, 3, T // 2, T - 1], np.random.default_rng(1).integers(0, T, 60)]))
+    w13, w2 = _dense(ex)
+    want, tol = ref.moe(_f64(x)[some], w13, w2, ids[some], w[some].astype(np.float64), limit, EPS[dt])
+    # (32 pairs a token: their sum is rounded once a pair, on sums of up to all their magnitudes)
+    each = sum(np.abs(ref.moe(_f64(x)[some], w13, w2, ids[some, j:j + 1], w[some, j:j + 1].astype(np.float64), limit, 0.0)[0]) for j in range(k))
+    assert (np.abs(_f64(out)[some] - want) <= tol + each * k * 2.0 ** -24 + TINY[dt]).all()
+    with pytest.raises(ValueError, match="unsupported size"):
+        mxfp4.moe_forward_ids(ex, x.new_zeros(65537, H), torch.zeros(65537, 1, dtype=torch.int32, device="cuda"), torch.zeros(65537, 1, device="cuda"))
