@@ -2032,7 +2032,7 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
     f.wdt = r.wdt;
     if (mxfp4_direct(T, topk, n, expert_map ? std::max(n, n_global) : n, K, N)) return rc_launch(launch_mxfp4_direct(f, stream));
     if (int rc = launch_route(r, stream)) return rc_launch(rc);
-    return rc_launch(launch_mxfp4(f, stream, 15));
+    return rc_launch(launch_mxfp4(f, stream));
 }
 
 int64_t mi355moe_gated_forward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate) {
@@ -2072,7 +2072,7 @@ int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, 
 int64_t mi355moe_gated_backward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate) {
     if (gated_ok(MI355MOE_BF16, T, hidden, intermediate)) return -1;
     return (int64_t)(align_up(T * 2 * intermediate * 2) + align_up(4 * (GATED_TOPS + 1))) +
-           4 * gated_part_floats(T, hidden, intermediate, true, true);
+           4 * gated_part_floats(T, hidden, intermediate);
 }
 
 int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, const void* x, int dtype, int64_t T,

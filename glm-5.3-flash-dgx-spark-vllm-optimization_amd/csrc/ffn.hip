@@ -425,11 +425,11 @@ static int gemm16(Gemm16Args a, hipStream_t st) {
     return 0;
 }
 
-int64_t gated_part_floats(int64_t T, int64_t K, int64_t N, bool dx, bool dw) {
+int64_t gated_part_floats(int64_t T, int64_t K, int64_t N) {
     const Gemm16Plan px = plan_gemm16(T, K, 2 * N), pw = plan_gemm16(2 * N, K, T);
     int64_t f = 0;
-    if (dx && px.splits > 1) f = std::max(f, px.splits * T * K);
-    if (dw && pw.splits > 1) f = std::max(f, pw.splits * 2 * N * K);
+    if (px.splits > 1) f = std::max(f, px.splits * T * K);
+    if (pw.splits > 1) f = std::max(f, pw.splits * 2 * N * K);
     return f;
 }
 

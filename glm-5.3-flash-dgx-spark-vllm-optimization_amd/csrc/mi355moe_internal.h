@@ -301,7 +301,8 @@ int launch_fp8(const Fp8Args& a, hipStream_t st, int kernels);
 int launch_quant_rows(const void* x, int xdt, int64_t stride, int rows, int K, uint8_t* q, float* s, hipStream_t st);
 
 // MXFP4 (mxfp4.hip). Codes two a byte, rows K / 2 bytes apart. Scales: the 8 of steps of 256 values together, those of row
-// r and step k at p + r * row + k * step: rows of K / 32 bytes (row = K / 32, a multiple of 4, step = 8), or arranged by
+// r and step k at p + r * row + k * step: rows of K / 32 bytes (row = K / 32, of any value where the reader takes
+// bytes or dwords at any address, a multiple of 4 where tiles load dwords by it; step = 8), or arranged by
 // steps (row = 8, step = 8 rows; the steps' bytes behind a row's last scale are 127).
 struct MxScales {
     const uint8_t* p;
@@ -356,8 +357,8 @@ constexpr int MX_FEW = 16, MX_TILE = 64, MX_WIDE = 128;
 constexpr int mxfp4_seg_rows(int64_t P, int64_t n) { return P <= 8 * n ? MX_FEW : P < 96 * n ? MX_TILE : MX_WIDE; }
 // a call whose pairs hardly share experts, in two launches and without a permutation (a.ids, a.wts)
 int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st);
-// kernels: bit 0 quantise inputs, bit 1 gate/up, bit 2 down, bit 3 slot-order combine
-int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels);
+// the others: quantise inputs, gate/up, down, slot-order combine (the route has run)
+int launch_mxfp4(const Mxfp4Args& a, hipStream_t st);
 // rows x K values to codes [rows][ceil(K/2)] and scales [rows][ceil(K/32)] or (steps) arranged by steps
 int launch_mx_quant(const void* x, int xdt, int64_t stride, int64_t rows, int K, uint8_t* q, uint8_t* s, int steps,
                     hipStream_t st);
@@ -418,7 +419,7 @@ int64_t gated_forward_floats(int64_t T, int64_t K, int64_t N);
 int launch_gated_forward(const GatedArgs& a, hipStream_t st);
 // d from gu and dh; then dx (if set) = d W13 and dw (if set) = d^T x
 int launch_gated_backward(const GatedArgs& a, hipStream_t st);
-int64_t gated_part_floats(int64_t T, int64_t K, int64_t N, bool dx, bool dw);
+int64_t gated_part_floats(int64_t T, int64_t K, int64_t N);
 
 int launch_router_logits(const uint16_t* x, int64_t x_stride, const uint16_t* w, int T, int K, int E, float* logits,
                          hipStream_t st);

@@ -913,24 +913,20 @@ int launch_mxfp4_direct(const Mxfp4Args& a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-int launch_mxfp4(const Mxfp4Args& a, hipStream_t st, int kernels) {
-    if ((kernels & 1) && launch_mx_quant(a.x, a.xdt, a.x_stride, a.T, a.K, a.qx, a.sx, 1, st)) return -1;
+int launch_mxfp4(const Mxfp4Args& a, hipStream_t st) {
+    if (launch_mx_quant(a.x, a.xdt, a.x_stride, a.T, a.K, a.qx, a.sx, 1, st)) return -1;
     const bool few = a.seg == MX_FEW;
-    if (kernels & 2) {
-        if (few) hipLaunchKernelGGL(mx_gateup_few_kernel<4>, dim3(a.N / 32, a.S_cap), dim3(256), 0, st, a);
-        else if (a.seg == MX_TILE ? run_mx_gateup<128, 64, 2, 2, 3>(a, st) : run_mx_gateup<128, 128, 2, 2, 2>(a, st)) return -1;
-    }
-    if (kernels & 4) {
-        if (few) {
-            const int nblk = a.N >> 5;
-            auto grid = [&](int cols) { return dim3((a.K + cols - 1) / cols, a.S_cap); };
-            if (nblk > 64) hipLaunchKernelGGL((mx_down_few_kernel<2, 8>), grid(32), dim3(512), 0, st, a);
-            else if (nblk > 32) hipLaunchKernelGGL((mx_down_few_kernel<2, 4>), grid(64), dim3(512), 0, st, a);
-            else if (nblk > 16) hipLaunchKernelGGL((mx_down_few_kernel<2, 2>), grid(128), dim3(512), 0, st, a);
-            else hipLaunchKernelGGL((mx_down_few_kernel<2, 1>), grid(256), dim3(512), 0, st, a);
-        } else if (a.seg == MX_TILE ? run_mx_down<128, 64, 2, 2, 3>(a, st) : run_mx_down<128, 128, 2, 2, 2>(a, st)) return -1;
-    }
-    if (kernels & 8) hipLaunchKernelGGL(mx_combine_kernel, dim3(a.T, (a.K + 1023) / 1024), dim3(256), 0, st, a);
+    if (few) hipLaunchKernelGGL(mx_gateup_few_kernel<4>, dim3(a.N / 32, a.S_cap), dim3(256), 0, st, a);
+    else if (a.seg == MX_TILE ? run_mx_gateup<128, 64, 2, 2, 3>(a, st) : run_mx_gateup<128, 128, 2, 2, 2>(a, st)) return -1;
+    if (few) {
+        const int nblk = a.N >> 5;
+        auto grid = [&](int cols) { return dim3((a.K + cols - 1) / cols, a.S_cap); };
+        if (nblk > 64) hipLaunchKernelGGL((mx_down_few_kernel<2, 8>), grid(32), dim3(512), 0, st, a);
+        else if (nblk > 32) hipLaunchKernelGGL((mx_down_few_kernel<2, 4>), grid(64), dim3(512), 0, st, a);
+        else if (nblk > 16) hipLaunchKernelGGL((mx_down_few_kernel<2, 2>), grid(128), dim3(512), 0, st, a);
+        else hipLaunchKernelGGL((mx_down_few_kernel<2, 1>), grid(256), dim3(512), 0, st, a);
+    } else if (a.seg == MX_TILE ? run_mx_down<128, 64, 2, 2, 3>(a, st) : run_mx_down<128, 128, 2, 2, 2>(a, st)) return -1;
+    hipLaunchKernelGGL(mx_combine_kernel, dim3(a.T, (a.K + 1023) / 1024), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
