@@ -335,7 +335,8 @@ void carve_mxfp4(void* ws, int64_t P, int64_t T, int64_t n, int64_t K, int64_t N
 // combine launches (10 us) and reads an expert again for every further pair of it (6.7 MB in 1.2 us at hidden 4096,
 // intermediate 1024). us without / with, top-8, pairs beyond the first of their expert (uniform routing): 288 experts T = 1
 // (0) 26.8 / 17.2, 4 (1.3) 50 / 42, 8 (6) 93 / 84, 16 (23) 143 / 155, 32 (86) 204 / 292; 36 experts T = 4 (9) 43 / 38, 8
-// (33) 50 / 66; 8 experts T = 2 (8) 27 / 23.
+// (33) 50 / 66; 8 experts T = 2 (8) 27 / 23. Skewed routing shares more pairs than this counts, out of caches: 288 experts, Zipf(1.2)
+// picks, T = 2 37.0 / 26.5, 4 48.5 / 42.0, 6 56.8 / 56.0, 8 65.6 / 70.4 (from 16 on the permutation is taken).
 bool mxfp4_direct(int64_t T, int64_t topk, int64_t n, int64_t total, int64_t K, int64_t N) {
     const double local = (double)T * (double)topk * (double)n / (double)total;
     const double again = local - std::min(local, expected_experts((double)T, topk, n, total));

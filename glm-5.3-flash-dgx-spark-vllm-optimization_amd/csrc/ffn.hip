@@ -42,7 +42,7 @@ __device__ __forceinline__ f32x4 few_mma16(u32x4 a, u32x4 b, f32x4 c) {
 // Lane (c = lane % 16, g = lane / 16) holds the chunks g, 4 + g, 8 + g, 12 + g of weight row c and of token c, so that a load
 // takes 64 bytes in a row (128 of the contraction a wave step, in the same order on both sides); the contraction is cut over
 // the sixteen waves, whose sums join in LDS in wave order. Bound: the latency of the two or three loads a wave makes and the
-// join (one token, 4096 -> 1024, 16.8 MB of weights: 7.1 us, 2.4 TB/s; 4096 -> 4096: 13.4 us, 5.0 TB/s); more than one group
+// join (one token, 4096 -> 1024, 16.8 MB of weights by 128 workgroups, two rounds of loads each: 7.1 us, 2.4 TB/s; 4096 -> 4096: 13.4 us, 5.0 TB/s); more than one group
 // of tokens reads the weights and the tokens through L2 again, 16.8 us at 512 workgroups, all that the card holds at once.
 // Two or four groups a workgroup, which read the weights once: 13.7 us for 32 tokens (9.9 by two workgroups), 21 for 64 (16.8).
 template <int DT>
@@ -105,8 +105,10 @@ __global__ __launch_bounds__(1024) void gated_few_kernel(GatedArgs a) {
 
 // Workgroup tiles of BP / 2 columns x BQ tokens; a wave's P rows are its gate columns, then the same up columns, so the SwiGLU
 // is local to a lane. 8192 tokens, 4096 -> 2048, 275 GFLOP with g and u kept: 267 us, 1.03 PFLOP/s (without them 235 us, 1.17; a
-// library product alone takes 218): the matrix cores' power, then 134 MB of fp32 sums. 1791 tokens -> 1024: 36 us, 0.83 PFLOP/s,
-// 240 tiles for 256 CUs. Few tokens: the latency of a stage, 0.33 us whatever the tile (4096 -> 1024, 700 tokens: 24 us).
+// library product alone takes 218): the matrix cores, busy in half of the cycles at 2.0 GHz, then 134 MB of fp32 sums. 1791 tokens
+// -> 1024: 36 us, 0.83 PFLOP/s, 224 tiles on 256 CUs at 0.57 us a stage, of which the matrix cores work half and LDS 38 %, and
+// waves wait 39 %, next to nothing of it for LDS: the stage's loads and its barrier. Few tokens: the latency of a stage, 0.33 us
+// whatever the tile (4096 -> 1024, 700 tokens: 24 us).
 template <int DT, int BP, int BQ, int WP, int WQ, int ST>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void gated_kernel(GatedArgs a, int nt, int mt) {
     using G = GemmTile<KindOf<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
@@ -251,7 +253,8 @@ __device__ __forceinline__ int gated_shift(const uint32_t* tops, int n) {
 __device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast(float, (uint32_t)(127 + k) << 23); }
 
 // d = [dg | du], eight columns a thread. Bound: memory; 8192 x 2048, 235 MB: 35 us, 6.7 TB/s (part of it from cache). Rounded
-// once to the operand type, which the matrix cores take; unrounded, the two products would be fp32 ones, at a tenth of the rate.
+// once to the operand type, which the matrix cores take; unrounded, the two products would be fp32 ones, at a tenth of the rate
+// (the gradients' error against float64 grows from 0.0017 to 0.0024 of their norm in bf16, their own last rounding's share 0.0017).
 // fp16: times 2^k by the maxima of gated_top_kernel, and 2^-k left for the products.
 template <int DT>
 __global__ __launch_bounds__(256) void gated_d_kernel(GatedArgs a) {
@@ -293,9 +296,10 @@ struct Gemm16Args {
     const float* unscale;   // fp16: the factor of the sums (nullptr: none)
 };
 
-// out[m][n] = sum over k of P Q, dtype DT, or fp32 partials of the contraction's splits (grid y). Bound: the matrix cores' power
-// and the transposing LDS reads; 8192 tokens, 4096 -> 2048, 275 GFLOP each: dx (8192 x 4096 from 4096) 235 us, dw (4096 x 4096
-// from 8192) 230, 1.17 and 1.19 PFLOP/s (library products of these sizes and layouts: 238 and 256).
+// out[m][n] = sum over k of P Q, dtype DT, or fp32 partials of the contraction's splits (grid y). Bound: the matrix cores, busy
+// in 60 and 64 % of the cycles at 1.8 GHz (memory-bound kernels run at 2.2); 8192 tokens, 4096 -> 2048, 275 GFLOP each: dx (8192 x
+// 4096 from 4096) 235 us, dw (4096 x 4096 from 8192) 230, 1.17 and 1.19 PFLOP/s (library products of these sizes and layouts: 238
+// and 256). Of few tiles (dx below 2000 tokens): a stage's latency, 0.6 us on the small tiles.
 template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void gemm16_kernel(Gemm16Args a, int nt, int mt) {
     using G = GemmTile<KindOf<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
@@ -374,7 +378,8 @@ static int gated_parts(int64_t T, int64_t K, int64_t N) {
 // The forward streams the weights for one group of 16 tokens, and for more while their workgroups are at most three a CU, or, where
 // the contraction would be cut, two of 4096 values. us streamed / by tiles, cold weights: 4096 -> 1024, T = 16 9.7 / 26, 64
 // 16.8 / 30, 96 23.5 / 29 (in parts 15), 128 30.5 / 29; 4096 -> 4096, 16 18 / 28, 32 31.7 / 29.5; 4096 -> 12288, 1 34 / 44, 16
-// 50 / 45; 2048 -> 768, 128 13.1 / 16.6; 8192 -> 512, 64 16.6 / 53 (in parts 15.5), 100 31 / 53 (in parts 15.5).
+// 50 / 45; 2048 -> 768, 128 13.1 / 16.6; 8192 -> 512, 64 16.6 / 53 (in parts 15.5), 100 31 / 53 (in parts 15.5). What so simple a
+// rule leaves by these figures: 5 us at 12288 columns and 16 tokens, 1 at 8192 -> 512 and 64.
 static bool gated_streams(int64_t T, int64_t K, int64_t N) {
     const int64_t wgs = (T + 15) / 16 * (N / 8);
     return T <= 16 || (wgs <= 768 && (wgs * K <= 512 * 4096 || gated_parts(T, K, N) == 1));
@@ -389,8 +394,8 @@ struct Gemm16Plan {
     int tile, splits;
 };
 // By the rule of plan_mx_matmul. us by kind 256 / 128 / 128 deep / 64, dx of 4096 columns from 2048: T = 128 42 / 29 / 20.7 /
-// 20.4, 512 46 / 32 / 24.0 / 22.5, 1791 51 / 41.8 / 47.7 / 61.7, 4096 71 / 83 / 95 / 120. A long contraction of few tiles (128 x
-// 512 x 8192): 36 us, in 4 parts 21.
+// 20.4, 512 46 / 32 / 24.0 / 22.5 (512 tiles of 64: the deep one is taken), 1791 51 / 41.8 / 47.7 / 61.7, 4096 71 / 83 / 95 / 120.
+// A long contraction of few tiles (128 x 512 x 8192): 36 us, in 4 parts 21.
 static Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
     Gemm16Plan p{TILE_256, 1};
     auto tiles = [&](int64_t b) { return ((N + b - 1) / b) * ((M + b - 1) / b); };

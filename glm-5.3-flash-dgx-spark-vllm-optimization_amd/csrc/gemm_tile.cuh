@@ -156,7 +156,7 @@ __device__ __forceinline__ u32x4 fragment(const unsigned char* st, int r0, int s
 // Scale dwords of an MXFP4 operand: a stage holds 8 bytes of each row's scales (the dword of half h at 4h), 256 bytes (32
 // rows) a wave instruction of 4 bytes a lane. Row R's scales of stage kb lie at rowoff(R) + kb * step: back to back for the
 // rows of a tile where the scales were arranged by steps; in rows of K / 32 bytes they touch as many lines as the stage's
-// codes do, for a sixteenth of the bytes (256 x 256 tiles, K 16384: 3390 cycles a stage, 2470 without these loads).
+// codes do, for a sixteenth of the bytes.
 template <int R, int NW>
 struct ScaleStager {
     static constexpr int INST = (R / 32 + NW - 1) / NW;

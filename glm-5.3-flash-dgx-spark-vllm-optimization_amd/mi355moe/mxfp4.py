@@ -184,8 +184,10 @@ def _arranged(scale: torch.Tensor) -> torch.Tensor:
 
 class Mxfp4Experts:
     """A layer's MXFP4 experts plus the C descriptor. The codes stay the caller's tensors; the scales are copied once into
-    the order the kernels read (a seventeenth of the layer's bytes; arrange=False keeps the caller's, which costs time in
-    every call and needs H and I to be multiples of 128)."""
+    the order the kernels read (a seventeenth of the layer's bytes; arrange=False keeps the caller's, which needs H
+    and I to be multiples of 128 and costs 0 to 6 % of a call: hidden 4096, intermediate 1024, 288 experts, top-8, 8 tokens 78 us
+    arranged and 83 as they come, 64 tokens 286 and 296, 2047 tokens 547 and 555). Built on the current stream: as with any
+    tensor, another stream waits for it before its first call."""
 
     def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
                  arrange: bool = True):
