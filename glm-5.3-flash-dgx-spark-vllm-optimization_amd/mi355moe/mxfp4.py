@@ -183,8 +183,8 @@ def _arranged(scale: torch.Tensor) -> torch.Tensor:
 
 
 class Mxfp4Experts:
-    """A layer's MXFP4 experts plus the C descriptor. The codes stay the caller's tensors; the scales are copied once into
-    the order the kernels read (a seventeenth of the layer's bytes; arrange=False keeps the caller's, which needs H
+    """A layer's MXFP4 experts plus the C descriptor. The codes stay the caller's tensors; the scales are copied once (later
+    changes of the caller's do not reach them) into the order the kernels read (a seventeenth of the layer's bytes; arrange=False keeps the caller's, which needs H
     and I to be multiples of 128 and costs 0 to 6 % of a call: hidden 4096, intermediate 1024, 288 experts, top-8, 8 tokens 78 us
     arranged and 83 as they come, 64 tokens 286 and 296, 2047 tokens 547 and 555). Built on the current stream: as with any
     tensor, another stream waits for it before its first call."""
@@ -268,6 +268,8 @@ def moe_forward_ids(experts: Mxfp4Experts, x: torch.Tensor, topk_ids: torch.Tens
         raise ValueError(f"activations on {dev}, experts on {experts.device}")
     if x.dim() != 2 or x.shape[1] != experts.K:
         raise ValueError(f"x must be [T, {experts.K}], got {tuple(x.shape)}")
+    if expert_map is not None and expert_map.numel() == 0:
+        raise ValueError("expert_map has no entries")        # (its address would read as no map: ids taken as local ones)
     _rows(x)
     T = x.shape[0]
     if topk_ids.dim() not in (1, 2) or topk_ids.shape[0] != T or topk_weights.shape != topk_ids.shape:
