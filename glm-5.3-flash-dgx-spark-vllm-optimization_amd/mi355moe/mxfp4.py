@@ -53,9 +53,9 @@ def _rows(x: torch.Tensor, name: str = "x") -> torch.Tensor:
 
 
 def _may_write(out: torch.Tensor, what: str, adds: bool, *inputs: torch.Tensor) -> None:
-    """Refuses an `out` whose gradient a call that writes through its address would falsify: one that is overwritten or a leaf (or
-    a view of one) where it needs a gradient itself, and any where the inputs do. What is added to an intermediate result leaves its gradient
-    as it is."""
+    """Refuses an `out` whose gradient a call that writes through its address would falsify: one that is overwritten, or a
+    leaf or a view of one, where it needs a gradient itself, and any where the inputs do. What is added to an intermediate
+    result leaves its gradient as it is."""
     _no_tangents(what, out, *inputs)
     if torch.is_grad_enabled():
         if any(t.requires_grad for t in inputs):
@@ -184,10 +184,10 @@ def _arranged(scale: torch.Tensor) -> torch.Tensor:
 
 class Mxfp4Experts:
     """A layer's MXFP4 experts plus the C descriptor. The codes stay the caller's tensors; the scales are copied once (later
-    changes of the caller's do not reach them) into the order the kernels read (a seventeenth of the layer's bytes; arrange=False keeps the caller's, which needs H
-    and I to be multiples of 128 and costs 0 to 6 % of a call: hidden 4096, intermediate 1024, 288 experts, top-8, 8 tokens 78 us
-    arranged and 83 as they come, 64 tokens 286 and 296, 2047 tokens 547 and 555). Built on the current stream: as with any
-    tensor, another stream waits for it before its first call."""
+    changes of the caller's do not reach them) into the order the kernels read, a seventeenth of the layer's bytes.
+    arrange=False keeps the caller's, which needs H and I to be multiples of 128 and costs 0 to 6 % of a call (hidden 4096,
+    intermediate 1024, 288 experts, top-8: 8 tokens 78 us arranged and 83 as they come, 64 tokens 286 and 296, 2047 tokens
+    547 and 555). Built on the current stream: as with any tensor, another stream waits for it before its first call."""
 
     def __init__(self, w13: torch.Tensor, w13_scale: torch.Tensor, w2: torch.Tensor, w2_scale: torch.Tensor,
                  arrange: bool = True):
