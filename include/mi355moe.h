@@ -491,8 +491,8 @@ int mi355moe_mxfp4_moe_forward_ids(const mi355moe_mxfp4_layer* layer, const void
  * once: both projections, the activation and the product (what the model's shared expert computes before
  * its down projection). x [T][hidden] (row stride x_stride), w13 [2 * intermediate][hidden] (gate rows, then up rows)
  * and h (row stride h_stride) of one dtype, F16 or BF16; hidden and intermediate multiples of 8; x, w13 and h
- * 16-byte aligned, x_stride and h_stride multiples of 8, x_stride at most 2^22. gu (optional, fp32 [T][2 * intermediate], 16-byte aligned) receives g and u for
- * the backward pass. The workspace (may be NULL if the size query says 0) is 16-byte aligned, uninitialised. */
+ * 16-byte aligned, x_stride and h_stride multiples of 8, x_stride at most 2^22. gu (optional, fp32 [T][2 * intermediate],
+ * 16-byte aligned) receives g and u for the backward pass. The workspace (may be NULL if the size query says 0) is 16-byte aligned, uninitialised. */
 int64_t mi355moe_gated_forward_workspace_bytes(int64_t T, int64_t hidden, int64_t intermediate);
 int mi355moe_gated_forward(const void* x, int dtype, int64_t T, int64_t hidden, int64_t x_stride, const void* w13,
                            int64_t intermediate, float limit, void* h, int64_t h_stride, float* gu, void* workspace,
