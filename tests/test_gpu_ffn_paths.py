@@ -117,3 +117,19 @@ def test_most_rows(cuda):
     assert ((dw.double() - v).abs() <= tol).all()
     with pytest.raises(RuntimeError, match="code 3"):
         ffn.gated_forward(x.new_empty(T + 1, H), w, limit)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("size", [(8192, 4096, 2048), (130, 264, 2056), (8203, 136, 72)], ids=_id)
+def test_training_steps_repeat(cuda, size, dt):
+    """The same step gives the same bits: on the largest tiles, and where a gradient's sum is cut into parts."""
+    from mi355moe import ffn
+    x, w, dh = _inputs(*size, dt, 3)
+
+    def step():
+        h, gu = ffn.gated_forward(x, w, 10.0, save=True)
+        return (h, gu, *ffn.gated_backward(dh, gu, x, w, 10.0))
+
+    first = step()
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
