@@ -351,6 +351,32 @@ int gated_ok(int dtype, int64_t T, int64_t K, int64_t N) {
     if (T > (1 << 24) || K > 65536 || N > 16384) return MI355MOE_ELIMIT;
     return 0;
 }
+// The dense product's sizes; K % 8 == 0: its operands as the gated block's.
+int linear_ok(int dtype, int64_t M, int64_t K, int64_t N, int activation) {
+    if (dtype != MI355MOE_F16 && dtype != MI355MOE_BF16) return MI355MOE_EDTYPE;
+    if (M < 0 || K < 1 || N < 1) return MI355MOE_ESHAPE;
+    if (M > (1 << 24) || K > 65536 || N > (1 << 18)) return MI355MOE_ELIMIT;
+    if (activation < ACT_NONE || activation > ACT_GELU_TANH) return MI355MOE_EINVAL;
+    return 0;
+}
+int linear_operands(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t K) {
+    if (x_stride < K || w_stride < K) return MI355MOE_ESHAPE;
+    if ((reinterpret_cast<uintptr_t>(x) & 1) || (reinterpret_cast<uintptr_t>(w) & 1)) return MI355MOE_EINVAL;
+    if (K % 8) return 0;
+    if (!rows16_ok(x, x_stride) || !rows16_ok(w, w_stride)) return MI355MOE_EINVAL;
+    return x_stride > (1 << 22) || w_stride > (1 << 22) ? MI355MOE_ESHAPE : 0;
+}
+int rows_ok(int dtype, int64_t T, int64_t H, int64_t topk) {
+    if (dtype != MI355MOE_F32 && dtype != MI355MOE_F16 && dtype != MI355MOE_BF16) return MI355MOE_EDTYPE;
+    if (T < 0 || H < 1) return MI355MOE_ESHAPE;
+    if (topk < 1 || topk > MAX_TOPK || T * topk > (1 << 24) || T > (1 << 24) || H > 65536) return MI355MOE_ELIMIT;
+    return 0;
+}
+int norm_ok(int dtype, int64_t rows, int64_t H) {
+    if (dtype != MI355MOE_F32 && dtype != MI355MOE_F16 && dtype != MI355MOE_BF16) return MI355MOE_EDTYPE;
+    if (rows < 0 || H < 1) return MI355MOE_ESHAPE;
+    return H > 16384 || rows > (1 << 26) ? MI355MOE_ELIMIT : 0;
+}
 int dt_w(int dt) {
     return dt == MI355MOE_F32 ? DT_F32 : dt == MI355MOE_F16 ? DT_F16 : dt == MI355MOE_BF16 ? DT_BF16 : -1;
 }
@@ -2108,6 +2134,272 @@ int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, 
     g.unscale = reinterpret_cast<float*>(g.tops + GATED_TOPS);
     g.part = reinterpret_cast<float*>(reinterpret_cast<char*>(g.tops) + align_up(4 * (GATED_TOPS + 1)));
     return rc_launch(launch_gated_backward(g, stream));
+}
+
+int64_t mi355moe_sort_tokens_workspace_bytes(int64_t T, int64_t topk, int64_t n) {
+    if (rows_ok(MI355MOE_BF16, T, 1, topk) || n < 1 || n > MAX_EXPERTS) return -1;
+    return 4 * sort_count_words(T * topk, n);
+}
+
+int mi355moe_sort_tokens(const void* ids, int ids_dtype, int64_t T, int64_t topk, const int64_t* expert_map, int64_t n_global,
+                         int64_t n, int32_t* row, int32_t* pair, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                         hipStream_t stream) {
+    if (ids_dtype != MI355MOE_I32 && ids_dtype != MI355MOE_I64) return MI355MOE_EDTYPE;
+    if (int r = rows_ok(MI355MOE_BF16, T, 1, topk)) return r;
+    if (n < 1 || n > MAX_EXPERTS) return MI355MOE_ELIMIT;
+    if (expert_map && n_global < 0) return MI355MOE_EINVAL;
+    if (!offsets || (T > 0 && (!ids || !row || !pair))) return MI355MOE_EINVAL;
+    const int64_t need = mi355moe_sort_tokens_workspace_bytes(T, topk, n);
+    if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3))) return MI355MOE_EINVAL;
+    if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
+    SortArgs a{};
+    a.ids = ids;
+    a.ids64 = ids_dtype == MI355MOE_I64;
+    a.emap = expert_map;
+    a.n_global = n_global;
+    a.n = (int)n;
+    a.P = T * topk;
+    a.row = row;
+    a.pair = pair;
+    a.offsets = offsets;
+    a.counts = static_cast<int*>(workspace);
+    return rc_launch(launch_sort(a, stream));
+}
+
+int mi355moe_rows_to_experts(const void* x, int dtype, int64_t T, int64_t H, int64_t x_stride, const int32_t* row, int64_t topk,
+                             void* rows, hipStream_t stream) {
+    if (int r = rows_ok(dtype, T, H, topk)) return r;
+    if (x_stride < H) return MI355MOE_ESHAPE;
+    if (T == 0) return 0;
+    if (!x || !row || !rows) return MI355MOE_EINVAL;
+    RowsArgs a{};
+    a.dt = dt_w(dtype);
+    a.T = T;
+    a.P = T * topk;
+    a.H = (int)H;
+    a.topk = (int)topk;
+    a.row = row;
+    a.x = x;
+    a.x_stride = x_stride;
+    a.rows = rows;
+    return rc_launch(launch_rows_scatter(a, stream));
+}
+
+int mi355moe_rows_from_experts(const void* rows, int dtype, int64_t T, int64_t H, const int32_t* row, int64_t topk,
+                               const void* weights, int weights_dtype, const void* shared, int64_t shared_stride, void* out,
+                               int64_t out_stride, hipStream_t stream) {
+    if (int r = rows_ok(dtype, T, H, topk)) return r;
+    if (weights && dt_w(weights_dtype) < 0) return MI355MOE_EDTYPE;
+    if (out_stride < H || (shared && shared_stride < H)) return MI355MOE_ESHAPE;
+    if (T == 0) return 0;
+    if (!rows || !row || !out) return MI355MOE_EINVAL;
+    RowsArgs a{};
+    a.dt = dt_w(dtype);
+    a.T = T;
+    a.P = T * topk;
+    a.H = (int)H;
+    a.topk = (int)topk;
+    a.row = row;
+    a.rows = const_cast<void*>(rows);
+    a.w = weights;
+    a.wdt = dt_w(weights_dtype);
+    a.shared = shared;
+    a.shared_stride = shared_stride;
+    a.out = out;
+    a.out_stride = out_stride;
+    return rc_launch(launch_rows_gather(a, stream));
+}
+
+int mi355moe_rows_from_experts_backward(const void* dout, int dtype, int64_t T, int64_t H, int64_t dout_stride, const int32_t* row,
+                                        int64_t topk, const void* weights, int weights_dtype, const void* rows, void* drows,
+                                        void* dweights, hipStream_t stream) {
+    if (int r = rows_ok(dtype, T, H, topk)) return r;
+    if (dt_w(weights_dtype) < 0) return MI355MOE_EDTYPE;
+    if (dout_stride < H) return MI355MOE_ESHAPE;
+    if (T == 0 || (!drows && !dweights)) return 0;
+    if (!dout || !row || !weights || (dweights && !rows)) return MI355MOE_EINVAL;
+    RowsArgs a{};
+    a.dt = dt_w(dtype);
+    a.T = T;
+    a.P = T * topk;
+    a.H = (int)H;
+    a.topk = (int)topk;
+    a.row = row;
+    a.x = dout;
+    a.x_stride = dout_stride;
+    a.w = weights;
+    a.wdt = dt_w(weights_dtype);
+    a.y = rows;
+    a.rows = drows;
+    a.dw = dweights;
+    return rc_launch(launch_rows_grad(a, stream));
+}
+
+int64_t mi355moe_linear_forward_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+    if (linear_ok(MI355MOE_BF16, M, K, N, ACT_NONE)) return -1;
+    return linear_forward_bytes(M, N, K);
+}
+
+int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w, int64_t N,
+                            int64_t w_stride, const void* bias, int bias_dtype, int activation, const void* residual,
+                            int64_t residual_stride, void* out, int64_t out_stride, float* z, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream) {
+    if (int r = linear_ok(dtype, M, K, N, activation)) return r;
+    if (bias && dt_w(bias_dtype) < 0) return MI355MOE_EDTYPE;
+    if (out_stride < N || (residual && residual_stride < N)) return MI355MOE_ESHAPE;
+    if (M == 0) return 0;
+    if (!x || !w || !out) return MI355MOE_EINVAL;
+    if (int r = linear_operands(x, x_stride, w, w_stride, K)) return r;
+    const int64_t need = linear_forward_bytes(M, N, K);
+    if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MI355MOE_EINVAL;
+    if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
+    LinearArgs a{};
+    a.dt = dt_act(dtype);
+    a.M = M;
+    a.N = (int)N;
+    a.K = (int)K;
+    a.x = static_cast<const uint16_t*>(x);
+    a.x_stride = x_stride;
+    a.w = static_cast<const uint16_t*>(w);
+    a.w_stride = w_stride;
+    a.bias = bias;
+    a.bdt = dt_w(bias_dtype);
+    a.act = activation;
+    a.res = residual;
+    a.res_stride = residual_stride;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.z = z;
+    a.splits = 1;
+    return rc_launch(launch_linear(a, workspace, stream));
+}
+
+int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+    if (linear_ok(MI355MOE_BF16, M, K, N, ACT_NONE)) return -1;
+    return linear_backward_bytes(M, N, K);
+}
+
+int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, const void* x, int dtype, int64_t M, int64_t K,
+                             int64_t x_stride, const void* w, int64_t N, int64_t w_stride, int activation, void* dx, void* dw,
+                             void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (int r = linear_ok(dtype, M, K, N, activation)) return r;
+    if (dbias && dt_w(bias_dtype) < 0) return MI355MOE_EDTYPE;
+    if (dy_stride < N) return MI355MOE_ESHAPE;
+    if (!dx && !dw && !dbias) return 0;
+    if (M == 0) return dw || dbias ? MI355MOE_ESHAPE : 0;
+    if (!dy || !workspace || (activation != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return MI355MOE_EINVAL;
+    if (int r = linear_operands(dw ? x : nullptr, dw ? x_stride : (K + 7) / 8 * 8, dx ? w : nullptr, dx ? w_stride : (K + 7) / 8 * 8, K)) return r;
+    if (K % 8 == 0 && (!rows16_ok(dx, 0) || !rows16_ok(dw, 0))) return MI355MOE_EINVAL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return MI355MOE_EINVAL;
+    if ((int64_t)workspace_bytes < linear_backward_bytes(M, N, K)) return MI355MOE_EWORKSPACE;
+    LinearArgs a{};
+    a.dt = dt_act(dtype);
+    a.M = M;
+    a.N = (int)N;
+    a.K = (int)K;
+    a.x = static_cast<const uint16_t*>(x);
+    a.x_stride = x_stride;
+    a.w = static_cast<const uint16_t*>(w);
+    a.w_stride = w_stride;
+    a.bdt = dt_w(bias_dtype);
+    a.act = activation;
+    a.z = const_cast<float*>(z);
+    a.dy = dy;
+    a.dy_stride = dy_stride;
+    a.dx = dx;
+    a.dw = dw;
+    a.dbias = dbias;
+    a.splits = 1;
+    return rc_launch(launch_linear_backward(a, workspace, stream));
+}
+
+int mi355moe_norm_forward(const void* branch, int dtype, int64_t rows, int64_t H, int64_t branch_stride, const void* residual,
+                          int64_t residual_stride, const void* post, const void* pre, int weights_dtype, const void* gate,
+                          int gate_dtype, int gate_kind, float eps, float scale, float residual_scale, void* s, void* y,
+                          float* stats, hipStream_t stream) {
+    if (int r = norm_ok(dtype, rows, H)) return r;
+    if ((post || pre) && dt_w(weights_dtype) < 0) return MI355MOE_EDTYPE;
+    if (gate_kind < GATE_NONE || gate_kind > GATE_FULL || (gate_kind != GATE_NONE) != (gate != nullptr)) return MI355MOE_EINVAL;
+    if (gate && dt_w(gate_dtype) < 0) return MI355MOE_EDTYPE;
+    if (branch_stride < H || (residual && residual_stride < H)) return MI355MOE_ESHAPE;
+    if (!(eps >= 0.0f) || (pre != nullptr) != (y != nullptr) || (!s && !y)) return MI355MOE_EINVAL;
+    if (rows == 0) return 0;
+    if (!branch) return MI355MOE_EINVAL;
+    NormArgs a{};
+    a.dt = dt_w(dtype);
+    a.rows = rows;
+    a.H = (int)H;
+    a.branch = branch;
+    a.branch_stride = branch_stride;
+    a.res = residual;
+    a.res_stride = residual_stride;
+    a.post = post;
+    a.pre = pre;
+    a.wdt = dt_w(weights_dtype);
+    a.gate = gate;
+    a.gdt = dt_w(gate_dtype);
+    a.gate_kind = gate_kind;
+    a.eps = eps;
+    a.alpha = residual_scale;
+    a.beta = scale;
+    a.s = s;
+    a.y = y;
+    a.stats = stats;
+    return rc_launch(launch_norm(a, stream));
+}
+
+int64_t mi355moe_norm_backward_workspace_bytes(int64_t rows, int64_t H) {
+    if (norm_ok(MI355MOE_BF16, rows, H)) return -1;
+    return 4 * norm_part_floats(rows, (int)H);
+}
+
+int mi355moe_norm_backward(const void* ds, int64_t ds_stride, const void* dy, int64_t dy_stride, const void* branch, int dtype,
+                           int64_t rows, int64_t H, int64_t branch_stride, const void* residual, int64_t residual_stride,
+                           const void* post, const void* pre, int weights_dtype, const void* gate, int gate_dtype, int gate_kind,
+                           float scale, float residual_scale, const float* stats, void* dbranch, void* dresidual, void* dpost,
+                           void* dpre, void* dgate, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (int r = norm_ok(dtype, rows, H)) return r;
+    if ((post || pre) && dt_w(weights_dtype) < 0) return MI355MOE_EDTYPE;
+    if (gate_kind < GATE_NONE || gate_kind > GATE_FULL || (gate_kind != GATE_NONE) != (gate != nullptr)) return MI355MOE_EINVAL;
+    if (gate && dt_w(gate_dtype) < 0) return MI355MOE_EDTYPE;
+    if ((ds && ds_stride < H) || (dy && dy_stride < H) || branch_stride < H || (residual && residual_stride < H)) return MI355MOE_ESHAPE;
+    if ((dy && !pre) || (dpre && !dy) || (dpost && !post) || (dgate && !gate)) return MI355MOE_EINVAL;
+    if (!dbranch && !dresidual && !dpost && !dpre && !dgate) return 0;
+    const bool joined = dpost || dpre || (dgate && gate_kind == GATE_CHANNEL);
+    if (rows == 0) return joined ? MI355MOE_ESHAPE : 0;
+    if ((!ds && !dy) || !branch || !stats) return MI355MOE_EINVAL;
+    if (joined) {
+        if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)) return MI355MOE_EINVAL;
+        if ((int64_t)workspace_bytes < mi355moe_norm_backward_workspace_bytes(rows, H)) return MI355MOE_EWORKSPACE;
+    }
+    NormArgs a{};
+    a.dt = dt_w(dtype);
+    a.rows = rows;
+    a.H = (int)H;
+    a.branch = branch;
+    a.branch_stride = branch_stride;
+    a.res = residual;
+    a.res_stride = residual_stride;
+    a.post = post;
+    a.pre = pre;
+    a.wdt = dt_w(weights_dtype);
+    a.gate = gate;
+    a.gdt = dt_w(gate_dtype);
+    a.gate_kind = gate_kind;
+    a.alpha = residual_scale;
+    a.beta = scale;
+    a.stats = const_cast<float*>(stats);
+    a.ds = ds;
+    a.ds_stride = ds_stride;
+    a.dy = dy;
+    a.dy_stride = dy_stride;
+    a.dbranch = dbranch;
+    a.dres = dresidual;
+    a.dpost = dpost;
+    a.dpre = dpre;
+    a.dgate = dgate;
+    a.part = joined ? static_cast<float*>(workspace) : nullptr;
+    return rc_launch(launch_norm_grad(a, stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,552 @@
+// The dense product with its epilogue, and its gradients, on the 16-bit matrix cores.
+//
+//   z = x W^T + bias (fp32 sums);   out = act(z) + residual, rounded once
+//   dz = dy act'(z) from the fp32 z that the forward pass keeps;   dx = dz W,   dW = dz^T x,   dbias = sum over rows of dz
+//   (fp32 sums; dbias sums the unrounded dz, the products take it rounded once to the operand type, in fp16 times a power of
+//   two that the call's largest value sets where the activation has a slope other than 0 and 1)
+//
+//   relu max(z, 0);   silu z s(z);   gelu z Phi(z), Phi the normal distribution's integral;   gelu_tanh z s(2 sqrt(2/pi) (z +
+//   0.044715 z^3)), which is z (1 + tanh(half of that)) / 2;   s(v) = 1 / (1 + e^-v)
+#include <algorithm>
+
+#include "gemm_tile.cuh"
+#include "rows.cuh"
+
+namespace mi355moe {
+
+template <int DT>
+struct LinearKind {
+    static constexpr int value = DT == DT_BF16 ? MM_BF16 : MM_F16;
+};
+
+// ------------------------------------------------------------------------------------------------ activations
+
+__device__ __forceinline__ float sigmoid_rcp(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+// Phi(z) by Abramowitz and Stegun 7.1.26: erfc(x) = t (a1 + t (a2 + ...)) e^(-x^2), t = 1 / (1 + p x), within 1.5e-7 (of the
+// order of fp32's own step at 1; the library's erfcf takes three times the instructions). e: e^(-z^2 / 2).
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    e = __expf(-x * x);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    const float half = 0.5f * p * t * e;
+    return z < 0.0f ? half : 1.0f - half;
+}
+constexpr float GELU_A = 1.5957691216057308f;                        // 2 sqrt(2 / pi)
+
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+    if (act == ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];       // (NaN stays)
+    } else if (act == ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] *= sigmoid_rcp(v[j]);
+    } else if (act == ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float e;
+            v[j] *= normal_cdf(v[j], e);
+        }
+    } else if (act == ACT_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] *= sigmoid_rcp(GELU_A * (v[j] + 0.044715f * v[j] * v[j] * v[j]));
+    }
+}
+__device__ __forceinline__ float act_slope(int act, float z) {
+    if (act == ACT_RELU) return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;     // (NaN stays)
+    if (act == ACT_SILU) {
+        const float s = sigmoid_rcp(z);
+        return s * (1.0f + z * (1.0f - s));
+    }
+    if (act == ACT_GELU) {
+        float e;
+        const float c = normal_cdf(z, e);
+        return __builtin_fmaf(z * 0.3989422804014327f, e, c);
+    }
+    if (act == ACT_GELU_TANH) {
+        const float s = sigmoid_rcp(GELU_A * (z + 0.044715f * z * z * z));
+        return s + z * s * (1.0f - s) * GELU_A * (1.0f + 3.0f * 0.044715f * z * z);
+    }
+    return 1.0f;
+}
+
+// Columns c .. of row m from their sums: bias (b: theirs), activation, residual and the one rounding.
+template <int DT>
+__device__ __forceinline__ void linear_out8(const LinearArgs& a, int64_t m, int c, float (&v)[8], const float (&b)[8]) {
+    const int n = a.N - c;
+    if (a.bias)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += b[j];
+    if (a.z) store8<DT_F32>(a.z, (size_t)m * a.N + c, n, v);
+    activate(a.act, v);
+    if (a.res) {
+        float r[8];
+        load8<DT>(a.res, (size_t)m * a.res_stride + c, n, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+    }
+    store8<DT>(a.out, (size_t)m * a.out_stride + c, n, v);
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+
+template <int DT>
+__device__ __forceinline__ f32x4 linear_mma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (DT == DT_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+// Chunk (eight values) i of a row of K values, what lies behind the row's end as zero.
+__device__ __forceinline__ u32x4 row_chunk(const uint16_t* row, int i, int K) {
+    const int n = K - 8 * i;
+    u32x4 v = {0, 0, 0, 0};
+    if (n >= 8) return *reinterpret_cast<const rows_u32x4*>(row + 8 * i);
+    for (int j = 0; j < n; ++j) v[j >> 1] |= (uint32_t)row[8 * i + j] << (16 * (j & 1));
+    return v;
+}
+
+// grid (ceil(N / 16), ceil(M / 16)), W waves: 16 weight rows as one 16-row MFMA operand, for 16 rows of x; any K, stride and
+// address. Lane (c = lane % 16, g = lane / 16) holds the chunks g, 4 + g, 8 + g, 12 + g of weight row c and of row c of x, so
+// that a load takes 64 bytes in a row (128 of the contraction a wave step, in the same order on both sides); the contraction is
+// cut over the waves, whose sums join in LDS in wave order.
+template <int DT, int W>
+__global__ __launch_bounds__(64 * W) void linear_few_kernel(LinearArgs a) {
+    __shared__ __align__(16) float red[W][256];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 16;
+    const int64_t m0 = (int64_t)blockIdx.y * 16;
+    const int rows = (int)min((int64_t)16, a.M - m0);
+    const int chunks = (a.K + 7) >> 3;
+    const uint16_t* w = a.w + (size_t)min(n0 + c, a.N - 1) * a.w_stride;
+    const uint16_t* x = a.x + (size_t)(m0 + min(c, rows - 1)) * a.x_stride;
+    f32x4 acc = {};
+    for (int b0 = wv * 16; b0 < chunks; b0 += 16 * W) {
+        u32x4 p[4], q[4];
+        if ((b0 + 16) * 8 <= a.K) {                                  // (uniform)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const rows_u32x4*>(w + 8 * (b0 + g + 4 * i));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const rows_u32x4*>(x + 8 * (b0 + g + 4 * i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = row_chunk(w, b0 + g + 4 * i, a.K);
+                q[i] = row_chunk(x, b0 + g + 4 * i, a.K);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = linear_mma16<DT>(p[i], q[i], acc);
+    }
+    *reinterpret_cast<f32x4*>(&red[wv][lane * 4]) = acc;
+    __syncthreads();
+    if (tid >= 256) return;
+    const int m = tid >> 4, n = tid & 15, col = n0 + n;
+    if (m >= rows || col >= a.N) return;
+    float v[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[0] += red[i][((n >> 2) * 16 + m) * 4 + (n & 3)];
+    if (a.bias) v[0] += any_value(a.bias, a.bdt, col);
+    if (a.z) a.z[(size_t)(m0 + m) * a.N + col] = v[0];
+    activate(a.act, v);
+    if (a.res) v[0] += row_value<DT>(a.res, (size_t)(m0 + m) * a.res_stride + col);
+    store_any(a.out, DT, (size_t)(m0 + m) * a.out_stride + col, v[0]);
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+
+// A workgroup's BP columns x BQ rows, the contraction in a.splits parts (grid y). The sums pass through LDS in fp32, 32 rows of a
+// wave at a time, so that a lane ends up with eight columns of a row: bias, residual and output are whole 16-byte accesses
+// in whole lines, and the residual is added before the one rounding.
+template <int DT, int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(LinearArgs a, int nt, int mt) {
+    using G = GemmTile<LinearKind<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int2 tile = tile_order(blockIdx.x, nt, mt);
+    const int n0 = tile.x * BP;
+    const int64_t m0 = (int64_t)tile.y * BQ;
+    const int stages = (a.K + SB / 2 - 1) / (SB / 2), per = (stages + a.splits - 1) / a.splits;
+    const int kb0 = blockIdx.y * per, kb1 = min(stages, kb0 + per);
+    const uint32_t wp = 2u * (uint32_t)a.w_stride, xp = 2u * (uint32_t)a.x_stride;
+    const int pl = min(BP, a.N - n0) - 1, ql = (int)min((int64_t)BQ, a.M - m0) - 1;
+    G t;
+    t.p.init_row(uniform_ptr(a.w + (size_t)n0 * a.w_stride + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, pl) * wp; });
+    t.q.init_row(uniform_ptr(a.x + (size_t)m0 * a.x_stride + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, ql) * xp; });
+    const int tail = kb1 == stages ? a.K % (SB / 2) / 8 : 0;
+    if (kb0 < kb1) t.run(lds, kb0, kb1, tail, tail, 0, 0);
+    else
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
+
+    constexpr int UNITS = 8 * G::TP, CH = UNITS / 2;                 // 16-byte units and 8-column chunks of a wave's row
+    static_assert(G::NW * 32 * 16 * UNITS <= G::LDS, "the stages hold the waves' rows");
+    unsigned char* mine = lds + wv * (32 * 16 * UNITS);
+    const int64_t m1 = m0 + (wv / WP) * (BQ / WQ);
+    const int c = n0 + (wv % WP) * (BP / WP) + 8 * (lane % CH), n = a.N - c;
+    const int m = lane & 31, h = lane >> 5;
+    float b[8] = {};
+    if (a.bias && a.splits == 1) load8_any(a.bias, a.bdt, c, n, b);
+    float* part = a.splits > 1 ? a.part + (size_t)blockIdx.y * a.M * a.part_stride : nullptr;
+    __syncthreads();                                                 // no wave reads a stage any more
+#pragma unroll
+    for (int j = 0; j < G::TQ; ++j) {
+        unsigned char* row = mine + m * (16 * UNITS);
+#pragma unroll
+        for (int i = 0; i < G::TP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f32x16& v = t.acc[i][j];
+                *reinterpret_cast<f32x4*>(row + (((8 * i + 2 * r + h) ^ (m & (UNITS - 1))) << 4)) =
+                    f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
+            }
+        asm volatile("" ::: "memory");                               // (a wave's LDS accesses are performed in order)
+#pragma unroll
+        for (int s = 0; s < CH / 2; ++s) {
+            const int rr = s * (64 / CH) + lane / CH, u = 2 * (lane % CH), x = rr & (UNITS - 1);
+            const unsigned char* from = mine + rr * (16 * UNITS);
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(from + ((u ^ x) << 4)), hi = *reinterpret_cast<const f32x4*>(from + (((u + 1) ^ x) << 4));
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            const int64_t mm = m1 + 32 * j + rr;
+            if (mm >= a.M || n <= 0) continue;
+            if (part) store8<DT_F32>(part, (size_t)mm * a.part_stride + c, 8, v);
+            else linear_out8<DT>(a, mm, c, v, b);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// out from the sums of the contraction's parts [splits][M][part_stride], added in order: eight columns a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
+    const int per = (a.N + 7) / 8;
+    const int64_t items = a.M * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per;
+        const int c = (int)(i - m * per) * 8;
+        float v[8] = {}, b[8] = {};
+        for (int s = 0; s < a.splits; ++s) {
+            float p[8];
+            load8<DT_F32>(a.part, ((size_t)s * a.M + m) * a.part_stride + c, 8, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += p[j];
+        }
+        if (a.bias) load8_any(a.bias, a.bdt, c, a.N - c, b);
+        linear_out8<DT>(a, m, c, v, b);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ copies
+
+// dst [drows][dw] = src [rows][cols] (row stride ss), the rest zero: dw and dst's rows in whole 16 bytes.
+__global__ __launch_bounds__(256) void linear_pad_kernel(const uint16_t* __restrict__ src, int64_t ss, int64_t rows, int cols,
+                                                         uint16_t* __restrict__ dst, int64_t drows, int dw) {
+    const int per = dw / 8;
+    const int64_t items = drows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i - r * per) * 8;
+        u32x4 v = {0, 0, 0, 0};
+        if (r < rows) {
+            const uint16_t* p = src + (size_t)r * ss + c;
+            if (c + 8 <= cols) v = *reinterpret_cast<const rows_u32x4*>(p);
+            else
+                for (int j = 0; c + j < cols; ++j) v[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+        }
+        *reinterpret_cast<u32x4*>(dst + (size_t)r * dw + c) = v;
+    }
+}
+// dst [rows][cols] = the first columns of src [rows][sw].
+__global__ __launch_bounds__(256) void linear_crop_kernel(const uint16_t* __restrict__ src, int sw, uint16_t* __restrict__ dst, int64_t rows, int cols) {
+    const int per = (cols + 7) / 8;
+    const int64_t items = rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i - r * per) * 8;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(src + (size_t)r * sw + c);
+        uint16_t* p = dst + (size_t)r * cols + c;
+        if (c + 8 <= cols) *reinterpret_cast<rows_u32x4*>(p) = v;
+        else
+            for (int j = 0; c + j < cols; ++j) p[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ gradient
+
+constexpr int DZ_ROWS = 64;                                          // rows of a workgroup of linear_dz_kernel
+
+template <int DT>
+__device__ __forceinline__ void slope8(const LinearArgs& a, int64_t m, int c, float (&d)[8]) {
+    const int n = a.N - c;
+    load8<DT>(a.dy, (size_t)m * a.dy_stride + c, n, d);
+    if (a.act != ACT_NONE) {
+        float z[8];
+        load8<DT_F32>(a.z, (size_t)m * a.N + c, n, z);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] *= act_slope(a.act, z[j]);
+    }
+}
+
+// The largest finite magnitude of dz, as fp32 bits, of each workgroup's share (fp16 only: dz = dy act'(z) can lie among fp16's
+// subnormals, or beyond its range, where the sums over it are ordinary fp16 numbers).
+template <int DT>
+__global__ __launch_bounds__(256) void linear_top_kernel(LinearArgs a) {
+    __shared__ uint32_t red[4];
+    const int per = (a.N + 7) / 8;
+    const int64_t items = a.M * per;
+    uint32_t top = 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / per;
+        float d[8];
+        slope8<DT>(a, m, (int)(i - m * per) * 8, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, d[j]) & 0x7FFFFFFFu;
+            top = max(top, b < 0x7F800000u ? b : 0u);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) a.tops[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+}
+// k of the 2^k that brings the largest of `n` maxima into [2^14, 2^15) (0 where all are zero): every thread gets it.
+__device__ __forceinline__ int linear_shift(const uint32_t* tops, int n) {
+    __shared__ uint32_t red[4];
+    uint32_t top = 0;
+    for (int i = threadIdx.x; i < n; i += 256) top = max(top, tops[i]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = max(max(red[0], red[1]), max(red[2], red[3]));
+    return top ? min(14 - ((int)(top >> 23) - 127), 120) : 0;
+}
+
+// dz of 256 columns and DZ_ROWS rows: 32 threads across the columns, eight values each, eight down the rows. dz [M][dz_stride]
+// in the operand type (its columns behind N zero), where a.dz is set; the sums of the unrounded dz over the workgroup's rows
+// to part [grid x][part_stride] where that is set.
+template <int DT>
+__global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a) {
+    __shared__ __align__(16) float red[8][256];
+    float f = 1.0f;
+    if constexpr (DT == DT_F16)
+        if (a.ntops) {                                               // (uniform)
+            const int k = linear_shift(a.tops, a.ntops);
+            f = __builtin_bit_cast(float, (uint32_t)(127 + k) << 23);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.unscale = __builtin_bit_cast(float, (uint32_t)(127 - k) << 23);
+        }
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int c = blockIdx.y * 256 + tx * 8;
+    const int64_t m0 = (int64_t)blockIdx.x * DZ_ROWS, m1 = min(a.M, m0 + DZ_ROWS);
+    float sum[8] = {};
+    if (c < a.N)
+        for (int64_t m = m0 + ty; m < m1; m += 8) {
+            float d[8];
+            slope8<DT>(a, m, c, d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += d[j];
+            if (a.dz) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[j] = c + j < a.N ? d[j] * f : 0.0f;
+                store8<DT>(a.dz, (size_t)m * a.dz_stride + c, 8, d);
+            }
+        }
+    if (!a.dbias) return;                                            // (uniform)
+    store8<DT_F32>(red[ty], tx * 8, 8, sum);
+    __syncthreads();
+    const int col = blockIdx.y * 256 + threadIdx.x;
+    if (col >= a.N) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+    a.part[(size_t)blockIdx.x * a.part_stride + col] = s;
+}
+// dbias: the parts' sums in order, 64 columns a workgroup, the parts cut over its sixteen waves.
+__global__ __launch_bounds__(1024) void linear_dbias_kernel(LinearArgs a, int parts) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    const int per = (parts + 15) / 16, g0 = wv * per, g1 = min(parts, g0 + per);
+    float v = 0.0f;
+    if (c < a.N) {
+#pragma unroll 8
+        for (int g = g0; g < g1; ++g) v += a.part[(size_t)g * a.part_stride + c];
+    }
+    red[wv][lane] = v;
+    __syncthreads();
+    if (wv || c >= a.N) return;
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) v += red[w][lane];
+    store_any(a.dbias, a.bdt, c, v);
+}
+
+// ------------------------------------------------------------------------------------------------ launchers
+
+static unsigned linear_grid(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, 8192); }
+static int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
+
+static bool linear_streams(int64_t M, int64_t N, int64_t K) {
+    (void)K;
+    return M <= 16 || (M + 15) / 16 * ((N + 15) / 16) <= 512;
+}
+static Gemm16Plan linear_plan(int64_t M, int64_t N, int64_t K) { return plan_gemm16(M, N, K); }
+
+// Where the parts of a workspace begin, in bytes (256-byte steps); -1: not there.
+struct LinearSpace {
+    int64_t x = -1, w = -1, part = -1, dz = -1, dx = -1, dw = -1, tops = -1, bytes = 0;
+    int64_t take(int64_t n) {
+        const int64_t at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    }
+};
+static LinearSpace forward_space(int64_t M, int64_t N, int64_t K) {
+    LinearSpace s;
+    if (M == 0 || linear_streams(M, N, K)) return s;
+    if (K % 8) s.x = s.take(M * up8(K) * 2), s.w = s.take(N * up8(K) * 2);
+    const Gemm16Plan p = linear_plan(M, N, K);
+    if (p.splits > 1) s.part = s.take(p.splits * M * up8(N) * 4);
+    return s;
+}
+int64_t linear_forward_bytes(int64_t M, int64_t N, int64_t K) { return forward_space(M, N, K).bytes; }
+
+static int pad(const uint16_t* src, int64_t ss, int64_t rows, int64_t cols, uint16_t* dst, int64_t drows, int64_t dw, hipStream_t st) {
+    hipLaunchKernelGGL(linear_pad_kernel, dim3(linear_grid(drows * dw / 8)), dim3(256), 0, st, src, ss, rows, (int)cols, dst, drows, (int)dw);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+static int crop(const uint16_t* src, int64_t sw, uint16_t* dst, int64_t rows, int64_t cols, hipStream_t st) {
+    hipLaunchKernelGGL(linear_crop_kernel, dim3(linear_grid(rows * ((cols + 7) / 8))), dim3(256), 0, st, src, (int)sw, dst, rows, (int)cols);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int DT, int BP, int BQ, int WP, int WQ, int ST>
+static int run_linear(const LinearArgs& a, hipStream_t st) {
+    using G = GemmTile<LinearKind<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
+    if (!allow_lds<linear_kernel<DT, BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
+    const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
+    hipLaunchKernelGGL((linear_kernel<DT, BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int DT>
+static int linear_forward(LinearArgs a, char* ws, hipStream_t st) {
+    if (linear_streams(a.M, a.N, a.K)) {
+        const dim3 g((a.N + 15) / 16, (unsigned)((a.M + 15) / 16));
+        if (a.K > 1024) hipLaunchKernelGGL((linear_few_kernel<DT, 16>), g, dim3(1024), 0, st, a);
+        else hipLaunchKernelGGL((linear_few_kernel<DT, 4>), g, dim3(256), 0, st, a);
+        return hipGetLastError() == hipSuccess ? 0 : -1;
+    }
+    const LinearSpace s = forward_space(a.M, a.N, a.K);
+    if (s.x >= 0) {
+        uint16_t *x = reinterpret_cast<uint16_t*>(ws + s.x), *w = reinterpret_cast<uint16_t*>(ws + s.w);
+        const int64_t K8 = up8(a.K);
+        if (int r = pad(a.x, a.x_stride, a.M, a.K, x, a.M, K8, st)) return r;
+        if (int r = pad(a.w, a.w_stride, a.N, a.K, w, a.N, K8, st)) return r;
+        a.x = x, a.w = w, a.x_stride = a.w_stride = K8, a.K = (int)K8;
+    }
+    const Gemm16Plan p = linear_plan(a.M, a.N, a.K);
+    a.splits = p.splits;
+    a.part = s.part >= 0 ? reinterpret_cast<float*>(ws + s.part) : nullptr;
+    a.part_stride = up8(a.N);
+    const int r = p.tile == TILE_256        ? run_linear<DT, 256, 256, 2, 4, 2>(a, st)
+                  : p.tile == TILE_128      ? run_linear<DT, 128, 128, 2, 2, 2>(a, st)
+                  : p.tile == TILE_128_DEEP ? run_linear<DT, 128, 128, 2, 4, 4>(a, st)
+                                            : run_linear<DT, 64, 64, 2, 2, 4>(a, st);
+    if (r || a.splits == 1) return r;
+    hipLaunchKernelGGL(linear_join_kernel<DT>, dim3(linear_grid(a.M * ((a.N + 7) / 8))), dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+int launch_linear(const LinearArgs& a, void* ws, hipStream_t st) {
+    return a.dt == DT_BF16 ? linear_forward<DT_BF16>(a, static_cast<char*>(ws), st) : linear_forward<DT_F16>(a, static_cast<char*>(ws), st);
+}
+
+// Whether the products can take dy as it is (its rows then lie as an operand's do).
+static bool dz_is_dy(const LinearArgs& a) {
+    return a.act == ACT_NONE && a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dy) & 15) == 0 && a.dy_stride % 8 == 0 && a.dy_stride <= (1 << 22);
+}
+static LinearSpace backward_space(int64_t M, int64_t N, int64_t K) {
+    LinearSpace s;
+    const int64_t N8 = up8(N), K8 = up8(K);
+    s.dz = s.take(M * N8 * 2);
+    s.tops = s.take(4 * (LINEAR_TOPS + 1));
+    if (K % 8) s.x = s.take(M * K8 * 2), s.dx = s.take(M * K8 * 2);
+    if (K % 8 || N % 8) s.w = s.take(N8 * K8 * 2), s.dw = s.take(N8 * K8 * 2);
+    const int64_t parts = std::max({gemm16_part_floats(M, K8, N8), gemm16_part_floats(N8, K8, M), (M + DZ_ROWS - 1) / DZ_ROWS * N8});
+    s.part = s.take(4 * parts);
+    return s;
+}
+int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K) { return backward_space(M, N, K).bytes; }
+
+template <int DT>
+static int linear_backward(LinearArgs a, char* ws, hipStream_t st) {
+    const LinearSpace s = backward_space(a.M, a.N, a.K);
+    const int64_t N8 = up8(a.N), K8 = up8(a.K);
+    auto at = [&](int64_t o) { return reinterpret_cast<uint16_t*>(ws + o); };
+    const bool products = a.dx || a.dw, direct = dz_is_dy(a);
+    a.part = reinterpret_cast<float*>(ws + s.part);
+    a.part_stride = N8;
+    a.dz = products && !direct ? at(s.dz) : nullptr;
+    a.dz_stride = N8;
+    a.tops = reinterpret_cast<uint32_t*>(ws + s.tops);
+    a.unscale = reinterpret_cast<float*>(a.tops + LINEAR_TOPS);
+    a.ntops = 0;
+    if (DT == DT_F16 && a.dz && a.act != ACT_NONE && a.act != ACT_RELU) {
+        a.ntops = (int)std::min<int64_t>((a.M * ((a.N + 7) / 8) + 255) / 256, LINEAR_TOPS);
+        hipLaunchKernelGGL(linear_top_kernel<DT>, dim3(a.ntops), dim3(256), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return -1;
+    }
+    if (a.dz || a.dbias) {
+        const int parts = (int)((a.M + DZ_ROWS - 1) / DZ_ROWS);
+        hipLaunchKernelGGL(linear_dz_kernel<DT>, dim3(parts, (a.N + 255) / 256), dim3(256), 0, st, a);
+        if (hipGetLastError() != hipSuccess) return -1;
+        if (a.dbias) {
+            hipLaunchKernelGGL(linear_dbias_kernel, dim3((a.N + 63) / 64), dim3(1024), 0, st, a, parts);
+            if (hipGetLastError() != hipSuccess) return -1;
+        }
+    }
+    const uint16_t* dz = direct ? static_cast<const uint16_t*>(a.dy) : at(s.dz);
+    const int64_t ldz = direct ? a.dy_stride : N8;
+    const float* unscale = a.ntops ? a.unscale : nullptr;
+    if (a.dx) {
+        Gemm16Args g{};
+        g.p = a.w, g.ldp = a.w_stride;
+        if (s.w >= 0) {
+            if (int r = pad(a.w, a.w_stride, a.N, a.K, at(s.w), N8, K8, st)) return r;
+            g.p = at(s.w), g.ldp = K8;
+        }
+        g.q = dz, g.ldq = ldz, g.M = a.M, g.N = (int)K8, g.C = N8, g.unscale = unscale, g.part = a.part;
+        g.out = s.dx >= 0 ? at(s.dx) : a.dx, g.out_stride = K8;
+        if (int r = launch_gemm16_col_row(DT, g, st)) return r;
+        if (s.dx >= 0)
+            if (int r = crop(at(s.dx), K8, static_cast<uint16_t*>(a.dx), a.M, a.K, st)) return r;
+    }
+    if (a.dw) {
+        Gemm16Args g{};
+        g.p = a.x, g.ldp = a.x_stride;
+        if (s.x >= 0) {
+            if (int r = pad(a.x, a.x_stride, a.M, a.K, at(s.x), a.M, K8, st)) return r;
+            g.p = at(s.x), g.ldp = K8;
+        }
+        g.q = dz, g.ldq = ldz, g.M = N8, g.N = (int)K8, g.C = a.M, g.unscale = unscale, g.part = a.part;
+        g.out = s.dw >= 0 ? at(s.dw) : a.dw, g.out_stride = K8;
+        if (int r = launch_gemm16_col_col(DT, g, st)) return r;
+        if (s.dw >= 0)
+            if (int r = crop(at(s.dw), K8, static_cast<uint16_t*>(a.dw), a.N, a.K, st)) return r;
+    }
+    return 0;
+}
+int launch_linear_backward(const LinearArgs& a, void* ws, hipStream_t st) {
+    return a.dt == DT_BF16 ? linear_backward<DT_BF16>(a, static_cast<char*>(ws), st) : linear_backward<DT_F16>(a, static_cast<char*>(ws), st);
+}
+
+}  // namespace mi355moe

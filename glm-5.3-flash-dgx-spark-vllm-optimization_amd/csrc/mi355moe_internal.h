@@ -466,4 +466,132 @@ int launch_sigmoid(const float* g, int64_t n, int variant, float* out, hipStream
 int launch_rot_in(const void* x, int xdt, int64_t x_stride, const int* tok, const int* pe, const int64_t* suh_tab,
                   int P, int K, uint16_t* out, hipStream_t st);
 
+// Tokens sorted by expert, and back (dispatch.hip).
+struct SortArgs {
+    const void* ids;        // [P] int32 or int64
+    int ids64;
+    const int64_t* emap;    // optional [n_global]: global id -> local id, anything outside [0, n) dropped
+    int64_t n_global;
+    int n;
+    int64_t P;
+    int* row;               // [P] place of each pair, ~place where no local expert takes it
+    int* pair;              // [P] the inverse
+    int* offsets;           // [n + 1]
+    int* counts;            // [workgroups][n + 1] (sort_count_words of them)
+    int64_t chunk;          // pairs of a workgroup (set by the launcher)
+};
+int64_t sort_count_words(int64_t P, int64_t n);
+int launch_sort(const SortArgs& a, hipStream_t st);
+struct RowsArgs {
+    int dt;
+    int64_t T, P;
+    int H, topk;
+    const int* row;         // [P], of launch_sort
+    const void* x;          // [T][x_stride]: the tokens (scatter) or dout (gradient)
+    int64_t x_stride;
+    void* rows;             // [P][H]: written by scatter and gradient (there optional), read by gather
+    const void* y;          // [P][H]: the rows that dw reads
+    const void* w;          // [P] weights of type wdt (gather: nullptr for ones)
+    int wdt;
+    const void* shared;     // gather: optional [T][shared_stride]
+    int64_t shared_stride;
+    void* out;              // gather: [T][out_stride]
+    int64_t out_stride;
+    void* dw;               // gradient: optional [P] of type wdt
+};
+int launch_rows_scatter(const RowsArgs& a, hipStream_t st);
+int launch_rows_gather(const RowsArgs& a, hipStream_t st);
+int launch_rows_grad(const RowsArgs& a, hipStream_t st);
+
+// The norms around a block (norm.hip).
+enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_FULL = 3 };
+struct NormArgs {
+    int dt;                 // of branch, res, s, y and their gradients
+    int64_t rows;
+    int H;
+    const void* branch;     // [rows][branch_stride]
+    int64_t branch_stride;
+    const void* res;        // optional [rows][res_stride]
+    int64_t res_stride;
+    const void *post, *pre; // optional [H], of type wdt
+    int wdt;
+    const void* gate;       // [H], [rows] or [rows][H] by gate_kind, of type gdt
+    int gdt, gate_kind;
+    float eps, alpha, beta; // alpha: the residual's factor, beta: the branch's
+    void *s, *y;            // optional [rows][H] (y iff pre)
+    float* stats;           // [rows][2]: the two norms' factors (forward: optional)
+    // backward
+    const void* ds;         // optional [rows][ds_stride]
+    int64_t ds_stride;
+    const void* dy;         // optional [rows][dy_stride]
+    int64_t dy_stride;
+    void *dbranch, *dres;   // optional [rows][H]
+    void *dpost, *dpre;     // optional [H], of type wdt
+    void* dgate;            // optional, shaped like gate
+    float* part;            // norm_part_floats of them where dpost, dpre or a channel's dgate is asked for, else nullptr
+};
+int64_t norm_part_floats(int64_t rows, int H);
+int launch_norm(const NormArgs& a, hipStream_t st);
+int launch_norm_grad(const NormArgs& a, hipStream_t st);
+
+// 16-bit tile products (ffn.hip): out[m][n] = sum over k of P Q.
+struct Gemm16Args {
+    const uint16_t* p;      // ROW: [N][ldp], COL: [C][ldp]
+    const uint16_t* q;      // ROW: [M][ldq], COL: [C][ldq]
+    int64_t ldp, ldq;       // elements
+    int64_t M;
+    int N;
+    int64_t C;              // contraction
+    void* out;
+    int64_t out_stride;
+    int splits;
+    float* part;
+    const float* unscale;   // fp16: the factor of the sums (nullptr: none)
+};
+struct Gemm16Plan {
+    int tile, splits;
+};
+Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C);
+int64_t gemm16_part_floats(int64_t M, int64_t N, int64_t C);
+// P with the contraction as its row index, Q by rows or likewise
+int launch_gemm16_col_row(int dt, const Gemm16Args& a, hipStream_t st);
+int launch_gemm16_col_col(int dt, const Gemm16Args& a, hipStream_t st);
+
+// The dense product with its epilogue (linear.hip).
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
+struct LinearArgs {
+    int dt;                 // DT_F16 or DT_BF16
+    int64_t M;
+    int N, K;
+    const uint16_t* x;      // [M][x_stride]; K % 8 == 0: rows at 16-byte addresses (w's too)
+    int64_t x_stride;
+    const uint16_t* w;      // [N][w_stride]
+    int64_t w_stride;
+    const void* bias;       // optional [N] of type bdt
+    int bdt, act;
+    const void* res;        // optional [M][res_stride]
+    int64_t res_stride;
+    void* out;              // [M][out_stride]
+    int64_t out_stride;
+    float* z;               // [M][N]: x W^T + bias (forward: optional)
+    // set by the launchers
+    int splits;
+    float* part;            // [splits][M][part_stride]; backward: [row blocks][part_stride], or the products' parts
+    int64_t part_stride;
+    uint16_t* dz;           // [M][dz_stride]
+    int64_t dz_stride;
+    uint32_t* tops;
+    int ntops;
+    float* unscale;
+    // backward
+    const void* dy;         // [M][dy_stride]
+    int64_t dy_stride;
+    void *dx, *dw, *dbias;  // optional [M][K], [N][K], [N] of type bdt
+};
+constexpr int LINEAR_TOPS = 1024;
+int64_t linear_forward_bytes(int64_t M, int64_t N, int64_t K);
+int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K);
+int launch_linear(const LinearArgs& a, void* workspace, hipStream_t st);
+int launch_linear_backward(const LinearArgs& a, void* workspace, hipStream_t st);
+
 }  // namespace mi355moe

@@ -141,6 +141,22 @@ _SIGS = {
     "mi355moe_gated_backward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "mi355moe_gated_backward": (_int, [_c_p, _i64, _c_p, _c_p, _int, _i64, _i64, _i64, _c_p, _i64, _f, _c_p, _c_p, _c_p,
                                        _sz, _c_p]),
+    "mi355moe_sort_tokens_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mi355moe_sort_tokens": (_int, [_c_p, _int, _i64, _i64, _c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _sz, _c_p]),
+    "mi355moe_rows_to_experts": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _c_p, _c_p]),
+    "mi355moe_rows_from_experts": (_int, [_c_p, _int, _i64, _i64, _c_p, _i64, _c_p, _int, _c_p, _i64, _c_p, _i64, _c_p]),
+    "mi355moe_rows_from_experts_backward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _c_p, _int, _c_p, _c_p, _c_p, _c_p]),
+    "mi355moe_linear_forward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mi355moe_linear_forward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _i64, _c_p, _int, _int, _c_p, _i64, _c_p, _i64,
+                                       _c_p, _c_p, _sz, _c_p]),
+    "mi355moe_linear_backward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mi355moe_linear_backward": (_int, [_c_p, _i64, _c_p, _c_p, _int, _i64, _i64, _i64, _c_p, _i64, _i64, _int, _c_p, _c_p, _c_p,
+                                        _int, _c_p, _sz, _c_p]),
+    "mi355moe_norm_forward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _c_p, _c_p, _int, _c_p, _int, _int, _f, _f, _f, _c_p,
+                                     _c_p, _c_p, _c_p]),
+    "mi355moe_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "mi355moe_norm_backward": (_int, [_c_p, _i64, _c_p, _i64, _c_p, _int, _i64, _i64, _i64, _c_p, _i64, _c_p, _c_p, _int, _c_p, _int,
+                                      _int, _f, _f, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz, _c_p]),
     "mi355moe_sched_item": (_int, [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_int), ctypes.POINTER(_int),
                                    ctypes.POINTER(_int)]),
     "mi355moe_exl3_moe": (_int, [ctypes.POINTER(Exl3LayerDesc), _c_p, _i64, _c_p, _c_p, _c_p, _c_p, _i64, _i64,

@@ -1,0 +1,202 @@
+"""Tokens sorted by expert, and back with weights applied, with gradients.
+
+For callers whose experts are not this package's (its own experts sort inside their calls): 16-bit experts that are tuned, or
+an exchange between expert-parallel ranks.
+
+    plan = sort_tokens(topk_ids, n)                                # rows, by expert; no host synchronisation
+    rows = to_experts(x, plan)                                     # [T * topk, H]; expert e: plan.offsets[e] .. offsets[e + 1]
+    out = from_experts(experts(rows), topk_weights, plan, shared)  # [T, H]: shared + the weighted rows of each token
+
+  sort_tokens            the order: pairs by (local expert, pair index)
+  to_experts             every pair's token row in that order, differentiable in x
+  from_experts           the weighted sum per token in fp32, differentiable in rows, weights and shared
+  from_experts_backward  its explicit gradients (for capture; to_experts' gradient is from_experts without weights)
+
+Rows are fp32, fp16 or bf16. Every call runs on the current stream of its tensors' device; outputs and scratch come from torch's
+caching allocator. No atomics on values: two calls give the same bits.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, _row_stride,
+                  ids_dtype_code, weight_dtype_code)
+
+
+class SortedTokens:
+    """The order of a router's picks, made by sort_tokens. row int32 [T, topk]: each pair's row, or ~row (negative) for a pair
+    that no local expert takes (their rows come behind the others, and hold zeros); pair int32 [T * topk]: the pair of each
+    row, or ~pair; offsets int32 [n + 1]: where each expert's rows begin, offsets[n] the number of rows that experts have."""
+
+    __slots__ = ("row", "pair", "offsets", "tokens", "topk", "n")
+
+    def __init__(self, row: torch.Tensor, pair: torch.Tensor, offsets: torch.Tensor):
+        self.row, self.pair, self.offsets = row, pair, offsets
+        self.tokens, self.topk = row.shape
+        self.n = offsets.numel() - 1
+
+
+def sort_tokens(topk_ids: torch.Tensor, n: int, expert_map: torch.Tensor | None = None) -> SortedTokens:
+    """The pairs of topk_ids [T, topk] (int32 or int64) in the order (local expert, pair index). Without expert_map an id in [0,
+    n) is its local expert; with it ([ids] of global id -> local id) an id's entry is. Every other pair is dropped: it is no
+    expert's, its row comes behind offsets[n]."""
+    dev = _need_cuda(topk_ids, expert_map)
+    code = ids_dtype_code(topk_ids.dtype)
+    if topk_ids.dim() != 2 or topk_ids.shape[1] == 0:
+        raise ValueError(f"topk_ids must be [T, topk], got {tuple(topk_ids.shape)}")
+    if expert_map is not None:
+        if expert_map.dim() != 1 or expert_map.dtype.is_floating_point or expert_map.dtype == torch.bool:
+            raise ValueError(f"expert_map must be a vector of whole numbers, got {expert_map.dtype} {tuple(expert_map.shape)}")
+    T, topk = topk_ids.shape
+    L = _lib.lib()
+    nb = L.mi355moe_sort_tokens_workspace_bytes(T, topk, int(n))
+    with _on_device(dev):
+        ids = topk_ids.contiguous()
+        em = None if expert_map is None else expert_map.to(torch.int64).contiguous()
+        n_global = 0 if em is None else em.numel()
+        if em is not None and n_global == 0:
+            em = ids.new_zeros(1, dtype=torch.int64)             # (no id has an entry; the address only says that there is a map)
+        words = torch.empty(2 * T * topk + max(int(n), 0) + 1, dtype=torch.int32, device=dev)
+        row, pair, offsets = words[:T * topk], words[T * topk:2 * T * topk], words[2 * T * topk:]
+        ws = words.new_empty(nb // 4) if nb > 0 else None
+        _lib.check("mi355moe_sort_tokens", L.mi355moe_sort_tokens(
+            _addr(ids), code, T, topk, _addr(em), n_global, int(n), row.data_ptr(), pair.data_ptr(), offsets.data_ptr(), _addr(ws),
+            max(nb, 0), _raw_stream(dev)))
+    return SortedTokens(row.view(T, topk), pair, offsets)
+
+
+def _check(plan: SortedTokens, what: str, t: torch.Tensor, rows: int, dev: torch.device) -> int:
+    code = weight_dtype_code(t.dtype)
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] == 0:
+        raise ValueError(f"{what} must be [{rows}, H], got {tuple(t.shape)}")
+    if plan.row.device != dev:
+        raise ValueError(f"the order is on {plan.row.device}, {what} on {dev}")
+    return code
+
+
+def _to_experts(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    dev = _need_cuda(x)
+    code = _check(plan, "x", x, plan.tokens, dev)
+    H = x.shape[1]
+    with _on_device(dev):
+        x = _rows_any(_plain(x))
+        rows = x.new_empty((plan.tokens * plan.topk, H))
+        _lib.check("mi355moe_rows_to_experts", _lib.lib().mi355moe_rows_to_experts(
+            x.data_ptr(), code, plan.tokens, H, _row_stride(x), plan.row.data_ptr(), plan.topk, rows.data_ptr(), _raw_stream(dev)))
+    return rows
+
+
+def _check_back(rows, weights, plan, shared):
+    dev = _need_cuda(rows, weights, shared)
+    code = _check(plan, "rows", rows, plan.tokens * plan.topk, dev)
+    if weights is not None and weights.shape != plan.row.shape:
+        raise ValueError(f"weights must be {tuple(plan.row.shape)}, got {tuple(weights.shape)}")
+    if shared is not None and (shared.dtype != rows.dtype or shared.shape != (plan.tokens, rows.shape[1])):
+        raise ValueError(f"shared must be {rows.dtype} {(plan.tokens, rows.shape[1])}, got {shared.dtype} {tuple(shared.shape)}")
+    return dev, code
+
+
+def _from_experts(rows, weights, plan, shared):
+    dev, code = _check_back(rows, weights, plan, shared)
+    wcode = _lib.F32 if weights is None else weight_dtype_code(weights.dtype)
+    H = rows.shape[1]
+    with _on_device(dev):
+        rows = _plain(rows).contiguous()
+        weights = None if weights is None else _plain(weights).contiguous()
+        shared = None if shared is None else _rows_any(_plain(shared))
+        out = rows.new_empty((plan.tokens, H))
+        _lib.check("mi355moe_rows_from_experts", _lib.lib().mi355moe_rows_from_experts(
+            rows.data_ptr(), code, plan.tokens, H, plan.row.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared),
+            H if shared is None else _row_stride(shared), out.data_ptr(), H, _raw_stream(dev)))
+    return out
+
+
+def from_experts_backward(dout: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, plan: SortedTokens, need_rows: bool = True,
+                          need_weights: bool = True):
+    """(drows, dweights), None where not needed, of from_experts(rows, weights, plan) from dout [T, H]: drows in rows' dtype, zero
+    behind offsets[n]; dweights in weights' dtype, zero for the pairs that no local expert takes. shared's gradient is dout."""
+    dev, code = _check_back(rows, weights, plan, None)
+    _need_cuda(rows, dout)
+    _no_tangents("from_experts_backward", dout, rows, weights)
+    H = rows.shape[1]
+    if dout.dtype != rows.dtype or dout.shape != (plan.tokens, H):
+        raise ValueError(f"dout must be {rows.dtype} {(plan.tokens, H)}, got {dout.dtype} {tuple(dout.shape)}")
+    with _on_device(dev):
+        dout, rows, weights = _rows_any(_plain(dout)), _plain(rows).contiguous(), _plain(weights).contiguous()
+        drows = torch.empty_like(rows) if need_rows else None
+        dw = torch.empty_like(weights) if need_weights else None
+        _lib.check("mi355moe_rows_from_experts_backward", _lib.lib().mi355moe_rows_from_experts_backward(
+            dout.data_ptr(), code, plan.tokens, H, _row_stride(dout), plan.row.data_ptr(), plan.topk, weights.data_ptr(),
+            weight_dtype_code(weights.dtype), rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev)))
+    return drows, dw
+
+
+_NOT_CAPTURED = ("mi355moe: {} cannot {} during graph capture; capture it under torch.no_grad with its explicit gradient "
+                 "(from_experts without weights, from_experts_backward)")
+
+
+class _To(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.plan = plan
+        return _to_experts(x, plan)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows):
+        if _capturing(drows.device):
+            raise RuntimeError(_NOT_CAPTURED.format("to_experts", "run an eager call's backward pass"))
+        return _from_experts(drows, None, ctx.plan, None), None
+
+
+class _From(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, plan, shared):
+        ctx.plan = plan
+        ctx.save_for_backward(rows, weights)
+        return _from_experts(rows, weights, plan, shared)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        if _capturing(dout.device):
+            raise RuntimeError(_NOT_CAPTURED.format("from_experts", "run an eager call's backward pass"))
+        rows, weights = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        drows = dw = None
+        if weights is None:
+            drows = _to_experts(dout, ctx.plan) if need[0] else None
+        elif need[0] or need[1]:
+            drows, dw = from_experts_backward(dout, rows, weights, ctx.plan, need[0], need[1])
+        return drows, dw, None, dout if need[3] else None
+
+
+def _records(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def to_experts(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    """rows [T * topk, H] of x [T, H]: row plan.row[t, j] is x[t]; the rows behind plan.offsets[n] are zero. Differentiable once in
+    x by reverse mode (forward-mode derivatives are refused). A call that would record a gradient, and the backward pass of an
+    eager one, are refused while a graph is captured."""
+    _no_tangents("to_experts", x)
+    if _records(x):
+        if _capturing(x.device):
+            raise RuntimeError(_NOT_CAPTURED.format("to_experts", "record a gradient"))
+        return _To.apply(x, plan)
+    return _to_experts(x, plan)
+
+
+def from_experts(rows: torch.Tensor, weights: torch.Tensor | None, plan: SortedTokens,
+                 shared: torch.Tensor | None = None) -> torch.Tensor:
+    """out [T, H] = shared + the sum over j of weights[t, j] * rows[plan.row[t, j]] (weights None: ones), j ascending, in fp32 with
+    one rounding to rows' dtype. Pairs that no local expert takes count as nothing, whatever their weight. Differentiable once
+    in rows, weights and shared, with the limits of to_experts."""
+    _no_tangents("from_experts", rows, weights, shared)
+    if _records(rows, weights, shared):
+        if _capturing(rows.device):
+            raise RuntimeError(_NOT_CAPTURED.format("from_experts", "record a gradient"))
+        return _From.apply(rows, weights, plan, shared)
+    return _from_experts(rows, weights, plan, shared)

@@ -1,13 +1,21 @@
-"""The gated feed-forward block of a layer's shared expert and its gradient.
+"""The gated feed-forward block of a layer's shared expert and the dense product with its epilogue, with their gradients.
 
     [g | u] = x W13^T;  h = silu(min(g, L)) * clamp(u, -L, L)   (the limit iff L != 0)
 
 in fp16 or bf16 with fp32 sums and one rounding: both projections, the activation and the product. The
-shared expert is h W2^T (a plain library product); its output is what the routed experts' `accumulate` adds to.
+shared expert is h W2^T (`linear`, which can add the residual stream to it); its output is what the routed experts'
+`accumulate` adds to.
+
+    out = act(x W^T + bias) + residual
+
+in the same types, likewise rounded once: a dense product with its epilogue.
 
   gated            h, differentiable in x and w13
   gated_forward    h, or h and the fp32 [g | u] that the gradient reads
   gated_backward   (dx, dw13) from dh and [g | u]
+  linear           out, differentiable in x, w, bias and residual
+  linear_forward   out, or out and the fp32 z = x W^T + bias that the gradient reads
+  linear_backward  (dx, dw, dbias) from dout and z
 
 The gradient reads g and u in fp32 (8 bytes per token and column, kept from the forward pass): read back they cost a
 fifth of the time that computing them again would, and the gradients carry one rounding less than with 16-bit copies.
@@ -21,13 +29,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _raw_stream, act_dtype_code
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Values between two rows of t. One row (or none) has none: its stride(0) can be anything, also in what torch calls
-    contiguous."""
-    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
+from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _row_stride, _rows_any,
+                  act_dtype_code, weight_dtype_code)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -48,10 +51,6 @@ def _forward_bytes(T: int, H: int, I: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def _backward_bytes(T: int, H: int, I: int) -> int:
     return _lib.lib().mi355moe_gated_backward_workspace_bytes(T, H, I)
-
-
-def _plain(t: torch.Tensor) -> torch.Tensor:
-    return t.detach() if t.requires_grad else t
 
 
 def _check(x: torch.Tensor, w13: torch.Tensor) -> tuple[torch.device, int]:
@@ -151,3 +150,131 @@ def gated(x: torch.Tensor, w13: torch.Tensor, limit: float = 0.0) -> torch.Tenso
                                "ffn.gated_forward(save=True) and ffn.gated_backward")
         return _Gated.apply(x, w13, float(limit))
     return gated_forward(x, w13, limit)
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(backward: bool, M: int, K: int, N: int) -> int:
+    L = _lib.lib()
+    return (L.mi355moe_linear_backward_workspace_bytes if backward else L.mi355moe_linear_forward_workspace_bytes)(M, K, N)
+
+
+def _linear_operand(t: torch.Tensor) -> torch.Tensor:
+    """t [rows, K] as the product reads it: where K is a multiple of 8 its rows lie at 16-byte addresses."""
+    return _rows16(t) if t.shape[1] % 8 == 0 else _rows_any(t)
+
+
+def _check_linear(x, w, bias, activation, residual):
+    dev = _need_cuda(x, w, bias, residual)
+    _no_tangents("the dense product", x, w, bias, residual)
+    code = act_dtype_code(x.dtype)
+    if w.dtype != x.dtype:
+        raise ValueError(f"x is {x.dtype}, w {w.dtype}")
+    if w.dim() != 2 or w.numel() == 0:
+        raise ValueError(f"w must be [N, K], got {tuple(w.shape)}")
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x must be [..., {w.shape[1]}], got {tuple(x.shape)}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != w.shape[0]):
+        raise ValueError(f"bias must be {(w.shape[0],)}, got {tuple(bias.shape)}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != (*x.shape[:-1], w.shape[0])):
+        raise ValueError(f"residual must be {x.dtype} {(*x.shape[:-1], w.shape[0])}, got {residual.dtype} {tuple(residual.shape)}")
+    return dev, code, _lib.F32 if bias is None else weight_dtype_code(bias.dtype)
+
+
+def linear_forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                   residual: torch.Tensor | None = None, save: bool = False):
+    """out [..., N] of x [..., K] and w [N, K], or with save (out, z), z fp32 [rows, N] = x W^T + bias for linear_backward (None
+    without an activation, whose gradient does not read it). No gradient is recorded."""
+    dev, code, bcode = _check_linear(x, w, bias, activation, residual)
+    N, K = w.shape
+    with _on_device(dev):
+        x2 = _plain(x)
+        x2 = _linear_operand(x2 if x.dim() == 2 else x2.reshape(-1, K))
+        w2 = _linear_operand(_plain(w))
+        b = None if bias is None else _plain(bias).contiguous()
+        r = None if residual is None else _plain(residual)
+        if r is not None:
+            r = _rows_any(r if r.dim() == 2 else r.reshape(-1, N))
+        M = x2.shape[0]
+        out = x2.new_empty((*x.shape[:-1], N))
+        z = x2.new_empty((M, N), dtype=torch.float32) if save and activation is not None else None
+        nb = _linear_bytes(False, M, K, N)
+        ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
+        _lib.check("mi355moe_linear_forward", _lib.lib().mi355moe_linear_forward(
+            x2.data_ptr(), code, M, K, _row_stride(x2), w2.data_ptr(), N, _row_stride(w2), _addr(b), bcode, ACTIVATIONS[activation],
+            _addr(r), N if r is None else _row_stride(r), out.data_ptr(), N, _addr(z), _addr(ws), max(nb, 0), _raw_stream(dev)))
+    return (out, z) if save else out
+
+
+def linear_backward(dout: torch.Tensor, z: torch.Tensor | None, x: torch.Tensor, w: torch.Tensor, activation: str | None = None,
+                    bias_dtype: torch.dtype | None = None, need_dx: bool = True, need_dw: bool = True):
+    """(dx, dw, dbias) from dout [..., N], the forward's z, x and w: fp32 sums, dx and dw in x's dtype, dbias in bias_dtype (None
+    where there is no bias or the gradient is not needed); the sums' order does not vary. residual's gradient is dout."""
+    dev, code, _ = _check_linear(x, w, None, activation, None)
+    _need_cuda(x, dout, z)
+    _no_tangents("the dense product's backward", dout, z)
+    N, K = w.shape
+    if dout.dtype != x.dtype or dout.shape != (*x.shape[:-1], N):
+        raise ValueError(f"dout must be {x.dtype} {(*x.shape[:-1], N)}, got {dout.dtype} {tuple(dout.shape)}")
+    bcode = _lib.F32 if bias_dtype is None else weight_dtype_code(bias_dtype)
+    with _on_device(dev):
+        x2, d2 = _plain(x), _plain(dout)
+        if x.dim() != 2:
+            x2, d2 = x2.reshape(-1, K), d2.reshape(-1, N)
+        x2, w2, d2 = _linear_operand(x2), _linear_operand(_plain(w)), _rows_any(d2)
+        M = x2.shape[0]
+        if activation is None:
+            z = None
+        elif z is None or z.dtype != torch.float32 or tuple(z.shape) != (M, N) or not z.is_contiguous():
+            raise ValueError(f"z must be contiguous float32 {(M, N)}, got {None if z is None else (z.dtype, tuple(z.shape))}")
+        new = torch.zeros if M == 0 else torch.empty
+        dx = new(x.shape, dtype=x.dtype, device=dev) if need_dx else None
+        dw = new((N, K), dtype=x.dtype, device=dev) if need_dw else None
+        db = new(N, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
+        if M == 0:
+            return dx, dw, db
+        nb = _linear_bytes(True, M, K, N)
+        ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
+        _lib.check("mi355moe_linear_backward", _lib.lib().mi355moe_linear_backward(
+            d2.data_ptr(), _row_stride(d2), _addr(z), x2.data_ptr(), code, M, K, _row_stride(x2), w2.data_ptr(), N, _row_stride(w2),
+            ACTIVATIONS[activation], _addr(dx), _addr(dw), _addr(db), bcode, ws.data_ptr(), max(nb, 0), _raw_stream(dev)))
+    return dx, dw, db
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, activation, residual):
+        out, z = linear_forward(x, w, bias, activation, residual, save=True)
+        ctx.save_for_backward(x, w, z)
+        ctx.activation, ctx.bias_dtype = activation, None if bias is None else bias.dtype
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        if _capturing(dout.device):
+            raise RuntimeError("mi355moe: the backward pass of an eagerly recorded ffn.linear cannot be captured; capture "
+                               "ffn.linear_forward(save=True) and ffn.linear_backward")
+        x, w, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = linear_backward(dout, z, x, w, ctx.activation, ctx.bias_dtype if need[2] else None, need[0], need[1])
+        return dx, dw, db, None, dout if need[4] else None
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """out [..., N] = act(x W^T + bias) + residual of x [..., K], w [N, K], bias [N] (any of fp32, fp16, bf16) and residual [..., N];
+    activation None, "relu", "silu", "gelu" or "gelu_tanh". Differentiable once in the four tensors by reverse mode
+    (forward-mode derivatives are refused). While a graph is captured, a call that would record a gradient, and the backward
+    pass of an eager one, are refused; capture linear_forward(save=True) and linear_backward instead."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
+        dev = _check_linear(x, w, bias, activation, residual)[0]
+        if _capturing(dev):
+            raise RuntimeError("mi355moe: linear cannot record a gradient during graph capture; capture "
+                               "ffn.linear_forward(save=True) and ffn.linear_backward")
+        return _Linear.apply(x, w, bias, activation, residual)
+    return linear_forward(x, w, bias, activation, residual)

@@ -59,6 +59,23 @@ def _need_cuda(*ts: torch.Tensor) -> torch.device:
     return dev
 
 
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    return t.detach() if t.requires_grad else t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Values between two rows of t. One row (or none) has none: its stride(0) can be anything, also in what torch calls
+    contiguous."""
+    return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
+
+
+def _rows_any(t: torch.Tensor) -> torch.Tensor:
+    """t [rows, H] itself where its values lie back to back in rows that do not overlap, else a contiguous copy."""
+    if t.is_contiguous() or ((t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
+        return t
+    return t.contiguous()
+
+
 def _no_tangents(what: str, *ts: torch.Tensor | None) -> None:
     """Refuses tensors that carry a forward-mode derivative: the kernels read their values alone, and the result would come
     without its derivative. (Such a tensor has requires_grad False, under torch.no_grad too.)"""

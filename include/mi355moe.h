@@ -507,6 +507,92 @@ int mi355moe_gated_backward(const void* dh, int64_t dh_stride, const float* gu, 
                             int64_t hidden, int64_t x_stride, const void* w13, int64_t intermediate, float limit, void* dx,
                             void* dw13, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---------------------------------------------------------------- tokens sorted by expert, and back
+ *
+ * For callers whose experts are not this library's: an expert-parallel exchange, 16-bit experts that are tuned. The P =
+ * T * topk pairs of a router's ids lie in the order (local expert, pair). Pairs that no local expert takes (an id outside
+ * [0, n), or with a map one outside [0, n_global) or mapped outside [0, n)) come behind the others, in pair order, so that
+ * every row of a [P][H] buffer has one pair. T * topk <= 2^24, topk <= 32, n <= 4096, H <= 65536. Deterministic. */
+
+/* row[t * topk + j] = the pair's row r, or ~r (negative) for a pair that no local expert takes; pair[r] = the pair of row r,
+ * or ~pair; offsets [n + 1]: expert e has the rows offsets[e] .. offsets[e + 1] - 1. The workspace (may be NULL if the size
+ * query says 0) is 4-byte aligned and needs no initialisation. */
+int64_t mi355moe_sort_tokens_workspace_bytes(int64_t T, int64_t topk, int64_t n);
+int mi355moe_sort_tokens(const void* ids, int ids_dtype, int64_t T, int64_t topk, const int64_t* expert_map, int64_t n_global,
+                         int64_t n, int32_t* row, int32_t* pair, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                         hipStream_t stream);
+/* rows [T * topk][H]: rows[row[t][j]] = x[t], zero in the rows behind offsets[n]. F32, F16 or BF16, any address of that type. */
+int mi355moe_rows_to_experts(const void* x, int dtype, int64_t T, int64_t H, int64_t x_stride, const int32_t* row, int64_t topk,
+                             void* rows, hipStream_t stream);
+/* out[t] = shared[t] + sum over j of weights[t][j] * rows[row[t][j]], j ascending, fp32, rounded once; pairs that no local
+ * expert takes are skipped (neither their row nor their weight is read). weights (F32, F16 or BF16 [T][topk]) NULL: ones, which
+ * makes it the gradient of mi355moe_rows_to_experts; shared NULL: none. Outputs overlap no input. */
+int mi355moe_rows_from_experts(const void* rows, int dtype, int64_t T, int64_t H, const int32_t* row, int64_t topk,
+                               const void* weights, int weights_dtype, const void* shared, int64_t shared_stride, void* out,
+                               int64_t out_stride, hipStream_t stream);
+/* Its gradients: drows [T * topk][H] = weights[t][j] * dout[t] (zero in the rows behind offsets[n]); dweights [T][topk] (of the
+ * weights' type) = the fp32 dot product of dout[t] and the pair's row (0 for a pair that no local expert takes). Either may
+ * be NULL (not computed); rows may be NULL without dweights. */
+int mi355moe_rows_from_experts_backward(const void* dout, int dtype, int64_t T, int64_t H, int64_t dout_stride, const int32_t* row,
+                                        int64_t topk, const void* weights, int weights_dtype, const void* rows, void* drows,
+                                        void* dweights, hipStream_t stream);
+
+/* ---------------------------------------------------------------- the dense product with its epilogue */
+
+enum {
+    MI355MOE_ACT_NONE = 0,
+    MI355MOE_ACT_RELU = 1,
+    MI355MOE_ACT_SILU = 2,
+    MI355MOE_ACT_GELU = 3,      /* z * Phi(z) */
+    MI355MOE_ACT_GELU_TANH = 4  /* z * (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+};
+
+/* out [M][N] = act(x W^T + bias) + residual: fp32 sums and epilogue, rounded once. x [M][K] (row stride x_stride), w [N][K]
+ * (row stride w_stride), residual [M][N] (optional) and out of one dtype, F16 or BF16; bias [N] (optional) F32, F16 or BF16. z
+ * (optional, fp32 [M][N]) receives x W^T + bias for the backward pass. M <= 2^24, N <= 2^18, K <= 65536, any of them odd. K % 8 ==
+ * 0: x and w at 16-byte addresses, their strides multiples of 8 and at most 2^22; other K: any address of their type, the call
+ * lays padded copies out in the workspace. Outputs overlap no input. The workspace (may be NULL if the size query says 0) is 16-byte
+ * aligned, uninitialised. */
+int64_t mi355moe_linear_forward_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w, int64_t N,
+                            int64_t w_stride, const void* bias, int bias_dtype, int activation, const void* residual,
+                            int64_t residual_stride, void* out, int64_t out_stride, float* z, void* workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+/* Its gradients (the residual's is dy itself): dz = dy act'(z) from the forward's z (NULL without an activation); dx [M][K] =
+ * dz W, dw [N][K] = dz^T x, dbias [N] (bias_dtype) = the sums of dz over the rows; fp32 sums rounded once, deterministic. dbias
+ * sums dz in fp32; the products take it rounded once to dtype (F16: times a power of two that brings the call's largest into
+ * its range). Each gradient may be NULL (not computed). M >= 1 if dw or dbias is asked for. dy at any address and stride; x, w
+ * (read for dw, dx) as for the forward; K % 8 == 0: dx and dw at 16-byte addresses. */
+int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, const void* x, int dtype, int64_t M, int64_t K,
+                             int64_t x_stride, const void* w, int64_t N, int64_t w_stride, int activation, void* dx, void* dw,
+                             void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------- the norms around a block */
+
+enum { MI355MOE_GATE_NONE = 0, MI355MOE_GATE_CHANNEL = 1, MI355MOE_GATE_TOKEN = 2, MI355MOE_GATE_FULL = 3 };
+
+/* The norm after a block, its gate, the scaled residual sum and the norm before the next block, in one pass:
+ *   u = branch r(branch) post (branch where post is NULL);  s = residual_scale residual + scale gate u;  y = s r(s) pre
+ * with r(v) = 1 / sqrt(mean of v^2 over the row + eps), in fp32, s and y rounded once (y goes by the unrounded s). branch
+ * [rows][H], residual (optional), s and y of one dtype, F32, F16 or BF16; s and y have rows back to back. post and pre (each
+ * optional, [H]) of one dtype, gate [H] (CHANNEL), [rows] (TOKEN) or [rows][H] (FULL) of its own. s may be NULL where y is asked
+ * for; y iff pre. stats (optional, fp32 [rows][2]): r(branch) and r(s), for the backward pass. Any address of a tensor's type;
+ * H <= 16384, rows <= 2^26. Outputs overlap no input. */
+int mi355moe_norm_forward(const void* branch, int dtype, int64_t rows, int64_t H, int64_t branch_stride, const void* residual,
+                          int64_t residual_stride, const void* post, const void* pre, int weights_dtype, const void* gate,
+                          int gate_dtype, int gate_kind, float eps, float scale, float residual_scale, void* s, void* y,
+                          float* stats, hipStream_t stream);
+/* Its gradients from ds and dy (one may be NULL: zero) and the forward's inputs and stats: dbranch, dresidual [rows][H], dpost,
+ * dpre [H] (weights_dtype), dgate (shaped and typed like gate); fp32, rounded once, deterministic. Each may be NULL. The
+ * workspace is read where dpost, dpre or a CHANNEL gate's gradient is asked for (rows >= 1 then): 16-byte aligned, uninitialised. */
+int64_t mi355moe_norm_backward_workspace_bytes(int64_t rows, int64_t H);
+int mi355moe_norm_backward(const void* ds, int64_t ds_stride, const void* dy, int64_t dy_stride, const void* branch, int dtype,
+                           int64_t rows, int64_t H, int64_t branch_stride, const void* residual, int64_t residual_stride,
+                           const void* post, const void* pre, int weights_dtype, const void* gate, int gate_dtype, int gate_kind,
+                           float scale, float residual_scale, const float* stats, void* dbranch, void* dresidual, void* dpost,
+                           void* dpre, void* dgate, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
