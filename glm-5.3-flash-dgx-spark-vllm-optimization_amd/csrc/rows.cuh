@@ -19,6 +19,11 @@ __device__ __forceinline__ float any_value(const void* p, int dt, size_t i) {
     return dt == DT_F32 ? row_value<DT_F32>(p, i) : dt == DT_BF16 ? row_value<DT_BF16>(p, i) : row_value<DT_F16>(p, i);
 }
 
+__device__ __forceinline__ void unpack8_f32(u32x4 lo, u32x4 hi, float (&v)[8]) {
+    const f32x4 a = __builtin_bit_cast(f32x4, lo), b = __builtin_bit_cast(f32x4, hi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+}
 __device__ __forceinline__ void unpack8_bf16(u32x4 w, float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -40,9 +45,7 @@ __device__ __forceinline__ void load8(const void* p, size_t i, int n, float (&v)
     if (n >= 8) {
         if constexpr (DT == DT_F32) {
             const rows_u32x4* q = reinterpret_cast<const rows_u32x4*>(static_cast<const float*>(p) + i);
-            const f32x4 a = __builtin_bit_cast(f32x4, (u32x4)q[0]), b = __builtin_bit_cast(f32x4, (u32x4)q[1]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+            unpack8_f32(q[0], q[1], v);
         } else {
             const u32x4 w = *reinterpret_cast<const rows_u32x4*>(static_cast<const uint16_t*>(p) + i);
             if constexpr (DT == DT_BF16) unpack8_bf16(w, v);
@@ -91,10 +94,63 @@ __device__ __forceinline__ void store_any(void* p, int dt, size_t i, float v) {
     else static_cast<uint16_t*>(p)[i] = (uint16_t)(dt == DT_BF16 ? pack2<DT_BF16>(v, 0.0f) : pack2<DT_F16>(v, 0.0f));
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
+// Eight values as they lie in memory: loaded first, made floats where they are used, so that a kernel's loads are all on their
+// way before the first is waited for.
+template <int DT>
+struct Raw8 {
+    u32x4 w[DT == DT_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* p, size_t i, int n) {
+        if (n >= 8) {
+            const rows_u32x4* q = reinterpret_cast<const rows_u32x4*>(static_cast<const unsigned char*>(p) + i * (DT == DT_F32 ? 4 : 2));
+            w[0] = q[0];
+            if constexpr (DT == DT_F32) w[1] = q[1];
+        } else {
+            w[0] = u32x4{0, 0, 0, 0};
+            if constexpr (DT == DT_F32) w[1] = u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+            for (int j = 0; j < 7; ++j)
+                if (j < n) {
+                    if constexpr (DT == DT_F32) w[j >> 2][j & 3] = static_cast<const uint32_t*>(p)[i + j];
+                    else w[0][j >> 1] |= (uint32_t)static_cast<const uint16_t*>(p)[i + j] << (16 * (j & 1));
+                }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (DT == DT_F32) unpack8_f32(w[0], w[1], v);
+        else if constexpr (DT == DT_BF16) unpack8_bf16(w[0], v);
+        else unpack8_f16(w[0], v);
+    }
+};
+// The same for a type known at run time only.
+struct RawAny8 {
+    u32x4 w[2];
+    __device__ __forceinline__ void load(const void* p, int dt, size_t i, int n) {
+        if (dt == DT_F32) {
+            Raw8<DT_F32> r;
+            r.load(p, i, n);
+            w[0] = r.w[0], w[1] = r.w[1];
+        } else {
+            Raw8<DT_BF16> r;
+            r.load(p, i, n);
+            w[0] = r.w[0];
+        }
+    }
+    __device__ __forceinline__ void get(int dt, float (&v)[8]) const {
+        if (dt == DT_F32) unpack8_f32(w[0], w[1], v);
+        else if (dt == DT_BF16) unpack8_bf16(w[0], v);
+        else unpack8_f16(w[0], v);
+    }
+};
+
+// The sum over a wave, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+    const int lane = threadIdx.x & 63;
+    v += xor_lane<1>(v, lane);
+    v += xor_lane<2>(v, lane);
+    v += xor_lane<4>(v, lane);
+    v += xor_lane<8>(v, lane);
+    v += xor_lane<16>(v, lane);
+    return v + xor_lane<32>(v, lane);
 }
 
 }  // namespace mi355moe
