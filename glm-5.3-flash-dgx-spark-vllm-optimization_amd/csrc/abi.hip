@@ -2270,7 +2270,6 @@ int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int6
     a.out = out;
     a.out_stride = out_stride;
     a.z = z;
-    a.splits = 1;
     return rc_launch(launch_linear(a, workspace, stream));
 }
 
@@ -2289,7 +2288,6 @@ int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, 
     if (M == 0) return dw || dbias ? MI355MOE_ESHAPE : 0;
     if (!dy || !workspace || (activation != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return MI355MOE_EINVAL;
     if (int r = linear_operands(dw ? x : nullptr, dw ? x_stride : (K + 7) / 8 * 8, dx ? w : nullptr, dx ? w_stride : (K + 7) / 8 * 8, K)) return r;
-    if (K % 8 == 0 && (!rows16_ok(dx, 0) || !rows16_ok(dw, 0))) return MI355MOE_EINVAL;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return MI355MOE_EINVAL;
     if ((int64_t)workspace_bytes < linear_backward_bytes(M, N, K)) return MI355MOE_EWORKSPACE;
     LinearArgs a{};
@@ -2309,7 +2307,6 @@ int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, 
     a.dx = dx;
     a.dw = dw;
     a.dbias = dbias;
-    a.splits = 1;
     return rc_launch(launch_linear_backward(a, workspace, stream));
 }
 

@@ -282,6 +282,20 @@ __global__ __launch_bounds__(256) void gated_d_kernel(GatedArgs a) {
     }
 }
 
+struct Gemm16Args {
+    const uint16_t* p;      // ROW: [N][ldp], COL: [C][ldp]
+    const uint16_t* q;      // ROW: [M][ldq], COL: [C][ldq]
+    int64_t ldp, ldq;       // elements
+    int64_t M;
+    int N;
+    int64_t C;              // contraction
+    void* out;
+    int64_t out_stride;
+    int splits;
+    float* part;
+    const float* unscale;   // fp16: the factor of the sums (nullptr: none)
+};
+
 // out[m][n] = sum over k of P Q, dtype DT, or fp32 partials of the contraction's splits (grid y). Bound: the matrix cores, busy
 // in 60 and 64 % of the cycles at 1.8 GHz (memory-bound kernels run at 2.2); 8192 tokens, 4096 -> 2048, 275 GFLOP each: dx (8192 x
 // 4096 from 4096) 235 us, dw (4096 x 4096 from 8192) 230, 1.17 and 1.19 PFLOP/s (library products of these sizes and layouts: 238
@@ -376,10 +390,13 @@ int64_t gated_forward_floats(int64_t T, int64_t K, int64_t N) {
     return s > 1 ? s * T * 2 * N : 0;
 }
 
+struct Gemm16Plan {
+    int tile, splits;
+};
 // By the rule of plan_mx_matmul. us by kind 256 / 128 / 128 deep / 64, dx of 4096 columns from 2048: T = 128 42 / 29 / 20.7 /
 // 20.4, 512 46 / 32 / 24.0 / 22.5 (512 tiles of 64: the deep one is taken), 1791 51 / 41.8 / 47.7 / 61.7, 4096 71 / 83 / 95 / 120.
 // A long contraction of few tiles (128 x 512 x 8192): 36 us, in 4 parts 21.
-Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
+static Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C) {
     Gemm16Plan p{TILE_256, 1};
     auto tiles = [&](int64_t b) { return ((N + b - 1) / b) * ((M + b - 1) / b); };
     const int64_t t64 = tiles(64), stages = (C + 63) / 64;
@@ -413,19 +430,12 @@ static int gemm16(Gemm16Args a, hipStream_t st) {
     return 0;
 }
 
-int64_t gemm16_part_floats(int64_t M, int64_t N, int64_t C) {
-    const int s = plan_gemm16(M, N, C).splits;
-    return s > 1 ? s * M * N : 0;
-}
-int launch_gemm16_col_row(int dt, const Gemm16Args& a, hipStream_t st) {
-    return dt == DT_BF16 ? gemm16<DT_BF16, LAY_COL, LAY_ROW>(a, st) : gemm16<DT_F16, LAY_COL, LAY_ROW>(a, st);
-}
-int launch_gemm16_col_col(int dt, const Gemm16Args& a, hipStream_t st) {
-    return dt == DT_BF16 ? gemm16<DT_BF16, LAY_COL, LAY_COL>(a, st) : gemm16<DT_F16, LAY_COL, LAY_COL>(a, st);
-}
-
 int64_t gated_part_floats(int64_t T, int64_t K, int64_t N) {
-    return std::max(gemm16_part_floats(T, K, 2 * N), gemm16_part_floats(2 * N, K, T));
+    const Gemm16Plan px = plan_gemm16(T, K, 2 * N), pw = plan_gemm16(2 * N, K, T);
+    int64_t f = 0;
+    if (px.splits > 1) f = std::max(f, px.splits * T * K);
+    if (pw.splits > 1) f = std::max(f, pw.splits * 2 * N * K);
+    return f;
 }
 
 template <int DT, int BP, int BQ, int WP, int WQ, int ST>

@@ -14,6 +14,38 @@
 
 namespace mi355moe {
 
+// One product with its epilogue, as the kernels take it: out [M][N], out[m][n] = act(sum over k of P Q + bias) + res.
+struct ProductArgs {
+    const uint16_t* p;      // ROW: [N][ldp], COL: [K][ldp]
+    const uint16_t* q;      // ROW: [M][ldq], COL: [K][ldq]
+    int64_t ldp, ldq;       // elements
+    int pcols, qcols;       // COL: how many of a row's values may be read (multiples of 8)
+    int64_t M, K;
+    int N;
+    const void* bias;       // optional [N] of type bdt
+    int bdt, act;
+    const void* res;        // optional [M][res_stride]
+    int64_t res_stride;
+    float* z;               // optional [M][N]: before the activation
+    const float* unscale;   // optional: a factor of the sums
+    void* out;
+    int64_t out_stride;
+    int splits;             // parts of the contraction
+    float* part;            // [splits][M][part_stride] (splits > 1)
+    int64_t part_stride;
+};
+// What the gradient's own kernels take beside the call's arguments.
+struct SlopeArgs {
+    LinearArgs a;
+    uint16_t* dz;           // optional [M][dz_stride]
+    int64_t dz_stride;
+    uint32_t* tops;
+    int ntops;
+    float* unscale;
+    float* part;            // [row blocks][part_stride]
+    int64_t part_stride;
+};
+
 template <int DT>
 struct LinearKind {
     static constexpr int value = DT == DT_BF16 ? MM_BF16 : MM_F16;
@@ -74,9 +106,9 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     return 1.0f;
 }
 
-// Columns c .. of row m from their sums: bias (b: theirs), activation, residual and the one rounding.
+// Columns c .. of row m from their sums: bias (b: theirs), activation, residual (r: theirs) and the one rounding.
 template <int DT>
-__device__ __forceinline__ void linear_out8(const LinearArgs& a, int64_t m, int c, float (&v)[8], const float (&b)[8]) {
+__device__ __forceinline__ void product_out8(const ProductArgs& a, int64_t m, int c, float (&v)[8], const float (&b)[8], const Raw8<DT>& r8) {
     const int n = a.N - c;
     if (a.bias)
 #pragma unroll
@@ -85,7 +117,7 @@ __device__ __forceinline__ void linear_out8(const LinearArgs& a, int64_t m, int 
     activate(a.act, v);
     if (a.res) {
         float r[8];
-        load8<DT>(a.res, (size_t)m * a.res_stride + c, n, r);
+        r8.get(r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += r[j];
     }
@@ -109,25 +141,27 @@ __device__ __forceinline__ u32x4 row_chunk(const uint16_t* row, int i, int K) {
     return v;
 }
 
-// grid (ceil(N / 16), ceil(M / 16)), W waves: 16 weight rows as one 16-row MFMA operand, for 16 rows of x; any K, stride and
+// grid (ceil(N / 16), ceil(M / 16)), eight waves: 16 weight rows as one 16-row MFMA operand, for 16 rows of x; any K, stride and
 // address. Lane (c = lane % 16, g = lane / 16) holds the chunks g, 4 + g, 8 + g, 12 + g of weight row c and of row c of x, so
 // that a load takes 64 bytes in a row (128 of the contraction a wave step, in the same order on both sides); the contraction is
 // cut over the waves, whose sums join in LDS in wave order.
-template <int DT, int W>
-__global__ __launch_bounds__(64 * W) void linear_few_kernel(LinearArgs a) {
+constexpr int FEW_WAVES = 8;
+template <int DT>
+__global__ __launch_bounds__(64 * FEW_WAVES) void linear_few_kernel(ProductArgs a) {
+    constexpr int W = FEW_WAVES;
     __shared__ __align__(16) float red[W][256];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n0 = blockIdx.x * 16;
     const int64_t m0 = (int64_t)blockIdx.y * 16;
     const int rows = (int)min((int64_t)16, a.M - m0);
-    const int chunks = (a.K + 7) >> 3;
-    const uint16_t* w = a.w + (size_t)min(n0 + c, a.N - 1) * a.w_stride;
-    const uint16_t* x = a.x + (size_t)(m0 + min(c, rows - 1)) * a.x_stride;
+    const int K = (int)a.K, chunks = (K + 7) >> 3;
+    const uint16_t* w = a.p + (size_t)min(n0 + c, a.N - 1) * a.ldp;
+    const uint16_t* x = a.q + (size_t)(m0 + min(c, rows - 1)) * a.ldq;
     f32x4 acc = {};
     for (int b0 = wv * 16; b0 < chunks; b0 += 16 * W) {
         u32x4 p[4], q[4];
-        if ((b0 + 16) * 8 <= a.K) {                                  // (uniform)
+        if ((b0 + 16) * 8 <= K) {                                  // (uniform)
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const rows_u32x4*>(w + 8 * (b0 + g + 4 * i));
 #pragma unroll
@@ -135,8 +169,8 @@ __global__ __launch_bounds__(64 * W) void linear_few_kernel(LinearArgs a) {
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[i] = row_chunk(w, b0 + g + 4 * i, a.K);
-                q[i] = row_chunk(x, b0 + g + 4 * i, a.K);
+                p[i] = row_chunk(w, b0 + g + 4 * i, K);
+                q[i] = row_chunk(x, b0 + g + 4 * i, K);
             }
         }
 #pragma unroll
@@ -161,25 +195,29 @@ __global__ __launch_bounds__(64 * W) void linear_few_kernel(LinearArgs a) {
 
 // A workgroup's BP columns x BQ rows, the contraction in a.splits parts (grid y). The sums pass through LDS in fp32, 32 rows of a
 // wave at a time, so that a lane ends up with eight columns of a row: bias, residual and output are whole 16-byte accesses
-// in whole lines, and the residual is added before the one rounding.
-template <int DT, int BP, int BQ, int WP, int WQ, int ST>
-__global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(LinearArgs a, int nt, int mt) {
-    using G = GemmTile<LinearKind<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
+// in whole lines, and the residual is added before the one rounding; it is requested before the sums go to LDS.
+template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
+__global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(ProductArgs a, int nt, int mt) {
+    using G = GemmTile<LinearKind<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int2 tile = tile_order(blockIdx.x, nt, mt);
     const int n0 = tile.x * BP;
     const int64_t m0 = (int64_t)tile.y * BQ;
-    const int stages = (a.K + SB / 2 - 1) / (SB / 2), per = (stages + a.splits - 1) / a.splits;
+    const int stages = (int)((a.K + SB / 2 - 1) / (SB / 2)), per = (stages + a.splits - 1) / a.splits;
     const int kb0 = blockIdx.y * per, kb1 = min(stages, kb0 + per);
-    const uint32_t wp = 2u * (uint32_t)a.w_stride, xp = 2u * (uint32_t)a.x_stride;
+    const uint32_t ldp = 2u * (uint32_t)a.ldp, ldq = 2u * (uint32_t)a.ldq;
     const int pl = min(BP, a.N - n0) - 1, ql = (int)min((int64_t)BQ, a.M - m0) - 1;
     G t;
-    t.p.init_row(uniform_ptr(a.w + (size_t)n0 * a.w_stride + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, pl) * wp; });
-    t.q.init_row(uniform_ptr(a.x + (size_t)m0 * a.x_stride + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, ql) * xp; });
-    const int tail = kb1 == stages ? a.K % (SB / 2) / 8 : 0;
-    if (kb0 < kb1) t.run(lds, kb0, kb1, tail, tail, 0, 0);
+    if constexpr (PL == LAY_ROW)
+        t.p.init_row(uniform_ptr(a.p + (size_t)n0 * a.ldp + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, pl) * ldp; });
+    else t.p.init_col(uniform_ptr(a.p + (size_t)kb0 * (SB / 2) * a.ldp + n0), wv, lane, ldp, min(BP, a.pcols - n0));
+    if constexpr (QL == LAY_ROW)
+        t.q.init_row(uniform_ptr(a.q + (size_t)m0 * a.ldq + (size_t)kb0 * (SB / 2)), wv, lane, [&](int r) { return (uint32_t)min(r, ql) * ldq; });
+    else t.q.init_col(uniform_ptr(a.q + (size_t)kb0 * (SB / 2) * a.ldq + m0), wv, lane, ldq, (int)min((int64_t)BQ, a.qcols - m0));
+    const int left = kb1 == stages ? (int)(a.K % (SB / 2)) : 0;      // (ROW operands hold whole chunks of eight, zeros in the last)
+    if (kb0 < kb1) t.run(lds, kb0, kb1, PL == LAY_ROW ? (left + 7) >> 3 : left, QL == LAY_ROW ? (left + 7) >> 3 : left, ldp, ldq);
     else
 #pragma unroll
         for (int i = 0; i < G::TP; ++i)
@@ -189,15 +227,23 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(LinearArgs a, i
     constexpr int UNITS = 8 * G::TP, CH = UNITS / 2;                 // 16-byte units and 8-column chunks of a wave's row
     static_assert(G::NW * 32 * 16 * UNITS <= G::LDS, "the stages hold the waves' rows");
     unsigned char* mine = lds + wv * (32 * 16 * UNITS);
-    const int64_t m1 = m0 + (wv / WP) * (BQ / WQ);
+    const int64_t m1 = m0 + (wv / WP) * (BQ / WQ) + lane / CH;
     const int c = n0 + (wv % WP) * (BP / WP) + 8 * (lane % CH), n = a.N - c;
     const int m = lane & 31, h = lane >> 5;
     float b[8] = {};
     if (a.bias && a.splits == 1) load8_any(a.bias, a.bdt, c, n, b);
+    const float f = a.unscale ? *a.unscale : 1.0f;
     float* part = a.splits > 1 ? a.part + (size_t)blockIdx.y * a.M * a.part_stride : nullptr;
     __syncthreads();                                                 // no wave reads a stage any more
 #pragma unroll
     for (int j = 0; j < G::TQ; ++j) {
+        Raw8<DT> r8[CH / 2];
+        if (a.res && !part)                                          // (uniform)
+#pragma unroll
+            for (int s = 0; s < CH / 2; ++s) {
+                const int64_t mm = m1 + 32 * j + s * (64 / CH);
+                r8[s].load(a.res, (size_t)mm * a.res_stride + c, mm < a.M ? n : 0);
+            }
         unsigned char* row = mine + m * (16 * UNITS);
 #pragma unroll
         for (int i = 0; i < G::TP; ++i)
@@ -213,11 +259,11 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(LinearArgs a, i
             const int rr = s * (64 / CH) + lane / CH, u = 2 * (lane % CH), x = rr & (UNITS - 1);
             const unsigned char* from = mine + rr * (16 * UNITS);
             const f32x4 lo = *reinterpret_cast<const f32x4*>(from + ((u ^ x) << 4)), hi = *reinterpret_cast<const f32x4*>(from + (((u + 1) ^ x) << 4));
-            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            const int64_t mm = m1 + 32 * j + rr;
+            float v[8] = {lo[0] * f, lo[1] * f, lo[2] * f, lo[3] * f, hi[0] * f, hi[1] * f, hi[2] * f, hi[3] * f};
+            const int64_t mm = m1 + 32 * j + s * (64 / CH);
             if (mm >= a.M || n <= 0) continue;
             if (part) store8<DT_F32>(part, (size_t)mm * a.part_stride + c, 8, v);
-            else linear_out8<DT>(a, mm, c, v, b);
+            else product_out8<DT>(a, mm, c, v, b, r8[s]);
         }
         asm volatile("" ::: "memory");
     }
@@ -225,56 +271,47 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(LinearArgs a, i
 
 // out from the sums of the contraction's parts [splits][M][part_stride], added in order: eight columns a thread.
 template <int DT>
-__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
+__global__ __launch_bounds__(256) void linear_join_kernel(ProductArgs a) {
     const int per = (a.N + 7) / 8;
     const int64_t items = a.M * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / per;
         const int c = (int)(i - m * per) * 8;
         float v[8] = {}, b[8] = {};
+        Raw8<DT> r8;
+        if (a.res) r8.load(a.res, (size_t)m * a.res_stride + c, a.N - c);
+        if (a.bias) load8_any(a.bias, a.bdt, c, a.N - c, b);
         for (int s = 0; s < a.splits; ++s) {
             float p[8];
             load8<DT_F32>(a.part, ((size_t)s * a.M + m) * a.part_stride + c, 8, p);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += p[j];
         }
-        if (a.bias) load8_any(a.bias, a.bdt, c, a.N - c, b);
-        linear_out8<DT>(a, m, c, v, b);
+        product_out8<DT>(a, m, c, v, b, r8);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ copies
 
-// dst [drows][dw] = src [rows][cols] (row stride ss), the rest zero: dw and dst's rows in whole 16 bytes.
-__global__ __launch_bounds__(256) void linear_pad_kernel(const uint16_t* __restrict__ src, int64_t ss, int64_t rows, int cols,
-                                                         uint16_t* __restrict__ dst, int64_t drows, int dw) {
-    const int per = dw / 8;
-    const int64_t items = drows * per;
+// Up to two matrices of `cols` columns copied to rows of whole 16 bytes ([rows][wide], the columns behind `cols` zero), as the
+// tiles read them.
+struct PadArgs {
+    const uint16_t* src[2];
+    int64_t stride[2], rows[2];
+    uint16_t* dst[2];
+    int cols, wide;
+};
+__global__ __launch_bounds__(256) void linear_pad_kernel(PadArgs a) {
+    const int per = a.wide / 8;
+    const int64_t items = (a.rows[0] + a.rows[1]) * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
+        int64_t r = i / per;
         const int c = (int)(i - r * per) * 8;
-        u32x4 v = {0, 0, 0, 0};
-        if (r < rows) {
-            const uint16_t* p = src + (size_t)r * ss + c;
-            if (c + 8 <= cols) v = *reinterpret_cast<const rows_u32x4*>(p);
-            else
-                for (int j = 0; c + j < cols; ++j) v[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-        }
-        *reinterpret_cast<u32x4*>(dst + (size_t)r * dw + c) = v;
-    }
-}
-// dst [rows][cols] = the first columns of src [rows][sw].
-__global__ __launch_bounds__(256) void linear_crop_kernel(const uint16_t* __restrict__ src, int sw, uint16_t* __restrict__ dst, int64_t rows, int cols) {
-    const int per = (cols + 7) / 8;
-    const int64_t items = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
-        const int c = (int)(i - r * per) * 8;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(src + (size_t)r * sw + c);
-        uint16_t* p = dst + (size_t)r * cols + c;
-        if (c + 8 <= cols) *reinterpret_cast<rows_u32x4*>(p) = v;
-        else
-            for (int j = 0; c + j < cols; ++j) p[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+        const int k = r >= a.rows[0];
+        r -= k ? a.rows[0] : 0;
+        Raw8<DT_BF16> v;
+        v.load(k ? a.src[1] : a.src[0], (size_t)r * (k ? a.stride[1] : a.stride[0]) + c, a.cols - c);
+        *reinterpret_cast<u32x4*>((k ? a.dst[1] : a.dst[0]) + (size_t)r * a.wide + c) = v.w[0];
     }
 }
 
@@ -297,7 +334,8 @@ __device__ __forceinline__ void slope8(const LinearArgs& a, int64_t m, int c, fl
 // The largest finite magnitude of dz, as fp32 bits, of each workgroup's share (fp16 only: dz = dy act'(z) can lie among fp16's
 // subnormals, or beyond its range, where the sums over it are ordinary fp16 numbers).
 template <int DT>
-__global__ __launch_bounds__(256) void linear_top_kernel(LinearArgs a) {
+__global__ __launch_bounds__(256) void linear_top_kernel(SlopeArgs g) {
+    const LinearArgs& a = g.a;
     __shared__ uint32_t red[4];
     const int per = (a.N + 7) / 8;
     const int64_t items = a.M * per;
@@ -316,7 +354,7 @@ __global__ __launch_bounds__(256) void linear_top_kernel(LinearArgs a) {
     for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) a.tops[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+    if (threadIdx.x == 0) g.tops[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
 }
 // k of the 2^k that brings the largest of `n` maxima into [2^14, 2^15) (0 where all are zero): every thread gets it.
 __device__ __forceinline__ int linear_shift(const uint32_t* tops, int n) {
@@ -332,17 +370,18 @@ __device__ __forceinline__ int linear_shift(const uint32_t* tops, int n) {
 }
 
 // dz of 256 columns and DZ_ROWS rows: 32 threads across the columns, eight values each, eight down the rows. dz [M][dz_stride]
-// in the operand type (its columns behind N zero), where a.dz is set; the sums of the unrounded dz over the workgroup's rows
+// in the operand type (its columns behind N zero), where g.dz is set; the sums of the unrounded dz over the workgroup's rows
 // to part [grid x][part_stride] where that is set.
 template <int DT>
-__global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a) {
+__global__ __launch_bounds__(256) void linear_dz_kernel(SlopeArgs g) {
+    const LinearArgs& a = g.a;
     __shared__ __align__(16) float red[8][256];
     float f = 1.0f;
     if constexpr (DT == DT_F16)
-        if (a.ntops) {                                               // (uniform)
-            const int k = linear_shift(a.tops, a.ntops);
+        if (g.ntops) {                                               // (uniform)
+            const int k = linear_shift(g.tops, g.ntops);
             f = __builtin_bit_cast(float, (uint32_t)(127 + k) << 23);
-            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.unscale = __builtin_bit_cast(float, (uint32_t)(127 - k) << 23);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *g.unscale = __builtin_bit_cast(float, (uint32_t)(127 - k) << 23);
         }
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int c = blockIdx.y * 256 + tx * 8;
@@ -354,10 +393,10 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a) {
             slope8<DT>(a, m, c, d);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += d[j];
-            if (a.dz) {
+            if (g.dz) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) d[j] = c + j < a.N ? d[j] * f : 0.0f;
-                store8<DT>(a.dz, (size_t)m * a.dz_stride + c, 8, d);
+                store8<DT>(g.dz, (size_t)m * g.dz_stride + c, 8, d);
             }
         }
     if (!a.dbias) return;                                            // (uniform)
@@ -368,10 +407,11 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
-    a.part[(size_t)blockIdx.x * a.part_stride + col] = s;
+    g.part[(size_t)blockIdx.x * g.part_stride + col] = s;
 }
 // dbias: the parts' sums in order, 64 columns a workgroup, the parts cut over its sixteen waves.
-__global__ __launch_bounds__(1024) void linear_dbias_kernel(LinearArgs a, int parts) {
+__global__ __launch_bounds__(1024) void linear_dbias_kernel(SlopeArgs g, int parts) {
+    const LinearArgs& a = g.a;
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int c = blockIdx.x * 64 + lane;
@@ -379,7 +419,7 @@ __global__ __launch_bounds__(1024) void linear_dbias_kernel(LinearArgs a, int pa
     float v = 0.0f;
     if (c < a.N) {
 #pragma unroll 8
-        for (int g = g0; g < g1; ++g) v += a.part[(size_t)g * a.part_stride + c];
+        for (int i = g0; i < g1; ++i) v += g.part[(size_t)i * g.part_stride + c];
     }
     red[wv][lane] = v;
     __syncthreads();
@@ -395,15 +435,86 @@ __global__ __launch_bounds__(1024) void linear_dbias_kernel(LinearArgs a, int pa
 static unsigned linear_grid(int64_t items) { return (unsigned)std::min<int64_t>((items + 255) / 256, 8192); }
 static int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
 
-static bool linear_streams(int64_t M, int64_t N, int64_t K) {
-    (void)K;
-    return M <= 16 || (M + 15) / 16 * ((N + 15) / 16) <= 512;
+// Which kernel, and in how many parts of the contraction, by an estimate of each one's time in us. Measured per stage of 64 (one
+// workgroup a CU; 64 x 64 also two): 64 x 64 0.30 (0.49 for two), 128 x 128 0.54, 256 x 128 0.91, 256 x 256 1.56, and per tile for
+// its ends 0.9 (2.8), 6, 11, 24: small tiles bring more workgroups, large ones read less. Parts pay a second launch and their
+// fp32 sums' way through memory. us measured, 64 / 128 / 256 x 128 / 256 (N = 4096 from 1024): M = 256 8.7 / 13.0 / 19.9 / 35, 768 19.7
+// / 16.5 / 24.3 / 44, 2048 43.7 / 32.6 / 27.4 / 46, 8192 - / 127 / 106 / 101; N = 1024 from 4096, M = 128 19.3, in four parts 11.9.
+struct ProductPlan {
+    int tile, splits;
+    double us;
+};
+static double tiles_us(int tile, int64_t tiles, int64_t stages) {
+    if (tile == TILE_64) {
+        const double one = 0.30 * stages + 0.9, two = 0.49 * stages + 2.8;
+        const int64_t rest = tiles % 512;
+        return 3.0 + (tiles / 512) * two + (rest == 0 ? 0.0 : rest <= 256 ? one : two);
+    }
+    const int64_t rounds = (tiles + 255) / 256;
+    return 3.0 + rounds * (tile == TILE_128_DEEP ? 0.54 * stages + 6.0 : tile == TILE_256_128 ? 0.91 * stages + 11.0 : 1.56 * stages + 24.0);
 }
-static Gemm16Plan linear_plan(int64_t M, int64_t N, int64_t K) { return plan_gemm16(M, N, K); }
+static ProductPlan plan_product(int64_t M, int64_t N, int64_t K) {
+    auto count = [&](int64_t p, int64_t q) { return ((N + p - 1) / p) * ((M + q - 1) / q); };
+    const int64_t stages = (K + 63) / 64;
+    ProductPlan best{TILE_64, 1, 1e30};
+    const struct {
+        int tile;
+        int64_t tiles;
+    } kinds[] = {{TILE_64, count(64, 64)}, {TILE_128_DEEP, count(128, 128)}, {TILE_256_128, count(256, 128)}, {TILE_256, count(256, 256)}};
+    for (const auto& k : kinds)
+        for (int s = 1; s <= 16; s *= 2) {
+            if (s > 1 && (k.tile == TILE_256 || k.tile == TILE_256_128 || stages / s < 8 || k.tiles * s > 512)) break;
+            double us = tiles_us(k.tile, k.tiles * s, (stages + s - 1) / s);
+            if (s > 1) us += 2.0 + s * (double)(M * N) * 8.0 / 6e6;
+            if (us < best.us) best = {k.tile, s, us};
+        }
+    return best;
+}
+// Few rows stream the weights. The streaming kernel takes about 3 us and, for every 256 workgroups of 16 columns and 16 rows, what
+// one CU takes to read its rows of both operands (7 us for 4096 of the contraction). us streamed / by tiles: 1024 from 4096, M = 64
+// 9.6 / 11.3, 96 16.5 / 11.6; 4096 from 1024, 16 4.6 / 7.3, 32 6.4 / 8.1, 64 9.9 / 8.2; 4096 from 4096, 16 10.7 / 12.8, 32 17 /
+// 13.2. It takes rows at any address; for tiles, rows of no whole 16 bytes are copied first.
+static bool linear_streams(int64_t M, int64_t N, int64_t K) {
+    const int64_t wgs = (M + 15) / 16 * ((N + 15) / 16);
+    const double few = 2.6 + (double)((wgs + 255) / 256) * (0.5 + 1.75e-3 * (double)K);
+    const double pad = K % 8 ? 4.0 + (double)((M + N) * K) * 4.0 / 4e6 : 0.0;
+    return M <= 4096 && few <= plan_product(M, N, K).us + pad;
+}
+static int64_t part_bytes(int64_t M, int64_t N, int64_t K) {
+    const int s = plan_product(M, N, K).splits;
+    return s > 1 ? 4 * s * M * up8(N) : 0;
+}
+
+template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
+static int run_tiles(const ProductArgs& a, hipStream_t st) {
+    using G = GemmTile<LinearKind<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
+    if (!allow_lds<linear_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
+    const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
+    hipLaunchKernelGGL((linear_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+template <int DT, int PL, int QL>
+static int run_product(ProductArgs a, float* part, hipStream_t st) {
+    const ProductPlan p = plan_product(a.M, a.N, a.K);
+    a.splits = p.splits;
+    a.part = part;
+    a.part_stride = up8(a.N);
+    const int r = p.tile == TILE_256        ? run_tiles<DT, PL, QL, 256, 256, 2, 4, 2>(a, st)
+                  : p.tile == TILE_256_128  ? run_tiles<DT, PL, QL, 256, 128, 2, 4, 3>(a, st)
+                  : p.tile == TILE_128_DEEP ? run_tiles<DT, PL, QL, 128, 128, 2, 4, 4>(a, st)
+                                            : run_tiles<DT, PL, QL, 64, 64, 2, 2, 4>(a, st);
+    if (r || a.splits == 1) return r;
+    hipLaunchKernelGGL(linear_join_kernel<DT>, dim3(linear_grid(a.M * ((a.N + 7) / 8))), dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+static int run_pad(const PadArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL(linear_pad_kernel, dim3(linear_grid((a.rows[0] + a.rows[1]) * (a.wide / 8))), dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
 
 // Where the parts of a workspace begin, in bytes (256-byte steps); -1: not there.
 struct LinearSpace {
-    int64_t x = -1, w = -1, part = -1, dz = -1, dx = -1, dw = -1, tops = -1, bytes = 0;
+    int64_t x = -1, w = -1, part = -1, dz = -1, tops = -1, bytes = 0;
     int64_t take(int64_t n) {
         const int64_t at = bytes;
         bytes += (n + 255) / 256 * 256;
@@ -414,57 +525,31 @@ static LinearSpace forward_space(int64_t M, int64_t N, int64_t K) {
     LinearSpace s;
     if (M == 0 || linear_streams(M, N, K)) return s;
     if (K % 8) s.x = s.take(M * up8(K) * 2), s.w = s.take(N * up8(K) * 2);
-    const Gemm16Plan p = linear_plan(M, N, K);
-    if (p.splits > 1) s.part = s.take(p.splits * M * up8(N) * 4);
+    if (const int64_t n = part_bytes(M, N, K)) s.part = s.take(n);
     return s;
 }
 int64_t linear_forward_bytes(int64_t M, int64_t N, int64_t K) { return forward_space(M, N, K).bytes; }
 
-static int pad(const uint16_t* src, int64_t ss, int64_t rows, int64_t cols, uint16_t* dst, int64_t drows, int64_t dw, hipStream_t st) {
-    hipLaunchKernelGGL(linear_pad_kernel, dim3(linear_grid(drows * dw / 8)), dim3(256), 0, st, src, ss, rows, (int)cols, dst, drows, (int)dw);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-static int crop(const uint16_t* src, int64_t sw, uint16_t* dst, int64_t rows, int64_t cols, hipStream_t st) {
-    hipLaunchKernelGGL(linear_crop_kernel, dim3(linear_grid(rows * ((cols + 7) / 8))), dim3(256), 0, st, src, (int)sw, dst, rows, (int)cols);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-
-template <int DT, int BP, int BQ, int WP, int WQ, int ST>
-static int run_linear(const LinearArgs& a, hipStream_t st) {
-    using G = GemmTile<LinearKind<DT>::value, LAY_ROW, LAY_ROW, BP, BQ, WP, WQ, ST>;
-    if (!allow_lds<linear_kernel<DT, BP, BQ, WP, WQ, ST>>(G::LDS)) return -1;
-    const int nt = (a.N + BP - 1) / BP, mt = (int)((a.M + BQ - 1) / BQ);
-    hipLaunchKernelGGL((linear_kernel<DT, BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-
 template <int DT>
 static int linear_forward(LinearArgs a, char* ws, hipStream_t st) {
+    ProductArgs g{};
+    g.M = a.M, g.N = a.N, g.K = a.K;
+    g.p = a.w, g.ldp = a.w_stride, g.q = a.x, g.ldq = a.x_stride;
+    g.bias = a.bias, g.bdt = a.bdt, g.act = a.act, g.res = a.res, g.res_stride = a.res_stride;
+    g.z = a.z, g.out = a.out, g.out_stride = a.out_stride;
     if (linear_streams(a.M, a.N, a.K)) {
-        const dim3 g((a.N + 15) / 16, (unsigned)((a.M + 15) / 16));
-        if (a.K > 1024) hipLaunchKernelGGL((linear_few_kernel<DT, 16>), g, dim3(1024), 0, st, a);
-        else hipLaunchKernelGGL((linear_few_kernel<DT, 4>), g, dim3(256), 0, st, a);
+        const dim3 grid((a.N + 15) / 16, (unsigned)((a.M + 15) / 16));
+        hipLaunchKernelGGL(linear_few_kernel<DT>, grid, dim3(64 * FEW_WAVES), 0, st, g);
         return hipGetLastError() == hipSuccess ? 0 : -1;
     }
     const LinearSpace s = forward_space(a.M, a.N, a.K);
     if (s.x >= 0) {
         uint16_t *x = reinterpret_cast<uint16_t*>(ws + s.x), *w = reinterpret_cast<uint16_t*>(ws + s.w);
         const int64_t K8 = up8(a.K);
-        if (int r = pad(a.x, a.x_stride, a.M, a.K, x, a.M, K8, st)) return r;
-        if (int r = pad(a.w, a.w_stride, a.N, a.K, w, a.N, K8, st)) return r;
-        a.x = x, a.w = w, a.x_stride = a.w_stride = K8, a.K = (int)K8;
+        if (int r = run_pad(PadArgs{{a.x, a.w}, {a.x_stride, a.w_stride}, {a.M, a.N}, {x, w}, a.K, (int)K8}, st)) return r;
+        g.p = w, g.q = x, g.ldp = g.ldq = K8;
     }
-    const Gemm16Plan p = linear_plan(a.M, a.N, a.K);
-    a.splits = p.splits;
-    a.part = s.part >= 0 ? reinterpret_cast<float*>(ws + s.part) : nullptr;
-    a.part_stride = up8(a.N);
-    const int r = p.tile == TILE_256        ? run_linear<DT, 256, 256, 2, 4, 2>(a, st)
-                  : p.tile == TILE_128      ? run_linear<DT, 128, 128, 2, 2, 2>(a, st)
-                  : p.tile == TILE_128_DEEP ? run_linear<DT, 128, 128, 2, 4, 4>(a, st)
-                                            : run_linear<DT, 64, 64, 2, 2, 4>(a, st);
-    if (r || a.splits == 1) return r;
-    hipLaunchKernelGGL(linear_join_kernel<DT>, dim3(linear_grid(a.M * ((a.N + 7) / 8))), dim3(256), 0, st, a);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return run_product<DT, LAY_ROW, LAY_ROW>(g, s.part >= 0 ? reinterpret_cast<float*>(ws + s.part) : nullptr, st);
 }
 int launch_linear(const LinearArgs& a, void* ws, hipStream_t st) {
     return a.dt == DT_BF16 ? linear_forward<DT_BF16>(a, static_cast<char*>(ws), st) : linear_forward<DT_F16>(a, static_cast<char*>(ws), st);
@@ -476,72 +561,65 @@ static bool dz_is_dy(const LinearArgs& a) {
 }
 static LinearSpace backward_space(int64_t M, int64_t N, int64_t K) {
     LinearSpace s;
-    const int64_t N8 = up8(N), K8 = up8(K);
-    s.dz = s.take(M * N8 * 2);
+    s.dz = s.take(M * up8(N) * 2);
     s.tops = s.take(4 * (LINEAR_TOPS + 1));
-    if (K % 8) s.x = s.take(M * K8 * 2), s.dx = s.take(M * K8 * 2);
-    if (K % 8 || N % 8) s.w = s.take(N8 * K8 * 2), s.dw = s.take(N8 * K8 * 2);
-    const int64_t parts = std::max({gemm16_part_floats(M, K8, N8), gemm16_part_floats(N8, K8, M), (M + DZ_ROWS - 1) / DZ_ROWS * N8});
-    s.part = s.take(4 * parts);
+    if (K % 8) s.x = s.take(M * up8(K) * 2), s.w = s.take(N * up8(K) * 2);
+    s.part = s.take(std::max({part_bytes(M, K, N), part_bytes(N, K, M), 4 * ((M + DZ_ROWS - 1) / DZ_ROWS) * up8(N)}));
     return s;
 }
 int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K) { return backward_space(M, N, K).bytes; }
 
 template <int DT>
-static int linear_backward(LinearArgs a, char* ws, hipStream_t st) {
+static int linear_backward(const LinearArgs& a, char* ws, hipStream_t st) {
     const LinearSpace s = backward_space(a.M, a.N, a.K);
     const int64_t N8 = up8(a.N), K8 = up8(a.K);
     auto at = [&](int64_t o) { return reinterpret_cast<uint16_t*>(ws + o); };
-    const bool products = a.dx || a.dw, direct = dz_is_dy(a);
-    a.part = reinterpret_cast<float*>(ws + s.part);
-    a.part_stride = N8;
-    a.dz = products && !direct ? at(s.dz) : nullptr;
-    a.dz_stride = N8;
-    a.tops = reinterpret_cast<uint32_t*>(ws + s.tops);
-    a.unscale = reinterpret_cast<float*>(a.tops + LINEAR_TOPS);
-    a.ntops = 0;
-    if (DT == DT_F16 && a.dz && a.act != ACT_NONE && a.act != ACT_RELU) {
-        a.ntops = (int)std::min<int64_t>((a.M * ((a.N + 7) / 8) + 255) / 256, LINEAR_TOPS);
-        hipLaunchKernelGGL(linear_top_kernel<DT>, dim3(a.ntops), dim3(256), 0, st, a);
+    const bool direct = dz_is_dy(a);
+    float* part = reinterpret_cast<float*>(ws + s.part);
+    SlopeArgs g{};
+    g.a = a;
+    g.part = part;
+    g.part_stride = N8;
+    g.dz = (a.dx || a.dw) && !direct ? at(s.dz) : nullptr;
+    g.dz_stride = N8;
+    g.tops = reinterpret_cast<uint32_t*>(ws + s.tops);
+    g.unscale = reinterpret_cast<float*>(g.tops + LINEAR_TOPS);
+    if (DT == DT_F16 && g.dz && a.act != ACT_NONE && a.act != ACT_RELU) {
+        g.ntops = (int)std::min<int64_t>((a.M * ((a.N + 7) / 8) + 255) / 256, LINEAR_TOPS);
+        hipLaunchKernelGGL(linear_top_kernel<DT>, dim3(g.ntops), dim3(256), 0, st, g);
         if (hipGetLastError() != hipSuccess) return -1;
     }
-    if (a.dz || a.dbias) {
+    if (g.dz || a.dbias) {
         const int parts = (int)((a.M + DZ_ROWS - 1) / DZ_ROWS);
-        hipLaunchKernelGGL(linear_dz_kernel<DT>, dim3(parts, (a.N + 255) / 256), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(linear_dz_kernel<DT>, dim3(parts, (a.N + 255) / 256), dim3(256), 0, st, g);
         if (hipGetLastError() != hipSuccess) return -1;
         if (a.dbias) {
-            hipLaunchKernelGGL(linear_dbias_kernel, dim3((a.N + 63) / 64), dim3(1024), 0, st, a, parts);
+            hipLaunchKernelGGL(linear_dbias_kernel, dim3((a.N + 63) / 64), dim3(1024), 0, st, g, parts);
             if (hipGetLastError() != hipSuccess) return -1;
         }
     }
-    const uint16_t* dz = direct ? static_cast<const uint16_t*>(a.dy) : at(s.dz);
-    const int64_t ldz = direct ? a.dy_stride : N8;
-    const float* unscale = a.ntops ? a.unscale : nullptr;
+    ProductArgs p{};
+    p.q = direct ? static_cast<const uint16_t*>(a.dy) : at(s.dz);
+    p.ldq = direct ? a.dy_stride : N8;
+    p.qcols = (int)N8;
+    p.pcols = (int)K8;
+    p.N = a.K;
+    p.out_stride = a.K;
+    p.unscale = g.ntops ? g.unscale : nullptr;
+    const uint16_t *x = a.x, *w = a.w;
+    int64_t ldx = a.x_stride, ldw = a.w_stride;
+    if (s.x >= 0 && (a.dx || a.dw)) {
+        const PadArgs pad{{a.x, a.w}, {ldx, ldw}, {a.dw ? a.M : 0, a.dx ? a.N : 0}, {at(s.x), at(s.w)}, a.K, (int)K8};
+        if (int r = run_pad(pad, st)) return r;
+        x = at(s.x), w = at(s.w), ldx = ldw = K8;
+    }
     if (a.dx) {
-        Gemm16Args g{};
-        g.p = a.w, g.ldp = a.w_stride;
-        if (s.w >= 0) {
-            if (int r = pad(a.w, a.w_stride, a.N, a.K, at(s.w), N8, K8, st)) return r;
-            g.p = at(s.w), g.ldp = K8;
-        }
-        g.q = dz, g.ldq = ldz, g.M = a.M, g.N = (int)K8, g.C = N8, g.unscale = unscale, g.part = a.part;
-        g.out = s.dx >= 0 ? at(s.dx) : a.dx, g.out_stride = K8;
-        if (int r = launch_gemm16_col_row(DT, g, st)) return r;
-        if (s.dx >= 0)
-            if (int r = crop(at(s.dx), K8, static_cast<uint16_t*>(a.dx), a.M, a.K, st)) return r;
+        p.p = w, p.ldp = ldw, p.M = a.M, p.K = a.N, p.out = a.dx;
+        if (int r = run_product<DT, LAY_COL, LAY_ROW>(p, part, st)) return r;
     }
     if (a.dw) {
-        Gemm16Args g{};
-        g.p = a.x, g.ldp = a.x_stride;
-        if (s.x >= 0) {
-            if (int r = pad(a.x, a.x_stride, a.M, a.K, at(s.x), a.M, K8, st)) return r;
-            g.p = at(s.x), g.ldp = K8;
-        }
-        g.q = dz, g.ldq = ldz, g.M = N8, g.N = (int)K8, g.C = a.M, g.unscale = unscale, g.part = a.part;
-        g.out = s.dw >= 0 ? at(s.dw) : a.dw, g.out_stride = K8;
-        if (int r = launch_gemm16_col_col(DT, g, st)) return r;
-        if (s.dw >= 0)
-            if (int r = crop(at(s.dw), K8, static_cast<uint16_t*>(a.dw), a.N, a.K, st)) return r;
+        p.p = x, p.ldp = ldx, p.M = a.N, p.K = a.M, p.out = a.dw;
+        if (int r = run_product<DT, LAY_COL, LAY_COL>(p, part, st)) return r;
     }
     return 0;
 }

@@ -368,7 +368,7 @@ int launch_mx_arrange(const uint8_t* a, int64_t mats, int64_t rows, uint8_t* ao,
                       hipStream_t st);
 // Kinds of workgroup tiles: the largest, 128 x 128 for two workgroups a CU, and three deeply buffered ones for products of
 // at most a workgroup a CU.
-enum TileKind { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_128_64 = 3, TILE_64 = 4 };
+enum TileKind { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_128_64 = 3, TILE_64 = 4, TILE_256_128 = 5 };
 struct MxMatmulPlan {
     int few, tile, splits, arrange;
 };
@@ -534,29 +534,6 @@ int64_t norm_part_floats(int64_t rows, int H);
 int launch_norm(const NormArgs& a, hipStream_t st);
 int launch_norm_grad(const NormArgs& a, hipStream_t st);
 
-// 16-bit tile products (ffn.hip): out[m][n] = sum over k of P Q.
-struct Gemm16Args {
-    const uint16_t* p;      // ROW: [N][ldp], COL: [C][ldp]
-    const uint16_t* q;      // ROW: [M][ldq], COL: [C][ldq]
-    int64_t ldp, ldq;       // elements
-    int64_t M;
-    int N;
-    int64_t C;              // contraction
-    void* out;
-    int64_t out_stride;
-    int splits;
-    float* part;
-    const float* unscale;   // fp16: the factor of the sums (nullptr: none)
-};
-struct Gemm16Plan {
-    int tile, splits;
-};
-Gemm16Plan plan_gemm16(int64_t M, int64_t N, int64_t C);
-int64_t gemm16_part_floats(int64_t M, int64_t N, int64_t C);
-// P with the contraction as its row index, Q by rows or likewise
-int launch_gemm16_col_row(int dt, const Gemm16Args& a, hipStream_t st);
-int launch_gemm16_col_col(int dt, const Gemm16Args& a, hipStream_t st);
-
 // The dense product with its epilogue (linear.hip).
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
 struct LinearArgs {
@@ -574,15 +551,6 @@ struct LinearArgs {
     void* out;              // [M][out_stride]
     int64_t out_stride;
     float* z;               // [M][N]: x W^T + bias (forward: optional)
-    // set by the launchers
-    int splits;
-    float* part;            // [splits][M][part_stride]; backward: [row blocks][part_stride], or the products' parts
-    int64_t part_stride;
-    uint16_t* dz;           // [M][dz_stride]
-    int64_t dz_stride;
-    uint32_t* tops;
-    int ntops;
-    float* unscale;
     // backward
     const void* dy;         // [M][dy_stride]
     int64_t dy_stride;

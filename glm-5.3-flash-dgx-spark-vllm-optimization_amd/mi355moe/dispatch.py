@@ -17,12 +17,19 @@ caching allocator. No atomics on values: two calls give the same bits.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, _row_stride,
-                  ids_dtype_code, weight_dtype_code)
+from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, ids_dtype_code,
+                  weight_dtype_code)
+
+
+@functools.lru_cache(maxsize=4096)
+def _sort_bytes(T: int, topk: int, n: int) -> int:
+    return _lib.lib().mi355moe_sort_tokens_workspace_bytes(T, topk, n)
 
 
 class SortedTokens:
@@ -30,12 +37,29 @@ class SortedTokens:
     that no local expert takes (their rows come behind the others, and hold zeros); pair int32 [T * topk]: the pair of each
     row, or ~pair; offsets int32 [n + 1]: where each expert's rows begin, offsets[n] the number of rows that experts have."""
 
-    __slots__ = ("row", "pair", "offsets", "tokens", "topk", "n")
+    __slots__ = ("_words", "tokens", "topk", "n")
 
-    def __init__(self, row: torch.Tensor, pair: torch.Tensor, offsets: torch.Tensor):
-        self.row, self.pair, self.offsets = row, pair, offsets
-        self.tokens, self.topk = row.shape
-        self.n = offsets.numel() - 1
+    def __init__(self, words: torch.Tensor, tokens: int, topk: int, n: int):
+        self._words, self.tokens, self.topk, self.n = words, tokens, topk, n      # row, pair, offsets, one behind the other
+
+    @property
+    def row(self) -> torch.Tensor:
+        P = self.tokens * self.topk
+        return self._words[:P].view(self.tokens, self.topk)
+
+    @property
+    def pair(self) -> torch.Tensor:
+        P = self.tokens * self.topk
+        return self._words[P:2 * P]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        P = self.tokens * self.topk
+        return self._words[2 * P:2 * P + self.n + 1]
+
+    @property
+    def device(self) -> torch.device:
+        return self._words.device
 
 
 def sort_tokens(topk_ids: torch.Tensor, n: int, expert_map: torch.Tensor | None = None) -> SortedTokens:
@@ -50,29 +74,31 @@ def sort_tokens(topk_ids: torch.Tensor, n: int, expert_map: torch.Tensor | None 
         if expert_map.dim() != 1 or expert_map.dtype.is_floating_point or expert_map.dtype == torch.bool:
             raise ValueError(f"expert_map must be a vector of whole numbers, got {expert_map.dtype} {tuple(expert_map.shape)}")
     T, topk = topk_ids.shape
-    L = _lib.lib()
-    nb = L.mi355moe_sort_tokens_workspace_bytes(T, topk, int(n))
+    n, P = int(n), T * topk
+    nb = _sort_bytes(T, topk, n)
     with _on_device(dev):
         ids = topk_ids.contiguous()
-        em = None if expert_map is None else expert_map.to(torch.int64).contiguous()
-        n_global = 0 if em is None else em.numel()
-        if em is not None and n_global == 0:
-            em = ids.new_zeros(1, dtype=torch.int64)             # (no id has an entry; the address only says that there is a map)
-        words = torch.empty(2 * T * topk + max(int(n), 0) + 1, dtype=torch.int32, device=dev)
-        row, pair, offsets = words[:T * topk], words[T * topk:2 * T * topk], words[2 * T * topk:]
-        ws = words.new_empty(nb // 4) if nb > 0 else None
-        _lib.check("mi355moe_sort_tokens", L.mi355moe_sort_tokens(
-            _addr(ids), code, T, topk, _addr(em), n_global, int(n), row.data_ptr(), pair.data_ptr(), offsets.data_ptr(), _addr(ws),
+        em, n_global = None, 0
+        if expert_map is not None:
+            em = expert_map.to(torch.int64).contiguous()
+            n_global = em.numel()
+            if n_global == 0:
+                em = ids.new_zeros(1, dtype=torch.int64)         # (no id has an entry; the address only says that there is a map)
+        # the scratch lies behind the three tables (a size that the library refuses: enough for its answer)
+        words = ids.new_empty(2 * P + max(n, 0) + 1 + max(nb, 0) // 4, dtype=torch.int32)
+        at = words.data_ptr()
+        _lib.check("mi355moe_sort_tokens", _lib.lib().mi355moe_sort_tokens(
+            _addr(ids), code, T, topk, _addr(em), n_global, n, at, at + 4 * P, at + 8 * P, at + 4 * (2 * P + n + 1) if nb > 0 else None,
             max(nb, 0), _raw_stream(dev)))
-    return SortedTokens(row.view(T, topk), pair, offsets)
+    return SortedTokens(words, T, topk, n)
 
 
 def _check(plan: SortedTokens, what: str, t: torch.Tensor, rows: int, dev: torch.device) -> int:
     code = weight_dtype_code(t.dtype)
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] == 0:
         raise ValueError(f"{what} must be [{rows}, H], got {tuple(t.shape)}")
-    if plan.row.device != dev:
-        raise ValueError(f"the order is on {plan.row.device}, {what} on {dev}")
+    if plan.device != dev:
+        raise ValueError(f"the order is on {plan.device}, {what} on {dev}")
     return code
 
 
@@ -81,18 +107,18 @@ def _to_experts(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     code = _check(plan, "x", x, plan.tokens, dev)
     H = x.shape[1]
     with _on_device(dev):
-        x = _rows_any(_plain(x))
+        x, ldx = _rows_any(_plain(x))
         rows = x.new_empty((plan.tokens * plan.topk, H))
         _lib.check("mi355moe_rows_to_experts", _lib.lib().mi355moe_rows_to_experts(
-            x.data_ptr(), code, plan.tokens, H, _row_stride(x), plan.row.data_ptr(), plan.topk, rows.data_ptr(), _raw_stream(dev)))
+            x.data_ptr(), code, plan.tokens, H, ldx, plan._words.data_ptr(), plan.topk, rows.data_ptr(), _raw_stream(dev)))
     return rows
 
 
 def _check_back(rows, weights, plan, shared):
     dev = _need_cuda(rows, weights, shared)
     code = _check(plan, "rows", rows, plan.tokens * plan.topk, dev)
-    if weights is not None and weights.shape != plan.row.shape:
-        raise ValueError(f"weights must be {tuple(plan.row.shape)}, got {tuple(weights.shape)}")
+    if weights is not None and weights.shape != (plan.tokens, plan.topk):
+        raise ValueError(f"weights must be {(plan.tokens, plan.topk)}, got {tuple(weights.shape)}")
     if shared is not None and (shared.dtype != rows.dtype or shared.shape != (plan.tokens, rows.shape[1])):
         raise ValueError(f"shared must be {rows.dtype} {(plan.tokens, rows.shape[1])}, got {shared.dtype} {tuple(shared.shape)}")
     return dev, code
@@ -105,11 +131,11 @@ def _from_experts(rows, weights, plan, shared):
     with _on_device(dev):
         rows = _plain(rows).contiguous()
         weights = None if weights is None else _plain(weights).contiguous()
-        shared = None if shared is None else _rows_any(_plain(shared))
+        shared, lds = (None, H) if shared is None else _rows_any(_plain(shared))
         out = rows.new_empty((plan.tokens, H))
         _lib.check("mi355moe_rows_from_experts", _lib.lib().mi355moe_rows_from_experts(
-            rows.data_ptr(), code, plan.tokens, H, plan.row.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared),
-            H if shared is None else _row_stride(shared), out.data_ptr(), H, _raw_stream(dev)))
+            rows.data_ptr(), code, plan.tokens, H, plan._words.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared), lds,
+            out.data_ptr(), H, _raw_stream(dev)))
     return out
 
 
@@ -123,12 +149,18 @@ def from_experts_backward(dout: torch.Tensor, rows: torch.Tensor, weights: torch
     H = rows.shape[1]
     if dout.dtype != rows.dtype or dout.shape != (plan.tokens, H):
         raise ValueError(f"dout must be {rows.dtype} {(plan.tokens, H)}, got {dout.dtype} {tuple(dout.shape)}")
+    return _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights)
+
+
+def _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights):
+    """from_experts_backward of arguments that have been looked at."""
+    H = rows.shape[1]
     with _on_device(dev):
-        dout, rows, weights = _rows_any(_plain(dout)), _plain(rows).contiguous(), _plain(weights).contiguous()
-        drows = torch.empty_like(rows) if need_rows else None
+        (dout, ldd), rows, weights = _rows_any(_plain(dout)), _plain(rows).contiguous(), _plain(weights).contiguous()
+        drows = torch.empty_like(rows) if need_rows else None        # (contiguous, like the two)
         dw = torch.empty_like(weights) if need_weights else None
         _lib.check("mi355moe_rows_from_experts_backward", _lib.lib().mi355moe_rows_from_experts_backward(
-            dout.data_ptr(), code, plan.tokens, H, _row_stride(dout), plan.row.data_ptr(), plan.topk, weights.data_ptr(),
+            dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(),
             weight_dtype_code(weights.dtype), rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev)))
     return drows, dw
 
@@ -169,7 +201,7 @@ class _From(torch.autograd.Function):
         if weights is None:
             drows = _to_experts(dout, ctx.plan) if need[0] else None
         elif need[0] or need[1]:
-            drows, dw = from_experts_backward(dout, rows, weights, ctx.plan, need[0], need[1])
+            drows, dw = _from_grads(rows.device, weight_dtype_code(rows.dtype), dout, rows, weights, ctx.plan, need[0], need[1])
         return drows, dw, None, dout if need[3] else None
 
 

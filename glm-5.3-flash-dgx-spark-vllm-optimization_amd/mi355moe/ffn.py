@@ -161,9 +161,15 @@ def _linear_bytes(backward: bool, M: int, K: int, N: int) -> int:
     return (L.mi355moe_linear_backward_workspace_bytes if backward else L.mi355moe_linear_forward_workspace_bytes)(M, K, N)
 
 
-def _linear_operand(t: torch.Tensor) -> torch.Tensor:
-    """t [rows, K] as the product reads it: where K is a multiple of 8 its rows lie at 16-byte addresses."""
-    return _rows16(t) if t.shape[1] % 8 == 0 else _rows_any(t)
+def _linear_operand(t: torch.Tensor, K: int) -> tuple[torch.Tensor, int]:
+    """t [rows, K] as the product reads it, and the values from one row to the next: where K is a multiple of 8 its rows lie at
+    16-byte addresses."""
+    if K & 7:
+        return _rows_any(t)
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t, K
+    t = _rows16(t)
+    return t, _row_stride(t)
 
 
 def _check_linear(x, w, bias, activation, residual):
@@ -172,16 +178,17 @@ def _check_linear(x, w, bias, activation, residual):
     code = act_dtype_code(x.dtype)
     if w.dtype != x.dtype:
         raise ValueError(f"x is {x.dtype}, w {w.dtype}")
-    if w.dim() != 2 or w.numel() == 0:
-        raise ValueError(f"w must be [N, K], got {tuple(w.shape)}")
-    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"x must be [..., {w.shape[1]}], got {tuple(x.shape)}")
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != w.shape[0]):
-        raise ValueError(f"bias must be {(w.shape[0],)}, got {tuple(bias.shape)}")
+    shape, ws = x.shape, w.shape
+    if len(ws) != 2 or w.numel() == 0:
+        raise ValueError(f"w must be [N, K], got {tuple(ws)}")
+    if not shape or shape[-1] != ws[1]:
+        raise ValueError(f"x must be [..., {ws[1]}], got {tuple(shape)}")
+    if bias is not None and bias.shape != ws[:1]:
+        raise ValueError(f"bias must be {(ws[0],)}, got {tuple(bias.shape)}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
-    if residual is not None and (residual.dtype != x.dtype or residual.shape != (*x.shape[:-1], w.shape[0])):
-        raise ValueError(f"residual must be {x.dtype} {(*x.shape[:-1], w.shape[0])}, got {residual.dtype} {tuple(residual.shape)}")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != (*shape[:-1], ws[0])):
+        raise ValueError(f"residual must be {x.dtype} {(*shape[:-1], ws[0])}, got {residual.dtype} {tuple(residual.shape)}")
     return dev, code, _lib.F32 if bias is None else weight_dtype_code(bias.dtype)
 
 
@@ -189,24 +196,30 @@ def linear_forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None =
                    residual: torch.Tensor | None = None, save: bool = False):
     """out [..., N] of x [..., K] and w [N, K], or with save (out, z), z fp32 [rows, N] = x W^T + bias for linear_backward (None
     without an activation, whose gradient does not read it). No gradient is recorded."""
-    dev, code, bcode = _check_linear(x, w, bias, activation, residual)
+    return _linear(_check_linear(x, w, bias, activation, residual), x, w, bias, activation, residual, save)
+
+
+def _linear(kinds, x, w, bias, activation, residual, save):
+    """linear_forward of arguments that have been looked at (kinds: what _check_linear said of them)."""
+    dev, code, bcode = kinds
     N, K = w.shape
     with _on_device(dev):
         x2 = _plain(x)
-        x2 = _linear_operand(x2 if x.dim() == 2 else x2.reshape(-1, K))
-        w2 = _linear_operand(_plain(w))
+        x2, ldx = _linear_operand(x2 if x2.dim() == 2 else x2.reshape(-1, K), K)
+        w2, ldw = _linear_operand(_plain(w), K)
         b = None if bias is None else _plain(bias).contiguous()
-        r = None if residual is None else _plain(residual)
-        if r is not None:
-            r = _rows_any(r if r.dim() == 2 else r.reshape(-1, N))
+        r, ldr = None, N
+        if residual is not None:
+            r = _plain(residual)
+            r, ldr = _rows_any(r if r.dim() == 2 else r.reshape(-1, N))
         M = x2.shape[0]
         out = x2.new_empty((*x.shape[:-1], N))
         z = x2.new_empty((M, N), dtype=torch.float32) if save and activation is not None else None
         nb = _linear_bytes(False, M, K, N)
         ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
         _lib.check("mi355moe_linear_forward", _lib.lib().mi355moe_linear_forward(
-            x2.data_ptr(), code, M, K, _row_stride(x2), w2.data_ptr(), N, _row_stride(w2), _addr(b), bcode, ACTIVATIONS[activation],
-            _addr(r), N if r is None else _row_stride(r), out.data_ptr(), N, _addr(z), _addr(ws), max(nb, 0), _raw_stream(dev)))
+            x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw, _addr(b), bcode, ACTIVATIONS[activation], _addr(r), ldr,
+            out.data_ptr(), N, _addr(z), _addr(ws), max(nb, 0), _raw_stream(dev)))
     return (out, z) if save else out
 
 
@@ -214,43 +227,51 @@ def linear_backward(dout: torch.Tensor, z: torch.Tensor | None, x: torch.Tensor,
                     bias_dtype: torch.dtype | None = None, need_dx: bool = True, need_dw: bool = True):
     """(dx, dw, dbias) from dout [..., N], the forward's z, x and w: fp32 sums, dx and dw in x's dtype, dbias in bias_dtype (None
     where there is no bias or the gradient is not needed); the sums' order does not vary. residual's gradient is dout."""
-    dev, code, _ = _check_linear(x, w, None, activation, None)
+    kinds = _check_linear(x, w, None, activation, None)
     _need_cuda(x, dout, z)
     _no_tangents("the dense product's backward", dout, z)
-    N, K = w.shape
+    N = w.shape[0]
     if dout.dtype != x.dtype or dout.shape != (*x.shape[:-1], N):
         raise ValueError(f"dout must be {x.dtype} {(*x.shape[:-1], N)}, got {dout.dtype} {tuple(dout.shape)}")
-    bcode = _lib.F32 if bias_dtype is None else weight_dtype_code(bias_dtype)
+    if bias_dtype is not None:
+        weight_dtype_code(bias_dtype)
+    M = dout.numel() // N
+    if activation is not None and (z is None or z.dtype != torch.float32 or tuple(z.shape) != (M, N) or not z.is_contiguous()):
+        raise ValueError(f"z must be contiguous float32 {(M, N)}, got {None if z is None else (z.dtype, tuple(z.shape))}")
+    return _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw)
+
+
+def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw):
+    """linear_backward of arguments that have been looked at."""
+    dev, code, _ = kinds
+    N, K = w.shape
     with _on_device(dev):
         x2, d2 = _plain(x), _plain(dout)
-        if x.dim() != 2:
+        if x2.dim() != 2:
             x2, d2 = x2.reshape(-1, K), d2.reshape(-1, N)
-        x2, w2, d2 = _linear_operand(x2), _linear_operand(_plain(w)), _rows_any(d2)
+        (x2, ldx), (w2, ldw), (d2, ldd) = _linear_operand(x2, K), _linear_operand(_plain(w), K), _rows_any(d2)
         M = x2.shape[0]
-        if activation is None:
-            z = None
-        elif z is None or z.dtype != torch.float32 or tuple(z.shape) != (M, N) or not z.is_contiguous():
-            raise ValueError(f"z must be contiguous float32 {(M, N)}, got {None if z is None else (z.dtype, tuple(z.shape))}")
-        new = torch.zeros if M == 0 else torch.empty
-        dx = new(x.shape, dtype=x.dtype, device=dev) if need_dx else None
-        dw = new((N, K), dtype=x.dtype, device=dev) if need_dw else None
-        db = new(N, dtype=bias_dtype, device=dev) if bias_dtype is not None else None
-        if M == 0:
+        new = x2.new_zeros if M == 0 else x2.new_empty
+        dx = new(x.shape) if need_dx else None
+        dw = new((N, K)) if need_dw else None
+        db = new(N, dtype=bias_dtype) if bias_dtype is not None else None
+        if M == 0 or (dx is None and dw is None and db is None):
             return dx, dw, db
         nb = _linear_bytes(True, M, K, N)
         ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
         _lib.check("mi355moe_linear_backward", _lib.lib().mi355moe_linear_backward(
-            d2.data_ptr(), _row_stride(d2), _addr(z), x2.data_ptr(), code, M, K, _row_stride(x2), w2.data_ptr(), N, _row_stride(w2),
-            ACTIVATIONS[activation], _addr(dx), _addr(dw), _addr(db), bcode, ws.data_ptr(), max(nb, 0), _raw_stream(dev)))
+            d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw,
+            ACTIVATIONS[activation], _addr(dx), _addr(dw), _addr(db), _lib.F32 if db is None else weight_dtype_code(bias_dtype),
+            ws.data_ptr(), max(nb, 0), _raw_stream(dev)))
     return dx, dw, db
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, activation, residual):
-        out, z = linear_forward(x, w, bias, activation, residual, save=True)
+    def forward(ctx, x, w, bias, residual, kinds, activation):
+        out, z = _linear(kinds, x, w, bias, activation, residual, True)
         ctx.save_for_backward(x, w, z)
-        ctx.activation, ctx.bias_dtype = activation, None if bias is None else bias.dtype
+        ctx.rest = kinds, activation, None if bias is None else bias.dtype
         return out
 
     @staticmethod
@@ -260,9 +281,10 @@ class _Linear(torch.autograd.Function):
             raise RuntimeError("mi355moe: the backward pass of an eagerly recorded ffn.linear cannot be captured; capture "
                                "ffn.linear_forward(save=True) and ffn.linear_backward")
         x, w, z = ctx.saved_tensors
+        kinds, activation, bias_dtype = ctx.rest
         need = ctx.needs_input_grad
-        dx, dw, db = linear_backward(dout, z, x, w, ctx.activation, ctx.bias_dtype if need[2] else None, need[0], need[1])
-        return dx, dw, db, None, dout if need[4] else None
+        dx, dw, db = _linear_grads(kinds, dout, z, x, w, activation, bias_dtype if need[2] else None, need[0], need[1])
+        return dx, dw, db, dout if need[3] else None, None, None
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -271,10 +293,11 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, a
     activation None, "relu", "silu", "gelu" or "gelu_tanh". Differentiable once in the four tensors by reverse mode
     (forward-mode derivatives are refused). While a graph is captured, a call that would record a gradient, and the backward
     pass of an eager one, are refused; capture linear_forward(save=True) and linear_backward instead."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
-        dev = _check_linear(x, w, bias, activation, residual)[0]
-        if _capturing(dev):
+    kinds = _check_linear(x, w, bias, activation, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        if _capturing(kinds[0]):
             raise RuntimeError("mi355moe: linear cannot record a gradient during graph capture; capture "
                                "ffn.linear_forward(save=True) and ffn.linear_backward")
-        return _Linear.apply(x, w, bias, activation, residual)
-    return linear_forward(x, w, bias, activation, residual)
+        return _Linear.apply(x, w, bias, residual, kinds, activation)
+    return _linear(kinds, x, w, bias, activation, residual, False)

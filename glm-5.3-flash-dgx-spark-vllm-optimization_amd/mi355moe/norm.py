@@ -21,7 +21,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, _row_stride, weight_dtype_code
+from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, weight_dtype_code
 
 _NONE, _CHANNEL, _TOKEN, _FULL = 0, 1, 2, 3
 
@@ -31,42 +31,41 @@ def _backward_bytes(rows: int, H: int) -> int:
     return _lib.lib().mi355moe_norm_backward_workspace_bytes(rows, H)
 
 
-def _gate_kind(branch: torch.Tensor, gate: torch.Tensor | None) -> int:
-    if gate is None:
-        return _NONE
-    if gate.shape == branch.shape:
+def _gate_kind(shape: torch.Size, gate: torch.Size) -> int:
+    if gate == shape:
         return _FULL
-    if gate.dim() == 1 and gate.shape[0] == branch.shape[-1]:
+    if gate == shape[-1:]:
         return _CHANNEL
-    if gate.shape == (*branch.shape[:-1], 1):
+    if gate == (*shape[:-1], 1):
         return _TOKEN
-    H = branch.shape[-1]
-    raise ValueError(f"gate must be {(H,)}, {(*branch.shape[:-1], 1)} or {tuple(branch.shape)}, got {tuple(gate.shape)}")
+    raise ValueError(f"gate must be {(shape[-1],)}, {(*shape[:-1], 1)} or {tuple(shape)}, got {tuple(gate)}")
 
 
 def _check(branch, residual, post, gate, pre):
     dev = _need_cuda(branch, residual, post, gate, pre)
     _no_tangents("the norms around a block", branch, residual, post, gate, pre)
-    code = weight_dtype_code(branch.dtype)
-    if branch.dim() < 1 or branch.shape[-1] == 0:
-        raise ValueError(f"branch must be [..., H], got {tuple(branch.shape)}")
-    H = branch.shape[-1]
-    if residual is not None and (residual.shape != branch.shape or residual.dtype != branch.dtype):
-        raise ValueError(f"residual must be {branch.dtype} {tuple(branch.shape)}, got {residual.dtype} {tuple(residual.shape)}")
+    dtype, shape = branch.dtype, branch.shape
+    code = weight_dtype_code(dtype)
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"branch must be [..., H], got {tuple(shape)}")
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype):
+        raise ValueError(f"residual must be {dtype} {tuple(shape)}, got {residual.dtype} {tuple(residual.shape)}")
     wcode = _lib.F32
-    for name, w in (("post", post), ("pre", pre)):
+    for w in (post, pre):
         if w is not None:
             wcode = weight_dtype_code(w.dtype)
-            if w.dim() != 1 or w.shape[0] != H:
-                raise ValueError(f"{name} must be {(H,)}, got {tuple(w.shape)}")
+            if w.shape != shape[-1:]:
+                raise ValueError(f"{'post' if w is post else 'pre'} must be {(shape[-1],)}, got {tuple(w.shape)}")
     if post is not None and pre is not None and post.dtype != pre.dtype:
         raise ValueError(f"post is {post.dtype}, pre {pre.dtype}")
-    return dev, code, wcode, _gate_kind(branch, gate), _lib.F32 if gate is None else weight_dtype_code(gate.dtype)
+    if gate is None:
+        return dev, code, wcode, _NONE, _lib.F32
+    return dev, code, wcode, _gate_kind(shape, gate.shape), weight_dtype_code(gate.dtype)
 
 
-def _rows(t: torch.Tensor | None, H: int) -> torch.Tensor | None:
+def _rows(t: torch.Tensor | None, H: int) -> tuple[torch.Tensor | None, int]:
     if t is None:
-        return None
+        return None, H
     t = _plain(t)
     return _rows_any(t if t.dim() == 2 else t.reshape(-1, H))
 
@@ -75,27 +74,33 @@ def _flat(t: torch.Tensor | None) -> torch.Tensor | None:
     return None if t is None else _plain(t).contiguous()
 
 
+def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, need_stats):
+    dev, code, wcode, kind, gcode = kinds
+    if pre is None and not need_s:
+        raise ValueError("neither s nor y is asked for")
+    shape = branch.shape
+    H = shape[-1]
+    with _on_device(dev):
+        (b, ldb), (r, ldr) = _rows(branch, H), _rows(residual, H)
+        n = b.shape[0]
+        post, pre, gate = _flat(post), _flat(pre), _flat(gate)
+        s = b.new_empty(shape) if need_s else None
+        y = b.new_empty(shape) if pre is not None else None
+        stats = b.new_empty((n, 2), dtype=torch.float32) if need_stats else None
+        if n:
+            _lib.check("mi355moe_norm_forward", _lib.lib().mi355moe_norm_forward(
+                b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode, kind, eps, scale,
+                residual_scale, _addr(s), _addr(y), _addr(stats), _raw_stream(dev)))
+    return s, y, stats
+
+
 def join_forward(branch: torch.Tensor, residual: torch.Tensor | None = None, post: torch.Tensor | None = None,
                  gate: torch.Tensor | None = None, pre: torch.Tensor | None = None, eps: float = 1e-6, scale: float = 1.0,
                  residual_scale: float = 1.0, need_s: bool = True):
     """(s, y, stats): s and y as join has them (None where there is none), stats fp32 [rows, 2] for join_backward. No gradient is
     recorded."""
-    dev, code, wcode, kind, gcode = _check(branch, residual, post, gate, pre)
-    if pre is None and not need_s:
-        raise ValueError("neither s nor y is asked for")
-    H = branch.shape[-1]
-    with _on_device(dev):
-        b, r = _rows(branch, H), _rows(residual, H)
-        n = b.shape[0]
-        post, pre, gate = _flat(post), _flat(pre), _flat(gate)
-        s = b.new_empty(branch.shape) if need_s else None
-        y = b.new_empty(branch.shape) if pre is not None else None
-        stats = b.new_empty((n, 2), dtype=torch.float32)
-        _lib.check("mi355moe_norm_forward", _lib.lib().mi355moe_norm_forward(
-            b.data_ptr(), code, n, H, _row_stride(b), _addr(r), H if r is None else _row_stride(r), _addr(post), _addr(pre), wcode,
-            _addr(gate), gcode, kind if n else _NONE, float(eps), float(scale), float(residual_scale), _addr(s), _addr(y),
-            stats.data_ptr(), _raw_stream(dev)) if n else 0)
-    return s, y, stats
+    return _forward(_check(branch, residual, post, gate, pre), branch, residual, post, gate, pre, float(eps), float(scale),
+                    float(residual_scale), need_s, True)
 
 
 def join_backward(ds: torch.Tensor | None, dy: torch.Tensor | None, stats: torch.Tensor, branch: torch.Tensor,
@@ -104,25 +109,31 @@ def join_backward(ds: torch.Tensor | None, dy: torch.Tensor | None, stats: torch
                   need: tuple = (True, True, True, True, True)):
     """(dbranch, dresidual, dpost, dgate, dpre) from ds and dy (None: zero), the forward's stats and its inputs, each shaped and
     typed like its input; None where the input is, or `need` (in that order) says no."""
-    dev, code, wcode, kind, gcode = _check(branch, residual, post, gate, pre)
+    kinds = _check(branch, residual, post, gate, pre)
     _need_cuda(branch, ds, dy, stats)
     _no_tangents("the norms' backward", ds, dy)
-    H = branch.shape[-1]
     for name, d in (("ds", ds), ("dy", dy)):
         if d is not None and (d.dtype != branch.dtype or d.shape != branch.shape):
             raise ValueError(f"{name} must be {branch.dtype} {tuple(branch.shape)}, got {d.dtype} {tuple(d.shape)}")
     if dy is not None and pre is None:
         raise ValueError("dy without pre")
+    n = branch.numel() // branch.shape[-1]
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
+        raise ValueError(f"stats must be contiguous float32 {(n, 2)}, got {stats.dtype} {tuple(stats.shape)}")
+    return _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, float(scale), float(residual_scale), need)
+
+
+def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, residual_scale, need):
+    """join_backward of arguments that have been looked at (kinds: what _check said of them)."""
+    dev, code, wcode, kind, gcode = kinds
+    H = branch.shape[-1]
     with _on_device(dev):
-        b, r, ds, dy = _rows(branch, H), _rows(residual, H), _rows(ds, H), _rows(dy, H)
+        (b, ldb), (r, ldr), (ds, lds), (dy, ldy) = _rows(branch, H), _rows(residual, H), _rows(ds, H), _rows(dy, H)
         n = b.shape[0]
-        if stats.dtype != torch.float32 or tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
-            raise ValueError(f"stats must be contiguous float32 {(n, 2)}, got {stats.dtype} {tuple(stats.shape)}")
         nothing = n == 0 or (ds is None and dy is None)
-        new = torch.zeros if nothing else torch.empty
 
         def like(t, wanted):
-            return new(t.shape, dtype=t.dtype, device=dev) if t is not None and wanted else None
+            return None if t is None or not wanted else t.new_zeros(t.shape) if nothing else t.new_empty(t.shape)
 
         db, dr, dpost, dgate = like(branch, need[0]), like(residual, need[1]), like(post, need[2]), like(gate, need[3])
         dpre = like(pre, need[4])
@@ -135,20 +146,18 @@ def join_backward(ds: torch.Tensor | None, dy: torch.Tensor | None, stats: torch
         nb = _backward_bytes(n, H) if join else 0
         ws = b.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
         _lib.check("mi355moe_norm_backward", _lib.lib().mi355moe_norm_backward(
-            _addr(ds), H if ds is None else _row_stride(ds), _addr(dy), H if dy is None else _row_stride(dy), b.data_ptr(), code, n, H,
-            _row_stride(b), _addr(r), H if r is None else _row_stride(r), _addr(post), _addr(pre), wcode, _addr(gate), gcode, kind,
-            float(scale), float(residual_scale), stats.data_ptr(), _addr(db), _addr(dr), _addr(dpost),
+            _addr(ds), lds, _addr(dy), ldy, b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode,
+            _addr(gate), gcode, kind, scale, residual_scale, stats.data_ptr(), _addr(db), _addr(dr), _addr(dpost),
             None if dy is None else _addr(dpre), _addr(dgate), _addr(ws), max(nb, 0), _raw_stream(dev)))
     return db, dr, dpost, dgate, dpre
 
 
 class _Join(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s):
-        s, y, stats = join_forward(branch, residual, post, gate, pre, eps, scale, residual_scale, need_s)
+    def forward(ctx, branch, residual, post, gate, pre, kinds, eps, scale, residual_scale, need_s):
+        s, y, stats = _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, True)
         ctx.save_for_backward(branch, residual, post, gate, pre, stats)
-        ctx.scales = scale, residual_scale
-        ctx.outputs = s is not None, y is not None
+        ctx.rest = kinds, scale, residual_scale, s is not None, y is not None
         ctx.set_materialize_grads(False)
         return (s, y) if s is not None and y is not None else s if y is None else y
 
@@ -159,20 +168,19 @@ class _Join(torch.autograd.Function):
         if _capturing(branch.device):
             raise RuntimeError("mi355moe: the backward pass of an eagerly recorded norm cannot be captured; capture "
                                "norm.join_forward and norm.join_backward")
-        ds = grads[0] if ctx.outputs[0] else None
-        dy = grads[-1] if ctx.outputs[1] else None
-        return (*join_backward(ds, dy, stats, branch, residual, post, gate, pre, *ctx.scales, need=ctx.needs_input_grad[:5]),
-                None, None, None, None)
+        kinds, scale, residual_scale, has_s, has_y = ctx.rest
+        return (*_backward(kinds, grads[0] if has_s else None, grads[-1] if has_y else None, stats, branch, residual, post, gate, pre,
+                           scale, residual_scale, ctx.needs_input_grad), None, None, None, None, None)
 
 
 def _call(branch, residual, post, gate, pre, eps, scale, residual_scale, need_s):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (branch, residual, post, gate, pre)):
-        dev = _check(branch, residual, post, gate, pre)[0]
-        if _capturing(dev):
+    kinds = _check(branch, residual, post, gate, pre)
+    if torch.is_grad_enabled() and (branch.requires_grad or any(t is not None and t.requires_grad for t in (residual, post, gate, pre))):
+        if _capturing(kinds[0]):
             raise RuntimeError("mi355moe: a norm cannot record a gradient during graph capture; capture norm.join_forward and "
                                "norm.join_backward")
-        return _Join.apply(branch, residual, post, gate, pre, eps, scale, residual_scale, need_s)
-    s, y, _ = join_forward(branch, residual, post, gate, pre, eps, scale, residual_scale, need_s)
+        return _Join.apply(branch, residual, post, gate, pre, kinds, eps, scale, residual_scale, need_s)
+    s, y, _ = _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, False)
     return (s, y) if s is not None and y is not None else s if y is None else y
 
 
@@ -184,11 +192,11 @@ def join(branch: torch.Tensor, residual: torch.Tensor | None = None, post: torch
     dtype; gate is [H], [..., 1] or [..., H] of any. Differentiable once in the five tensors by reverse mode (forward-mode
     derivatives are refused). While a graph is captured, a call that would record a gradient, and the backward pass of an
     eager one, are refused."""
-    return _call(branch, residual, post, gate, pre, eps, scale, residual_scale, True)
+    return _call(branch, residual, post, gate, pre, float(eps), float(scale), float(residual_scale), True)
 
 
 def rms(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """x * r(x) * weight over the last dimension, with join's types and gradients."""
     if weight is None:
         raise ValueError("rms needs a weight")
-    return _call(x, None, None, None, weight, eps, 1.0, 1.0, False)
+    return _call(x, None, None, None, weight, float(eps), 1.0, 1.0, False)

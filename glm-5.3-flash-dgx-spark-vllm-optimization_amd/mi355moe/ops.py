@@ -69,11 +69,15 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.shape[1] if t.shape[0] <= 1 else t.stride(0)
 
 
-def _rows_any(t: torch.Tensor) -> torch.Tensor:
-    """t [rows, H] itself where its values lie back to back in rows that do not overlap, else a contiguous copy."""
-    if t.is_contiguous() or ((t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
-        return t
-    return t.contiguous()
+def _rows_any(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """t [rows, H] itself where its values lie back to back in rows that do not overlap, else a contiguous copy, and the values
+    from one row to the next."""
+    H = t.shape[1]
+    if t.is_contiguous():
+        return t, H
+    if (H == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= H):
+        return t, _row_stride(t)
+    return t.contiguous(), H
 
 
 def _no_tangents(what: str, *ts: torch.Tensor | None) -> None:

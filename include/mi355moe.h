@@ -561,8 +561,8 @@ int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int6
 /* Its gradients (the residual's is dy itself): dz = dy act'(z) from the forward's z (NULL without an activation); dx [M][K] =
  * dz W, dw [N][K] = dz^T x, dbias [N] (bias_dtype) = the sums of dz over the rows; fp32 sums rounded once, deterministic. dbias
  * sums dz in fp32; the products take it rounded once to dtype (F16: times a power of two that brings the call's largest into
- * its range). Each gradient may be NULL (not computed). M >= 1 if dw or dbias is asked for. dy at any address and stride; x, w
- * (read for dw, dx) as for the forward; K % 8 == 0: dx and dw at 16-byte addresses. */
+ * its range). Each gradient may be NULL (not computed). M >= 1 if dw or dbias is asked for. dy, dx and dw at any address of
+ * their type; x, w (read for dw, dx) as for the forward. */
 int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, const void* x, int dtype, int64_t M, int64_t K,
                              int64_t x_stride, const void* w, int64_t N, int64_t w_stride, int activation, void* dx, void* dw,
