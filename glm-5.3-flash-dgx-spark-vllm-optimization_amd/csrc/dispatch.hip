@@ -10,6 +10,7 @@
 //
 // Without atomics on values: two calls give the same bits.
 #include <algorithm>
+#include <climits>
 
 #include "gemm_tile.cuh"
 #include "rows.cuh"
@@ -19,7 +20,6 @@ namespace mi355moe {
 // ------------------------------------------------------------------------------------------------ sort
 
 constexpr int SORT_ONE = 4096;          // pairs that one workgroup sorts alone
-constexpr int SORT_BLOCKS = 128;        // most workgroups of a call
 
 template <typename IT>
 __device__ __forceinline__ int sort_local(const SortArgs& a, int64_t i) {
@@ -130,17 +130,21 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(SortArgs a, int blocks
     }
 }
 
-static int64_t sort_chunk(int64_t P) {
+// Pairs of a workgroup: up to SORT_ONE one sorts alone (us alone / by eight: 4096 pairs 7.9 / -, 8192 12.0 / 7.9); else 1024, and in at
+// most 128 workgroups, with many experts, whose counts each of them reads, in 32 (us by 128 / 64 / 32 workgroups, 288 experts: 65536
+// pairs - / 10.9 / 10.5, 2^20 23.7 / 29 / 47; 4096 experts: 65536 - / 37.7 / 28.6, 2^18 62 / 46 / 44).
+static int64_t sort_chunk(int64_t P, int64_t n) {
     if (P <= SORT_ONE) return std::max<int64_t>(1024, (P + 1023) / 1024 * 1024);
-    return std::max<int64_t>(1024, ((P + SORT_BLOCKS - 1) / SORT_BLOCKS + 1023) / 1024 * 1024);
+    const int64_t most = n <= 1024 ? 128 : 32;
+    return ((P + most - 1) / most + 1023) / 1024 * 1024;
 }
-static int sort_blocks(int64_t P) { return P <= SORT_ONE ? 1 : (int)((P + sort_chunk(P) - 1) / sort_chunk(P)); }
-int64_t sort_count_words(int64_t P, int64_t n) { return sort_blocks(P) > 1 ? sort_blocks(P) * (n + 1) : 0; }
+static int sort_blocks(int64_t P, int64_t n) { return P <= SORT_ONE ? 1 : (int)((P + sort_chunk(P, n) - 1) / sort_chunk(P, n)); }
+int64_t sort_count_words(int64_t P, int64_t n) { return sort_blocks(P, n) > 1 ? sort_blocks(P, n) * (n + 1) : 0; }
 
 template <typename IT>
 static int run_sort(SortArgs a, hipStream_t st) {
-    const int blocks = sort_blocks(a.P), n1 = a.n + 1;
-    a.chunk = sort_chunk(a.P);
+    const int blocks = sort_blocks(a.P, a.n), n1 = a.n + 1;
+    a.chunk = sort_chunk(a.P, a.n);
     if (blocks > 1) {
         hipLaunchKernelGGL(sort_count_kernel<IT>, dim3(blocks), dim3(1024), n1 * 4, st, a);
         if (hipGetLastError() != hipSuccess) return -1;
@@ -155,24 +159,26 @@ int launch_sort(const SortArgs& a, hipStream_t st) { return a.ids64 ? run_sort<i
 
 // ------------------------------------------------------------------------------------------------ rows
 
-// The threads of a workgroup lie over 256 / lanes tokens, `lanes` (a power of two) over the 16-byte units of a row; UNI: a wave
-// has one token (lanes >= 64), whose table entries are then scalar.
+// The threads of a workgroup lie over 256 / lanes tokens and `lanes` = 2^shift of the 16-byte units of a row; the workgroups of a
+// token's `segs` pieces follow one another. UNI: a wave has one token (lanes >= 64), whose table entries are then scalar.
+struct RowsPlace {
+    int64_t t;
+    int unit;
+};
 template <bool UNI>
-__device__ __forceinline__ int64_t token_of(int shift) {
-    const int64_t t = ((int64_t)blockIdx.x << (8 - shift)) + (threadIdx.x >> shift);
-    if constexpr (UNI) return __builtin_amdgcn_readfirstlane((int)t);
-    else return t;
+__device__ __forceinline__ RowsPlace rows_place(int shift, int segs) {
+    const uint32_t g = blockIdx.x / (uint32_t)segs, seg = blockIdx.x - g * segs;
+    const int64_t t = ((int64_t)g << (8 - shift)) + (threadIdx.x >> shift);
+    return {UNI ? (int64_t)__builtin_amdgcn_readfirstlane((int)t) : t, (int)(seg << shift) + (int)(threadIdx.x & ((1 << shift) - 1))};
 }
 
 // rows[row] = x[t] (live) or zero, 16 bytes a thread and store; ES: bytes of a value.
 template <int ES, bool UNI>
-__global__ __launch_bounds__(256) void rows_scatter_kernel(RowsArgs a, int shift) {
-    const int64_t t = token_of<UNI>(shift);
-    const int64_t u = ((int64_t)blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1));
-    const int64_t RB = (int64_t)a.H * ES;                            // bytes of a row
-    const int64_t b = u * 16;
+__global__ __launch_bounds__(256) void rows_scatter_kernel(RowsArgs a, int shift, int segs) {
+    const auto [t, u] = rows_place<UNI>(shift, segs);
+    const int RB = a.H * ES, b = u * 16;                             // bytes of a row, and this thread's first
     if (t >= a.T || b >= RB) return;
-    const int left = (int)min((int64_t)16, RB - b);
+    const int left = min(16, RB - b);
     const unsigned char* src = static_cast<const unsigned char*>(a.x) + (size_t)t * a.x_stride * ES + b;
     u32x4 v = {0, 0, 0, 0};
     if (left == 16) v = *reinterpret_cast<const rows_u32x4*>(src);
@@ -191,58 +197,142 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(RowsArgs a, int shift
     }
 }
 
-// out[t] = shared[t] + the weighted rows of t, eight values a thread.
-template <int DT, bool UNI>
-__global__ __launch_bounds__(256) void rows_gather_kernel(RowsArgs a, int shift) {
-    const int64_t t = token_of<UNI>(shift);
-    const int64_t c = (((int64_t)blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1))) * 8;
-    const int n = (int)min((int64_t)8, a.H - c);
-    if (t >= a.T || n <= 0) return;
-    float acc[8] = {};
-    if (a.shared) load8<DT>(a.shared, (size_t)t * a.shared_stride + c, n, acc);
-    for (int j = 0; j < a.topk; ++j) {
-        const int64_t p = t * a.topk + j;
-        const int r = a.row[p];
-        if (r < 0 || r >= a.P) continue;
-        const float w = a.w ? any_value(a.w, a.wdt, p) : 1.0f;
-        float v[8];
-        load8<DT>(a.rows, (size_t)r * a.H + c, n, v);
+// The next N live slots' rows, requested together, then added in order.
+template <int DT, bool ONCE, int N>
+__device__ __forceinline__ void add_rows(const RowsArgs& a, uint64_t& live, int rv, float wv, int c, int n, float (&acc)[8]) {
+    Raw8<DT> v[N];
+    float w[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+    for (int k = 0; k < N; ++k) {
+        const int j = __builtin_ctzll(live);
+        live &= live - 1;
+        v[k].template load<ONCE>(a.rows, (size_t)__builtin_amdgcn_readlane(rv, j) * a.H + c, n);
+        w[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wv), j));
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        float x[8];
+        v[k].get(x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w[k], x[i], acc[i]);
+    }
+}
+
+// out[t] = shared[t] + the weighted rows of t, eight values a thread. A wave's lanes read the table entries of its token's slots
+// (at most 32), and the rows of up to eight slots are on their way at once.
+template <int DT, bool UNI, bool ONCE>
+__global__ __launch_bounds__(256) void rows_gather_kernel(RowsArgs a, int shift, int segs) {
+    const auto [t, u] = rows_place<UNI>(shift, segs);
+    const int c = u * 8, n = min(8, a.H - c);
+    if (t >= a.T || (!UNI && n <= 0)) return;
+    float acc[8] = {};
+    Raw8<DT> sh;
+    if (a.shared) sh.load(a.shared, (size_t)t * a.shared_stride + c, n);
+    if constexpr (UNI) {
+        const int lane = threadIdx.x & 63;
+        const int64_t p = t * a.topk + min(lane, a.topk - 1);
+        const int rv = lane < a.topk ? a.row[p] : -1;
+        const float wv = a.w ? any_value(a.w, a.wdt, p) : 1.0f;
+        uint64_t live = __ballot(rv >= 0 && rv < a.P);
+        if (a.shared) sh.get(acc);
+        int left = __popcll(live);
+        for (; left >= 8; left -= 8) add_rows<DT, ONCE, 8>(a, live, rv, wv, c, n, acc);
+        if (left & 4) add_rows<DT, ONCE, 4>(a, live, rv, wv, c, n, acc);
+        if (left & 2) add_rows<DT, ONCE, 2>(a, live, rv, wv, c, n, acc);
+        if (left & 1) add_rows<DT, ONCE, 1>(a, live, rv, wv, c, n, acc);
+    } else {
+        if (a.shared) sh.get(acc);
+        for (int j = 0; j < a.topk; ++j) {
+            const int64_t p = t * a.topk + j;
+            const int r = a.row[p];
+            if (r < 0 || r >= a.P) continue;
+            const float w = a.w ? any_value(a.w, a.wdt, p) : 1.0f;
+            float v[8];
+            load8<DT>(a.rows, (size_t)r * a.H + c, n, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w, v[i], acc[i]);
+        }
     }
     store8<DT>(a.out, (size_t)t * a.out_stride + c, n, acc);
 }
 
-// drows and dw of one pair a wave: the waves of a workgroup are neighbours, mostly slots of one token.
-template <int DT>
-__global__ __launch_bounds__(256) void rows_grad_kernel(RowsArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t p = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (p >= a.P) return;
-    const int r = a.row[p];
-    const int64_t to = r < 0 ? ~r : r, t = p / a.topk;
-    if (to >= a.P) return;
-    const float w = r < 0 ? 0.0f : any_value(a.w, a.wdt, p);
-    float dot = 0.0f;
-    for (int c = lane * 8; c < a.H; c += 512) {
+// drows and dw of the next N live slots of token t.
+template <int DT, bool ONCE, int N>
+__device__ __forceinline__ void grad_rows(const RowsArgs& a, int64_t t, uint64_t& live, int rv, float wv, float (*red)[4]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int slot[N];
+    size_t row[N];
+    float w[N], dot[N] = {};
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        slot[k] = __builtin_ctzll(live);
+        live &= live - 1;
+        row[k] = (size_t)__builtin_amdgcn_readlane(rv, slot[k]) * a.H;
+        w[k] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wv), slot[k]));
+    }
+    for (int c = threadIdx.x * 8; c < a.H; c += blockDim.x * 8) {
         const int n = a.H - c;
-        float d[8] = {}, y[8];
-        if (r >= 0) {                                                // (uniform)
-            load8<DT>(a.x, (size_t)t * a.x_stride + c, n, d);
+        Raw8<DT> d8, y8[N];
+        d8.load(a.x, (size_t)t * a.x_stride + c, n);
+        if (a.dw)                                                    // (uniform)
+#pragma unroll
+            for (int k = 0; k < N; ++k) y8[k].template load<ONCE>(a.y, row[k] + c, n);
+        float d[8];
+        d8.get(d);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float v[8];
             if (a.dw) {
-                load8<DT>(a.y, (size_t)to * a.H + c, n, y);
+                y8[k].get(v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(d[i], y[i], dot);
+                for (int i = 0; i < 8; ++i) dot[k] = __builtin_fmaf(d[i], v[i], dot[k]);
             }
+            if (a.rows) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] *= w;
+                for (int i = 0; i < 8; ++i) v[i] = w[k] * d[i];
+                store8<DT>(a.rows, row[k] + c, n, v);
+            }
         }
-        if (a.rows) store8<DT>(a.rows, (size_t)to * a.H + c, n, d);
     }
-    if (a.dw) {
-        dot = wave_sum(dot);
-        if (lane == 0) store_any(a.dw, a.wdt, p, dot);
+    if (!a.dw) return;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        dot[k] = wave_sum(dot[k]);
+        if (lane == 0) red[k][wave] = dot[k];
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if ((int)threadIdx.x == k) {
+            float s = 0.0f;
+            for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[k][i];
+            store_any(a.dw, a.wdt, t * a.topk + slot[k], s);
+        }
+    __syncthreads();                                                 // (the sums have been read: the next slots write them)
+}
+
+// A workgroup a token: dout[t] is read once for eight slots, whose rows are on their way at once; at most four waves.
+template <int DT, bool ONCE>
+__global__ __launch_bounds__(256) void rows_grad_kernel(RowsArgs a) {
+    __shared__ float red[8][4];
+    const int64_t t = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    const int64_t p = t * a.topk + min(lane, a.topk - 1);
+    const int rv = lane < a.topk ? a.row[p] : INT_MAX;
+    const float wv = any_value(a.w, a.wdt, p);
+    uint64_t live = __ballot(rv >= 0 && rv < a.P), dead = __ballot(rv < 0 && ~rv < a.P);      // (the same in every wave)
+    if (a.dw && threadIdx.x < 64 && (dead >> lane & 1)) store_any(a.dw, a.wdt, p, 0.0f);
+    if (a.rows)
+        for (; dead; dead &= dead - 1) {
+            const size_t row = (size_t)~__builtin_amdgcn_readlane(rv, __builtin_ctzll(dead)) * a.H;
+            const float zero[8] = {};
+            for (int c = threadIdx.x * 8; c < a.H; c += blockDim.x * 8) store8<DT>(a.rows, row + c, a.H - c, zero);
+        }
+    int left = __popcll(live);
+    for (; left >= 8; left -= 8) grad_rows<DT, ONCE, 8>(a, t, live, rv, wv, red);
+    if (left & 4) grad_rows<DT, ONCE, 4>(a, t, live, rv, wv, red);
+    if (left & 2) grad_rows<DT, ONCE, 2>(a, t, live, rv, wv, red);
+    if (left & 1) grad_rows<DT, ONCE, 1>(a, t, live, rv, wv, red);
 }
 
 // log2 of the threads on a row of `units` pieces: all of them, 8 to 256.
@@ -251,25 +341,31 @@ static int row_shift(int64_t units) {
     while (s < 8 && (1 << s) < units) ++s;
     return s;
 }
+// (T <= 2^24 tokens of at most 64 pieces where a workgroup has one token, else of one)
+static unsigned rows_grid(int64_t T, int shift, int segs) { return (unsigned)((T + (256 >> shift) - 1) / (256 >> shift) * segs); }
 
 template <int ES>
 static int run_scatter(const RowsArgs& a, hipStream_t st) {
-    const int64_t units = ((int64_t)a.H * ES + 15) / 16;
-    const int s = row_shift(units), per = 256 >> s;
-    const dim3 g((unsigned)((a.T + per - 1) / per), (unsigned)((units + (1 << s) - 1) >> s));
-    if (s >= 6) hipLaunchKernelGGL((rows_scatter_kernel<ES, true>), g, dim3(256), 0, st, a, s);
-    else hipLaunchKernelGGL((rows_scatter_kernel<ES, false>), g, dim3(256), 0, st, a, s);
+    const int units = (a.H * ES + 15) / 16, s = row_shift(units), segs = (units + (1 << s) - 1) >> s;
+    const dim3 g(rows_grid(a.T, s, segs));
+    if (s >= 6) hipLaunchKernelGGL((rows_scatter_kernel<ES, true>), g, dim3(256), 0, st, a, s, segs);
+    else hipLaunchKernelGGL((rows_scatter_kernel<ES, false>), g, dim3(256), 0, st, a, s, segs);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 int launch_rows_scatter(const RowsArgs& a, hipStream_t st) { return a.dt == DT_F32 ? run_scatter<4>(a, st) : run_scatter<2>(a, st); }
 
+// Rows of 64 MB and more are marked as read once. us plain / marked, bf16 rows of 4096, top 8: gather, 512 tokens (34 MB) 8.7 / 8.7, 1024
+// 21 / 15.6, 4096 79 / 59, 8192 130 / 106; gradient, 512 17.8 / 18.6, and after a gather that left nothing of them in the caches,
+// as in a training step, 2048 75 / 60, 4096 136 / 116.
+static bool rows_once(const RowsArgs& a) { return a.P * a.H * (a.dt == DT_F32 ? 4 : 2) >= (64 << 20); }
+
 template <int DT>
 static int run_gather(const RowsArgs& a, hipStream_t st) {
-    const int64_t units = (a.H + 7) / 8;
-    const int s = row_shift(units), per = 256 >> s;
-    const dim3 g((unsigned)((a.T + per - 1) / per), (unsigned)((units + (1 << s) - 1) >> s));
-    if (s >= 6) hipLaunchKernelGGL((rows_gather_kernel<DT, true>), g, dim3(256), 0, st, a, s);
-    else hipLaunchKernelGGL((rows_gather_kernel<DT, false>), g, dim3(256), 0, st, a, s);
+    const int units = (a.H + 7) / 8, s = row_shift(units), segs = (units + (1 << s) - 1) >> s;
+    const dim3 g(rows_grid(a.T, s, segs));
+    if (s >= 6 && rows_once(a)) hipLaunchKernelGGL((rows_gather_kernel<DT, true, true>), g, dim3(256), 0, st, a, s, segs);
+    else if (s >= 6) hipLaunchKernelGGL((rows_gather_kernel<DT, true, false>), g, dim3(256), 0, st, a, s, segs);
+    else hipLaunchKernelGGL((rows_gather_kernel<DT, false, false>), g, dim3(256), 0, st, a, s, segs);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 int launch_rows_gather(const RowsArgs& a, hipStream_t st) {
@@ -278,7 +374,9 @@ int launch_rows_gather(const RowsArgs& a, hipStream_t st) {
 
 template <int DT>
 static int run_rows_grad(const RowsArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(rows_grad_kernel<DT>, dim3((unsigned)((a.P + 3) / 4)), dim3(256), 0, st, a);
+    const dim3 g((unsigned)a.T), b(std::min(256, (a.H + 511) / 512 * 64));
+    if (rows_once(a)) hipLaunchKernelGGL((rows_grad_kernel<DT, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((rows_grad_kernel<DT, false>), g, b, 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 int launch_rows_grad(const RowsArgs& a, hipStream_t st) {

@@ -322,13 +322,17 @@ constexpr int DZ_ROWS = 64;                                          // rows of 
 template <int DT>
 __device__ __forceinline__ void slope8(const LinearArgs& a, int64_t m, int c, float (&d)[8]) {
     const int n = a.N - c;
-    load8<DT>(a.dy, (size_t)m * a.dy_stride + c, n, d);
+    Raw8<DT> d8;
+    d8.load(a.dy, (size_t)m * a.dy_stride + c, n);
     if (a.act != ACT_NONE) {
+        Raw8<DT_F32> z8;
+        z8.load(a.z, (size_t)m * a.N + c, n);
         float z[8];
-        load8<DT_F32>(a.z, (size_t)m * a.N + c, n, z);
+        z8.get(z);
+        d8.get(d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) d[j] *= act_slope(a.act, z[j]);
-    }
+    } else d8.get(d);
 }
 
 // The largest finite magnitude of dz, as fp32 bits, of each workgroup's share (fp16 only: dz = dy act'(z) can lie among fp16's

@@ -44,7 +44,7 @@ __device__ __forceinline__ float inv_rms(float sum, int H, float eps) { return _
 
 // A row of up to 8 NV values a thread: by a wave, four rows a workgroup (WG false), or by a workgroup of as many threads as the row
 // needs. Everything that the row reads is requested before the first sum.
-template <int DT, bool WG, int NV>
+template <int DT, bool WG, int NV, bool ONCE>
 __global__ __launch_bounds__(WG ? 1024 : 256) void norm_kernel(NormArgs a) {
     __shared__ float red[2][16];
     const int tpr = WG ? blockDim.x : 64, tid = WG ? threadIdx.x : threadIdx.x & 63;
@@ -56,8 +56,8 @@ __global__ __launch_bounds__(WG ? 1024 : 256) void norm_kernel(NormArgs a) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int c = (v * tpr + tid) * 8, n = a.H - c;
-        rb8[v].load(a.branch, (size_t)r * a.branch_stride + c, n);
-        if (a.res) rr8[v].load(a.res, (size_t)r * a.res_stride + c, n);
+        rb8[v].template load<ONCE>(a.branch, (size_t)r * a.branch_stride + c, n);
+        if (a.res) rr8[v].template load<ONCE>(a.res, (size_t)r * a.res_stride + c, n);
         if (a.post) post8[v].load(a.post, a.wdt, c, n);
         if (a.gate_kind == GATE_CHANNEL) gate8[v].load(a.gate, a.gdt, c, n);
         if (a.gate_kind == GATE_FULL) gate8[v].load(a.gate, a.gdt, (size_t)r * a.H + c, n);
@@ -339,12 +339,17 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(NormArgs a, int parts) 
 // Threads of a row: eight values each up to 8192, sixteen beyond; whole waves.
 static int norm_threads(int H) { return H <= 8192 ? (H + 511) / 512 * 64 : 1024; }
 
+// Tensors of 64 MB and more are marked as read once (us plain / marked, bf16 rows of 4096: 1237 rows 11.2 / 11.7, 8192 47.5 / 46.0,
+// 16384 94.6 / 86.5; the gradient, which reads and writes more besides: no difference).
+static bool norm_once(const NormArgs& a) { return a.rows * a.H * (a.dt == DT_F32 ? 4 : 2) >= (64 << 20); }
+
 template <int DT>
 static int run_norm(const NormArgs& a, hipStream_t st) {
     const int t = norm_threads(a.H);
-    if (t == 64) hipLaunchKernelGGL((norm_kernel<DT, false, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
-    else if (a.H <= 8192) hipLaunchKernelGGL((norm_kernel<DT, true, 1>), dim3((unsigned)a.rows), dim3(t), 0, st, a);
-    else hipLaunchKernelGGL((norm_kernel<DT, true, 2>), dim3((unsigned)a.rows), dim3(t), 0, st, a);
+    if (t == 64) hipLaunchKernelGGL((norm_kernel<DT, false, 1, false>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, st, a);
+    else if (a.H <= 8192 && norm_once(a)) hipLaunchKernelGGL((norm_kernel<DT, true, 1, true>), dim3((unsigned)a.rows), dim3(t), 0, st, a);
+    else if (a.H <= 8192) hipLaunchKernelGGL((norm_kernel<DT, true, 1, false>), dim3((unsigned)a.rows), dim3(t), 0, st, a);
+    else hipLaunchKernelGGL((norm_kernel<DT, true, 2, false>), dim3((unsigned)a.rows), dim3(t), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 int launch_norm(const NormArgs& a, hipStream_t st) {

@@ -99,11 +99,13 @@ __device__ __forceinline__ void store_any(void* p, int dt, size_t i, float v) {
 template <int DT>
 struct Raw8 {
     u32x4 w[DT == DT_F32 ? 2 : 1];
+    // ONCE: marked as read once, so that a stream larger than the caches does not push other lines out of them
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(const void* p, size_t i, int n) {
         if (n >= 8) {
             const rows_u32x4* q = reinterpret_cast<const rows_u32x4*>(static_cast<const unsigned char*>(p) + i * (DT == DT_F32 ? 4 : 2));
-            w[0] = q[0];
-            if constexpr (DT == DT_F32) w[1] = q[1];
+            w[0] = ONCE ? __builtin_nontemporal_load(q) : q[0];
+            if constexpr (DT == DT_F32) w[1] = ONCE ? __builtin_nontemporal_load(q + 1) : q[1];
         } else {
             w[0] = u32x4{0, 0, 0, 0};
             if constexpr (DT == DT_F32) w[1] = u32x4{0, 0, 0, 0};
