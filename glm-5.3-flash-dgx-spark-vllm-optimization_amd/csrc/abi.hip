@@ -351,6 +351,11 @@ int gated_ok(int dtype, int64_t T, int64_t K, int64_t N) {
     if (T > (1 << 24) || K > 65536 || N > 16384) return MI355MOE_ELIMIT;
     return 0;
 }
+// Whether an address is one of a dtype's (or absent).
+bool at_ok(const void* p, int dtype) {
+    const int size = dtype == MI355MOE_I64 ? 8 : dtype == MI355MOE_F32 || dtype == MI355MOE_I32 ? 4 : 2;
+    return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0;
+}
 // The dense product's sizes; K % 8 == 0: its operands as the gated block's.
 int linear_ok(int dtype, int64_t M, int64_t K, int64_t N, int activation) {
     if (dtype != MI355MOE_F16 && dtype != MI355MOE_BF16) return MI355MOE_EDTYPE;
@@ -361,7 +366,7 @@ int linear_ok(int dtype, int64_t M, int64_t K, int64_t N, int activation) {
 }
 int linear_operands(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int64_t K) {
     if (x_stride < K || w_stride < K) return MI355MOE_ESHAPE;
-    if ((reinterpret_cast<uintptr_t>(x) & 1) || (reinterpret_cast<uintptr_t>(w) & 1)) return MI355MOE_EINVAL;
+    if (!at_ok(x, MI355MOE_F16) || !at_ok(w, MI355MOE_F16)) return MI355MOE_EINVAL;
     if (K % 8) return 0;
     if (!rows16_ok(x, x_stride) || !rows16_ok(w, w_stride)) return MI355MOE_EINVAL;
     return x_stride > (1 << 22) || w_stride > (1 << 22) ? MI355MOE_ESHAPE : 0;
@@ -371,6 +376,10 @@ int rows_ok(int dtype, int64_t T, int64_t H, int64_t topk) {
     if (T < 0 || H < 1) return MI355MOE_ESHAPE;
     if (topk < 1 || topk > MAX_TOPK || T * topk > (1 << 24) || T > (1 << 24) || H > 65536) return MI355MOE_ELIMIT;
     return 0;
+}
+bool norm_inputs_ok(const void* branch, const void* residual, int dtype, const void* post, const void* pre, int weights_dtype,
+                    const void* gate, int gate_dtype) {
+    return at_ok(branch, dtype) && at_ok(residual, dtype) && at_ok(post, weights_dtype) && at_ok(pre, weights_dtype) && at_ok(gate, gate_dtype);
 }
 int norm_ok(int dtype, int64_t rows, int64_t H) {
     if (dtype != MI355MOE_F32 && dtype != MI355MOE_F16 && dtype != MI355MOE_BF16) return MI355MOE_EDTYPE;
@@ -2149,6 +2158,9 @@ int mi355moe_sort_tokens(const void* ids, int ids_dtype, int64_t T, int64_t topk
     if (n < 1 || n > MAX_EXPERTS) return MI355MOE_ELIMIT;
     if (expert_map && n_global < 0) return MI355MOE_EINVAL;
     if (!offsets || (T > 0 && (!ids || !row || !pair))) return MI355MOE_EINVAL;
+    if (!at_ok(ids, ids_dtype) || !at_ok(expert_map, MI355MOE_I64) || !at_ok(row, MI355MOE_I32) || !at_ok(pair, MI355MOE_I32) ||
+        !at_ok(offsets, MI355MOE_I32))
+        return MI355MOE_EINVAL;
     const int64_t need = mi355moe_sort_tokens_workspace_bytes(T, topk, n);
     if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 3))) return MI355MOE_EINVAL;
     if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
@@ -2172,6 +2184,7 @@ int mi355moe_rows_to_experts(const void* x, int dtype, int64_t T, int64_t H, int
     if (x_stride < H) return MI355MOE_ESHAPE;
     if (T == 0) return 0;
     if (!x || !row || !rows) return MI355MOE_EINVAL;
+    if (!at_ok(x, dtype) || !at_ok(row, MI355MOE_I32) || !at_ok(rows, dtype)) return MI355MOE_EINVAL;
     RowsArgs a{};
     a.dt = dt_w(dtype);
     a.T = T;
@@ -2193,6 +2206,8 @@ int mi355moe_rows_from_experts(const void* rows, int dtype, int64_t T, int64_t H
     if (out_stride < H || (shared && shared_stride < H)) return MI355MOE_ESHAPE;
     if (T == 0) return 0;
     if (!rows || !row || !out) return MI355MOE_EINVAL;
+    if (!at_ok(rows, dtype) || !at_ok(row, MI355MOE_I32) || !at_ok(weights, weights_dtype) || !at_ok(shared, dtype) || !at_ok(out, dtype))
+        return MI355MOE_EINVAL;
     RowsArgs a{};
     a.dt = dt_w(dtype);
     a.T = T;
@@ -2218,6 +2233,9 @@ int mi355moe_rows_from_experts_backward(const void* dout, int dtype, int64_t T, 
     if (dout_stride < H) return MI355MOE_ESHAPE;
     if (T == 0 || (!drows && !dweights)) return 0;
     if (!dout || !row || !weights || (dweights && !rows)) return MI355MOE_EINVAL;
+    if (!at_ok(dout, dtype) || !at_ok(row, MI355MOE_I32) || !at_ok(weights, weights_dtype) || !at_ok(rows, dtype) || !at_ok(drows, dtype) ||
+        !at_ok(dweights, weights_dtype))
+        return MI355MOE_EINVAL;
     RowsArgs a{};
     a.dt = dt_w(dtype);
     a.T = T;
@@ -2249,6 +2267,7 @@ int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int6
     if (out_stride < N || (residual && residual_stride < N)) return MI355MOE_ESHAPE;
     if (M == 0) return 0;
     if (!x || !w || !out) return MI355MOE_EINVAL;
+    if (!at_ok(bias, bias_dtype) || !at_ok(residual, dtype) || !at_ok(out, dtype) || !at_ok(z, MI355MOE_F32)) return MI355MOE_EINVAL;
     if (int r = linear_operands(x, x_stride, w, w_stride, K)) return r;
     const int64_t need = linear_forward_bytes(M, N, K);
     if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))) return MI355MOE_EINVAL;
@@ -2287,6 +2306,7 @@ int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, 
     if (!dx && !dw && !dbias) return 0;
     if (M == 0) return dw || dbias ? MI355MOE_ESHAPE : 0;
     if (!dy || !workspace || (activation != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return MI355MOE_EINVAL;
+    if (!at_ok(dy, dtype) || !at_ok(z, MI355MOE_F32) || !at_ok(dx, dtype) || !at_ok(dw, dtype) || !at_ok(dbias, bias_dtype)) return MI355MOE_EINVAL;
     if (int r = linear_operands(dw ? x : nullptr, dw ? x_stride : (K + 7) / 8 * 8, dx ? w : nullptr, dx ? w_stride : (K + 7) / 8 * 8, K)) return r;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return MI355MOE_EINVAL;
     if ((int64_t)workspace_bytes < linear_backward_bytes(M, N, K)) return MI355MOE_EWORKSPACE;
@@ -2321,7 +2341,8 @@ int mi355moe_norm_forward(const void* branch, int dtype, int64_t rows, int64_t H
     if (branch_stride < H || (residual && residual_stride < H)) return MI355MOE_ESHAPE;
     if (!(eps >= 0.0f) || (pre != nullptr) != (y != nullptr) || (!s && !y)) return MI355MOE_EINVAL;
     if (rows == 0) return 0;
-    if (!branch) return MI355MOE_EINVAL;
+    if (!branch || !norm_inputs_ok(branch, residual, dtype, post, pre, weights_dtype, gate, gate_dtype)) return MI355MOE_EINVAL;
+    if (!at_ok(s, dtype) || !at_ok(y, dtype) || !at_ok(stats, MI355MOE_F32)) return MI355MOE_EINVAL;
     NormArgs a{};
     a.dt = dt_w(dtype);
     a.rows = rows;
@@ -2365,6 +2386,10 @@ int mi355moe_norm_backward(const void* ds, int64_t ds_stride, const void* dy, in
     const bool joined = dpost || dpre || (dgate && gate_kind == GATE_CHANNEL);
     if (rows == 0) return joined ? MI355MOE_ESHAPE : 0;
     if ((!ds && !dy) || !branch || !stats) return MI355MOE_EINVAL;
+    if (!norm_inputs_ok(branch, residual, dtype, post, pre, weights_dtype, gate, gate_dtype) || !at_ok(stats, MI355MOE_F32) ||
+        !at_ok(ds, dtype) || !at_ok(dy, dtype) || !at_ok(dbranch, dtype) || !at_ok(dresidual, dtype) || !at_ok(dpost, weights_dtype) ||
+        !at_ok(dpre, weights_dtype) || !at_ok(dgate, gate_dtype))
+        return MI355MOE_EINVAL;
     if (joined) {
         if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)) return MI355MOE_EINVAL;
         if ((int64_t)workspace_bytes < mi355moe_norm_backward_workspace_bytes(rows, H)) return MI355MOE_EWORKSPACE;

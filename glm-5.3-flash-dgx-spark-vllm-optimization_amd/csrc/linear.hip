@@ -588,11 +588,12 @@ static int linear_backward(const LinearArgs& a, char* ws, hipStream_t st) {
     g.dz_stride = N8;
     g.tops = reinterpret_cast<uint32_t*>(ws + s.tops);
     g.unscale = reinterpret_cast<float*>(g.tops + LINEAR_TOPS);
-    if (DT == DT_F16 && g.dz && a.act != ACT_NONE && a.act != ACT_RELU) {
-        g.ntops = (int)std::min<int64_t>((a.M * ((a.N + 7) / 8) + 255) / 256, LINEAR_TOPS);
-        hipLaunchKernelGGL(linear_top_kernel<DT>, dim3(g.ntops), dim3(256), 0, st, g);
-        if (hipGetLastError() != hipSuccess) return -1;
-    }
+    if constexpr (DT == DT_F16)
+        if (g.dz && a.act != ACT_NONE && a.act != ACT_RELU) {
+            g.ntops = (int)std::min<int64_t>((a.M * ((a.N + 7) / 8) + 255) / 256, LINEAR_TOPS);
+            hipLaunchKernelGGL(linear_top_kernel<DT>, dim3(g.ntops), dim3(256), 0, st, g);
+            if (hipGetLastError() != hipSuccess) return -1;
+        }
     if (g.dz || a.dbias) {
         const int parts = (int)((a.M + DZ_ROWS - 1) / DZ_ROWS);
         hipLaunchKernelGGL(linear_dz_kernel<DT>, dim3(parts, (a.N + 255) / 256), dim3(256), 0, st, g);

@@ -20,10 +20,9 @@ from __future__ import annotations
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, ids_dtype_code,
+from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any, ids_dtype_code,
                   weight_dtype_code)
 
 
@@ -107,7 +106,7 @@ def _to_experts(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     code = _check(plan, "x", x, plan.tokens, dev)
     H = x.shape[1]
     with _on_device(dev):
-        x, ldx = _rows_any(_plain(x))
+        x, ldx = _rows_any(x)
         rows = x.new_empty((plan.tokens * plan.topk, H))
         _lib.check("mi355moe_rows_to_experts", _lib.lib().mi355moe_rows_to_experts(
             x.data_ptr(), code, plan.tokens, H, ldx, plan._words.data_ptr(), plan.topk, rows.data_ptr(), _raw_stream(dev)))
@@ -129,9 +128,9 @@ def _from_experts(rows, weights, plan, shared):
     wcode = _lib.F32 if weights is None else weight_dtype_code(weights.dtype)
     H = rows.shape[1]
     with _on_device(dev):
-        rows = _plain(rows).contiguous()
-        weights = None if weights is None else _plain(weights).contiguous()
-        shared, lds = (None, H) if shared is None else _rows_any(_plain(shared))
+        rows = _packed(rows)
+        weights = None if weights is None else _packed(weights)
+        shared, lds = (None, H) if shared is None else _rows_any(shared)
         out = rows.new_empty((plan.tokens, H))
         _lib.check("mi355moe_rows_from_experts", _lib.lib().mi355moe_rows_from_experts(
             rows.data_ptr(), code, plan.tokens, H, plan._words.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared), lds,
@@ -156,9 +155,9 @@ def _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights):
     """from_experts_backward of arguments that have been looked at."""
     H = rows.shape[1]
     with _on_device(dev):
-        (dout, ldd), rows, weights = _rows_any(_plain(dout)), _plain(rows).contiguous(), _plain(weights).contiguous()
-        drows = torch.empty_like(rows) if need_rows else None        # (contiguous, like the two)
-        dw = torch.empty_like(weights) if need_weights else None
+        (dout, ldd), rows, weights = _rows_any(dout), _packed(rows), _packed(weights)
+        drows = rows.new_empty(rows.shape) if need_rows else None
+        dw = weights.new_empty(weights.shape) if need_weights else None
         _lib.check("mi355moe_rows_from_experts_backward", _lib.lib().mi355moe_rows_from_experts_backward(
             dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(),
             weight_dtype_code(weights.dtype), rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev)))
@@ -176,7 +175,7 @@ class _To(torch.autograd.Function):
         return _to_experts(x, plan)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, drows):
         if _capturing(drows.device):
             raise RuntimeError(_NOT_CAPTURED.format("to_experts", "run an eager call's backward pass"))
@@ -191,7 +190,7 @@ class _From(torch.autograd.Function):
         return _from_experts(rows, weights, plan, shared)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         if _capturing(dout.device):
             raise RuntimeError(_NOT_CAPTURED.format("from_experts", "run an eager call's backward pass"))

@@ -29,8 +29,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _row_stride, _rows_any,
-                  act_dtype_code, weight_dtype_code)
+from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain, _raw_stream, _row_stride,
+                  _rows_any, act_dtype_code, weight_dtype_code)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -162,13 +162,14 @@ def _linear_bytes(backward: bool, M: int, K: int, N: int) -> int:
 
 
 def _linear_operand(t: torch.Tensor, K: int) -> tuple[torch.Tensor, int]:
-    """t [rows, K] as the product reads it, and the values from one row to the next: where K is a multiple of 8 its rows lie at
-    16-byte addresses."""
+    """t [..., K] as the product reads its rows, and the values from one row to the next: where K is a multiple of 8 the rows lie
+    at 16-byte addresses."""
     if K & 7:
         return _rows_any(t)
     if t.is_contiguous() and not t.data_ptr() & 15:
         return t, K
-    t = _rows16(t)
+    t = _plain(t)
+    t = _rows16(t if t.dim() == 2 else t.reshape(-1, K))
     return t, _row_stride(t)
 
 
@@ -204,15 +205,10 @@ def _linear(kinds, x, w, bias, activation, residual, save):
     dev, code, bcode = kinds
     N, K = w.shape
     with _on_device(dev):
-        x2 = _plain(x)
-        x2, ldx = _linear_operand(x2 if x2.dim() == 2 else x2.reshape(-1, K), K)
-        w2, ldw = _linear_operand(_plain(w), K)
-        b = None if bias is None else _plain(bias).contiguous()
-        r, ldr = None, N
-        if residual is not None:
-            r = _plain(residual)
-            r, ldr = _rows_any(r if r.dim() == 2 else r.reshape(-1, N))
-        M = x2.shape[0]
+        (x2, ldx), (w2, ldw) = _linear_operand(x, K), _linear_operand(w, K)
+        b = None if bias is None else _packed(bias)
+        r, ldr = (None, N) if residual is None else _rows_any(residual)
+        M = x2.numel() // K
         out = x2.new_empty((*x.shape[:-1], N))
         z = x2.new_empty((M, N), dtype=torch.float32) if save and activation is not None else None
         nb = _linear_bytes(False, M, K, N)
@@ -246,11 +242,8 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
     dev, code, _ = kinds
     N, K = w.shape
     with _on_device(dev):
-        x2, d2 = _plain(x), _plain(dout)
-        if x2.dim() != 2:
-            x2, d2 = x2.reshape(-1, K), d2.reshape(-1, N)
-        (x2, ldx), (w2, ldw), (d2, ldd) = _linear_operand(x2, K), _linear_operand(_plain(w), K), _rows_any(d2)
-        M = x2.shape[0]
+        (x2, ldx), (w2, ldw), (d2, ldd) = _linear_operand(x, K), _linear_operand(w, K), _rows_any(dout)
+        M = x2.numel() // K
         new = x2.new_zeros if M == 0 else x2.new_empty
         dx = new(x.shape) if need_dx else None
         dw = new((N, K)) if need_dw else None
@@ -275,7 +268,7 @@ class _Linear(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         if _capturing(dout.device):
             raise RuntimeError("mi355moe: the backward pass of an eagerly recorded ffn.linear cannot be captured; capture "

@@ -18,10 +18,9 @@ from __future__ import annotations
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _plain, _raw_stream, _rows_any, weight_dtype_code
+from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any, weight_dtype_code
 
 _NONE, _CHANNEL, _TOKEN, _FULL = 0, 1, 2, 3
 
@@ -64,14 +63,11 @@ def _check(branch, residual, post, gate, pre):
 
 
 def _rows(t: torch.Tensor | None, H: int) -> tuple[torch.Tensor | None, int]:
-    if t is None:
-        return None, H
-    t = _plain(t)
-    return _rows_any(t if t.dim() == 2 else t.reshape(-1, H))
+    return (None, H) if t is None else _rows_any(t)
 
 
 def _flat(t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else _plain(t).contiguous()
+    return None if t is None else _packed(t)
 
 
 def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, need_stats):
@@ -81,8 +77,8 @@ def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scal
     shape = branch.shape
     H = shape[-1]
     with _on_device(dev):
-        (b, ldb), (r, ldr) = _rows(branch, H), _rows(residual, H)
-        n = b.shape[0]
+        (b, ldb), (r, ldr) = _rows_any(branch), _rows(residual, H)
+        n = b.numel() // H
         post, pre, gate = _flat(post), _flat(pre), _flat(gate)
         s = b.new_empty(shape) if need_s else None
         y = b.new_empty(shape) if pre is not None else None
@@ -128,8 +124,8 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
     dev, code, wcode, kind, gcode = kinds
     H = branch.shape[-1]
     with _on_device(dev):
-        (b, ldb), (r, ldr), (ds, lds), (dy, ldy) = _rows(branch, H), _rows(residual, H), _rows(ds, H), _rows(dy, H)
-        n = b.shape[0]
+        (b, ldb), (r, ldr), (ds, lds), (dy, ldy) = _rows_any(branch), _rows(residual, H), _rows(ds, H), _rows(dy, H)
+        n = b.numel() // H
         nothing = n == 0 or (ds is None and dy is None)
 
         def like(t, wanted):
@@ -162,7 +158,7 @@ class _Join(torch.autograd.Function):
         return (s, y) if s is not None and y is not None else s if y is None else y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, *grads):
         branch, residual, post, gate, pre, stats = ctx.saved_tensors
         if _capturing(branch.device):

@@ -9,9 +9,11 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .layer import Exl3Experts
@@ -59,6 +61,18 @@ def _need_cuda(*ts: torch.Tensor) -> torch.device:
     return dev
 
 
+def _once(backward):
+    """A Function's backward pass that has no derivative of its own: torch's once_differentiable, whose wrapping is left out
+    where no graph of the backward pass is recorded."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
+
+
 def _plain(t: torch.Tensor) -> torch.Tensor:
     return t.detach() if t.requires_grad else t
 
@@ -70,14 +84,22 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _rows_any(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """t [rows, H] itself where its values lie back to back in rows that do not overlap, else a contiguous copy, and the values
-    from one row to the next."""
-    H = t.shape[1]
+    """t [..., H] as rows of H values: t itself where they lie back to back in rows that do not overlap, else a contiguous copy,
+    and the values from one row to the next. (What needs no copy is not detached either: the kernels take its address.)"""
+    H = t.shape[-1]
     if t.is_contiguous():
         return t, H
+    t = _plain(t)
+    if t.dim() != 2:
+        t = t.reshape(-1, H)
     if (H == 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= H):
         return t, _row_stride(t)
     return t.contiguous(), H
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """t with its values back to back."""
+    return t if t.is_contiguous() else _plain(t).contiguous()
 
 
 def _no_tangents(what: str, *ts: torch.Tensor | None) -> None:
