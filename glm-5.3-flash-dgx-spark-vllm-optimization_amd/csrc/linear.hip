@@ -134,11 +134,9 @@ __device__ __forceinline__ f32x4 linear_mma16(u32x4 a, u32x4 b, f32x4 c) {
 }
 // Chunk (eight values) i of a row of K values, what lies behind the row's end as zero.
 __device__ __forceinline__ u32x4 row_chunk(const uint16_t* row, int i, int K) {
-    const int n = K - 8 * i;
-    u32x4 v = {0, 0, 0, 0};
-    if (n >= 8) return *reinterpret_cast<const rows_u32x4*>(row + 8 * i);
-    for (int j = 0; j < n; ++j) v[j >> 1] |= (uint32_t)row[8 * i + j] << (16 * (j & 1));
-    return v;
+    Raw8<DT_BF16> v;                                                 // (the bits of either type)
+    v.load(row, 8 * i, K - 8 * i);
+    return v.w[0];
 }
 
 // grid (ceil(N / 16), ceil(M / 16)), eight waves: 16 weight rows as one 16-row MFMA operand, for 16 rows of x; any K, stride and
@@ -301,17 +299,22 @@ struct PadArgs {
     uint16_t* dst[2];
     int cols, wide;
 };
+// A wave a row.
 __global__ __launch_bounds__(256) void linear_pad_kernel(PadArgs a) {
-    const int per = a.wide / 8;
-    const int64_t items = (a.rows[0] + a.rows[1]) * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        int64_t r = i / per;
-        const int c = (int)(i - r * per) * 8;
-        const int k = r >= a.rows[0];
-        r -= k ? a.rows[0] : 0;
-        Raw8<DT_BF16> v;
-        v.load(k ? a.src[1] : a.src[0], (size_t)r * (k ? a.stride[1] : a.stride[0]) + c, a.cols - c);
-        *reinterpret_cast<u32x4*>((k ? a.dst[1] : a.dst[0]) + (size_t)r * a.wide + c) = v.w[0];
+    const int lane = threadIdx.x & 63;
+    int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (r >= a.rows[0] + a.rows[1]) return;
+    const int k = r >= a.rows[0];
+    r -= k ? a.rows[0] : 0;
+    const uint16_t* src = (k ? a.src[1] : a.src[0]) + (size_t)r * (k ? a.stride[1] : a.stride[0]);
+    uint16_t* dst = (k ? a.dst[1] : a.dst[0]) + (size_t)r * a.wide;
+    for (int c0 = lane * 8; c0 < a.wide; c0 += 2048) {
+        Raw8<DT_BF16> v[4];                                          // (on their way together)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i].load(src, c0 + 512 * i, a.cols - c0 - 512 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c0 + 512 * i < a.wide) *reinterpret_cast<u32x4*>(dst + c0 + 512 * i) = v[i].w[0];
     }
 }
 
@@ -512,7 +515,7 @@ static int run_product(ProductArgs a, float* part, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 static int run_pad(const PadArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(linear_pad_kernel, dim3(linear_grid((a.rows[0] + a.rows[1]) * (a.wide / 8))), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(linear_pad_kernel, dim3((unsigned)((a.rows[0] + a.rows[1] + 3) / 4)), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

@@ -43,18 +43,16 @@ class SortedTokens:
 
     @property
     def row(self) -> torch.Tensor:
-        P = self.tokens * self.topk
-        return self._words[:P].view(self.tokens, self.topk)
+        return self._words.as_strided((self.tokens, self.topk), (self.topk, 1))
 
     @property
     def pair(self) -> torch.Tensor:
         P = self.tokens * self.topk
-        return self._words[P:2 * P]
+        return self._words.as_strided((P,), (1,), P)
 
     @property
     def offsets(self) -> torch.Tensor:
-        P = self.tokens * self.topk
-        return self._words[2 * P:2 * P + self.n + 1]
+        return self._words.as_strided((self.n + 1,), (1,), 2 * self.tokens * self.topk)
 
     @property
     def device(self) -> torch.device:
