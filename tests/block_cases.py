@@ -112,10 +112,10 @@ DW = [
 
 # rows, H, the kernels of the forward pass, of the gradient (weights and the gate's among it)
 NORM = [
-    (9, 512, ["norm_kernel<2,0,1,0>"], ["norm_grad_kernel<2,1>", "norm_join_kernel"]),
+    (9, 512, ["norm_kernel<2,0,1,0>"], ["norm_grad_kernel<2,0>", "norm_join_kernel"]),
     (9, 520, ["norm_kernel<2,1,1,0>"], ["norm_grad_kernel<2,1>", "norm_join_kernel"]),
     (4098, 8190, ["norm_kernel<2,1,1,1>"], ["norm_grad_kernel<2,1>", "norm_join_kernel"]),
-    (5, 8200, ["norm_kernel<2,1,2,0>"], ["norm_grad_kernel<2,2>", "norm_join_kernel"]),
+    (5, 8200, ["norm_kernel<2,1,2,0>"], ["norm_grad_long_kernel<2>", "norm_join_kernel"]),
 ]
 
 # tokens, topk, H, the kernels of the way out, of the way back, of its gradient

@@ -83,6 +83,34 @@ def test_forward_and_gradients(cuda, R, H, gate, dt):
         assert v is None or torch.equal(leaf[k].grad, v), k
 
 
+# several rows a wave (8, 16, 32 or 64 lanes each) with a last workgroup that is part full, and more rows than the gradient has at once
+SHORT = [(1, 8), (70, 64), (69, 65), (37, 128), (35, 129), (18, 256), (33, 257), (7, 505), (40000, 33), (20000, 100), (5000, 300)]
+
+
+@pytest.mark.parametrize("R,H", SHORT)
+@pytest.mark.parametrize("dt", TYPES)
+def test_short_rows(cuda, R, H, dt):
+    from mi355moe import norm
+    i = SHORT.index((R, H))
+    for gate in ("channel", "token") if R > 100 else (None, "channel", "token", "full"):
+        t, ds, dy = _inputs(R, H, gate, dt, TYPES[i % 3], TYPES[(i + 1) % 3], R)
+        kw = dict(eps=1e-5, scale=0.5, residual_scale=1.25)
+        args = [t[k] for k in NAMES]
+        s, y, stats = norm.join_forward(*args, **kw)
+        (ws, es), (wy, ey) = ref.norm(*(_f64(v) for v in args), 1e-5, 0.5, 1.25, ref.HALF[_name(dt)], ref.TINY[_name(dt)])
+        _within(s, ws, es, "s")
+        _within(y, wy, ey, "y")
+        got = norm.join_backward(ds, dy, stats, *args, 0.5, 1.25)
+        _hold_grads(got, t, ds, dy, kw, R)
+        again = norm.join_backward(ds, dy, stats, *args, 0.5, 1.25)
+        assert all(a is b or torch.equal(a, b) for a, b in zip(got, again))
+        # a row's gradients are its own, whatever rows stand beside it
+        alone = norm.join_backward(ds[R // 2:R // 2 + 1], dy[R // 2:R // 2 + 1], stats[R // 2:R // 2 + 1], args[0][R // 2:R // 2 + 1],
+                                   args[1][R // 2:R // 2 + 1], args[2], args[3] if gate in (None, "channel") else args[3][R // 2:R // 2 + 1],
+                                   args[4], 0.5, 1.25)
+        assert torch.equal(alone[0][0], got[0][R // 2]) and torch.equal(alone[1][0], got[1][R // 2])
+
+
 @pytest.mark.parametrize("parts", ["b", "br", "bp", "bw", "brp", "brw", "bpw", "brpw"])
 @pytest.mark.parametrize("R,H", [(5, 72), (3, 1029), (700, 264)])
 def test_every_set_of_parts(cuda, parts, R, H):
