@@ -129,7 +129,7 @@ def test_norm_refusals(L):
     none = dict(db=NUL, dr=NUL, dpo=NUL, dpr=NUL, dg=NUL)
     assert back(**none) == 0 and back(R=0) == ESHAPE and back(R=0, dpo=NUL, dpr=NUL, dg=NUL) == 0
     assert back(ws=NUL) == EINVAL and back(ws=ODD) == EINVAL and back(nb=size(4, 64) - 1) == EWORKSPACE
-    assert size(4, 64) == 4 * 4 * 2 * 64 and size(1 << 20, 4096) == 4 * 512 * 2 * 4096 and size(4, 0) == -1
+    assert size(4, 64) == 4 * 2 * 64 and size(33, 64) == 2 * 4 * 2 * 64 and size(4, 600) == 4 * 4 * 2 * 600 and size(1 << 20, 4096) == 4 * 512 * 2 * 4096 and size(4, 0) == -1
 
 
 def test_python_refusals():
