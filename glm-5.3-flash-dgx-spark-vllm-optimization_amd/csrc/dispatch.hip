@@ -167,7 +167,7 @@ struct RowsPlace {
 };
 template <bool UNI>
 __device__ __forceinline__ RowsPlace rows_place(int shift, int segs) {
-    const uint32_t g = blockIdx.x / (uint32_t)segs, seg = blockIdx.x - g * segs;
+    const uint32_t i = wide_block(), g = i / (uint32_t)segs, seg = i - g * segs;
     const int64_t t = ((int64_t)g << (8 - shift)) + (threadIdx.x >> shift);
     return {UNI ? (int64_t)__builtin_amdgcn_readfirstlane((int)t) : t, (int)(seg << shift) + (int)(threadIdx.x & ((1 << shift) - 1))};
 }
@@ -315,7 +315,8 @@ __device__ __forceinline__ void grad_rows(const RowsArgs& a, int64_t t, uint64_t
 template <int DT, bool ONCE>
 __global__ __launch_bounds__(256) void rows_grad_kernel(RowsArgs a) {
     __shared__ float red[8][4];
-    const int64_t t = blockIdx.x;
+    const int64_t t = wide_block();
+    if (t >= a.T) return;                                            // (uniform)
     const int lane = threadIdx.x & 63;
     const int64_t p = t * a.topk + min(lane, a.topk - 1);
     const int rv = lane < a.topk ? a.row[p] : INT_MAX;
@@ -341,13 +342,13 @@ static int row_shift(int64_t units) {
     while (s < 8 && (1 << s) < units) ++s;
     return s;
 }
-// (T <= 2^24 tokens of at most 64 pieces where a workgroup has one token, else of one)
-static unsigned rows_grid(int64_t T, int shift, int segs) { return (unsigned)((T + (256 >> shift) - 1) / (256 >> shift) * segs); }
+// (at most 64 pieces of 2^24 tokens)
+static dim3 rows_grid(int64_t T, int shift, int segs) { return wide_grid((T + (256 >> shift) - 1) / (256 >> shift) * segs); }
 
 template <int ES>
 static int run_scatter(const RowsArgs& a, hipStream_t st) {
     const int units = (a.H * ES + 15) / 16, s = row_shift(units), segs = (units + (1 << s) - 1) >> s;
-    const dim3 g(rows_grid(a.T, s, segs));
+    const dim3 g = rows_grid(a.T, s, segs);
     if (s >= 6) hipLaunchKernelGGL((rows_scatter_kernel<ES, true>), g, dim3(256), 0, st, a, s, segs);
     else hipLaunchKernelGGL((rows_scatter_kernel<ES, false>), g, dim3(256), 0, st, a, s, segs);
     return hipGetLastError() == hipSuccess ? 0 : -1;
@@ -362,7 +363,7 @@ static bool rows_once(const RowsArgs& a) { return a.P * a.H * (a.dt == DT_F32 ? 
 template <int DT>
 static int run_gather(const RowsArgs& a, hipStream_t st) {
     const int units = (a.H + 7) / 8, s = row_shift(units), segs = (units + (1 << s) - 1) >> s;
-    const dim3 g(rows_grid(a.T, s, segs));
+    const dim3 g = rows_grid(a.T, s, segs);
     if (s >= 6 && rows_once(a)) hipLaunchKernelGGL((rows_gather_kernel<DT, true, true>), g, dim3(256), 0, st, a, s, segs);
     else if (s >= 6) hipLaunchKernelGGL((rows_gather_kernel<DT, true, false>), g, dim3(256), 0, st, a, s, segs);
     else hipLaunchKernelGGL((rows_gather_kernel<DT, false, false>), g, dim3(256), 0, st, a, s, segs);
@@ -374,7 +375,7 @@ int launch_rows_gather(const RowsArgs& a, hipStream_t st) {
 
 template <int DT>
 static int run_rows_grad(const RowsArgs& a, hipStream_t st) {
-    const dim3 g((unsigned)a.T), b(std::min(256, (a.H + 511) / 512 * 64));
+    const dim3 g = wide_grid(a.T), b(std::min(256, (a.H + 511) / 512 * 64));
     if (rows_once(a)) hipLaunchKernelGGL((rows_grad_kernel<DT, true>), g, b, 0, st, a);
     else hipLaunchKernelGGL((rows_grad_kernel<DT, false>), g, b, 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;

@@ -58,7 +58,9 @@ template <int DT, bool WG, int NV, bool ONCE>
 __global__ __launch_bounds__(WG ? 1024 : 256) void norm_kernel(NormArgs a, int shift) {
     __shared__ float red[2][16];
     const int tpr = WG ? blockDim.x : 1 << shift, tid = WG ? threadIdx.x : threadIdx.x & ((1 << shift) - 1);
-    const int64_t at = WG ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x << (8 - shift)) + (threadIdx.x >> shift);
+    const int64_t first = WG ? (int64_t)wide_block() : (int64_t)wide_block() << (8 - shift);
+    if (first >= a.rows) return;                                     // (uniform)
+    const int64_t at = WG ? first : first + (threadIdx.x >> shift);
     const int64_t r = min(at, a.rows - 1);                           // (lanes without a row repeat the last one's values)
     const bool mine = WG || at < a.rows;
     Raw8<DT> rb8[NV], rr8[NV];
@@ -512,8 +514,8 @@ static bool norm_once(const NormArgs& a) { return a.rows * a.H * (a.dt == DT_F32
 template <int DT>
 static int run_norm(const NormArgs& a, hipStream_t st) {
     const int t = norm_threads(a.H), shift = norm_shift(a.H);
-    const dim3 g((unsigned)a.rows);
-    if (a.H <= 512) hipLaunchKernelGGL((norm_kernel<DT, false, 1, false>), dim3((unsigned)((a.rows + (256 >> shift) - 1) >> (8 - shift))), dim3(256), 0, st, a, shift);
+    const dim3 g = wide_grid(a.H <= 512 ? (a.rows + (256 >> shift) - 1) >> (8 - shift) : a.rows);
+    if (a.H <= 512) hipLaunchKernelGGL((norm_kernel<DT, false, 1, false>), g, dim3(256), 0, st, a, shift);
     else if (a.H <= 8192 && norm_once(a)) hipLaunchKernelGGL((norm_kernel<DT, true, 1, true>), g, dim3(t), 0, st, a, 0);
     else if (a.H <= 8192) hipLaunchKernelGGL((norm_kernel<DT, true, 1, false>), g, dim3(t), 0, st, a, 0);
     else hipLaunchKernelGGL((norm_kernel<DT, true, 2, false>), g, dim3(t), 0, st, a, 0);

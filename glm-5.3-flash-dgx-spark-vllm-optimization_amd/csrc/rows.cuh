@@ -94,6 +94,13 @@ __device__ __forceinline__ void store_any(void* p, int dt, size_t i, float v) {
     else static_cast<uint16_t*>(p)[i] = (uint16_t)(dt == DT_BF16 ? pack2<DT_BF16>(v, 0.0f) : pack2<DT_F16>(v, 0.0f));
 }
 
+// A launch of n < 2^30 workgroups in a row. The runtime takes fewer than 2^32 threads a dimension, which 2^24 tokens of 256 threads
+// pass: beyond 2^20 workgroups a second dimension counts on, and the last ones of a launch can lie behind n.
+static inline dim3 wide_grid(int64_t n) {
+    return n <= 1 << 20 ? dim3((unsigned)n) : dim3(1 << 20, (unsigned)((n + (1 << 20) - 1) >> 20));
+}
+__device__ __forceinline__ uint32_t wide_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Eight values as they lie in memory: loaded first, made floats where they are used, so that a kernel's loads are all on their
 // way before the first is waited for.
 template <int DT>
