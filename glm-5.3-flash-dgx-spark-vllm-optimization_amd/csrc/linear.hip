@@ -101,7 +101,8 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     }
     if (act == ACT_GELU_TANH) {
         const float s = sigmoid_rcp(GELU_A * (z + 0.044715f * z * z * z));
-        return s + z * s * (1.0f - s) * GELU_A * (1.0f + 3.0f * 0.044715f * z * z);
+        const float c = __builtin_amdgcn_fmed3f(z, -64.0f, 64.0f);    // (beyond, s is 0 or 1, and z^2 may not be a number)
+        return s + z * s * (1.0f - s) * GELU_A * (1.0f + 3.0f * 0.044715f * c * c);
     }
     return 1.0f;
 }
@@ -142,7 +143,8 @@ __device__ __forceinline__ u32x4 row_chunk(const uint16_t* row, int i, int K) {
 // grid (ceil(N / 16), ceil(M / 16)), eight waves: 16 weight rows as one 16-row MFMA operand, for 16 rows of x; any K, stride and
 // address. Lane (c = lane % 16, g = lane / 16) holds the chunks g, 4 + g, 8 + g, 12 + g of weight row c and of row c of x, so
 // that a load takes 64 bytes in a row (128 of the contraction a wave step, in the same order on both sides); the contraction is
-// cut over the waves, whose sums join in LDS in wave order.
+// cut over the waves, whose sums join in LDS in wave order. Bound: the weights' way through a CU, 7 us for 4096 of the contraction (M = 1,
+// 4096 from 1024: 8.4 MB in 4.0 us, of which 2.6 are the launch and the chain of two loads); sixteen waves spilled.
 constexpr int FEW_WAVES = 8;
 template <int DT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void linear_few_kernel(ProductArgs a) {
@@ -193,7 +195,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void linear_few_kernel(ProductArgs 
 
 // A workgroup's BP columns x BQ rows, the contraction in a.splits parts (grid y). The sums pass through LDS in fp32, 32 rows of a
 // wave at a time, so that a lane ends up with eight columns of a row: bias, residual and output are whole 16-byte accesses
-// in whole lines, and the residual is added before the one rounding; it is requested before the sums go to LDS.
+// in whole lines, and the residual is added before the one rounding; it is requested before the sums go to LDS. Bound: the matrix cores
+// while the contraction runs and memory at its ends, which do not overlap where one workgroup has the CU (M = 8192, 4096 from 2048, bf16:
+// the product with relu 123 us, 1.1 PFLOP/s; + residual 146, + gelu_tanh 154, + z, 134 MB of fp32, 184 to 200; its gradients dx 124
+// to 150, dw 131 to 150). Gained nothing there: the residual requested before the product (206, for its registers), z in whole
+// lines by a second pass over LDS or marked as not read again (202, 210).
 template <int DT, int PL, int QL, int BP, int BQ, int WP, int WQ, int ST>
 __global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(ProductArgs a, int nt, int mt) {
     using G = GemmTile<LinearKind<DT>::value, PL, QL, BP, BQ, WP, WQ, ST>;
@@ -267,7 +273,8 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(ProductArgs a, 
     }
 }
 
-// out from the sums of the contraction's parts [splits][M][part_stride], added in order: eight columns a thread.
+// out from the sums of the contraction's parts [splits][M][part_stride], added in order: eight columns a thread. Bound: memory
+// (M = 1791, N = 1024 from two parts: 18 MB in 4.7 us).
 template <int DT>
 __global__ __launch_bounds__(256) void linear_join_kernel(ProductArgs a) {
     const int per = (a.N + 7) / 8;
@@ -299,7 +306,7 @@ struct PadArgs {
     uint16_t* dst[2];
     int cols, wide;
 };
-// A wave a row.
+// A wave a row. Bound: latency and rows that begin at odd addresses (333 and 2051 rows of 1027: 10 MB in 7.2 us).
 __global__ __launch_bounds__(256) void linear_pad_kernel(PadArgs a) {
     const int lane = threadIdx.x & 63;
     int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -378,7 +385,8 @@ __device__ __forceinline__ int linear_shift(const uint32_t* tops, int n) {
 
 // dz of 256 columns and DZ_ROWS rows: 32 threads across the columns, eight values each, eight down the rows. dz [M][dz_stride]
 // in the operand type (its columns behind N zero), where g.dz is set; the sums of the unrounded dz over the workgroup's rows
-// to part [grid x][part_stride] where that is set.
+// to part [grid x][part_stride] where that is set. A kernel of its own, because two products read dz and the tiles take 16-bit
+// operands from memory as they lie. Bound: HBM (8192 x 4096: 268 MB in 47 to 52 us, 5.3 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void linear_dz_kernel(SlopeArgs g) {
     const LinearArgs& a = g.a;
@@ -416,7 +424,8 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(SlopeArgs g) {
     for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
     g.part[(size_t)blockIdx.x * g.part_stride + col] = s;
 }
-// dbias: the parts' sums in order, 64 columns a workgroup, the parts cut over its sixteen waves.
+// dbias: the parts' sums in order, 64 columns a workgroup, the parts cut over its sixteen waves. Bound: latency (128 parts of 4096
+// columns: 5 us).
 __global__ __launch_bounds__(1024) void linear_dbias_kernel(SlopeArgs g, int parts) {
     const LinearArgs& a = g.a;
     __shared__ float red[16][64];

@@ -280,3 +280,23 @@ def test_rows_beyond_32_bit_offsets(cuda):
     _within(dx[s], *gx, "dx")
     d = out[:, :3].double() * torch.sigmoid(z[:, :3].double()) * (1 + z[:, :3].double() * torch.sigmoid(-z[:, :3].double()))
     assert ((db[:3].double() - d.sum(0)).abs() <= (M / 64 / 16 + 64) * ref.U * d.abs().sum(0) + 2.0 ** -20 * out[:, :3].double().abs().sum(0) * 8).all()
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "gelu_tanh"])
+def test_slopes_far_out(cuda, act):
+    """Where |z| is far beyond the activation's bend the slope is 1 or 0, also where z^2 passes fp32's range; a NaN stays one."""
+    from mi355moe import ffn
+    far = torch.tensor([100.0, 1e4, 1e15, 1e20, 3e38], device="cuda")
+    z = torch.cat([far, -far]).repeat(8, 1).contiguous()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dy = torch.randn(8, 10, generator=g, device="cuda").to(torch.bfloat16)
+    x, w = torch.ones(8, 16, device="cuda", dtype=torch.bfloat16), torch.ones(10, 16, device="cuda", dtype=torch.bfloat16)
+    _, dw, db = ffn.linear_backward(dy, z, x, w, act, torch.float32)
+    want = dy.double().sum(0)
+    want[5:] = 0
+    mag = dy.double().abs().sum(0)
+    assert bool(((db.double() - want).abs() <= 2.0 ** -20 * mag).all()), (db, want)      # (eight values and their sum)
+    assert bool(((dw[:, 0].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * mag).all())
+    z[3, 2] = float("nan")
+    db = ffn.linear_backward(dy, z, x, w, act, torch.float32, need_dx=False, need_dw=False)[2]
+    assert bool(db[2].isnan()) and not bool(db[[0, 1, 3, 4, 5, 6, 7, 8, 9]].isnan().any())
