@@ -300,3 +300,26 @@ def test_slopes_far_out(cuda, act):
     z[3, 2] = float("nan")
     db = ffn.linear_backward(dy, z, x, w, act, torch.float32, need_dx=False, need_dw=False)[2]
     assert bool(db[2].isnan()) and not bool(db[[0, 1, 3, 4, 5, 6, 7, 8, 9]].isnan().any())
+
+
+def test_long_contraction_beyond_32_bit_offsets(cuda):
+    """dW over rows whose bytes pass 32 bits, dx that has as many, and x read there by the forward pass."""
+    from mi355moe import ffn
+    M, K, N, dt = (1 << 21) + 3, 1032, 24, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(M, K, generator=g, device="cuda", dtype=dt)
+    dy = torch.randn(M, N, generator=g, device="cuda", dtype=dt)
+    w = torch.randn(N, K, generator=g, device="cuda", dtype=dt)
+    dx, dw, db = ffn.linear_backward(dy, None, x, w, None, torch.float32)
+    some = [0, 7, 511, 1031]
+    d, xs = dy.double(), x[:, some].double()
+    want, mag = (d.t().contiguous() @ xs), (d.abs().t().contiguous() @ xs.abs())
+    h = ref.HALF["bfloat16"]
+    assert bool(((dw[:, some].double() - want).abs() <= (M / 8 + 24) * 2 * ref.U * mag * (1 + h) + h * want.abs()).all())
+    assert bool(((db.double() - d.sum(0)).abs() <= (M / 8 + 32) * ref.U * d.abs().sum(0)).all())
+    out = ffn.linear_forward(x, w)
+    for s in (slice(0, 100), slice(M - 100, M)):
+        want, tol, _, _ = ref.linear(_f64(x[s]), _f64(w), None, None, None, h, ref.TINY["bfloat16"])
+        _within(out[s], want, tol, "out")
+        gx, _, _ = ref.linear_grads(_f64(dy[s]), None, _f64(x[s]), _f64(w), None, h, ref.TINY["bfloat16"], False)
+        _within(dx[s], *gx, "dx")
