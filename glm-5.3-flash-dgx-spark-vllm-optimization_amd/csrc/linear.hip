@@ -193,9 +193,55 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void linear_few_kernel(ProductArgs 
 
 // ------------------------------------------------------------------------------------------------ tiles
 
-// A workgroup's BP columns x BQ rows, the contraction in a.splits parts (grid y). The sums pass through LDS in fp32, 32 rows of a
-// wave at a time, so that a lane ends up with eight columns of a row: bias, residual and output are whole 16-byte accesses
-// in whole lines, and the residual is added before the one rounding; it is requested before the sums go to LDS. Bound: the matrix cores
+// What a wave does with its sums (32 TP columns from c0, 32 TQ rows from r0): they pass through LDS in fp32 (`mine`, 32 rows of 128 TP
+// bytes of the wave's own), 32 rows at a time, so that a lane ends up with eight columns of a row: bias, residual and output
+// are whole 16-byte accesses in whole lines, and the residual is added before the one rounding; it is requested before the sums
+// go to LDS.
+template <int DT, int TP, int TQ>
+__device__ __forceinline__ void linear_finish(const ProductArgs& a, const f32x16 (&acc)[TP][TQ], unsigned char* mine, int lane, int64_t r0, int c0) {
+    constexpr int UNITS = 8 * TP, CH = UNITS / 2;                    // 16-byte units and 8-column chunks of a wave's row
+    const int64_t m1 = r0 + lane / CH;
+    const int c = c0 + 8 * (lane % CH), n = a.N - c;
+    const int m = lane & 31, h = lane >> 5;
+    float b[8] = {};
+    if (a.bias && a.splits == 1) load8_any(a.bias, a.bdt, c, n, b);
+    const float f = a.unscale ? *a.unscale : 1.0f;
+    float* part = a.splits > 1 ? a.part + (size_t)blockIdx.y * a.M * a.part_stride : nullptr;
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) {
+        Raw8<DT> r8[CH / 2];
+        if (a.res && !part)                                          // (uniform)
+#pragma unroll
+            for (int s = 0; s < CH / 2; ++s) {
+                const int64_t mm = m1 + 32 * j + s * (64 / CH);
+                r8[s].load(a.res, (size_t)mm * a.res_stride + c, mm < a.M ? n : 0);
+            }
+        unsigned char* row = mine + m * (16 * UNITS);
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f32x16& v = acc[i][j];
+                *reinterpret_cast<f32x4*>(row + (((8 * i + 2 * r + h) ^ (m & (UNITS - 1))) << 4)) =
+                    f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
+            }
+        asm volatile("" ::: "memory");                               // (a wave's LDS accesses are performed in order)
+#pragma unroll
+        for (int s = 0; s < CH / 2; ++s) {
+            const int rr = s * (64 / CH) + lane / CH, u = 2 * (lane % CH), x = rr & (UNITS - 1);
+            const unsigned char* from = mine + rr * (16 * UNITS);
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(from + ((u ^ x) << 4)), hi = *reinterpret_cast<const f32x4*>(from + (((u + 1) ^ x) << 4));
+            float v[8] = {lo[0] * f, lo[1] * f, lo[2] * f, lo[3] * f, hi[0] * f, hi[1] * f, hi[2] * f, hi[3] * f};
+            const int64_t mm = m1 + 32 * j + s * (64 / CH);
+            if (mm >= a.M || n <= 0) continue;
+            if (part) store8<DT_F32>(part, (size_t)mm * a.part_stride + c, 8, v);
+            else product_out8<DT>(a, mm, c, v, b, r8[s]);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// A workgroup's BP columns x BQ rows, the contraction in a.splits parts (grid y). Bound: the matrix cores
 // while the contraction runs and memory at its ends, which do not overlap where one workgroup has the CU (M = 8192, 4096 from 2048, bf16:
 // the product with relu 123 us, 1.1 PFLOP/s; + residual 146, + gelu_tanh 154, + z, 134 MB of fp32, 184 to 200; its gradients dx 124
 // to 150, dw 131 to 150). Gained nothing there: the residual requested before the product (206, for its registers), z in whole
@@ -228,49 +274,79 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void linear_kernel(ProductArgs a, 
 #pragma unroll
             for (int j = 0; j < G::TQ; ++j) t.acc[i][j] = f32x16{};
 
-    constexpr int UNITS = 8 * G::TP, CH = UNITS / 2;                 // 16-byte units and 8-column chunks of a wave's row
-    static_assert(G::NW * 32 * 16 * UNITS <= G::LDS, "the stages hold the waves' rows");
-    unsigned char* mine = lds + wv * (32 * 16 * UNITS);
-    const int64_t m1 = m0 + (wv / WP) * (BQ / WQ) + lane / CH;
-    const int c = n0 + (wv % WP) * (BP / WP) + 8 * (lane % CH), n = a.N - c;
-    const int m = lane & 31, h = lane >> 5;
-    float b[8] = {};
-    if (a.bias && a.splits == 1) load8_any(a.bias, a.bdt, c, n, b);
-    const float f = a.unscale ? *a.unscale : 1.0f;
-    float* part = a.splits > 1 ? a.part + (size_t)blockIdx.y * a.M * a.part_stride : nullptr;
+    static_assert(G::NW * 32 * 128 * G::TP <= G::LDS, "the stages hold the waves' rows");
     __syncthreads();                                                 // no wave reads a stage any more
+    linear_finish<DT, G::TP, G::TQ>(a, t.acc, lds + wv * (32 * 128 * G::TP), lane, m0 + (wv / WP) * (BQ / WQ), n0 + (wv % WP) * (BP / WP));
+}
+
+// 64 columns x 64 rows of operands whose rows lie at any address (K no multiple of 8: the loads to LDS above take whole 16 bytes), so
+// that they need no copies: four stages of 64 are on their way to registers, from which a stage goes to one of two LDS buffers,
+// its 16-byte chunks exchanged by the row (lanes of one chunk then read different banks). The last, part stage is requested first.
+// Bound: the loads' way, which addresses off 16 bytes double (0.35 us a stage and workgroup of a CU, however many it has). us with the
+// copies and the tiles above / so: M = 130, 2051 from 1027 21.8 / 11.1, 333 15.4 / 10.3, 700 20.2 / 16.3, 1791 26.0 / 31.1; 1024 from
+// 4099, 130 20.6 / 13.5 (in parts), 1791 41 / 48.
+constexpr int ANY_AHEAD = 4;
+template <int DT>
+__global__ __launch_bounds__(256, 1) void linear_any_kernel(ProductArgs a, int nt, int mt) {
+    __shared__ __align__(16) unsigned char lds[2][2][64 * 128];
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int2 tile = tile_order(blockIdx.x, nt, mt);
+    const int n0 = tile.x * 64, K = (int)a.K;
+    const int64_t m0 = (int64_t)tile.y * 64;
+    const int stages = (K + 63) / 64, per = (stages + a.splits - 1) / a.splits;
+    const int kb0 = blockIdx.y * per, kb1 = min(min(stages, kb0 + per), K / 64);       // (whole stages)
+    const bool tail = kb0 < stages && kb0 + per >= stages && K % 64;
+    const int row = threadIdx.x >> 2, c4 = threadIdx.x & 3;          // what this thread loads: chunks c4 and c4 + 4 of a row of each
+    const uint16_t* p = a.p + (size_t)min(n0 + row, a.N - 1) * a.ldp;
+    const uint16_t* q = a.q + (size_t)min(m0 + row, a.M - 1) * a.ldq;
+    const int to0 = row * 128 + ((c4 ^ ((row >> 1) & 7)) << 4), to1 = row * 128 + (((c4 + 4) ^ ((row >> 1) & 7)) << 4);
+    u32x4 last[4], set[ANY_AHEAD][4];
+    if (tail)
 #pragma unroll
-    for (int j = 0; j < G::TQ; ++j) {
-        Raw8<DT> r8[CH / 2];
-        if (a.res && !part)                                          // (uniform)
+        for (int i = 0; i < 4; ++i) last[i] = row_chunk(i < 2 ? p : q, K / 64 * 8 + c4 + 4 * (i & 1), K);
+    auto load = [&](u32x4 (&v)[4], int kb) {
 #pragma unroll
-            for (int s = 0; s < CH / 2; ++s) {
-                const int64_t mm = m1 + 32 * j + s * (64 / CH);
-                r8[s].load(a.res, (size_t)mm * a.res_stride + c, mm < a.M ? n : 0);
-            }
-        unsigned char* row = mine + m * (16 * UNITS);
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const rows_u32x4*>((i < 2 ? p : q) + kb * 64 + 8 * (c4 + 4 * (i & 1)));
+    };
+    f32x16 acc[1][1] = {};
+    int cur = 0;
+    // one stage from registers, into which stage `next` is requested
+    auto step = [&](auto more, u32x4 (&v)[4], int next) {
+        unsigned char(*buf)[64 * 128] = lds[cur];
+        *reinterpret_cast<u32x4*>(buf[0] + to0) = v[0];
+        *reinterpret_cast<u32x4*>(buf[0] + to1) = v[1];
+        *reinterpret_cast<u32x4*>(buf[1] + to0) = v[2];
+        *reinterpret_cast<u32x4*>(buf[1] + to1) = v[3];
+        if constexpr (more) load(v, next);
+        __syncthreads();                                             // (the buffer before it is free: all have passed its reads)
+        const int pr = 32 * (wv & 1) + (lane & 31), qr = 32 * (wv >> 1) + (lane & 31), h = lane >> 5;
+        u32x4 x[4], y[4];
 #pragma unroll
-        for (int i = 0; i < G::TP; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x16& v = t.acc[i][j];
-                *reinterpret_cast<f32x4*>(row + (((8 * i + 2 * r + h) ^ (m & (UNITS - 1))) << 4)) =
-                    f32x4{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
-            }
-        asm volatile("" ::: "memory");                               // (a wave's LDS accesses are performed in order)
-#pragma unroll
-        for (int s = 0; s < CH / 2; ++s) {
-            const int rr = s * (64 / CH) + lane / CH, u = 2 * (lane % CH), x = rr & (UNITS - 1);
-            const unsigned char* from = mine + rr * (16 * UNITS);
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(from + ((u ^ x) << 4)), hi = *reinterpret_cast<const f32x4*>(from + (((u + 1) ^ x) << 4));
-            float v[8] = {lo[0] * f, lo[1] * f, lo[2] * f, lo[3] * f, hi[0] * f, hi[1] * f, hi[2] * f, hi[3] * f};
-            const int64_t mm = m1 + 32 * j + s * (64 / CH);
-            if (mm >= a.M || n <= 0) continue;
-            if (part) store8<DT_F32>(part, (size_t)mm * a.part_stride + c, 8, v);
-            else product_out8<DT>(a, mm, c, v, b, r8[s]);
+        for (int i = 0; i < 4; ++i) {
+            x[i] = *reinterpret_cast<const u32x4*>(buf[0] + pr * 128 + (((2 * i + h) ^ ((pr >> 1) & 7)) << 4));
+            y[i] = *reinterpret_cast<const u32x4*>(buf[1] + qr * 128 + (((2 * i + h) ^ ((qr >> 1) & 7)) << 4));
         }
-        asm volatile("" ::: "memory");
+        SCHED_FENCE();                                               // (all reads requested before the first multiplication)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[0][0] = mma16(std::integral_constant<int, LinearKind<DT>::value>{}, x[i], y[i], acc[0][0]);
+        cur ^= 1;
+    };
+    if (kb0 < kb1) {
+#pragma unroll
+        for (int i = 0; i < ANY_AHEAD; ++i) load(set[i], min(kb0 + i, kb1 - 1));
+        for (int kb = kb0;;) {                                       // (uniform; beyond the last stage the loads repeat it)
+#pragma unroll
+            for (int i = 0; i < ANY_AHEAD; ++i) {
+                step(std::true_type{}, set[i], min(kb + ANY_AHEAD, kb1 - 1));
+                if (++kb == kb1) break;
+            }
+            if (kb == kb1) break;
+        }
     }
+    if (tail) step(std::false_type{}, last, 0);
+    __syncthreads();                                                 // no wave reads a stage any more
+    linear_finish<DT, 1, 1>(a, acc, &lds[0][0][0] + wv * (32 * 128), lane, m0 + 32 * (wv >> 1), n0 + 32 * (wv & 1));
 }
 
 // out from the sums of the contraction's parts [splits][M][part_stride], added in order: eight columns a thread. Bound: memory
@@ -461,6 +537,7 @@ struct ProductPlan {
     double us;
 };
 static double tiles_us(int tile, int64_t tiles, int64_t stages) {
+    if (tile == TILE_ANY) return 3.5 + (double)((tiles + 255) / 256) * (0.35 * stages + 1.3);
     if (tile == TILE_64) {
         const double one = 0.30 * stages + 0.9, two = 0.49 * stages + 2.8;
         const int64_t rest = tiles % 512;
@@ -469,7 +546,9 @@ static double tiles_us(int tile, int64_t tiles, int64_t stages) {
     const int64_t rounds = (tiles + 255) / 256;
     return 3.0 + rounds * (tile == TILE_128_DEEP ? 0.54 * stages + 6.0 : tile == TILE_256_128 ? 0.91 * stages + 11.0 : 1.56 * stages + 24.0);
 }
-static ProductPlan plan_product(int64_t M, int64_t N, int64_t K) {
+static double join_us(int s, int64_t M, int64_t N) { return 2.0 + s * (double)(M * N) * 8.0 / 6e6; }
+// any: the operands lie at any address, so linear_any_kernel, or copies of them for the others.
+static ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool any = false) {
     auto count = [&](int64_t p, int64_t q) { return ((N + p - 1) / p) * ((M + q - 1) / q); };
     const int64_t stages = (K + 63) / 64;
     ProductPlan best{TILE_64, 1, 1e30};
@@ -481,23 +560,30 @@ static ProductPlan plan_product(int64_t M, int64_t N, int64_t K) {
         for (int s = 1; s <= 16; s *= 2) {
             if (s > 1 && (k.tile == TILE_256 || k.tile == TILE_256_128 || stages / s < 8 || k.tiles * s > 512)) break;
             double us = tiles_us(k.tile, k.tiles * s, (stages + s - 1) / s);
-            if (s > 1) us += 2.0 + s * (double)(M * N) * 8.0 / 6e6;
+            if (s > 1) us += join_us(s, M, N);
             if (us < best.us) best = {k.tile, s, us};
         }
+    if (any) {
+        best.us += 4.0 + (double)((M + N) * K) * 4.0 / 4e6;         // (the copies)
+        for (int s = 1; s <= 16 && (s == 1 || (stages / s >= 8 && count(64, 64) * s <= 512)); s *= 2) {
+            const double us = tiles_us(TILE_ANY, count(64, 64) * s, (stages + s - 1) / s) + (s > 1 ? join_us(s, M, N) : 0.0);
+            if (us < best.us) best = {TILE_ANY, s, us};
+        }
+    }
     return best;
 }
 // Few rows stream the weights. The streaming kernel takes about 3 us and, for every 256 workgroups of 16 columns and 16 rows, what
 // one CU takes to read its rows of both operands (7 us for 4096 of the contraction). us streamed / by tiles: 1024 from 4096, M = 64
 // 9.6 / 11.3, 96 16.5 / 11.6; 4096 from 1024, 16 4.6 / 7.3, 32 6.4 / 8.1, 64 9.9 / 8.2; 4096 from 4096, 16 10.7 / 12.8, 32 17 /
-// 13.2. It takes rows at any address; for tiles, rows of no whole 16 bytes are copied first.
+// 13.2. Rows at odd addresses (K no multiple of 8) take 1.7 times as long to read (us streamed / by linear_any_kernel, M = 65: 515 from
+// 131 4.4 / 6.0, 2051 from 1027 14.4 / 10.0).
 static bool linear_streams(int64_t M, int64_t N, int64_t K) {
     const int64_t wgs = (M + 15) / 16 * ((N + 15) / 16);
-    const double few = 2.6 + (double)((wgs + 255) / 256) * (0.5 + 1.75e-3 * (double)K);
-    const double pad = K % 8 ? 4.0 + (double)((M + N) * K) * 4.0 / 4e6 : 0.0;
-    return M <= 4096 && few <= plan_product(M, N, K).us + pad;
+    const double few = 2.6 + (double)((wgs + 255) / 256) * (0.5 + 1.75e-3 * (double)K) * (K % 8 ? 1.7 : 1.0);
+    return M <= 4096 && few <= plan_product(M, N, K, K % 8 != 0).us;
 }
-static int64_t part_bytes(int64_t M, int64_t N, int64_t K) {
-    const int s = plan_product(M, N, K).splits;
+static int64_t part_bytes(int64_t M, int64_t N, int64_t K, bool any = false) {
+    const int s = plan_product(M, N, K, any).splits;
     return s > 1 ? 4 * s * M * up8(N) : 0;
 }
 
@@ -509,13 +595,19 @@ static int run_tiles(const ProductArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((linear_kernel<DT, PL, QL, BP, BQ, WP, WQ, ST>), dim3(nt * mt, a.splits), dim3(G::THREADS), G::LDS, st, a, nt, mt);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
+template <int DT>
+static int run_any(const ProductArgs& a, hipStream_t st) {
+    const int nt = (a.N + 63) / 64, mt = (int)((a.M + 63) / 64);
+    hipLaunchKernelGGL(linear_any_kernel<DT>, dim3(nt * mt, a.splits), dim3(256), 0, st, a, nt, mt);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
 template <int DT, int PL, int QL>
-static int run_product(ProductArgs a, float* part, hipStream_t st) {
-    const ProductPlan p = plan_product(a.M, a.N, a.K);
+static int run_product(ProductArgs a, const ProductPlan& p, float* part, hipStream_t st) {
     a.splits = p.splits;
     a.part = part;
     a.part_stride = up8(a.N);
-    const int r = p.tile == TILE_256        ? run_tiles<DT, PL, QL, 256, 256, 2, 4, 2>(a, st)
+    const int r = p.tile == TILE_ANY        ? run_any<DT>(a, st)
+                  : p.tile == TILE_256      ? run_tiles<DT, PL, QL, 256, 256, 2, 4, 2>(a, st)
                   : p.tile == TILE_256_128  ? run_tiles<DT, PL, QL, 256, 128, 2, 4, 3>(a, st)
                   : p.tile == TILE_128_DEEP ? run_tiles<DT, PL, QL, 128, 128, 2, 4, 4>(a, st)
                                             : run_tiles<DT, PL, QL, 64, 64, 2, 2, 4>(a, st);
@@ -540,8 +632,8 @@ struct LinearSpace {
 static LinearSpace forward_space(int64_t M, int64_t N, int64_t K) {
     LinearSpace s;
     if (M == 0 || linear_streams(M, N, K)) return s;
-    if (K % 8) s.x = s.take(M * up8(K) * 2), s.w = s.take(N * up8(K) * 2);
-    if (const int64_t n = part_bytes(M, N, K)) s.part = s.take(n);
+    if (K % 8 && plan_product(M, N, K, true).tile != TILE_ANY) s.x = s.take(M * up8(K) * 2), s.w = s.take(N * up8(K) * 2);
+    if (const int64_t n = part_bytes(M, N, K, K % 8 != 0)) s.part = s.take(n);
     return s;
 }
 int64_t linear_forward_bytes(int64_t M, int64_t N, int64_t K) { return forward_space(M, N, K).bytes; }
@@ -565,7 +657,7 @@ static int linear_forward(LinearArgs a, char* ws, hipStream_t st) {
         if (int r = run_pad(PadArgs{{a.x, a.w}, {a.x_stride, a.w_stride}, {a.M, a.N}, {x, w}, a.K, (int)K8}, st)) return r;
         g.p = w, g.q = x, g.ldp = g.ldq = K8;
     }
-    return run_product<DT, LAY_ROW, LAY_ROW>(g, s.part >= 0 ? reinterpret_cast<float*>(ws + s.part) : nullptr, st);
+    return run_product<DT, LAY_ROW, LAY_ROW>(g, plan_product(a.M, a.N, a.K, a.K % 8 != 0), s.part >= 0 ? reinterpret_cast<float*>(ws + s.part) : nullptr, st);
 }
 int launch_linear(const LinearArgs& a, void* ws, hipStream_t st) {
     return a.dt == DT_BF16 ? linear_forward<DT_BF16>(a, static_cast<char*>(ws), st) : linear_forward<DT_F16>(a, static_cast<char*>(ws), st);
@@ -632,11 +724,11 @@ static int linear_backward(const LinearArgs& a, char* ws, hipStream_t st) {
     }
     if (a.dx) {
         p.p = w, p.ldp = ldw, p.M = a.M, p.K = a.N, p.out = a.dx;
-        if (int r = run_product<DT, LAY_COL, LAY_ROW>(p, part, st)) return r;
+        if (int r = run_product<DT, LAY_COL, LAY_ROW>(p, plan_product(p.M, p.N, p.K), part, st)) return r;
     }
     if (a.dw) {
         p.p = x, p.ldp = ldx, p.M = a.N, p.K = a.M, p.out = a.dw;
-        if (int r = run_product<DT, LAY_COL, LAY_COL>(p, part, st)) return r;
+        if (int r = run_product<DT, LAY_COL, LAY_COL>(p, plan_product(p.M, p.N, p.K), part, st)) return r;
     }
     return 0;
 }

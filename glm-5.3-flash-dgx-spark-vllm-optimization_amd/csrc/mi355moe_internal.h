@@ -368,7 +368,7 @@ int launch_mx_arrange(const uint8_t* a, int64_t mats, int64_t rows, uint8_t* ao,
                       hipStream_t st);
 // Kinds of workgroup tiles: the largest, 128 x 128 for two workgroups a CU, and three deeply buffered ones for products of
 // at most a workgroup a CU.
-enum TileKind { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_128_64 = 3, TILE_64 = 4, TILE_256_128 = 5 };
+enum TileKind { TILE_256 = 0, TILE_128 = 1, TILE_128_DEEP = 2, TILE_128_64 = 3, TILE_64 = 4, TILE_256_128 = 5, TILE_ANY = 6 };
 struct MxMatmulPlan {
     int few, tile, splits, arrange;
 };

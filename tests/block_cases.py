@@ -83,7 +83,9 @@ LINEAR = [
     (1, 136, 72, ["linear_few_kernel<2>"]),
     (33, 1027, 70, ["linear_few_kernel<2>"]),
     (300, 264, 776, [_tiles(0, 0, S64)]),
-    (900, 131, 777, [PAD, _tiles(0, 0, S64)]),
+    (900, 131, 777, ["linear_any_kernel<2>"]),
+    (4200, 37, 70, ["linear_any_kernel<2>"]),
+    (130, 4099, 1032, ["linear_any_kernel<2>", JOIN]),
     (130, 4104, 1032, [_tiles(0, 0, S64), JOIN]),
     (1030, 4104, 2056, [_tiles(0, 0, DEEP)]),
     (1030, 4099, 1032, [PAD, _tiles(0, 0, DEEP), JOIN]),
