@@ -105,7 +105,7 @@ def _to_experts(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     H = x.shape[1]
     with _on_device(dev):
         x, ldx = _rows_any(x)
-        rows = x.new_empty((plan.tokens * plan.topk, H))
+        rows = x.new_empty(plan.tokens * plan.topk, H)
         _lib.check("mi355moe_rows_to_experts", _lib.lib().mi355moe_rows_to_experts(
             x.data_ptr(), code, plan.tokens, H, ldx, plan._words.data_ptr(), plan.topk, rows.data_ptr(), _raw_stream(dev)))
     return rows
@@ -129,7 +129,7 @@ def _from_experts(rows, weights, plan, shared):
         rows = _packed(rows)
         weights = None if weights is None else _packed(weights)
         shared, lds = (None, H) if shared is None else _rows_any(shared)
-        out = rows.new_empty((plan.tokens, H))
+        out = rows.new_empty(plan.tokens, H)
         _lib.check("mi355moe_rows_from_experts", _lib.lib().mi355moe_rows_from_experts(
             rows.data_ptr(), code, plan.tokens, H, plan._words.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared), lds,
             out.data_ptr(), H, _raw_stream(dev)))
@@ -154,8 +154,8 @@ def _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights):
     H = rows.shape[1]
     with _on_device(dev):
         (dout, ldd), rows, weights = _rows_any(dout), _packed(rows), _packed(weights)
-        drows = rows.new_empty(rows.shape) if need_rows else None
-        dw = weights.new_empty(weights.shape) if need_weights else None
+        drows = torch.empty_like(rows) if need_rows else None
+        dw = torch.empty_like(weights) if need_weights else None
         _lib.check("mi355moe_rows_from_experts_backward", _lib.lib().mi355moe_rows_from_experts_backward(
             dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(),
             weight_dtype_code(weights.dtype), rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev)))

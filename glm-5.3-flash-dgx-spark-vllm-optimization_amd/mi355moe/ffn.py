@@ -209,8 +209,8 @@ def _linear(kinds, x, w, bias, activation, residual, save):
         b = None if bias is None else _packed(bias)
         r, ldr = (None, N) if residual is None else _rows_any(residual)
         M = x2.numel() // K
-        out = x2.new_empty((*x.shape[:-1], N))
-        z = x2.new_empty((M, N), dtype=torch.float32) if save and activation is not None else None
+        out = x2.new_empty(M, N) if x.dim() == 2 else x2.new_empty((*x.shape[:-1], N))
+        z = x2.new_empty(M, N, dtype=torch.float32) if save and activation is not None else None
         nb = _linear_bytes(False, M, K, N)
         ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
         _lib.check("mi355moe_linear_forward", _lib.lib().mi355moe_linear_forward(

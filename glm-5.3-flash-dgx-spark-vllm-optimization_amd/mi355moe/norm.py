@@ -20,7 +20,8 @@ import functools
 import torch
 
 from . import _lib
-from .ops import _addr, _capturing, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any, weight_dtype_code
+from .ops import (_addr, _capturing, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any,
+                  weight_dtype_code)
 
 _NONE, _CHANNEL, _TOKEN, _FULL = 0, 1, 2, 3
 
@@ -74,15 +75,14 @@ def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scal
     dev, code, wcode, kind, gcode = kinds
     if pre is None and not need_s:
         raise ValueError("neither s nor y is asked for")
-    shape = branch.shape
-    H = shape[-1]
+    H = branch.shape[-1]
     with _on_device(dev):
         (b, ldb), (r, ldr) = _rows_any(branch), _rows(residual, H)
         n = b.numel() // H
         post, pre, gate = _flat(post), _flat(pre), _flat(gate)
-        s = b.new_empty(shape) if need_s else None
-        y = b.new_empty(shape) if pre is not None else None
-        stats = b.new_empty((n, 2), dtype=torch.float32) if need_stats else None
+        s = _empty_like(branch) if need_s else None
+        y = _empty_like(branch) if pre is not None else None
+        stats = b.new_empty(n, 2, dtype=torch.float32) if need_stats else None
         if n:
             _lib.check("mi355moe_norm_forward", _lib.lib().mi355moe_norm_forward(
                 b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode, kind, eps, scale,
@@ -129,7 +129,7 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
         nothing = n == 0 or (ds is None and dy is None)
 
         def like(t, wanted):
-            return None if t is None or not wanted else t.new_zeros(t.shape) if nothing else t.new_empty(t.shape)
+            return None if t is None or not wanted else t.new_zeros(t.shape) if nothing else _empty_like(t)
 
         db, dr, dpost, dgate = like(branch, need[0]), like(residual, need[1]), like(post, need[2]), like(gate, need[3])
         dpre = like(pre, need[4])

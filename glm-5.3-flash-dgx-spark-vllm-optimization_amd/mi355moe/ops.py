@@ -97,6 +97,11 @@ def _rows_any(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t.contiguous(), H
 
 
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """A tensor of t's shape and type with its values back to back (torch.empty_like takes two thirds of new_empty's time)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _packed(t: torch.Tensor) -> torch.Tensor:
     """t with its values back to back."""
     return t if t.is_contiguous() else _plain(t).contiguous()

@@ -91,8 +91,8 @@ def test_linear_refusals(L):
     cut = dict(M=130, K=4104, xs=4104, wst=4104, N=1032, os=1032)
     nb = size(130, 4104, 1032)
     assert nb > 0 and call(**cut, ws=NUL) == EINVAL and call(**cut, ws=ODD) == EINVAL and call(**cut, nb=nb - 1) == EWORKSPACE
-    odd = size(900, 131, 777)
-    assert odd == (900 * 136 * 2 + 255) // 256 * 256 + (777 * 136 * 2 + 255) // 256 * 256
+    odd = size(4100, 1027, 2051)
+    assert size(900, 131, 777) == 0 and odd == (4100 * 1032 * 2 + 255) // 256 * 256 + (2051 * 1032 * 2 + 255) // 256 * 256
     assert back(ds=23) == ESHAPE and back(db=P, bdt=I32) == EDTYPE and back(d=NUL) == EINVAL and back(ws=NUL) == EINVAL and back(ws=ODD) == EINVAL
     assert back(act=2, z=NUL) == EINVAL and back(d=ODD) == EINVAL and back(dx=ODD) == EINVAL and back(dw=ODD) == EINVAL and back(db=TWO) == EINVAL
     assert back(act=2, z=TWO) == EINVAL
