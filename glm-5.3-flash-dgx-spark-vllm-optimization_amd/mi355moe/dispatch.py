@@ -81,8 +81,8 @@ def sort_tokens(topk_ids: torch.Tensor, n: int, expert_map: torch.Tensor | None 
             n_global = em.numel()
             if n_global == 0:
                 em = ids.new_zeros(1, dtype=torch.int64)         # (no id has an entry; the address only says that there is a map)
-        # the scratch lies behind the three tables (a size that the library refuses: enough for its answer)
-        words = ids.new_empty(2 * P + max(n, 0) + 1 + max(nb, 0) // 4, dtype=torch.int32)
+        # the scratch lies behind the three tables (sizes that the library refuses: nothing to write)
+        words = ids.new_empty(2 * P + n + 1 + nb // 4 if nb >= 0 else 1, dtype=torch.int32)
         at = words.data_ptr()
         _lib.check("mi355moe_sort_tokens", _lib.lib().mi355moe_sort_tokens(
             _addr(ids), code, T, topk, _addr(em), n_global, n, at, at + 4 * P, at + 8 * P, at + 4 * (2 * P + n + 1) if nb > 0 else None,

@@ -152,3 +152,16 @@ def test_saved_tensors_may_move(cuda):
             out = f(*leaf)
         got = torch.autograd.grad(out, leaf, torch.ones_like(out))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_refused_order_takes_no_memory(cuda):
+    from mi355moe import _lib, dispatch
+    ids = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    far = torch.zeros(1, dtype=torch.int32, device="cuda").expand(1 << 20, 32)
+    torch.cuda.synchronize()
+    for bad, n in ((ids, 10 ** 12), (ids, 1 << 30), (ids, -10 ** 12), (far[:, :17], 4)):
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(_lib.MoeError):
+            dispatch.sort_tokens(bad, n)
+        assert torch.cuda.max_memory_allocated() - before <= 4 * bad.numel() + (1 << 20)     # (the ids' copy, where they are a view)
