@@ -29,7 +29,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain, _raw_stream, _row_stride,
+from .ops import (_addr, _capturing, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain, _raw_stream, _row_stride,
                   _rows_any, act_dtype_code, weight_dtype_code)
 
 
@@ -244,12 +244,11 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
     with _on_device(dev):
         (x2, ldx), (w2, ldw), (d2, ldd) = _linear_operand(x, K), _linear_operand(w, K), _rows_any(dout)
         M = x2.numel() // K
-        new = x2.new_zeros if M == 0 else x2.new_empty
-        dx = new(x.shape) if need_dx else None
-        dw = new((N, K)) if need_dw else None
-        db = new(N, dtype=bias_dtype) if bias_dtype is not None else None
+        dx = _empty_like(x) if need_dx else None
+        dw = _empty_like(w) if need_dw else None
+        db = x2.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
         if M == 0 or (dx is None and dw is None and db is None):
-            return dx, dw, db
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
         nb = _linear_bytes(True, M, K, N)
         ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
         _lib.check("mi355moe_linear_backward", _lib.lib().mi355moe_linear_backward(
