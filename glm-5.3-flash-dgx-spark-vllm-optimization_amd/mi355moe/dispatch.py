@@ -22,8 +22,8 @@ import functools
 import torch
 
 from . import _lib
-from .ops import (_addr, _capturing, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any, ids_dtype_code,
-                  weight_dtype_code)
+from .ops import (_addr, _capturing, _current_device, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any,
+                  ids_dtype_code, weight_dtype_code)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -101,13 +101,20 @@ def _check(plan: SortedTokens, what: str, t: torch.Tensor, rows: int, dev: torch
 
 def _to_experts(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     dev = _need_cuda(x)
-    code = _check(plan, "x", x, plan.tokens, dev)
-    H = x.shape[1]
-    with _on_device(dev):
-        x, ldx = _rows_any(x)
-        rows = x.new_empty(plan.tokens * plan.topk, H)
-        _lib.check("mi355moe_rows_to_experts", _lib.lib().mi355moe_rows_to_experts(
-            x.data_ptr(), code, plan.tokens, H, ldx, plan._words.data_ptr(), plan.topk, rows.data_ptr(), _raw_stream(dev)))
+    return _scatter(dev, _check(plan, "x", x, plan.tokens, dev), x, plan)
+
+
+def _scatter(dev, code, x, plan):
+    """_to_experts of arguments that have been looked at."""
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _scatter(dev, code, x, plan)
+    T, topk, H = plan.tokens, plan.topk, x.shape[1]
+    x, ldx = (x, H) if x.is_contiguous() else _rows_any(x)
+    rows = x.new_empty(T * topk, H)
+    rc = _lib.lib().mi355moe_rows_to_experts(x.data_ptr(), code, T, H, ldx, plan._words.data_ptr(), topk, rows.data_ptr(), _raw_stream(dev))
+    if rc:
+        _lib.check("mi355moe_rows_to_experts", rc)
     return rows
 
 
@@ -123,16 +130,25 @@ def _check_back(rows, weights, plan, shared):
 
 def _from_experts(rows, weights, plan, shared):
     dev, code = _check_back(rows, weights, plan, shared)
+    return _gather(dev, code, rows, weights, plan, shared)
+
+
+def _gather(dev, code, rows, weights, plan, shared):
+    """_from_experts of arguments that have been looked at."""
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _gather(dev, code, rows, weights, plan, shared)
     wcode = _lib.F32 if weights is None else weight_dtype_code(weights.dtype)
-    H = rows.shape[1]
-    with _on_device(dev):
-        rows = _packed(rows)
-        weights = None if weights is None else _packed(weights)
-        shared, lds = (None, H) if shared is None else _rows_any(shared)
-        out = rows.new_empty(plan.tokens, H)
-        _lib.check("mi355moe_rows_from_experts", _lib.lib().mi355moe_rows_from_experts(
-            rows.data_ptr(), code, plan.tokens, H, plan._words.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared), lds,
-            out.data_ptr(), H, _raw_stream(dev)))
+    T, H = plan.tokens, rows.shape[1]
+    rows = _packed(rows)
+    weights = None if weights is None else _packed(weights)
+    shared, lds = (shared, H) if shared is None or shared.is_contiguous() else _rows_any(shared)
+    out = rows.new_empty(T, H)
+    rc = _lib.lib().mi355moe_rows_from_experts(
+        rows.data_ptr(), code, T, H, plan._words.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared), lds, out.data_ptr(), H,
+        _raw_stream(dev))
+    if rc:
+        _lib.check("mi355moe_rows_from_experts", rc)
     return out
 
 
@@ -151,14 +167,19 @@ def from_experts_backward(dout: torch.Tensor, rows: torch.Tensor, weights: torch
 
 def _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights):
     """from_experts_backward of arguments that have been looked at."""
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights)
     H = rows.shape[1]
-    with _on_device(dev):
-        (dout, ldd), rows, weights = _rows_any(dout), _packed(rows), _packed(weights)
-        drows = torch.empty_like(rows) if need_rows else None
-        dw = torch.empty_like(weights) if need_weights else None
-        _lib.check("mi355moe_rows_from_experts_backward", _lib.lib().mi355moe_rows_from_experts_backward(
-            dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(),
-            weight_dtype_code(weights.dtype), rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev)))
+    dout, ldd = (dout, H) if dout.is_contiguous() else _rows_any(dout)
+    rows, weights = _packed(rows), _packed(weights)
+    drows = torch.empty_like(rows) if need_rows else None
+    dw = torch.empty_like(weights) if need_weights else None
+    rc = _lib.lib().mi355moe_rows_from_experts_backward(
+        dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(), weight_dtype_code(weights.dtype),
+        rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev))
+    if rc:
+        _lib.check("mi355moe_rows_from_experts_backward", rc)
     return drows, dw
 
 
@@ -166,39 +187,44 @@ _NOT_CAPTURED = ("mi355moe: {} cannot {} during graph capture; capture it under 
                  "(from_experts without weights, from_experts_backward)")
 
 
+# (autograd gives a backward pass gradients of the outputs' shapes and types: they are not looked at again)
 class _To(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
-        ctx.plan = plan
-        return _to_experts(x, plan)
+        dev = _need_cuda(x)
+        ctx.rest = dev, _check(plan, "x", x, plan.tokens, dev), plan
+        return _scatter(dev, ctx.rest[1], x, plan)
 
     @staticmethod
     @_once
     def backward(ctx, drows):
-        if _capturing(drows.device):
+        dev, code, plan = ctx.rest
+        if _capturing(dev):
             raise RuntimeError(_NOT_CAPTURED.format("to_experts", "run an eager call's backward pass"))
-        return _from_experts(drows, None, ctx.plan, None), None
+        return _gather(dev, code, drows, None, plan, None), None
 
 
 class _From(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, plan, shared):
-        ctx.plan = plan
+        dev, code = _check_back(rows, weights, plan, shared)
+        ctx.rest = dev, code, plan
         ctx.save_for_backward(rows, weights)
-        return _from_experts(rows, weights, plan, shared)
+        return _gather(dev, code, rows, weights, plan, shared)
 
     @staticmethod
     @_once
     def backward(ctx, dout):
-        if _capturing(dout.device):
+        dev, code, plan = ctx.rest
+        if _capturing(dev):
             raise RuntimeError(_NOT_CAPTURED.format("from_experts", "run an eager call's backward pass"))
         rows, weights = ctx.saved_tensors
         need = ctx.needs_input_grad
         drows = dw = None
         if weights is None:
-            drows = _to_experts(dout, ctx.plan) if need[0] else None
+            drows = _scatter(dev, code, dout, plan) if need[0] else None
         elif need[0] or need[1]:
-            drows, dw = _from_grads(rows.device, weight_dtype_code(rows.dtype), dout, rows, weights, ctx.plan, need[0], need[1])
+            drows, dw = _from_grads(dev, code, dout, rows, weights, plan, need[0], need[1])
         return drows, dw, None, dout if need[3] else None
 
 

@@ -29,8 +29,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import (_addr, _capturing, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain, _raw_stream, _row_stride,
-                  _rows_any, act_dtype_code, weight_dtype_code)
+from .ops import (_addr, _capturing, _current_device, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain,
+                  _raw_stream, _row_stride, _rows_any, act_dtype_code, weight_dtype_code)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -203,19 +203,23 @@ def linear_forward(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None =
 def _linear(kinds, x, w, bias, activation, residual, save):
     """linear_forward of arguments that have been looked at (kinds: what _check_linear said of them)."""
     dev, code, bcode = kinds
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _linear(kinds, x, w, bias, activation, residual, save)
     N, K = w.shape
-    with _on_device(dev):
-        (x2, ldx), (w2, ldw) = _linear_operand(x, K), _linear_operand(w, K)
-        b = None if bias is None else _packed(bias)
-        r, ldr = (None, N) if residual is None else _rows_any(residual)
-        M = x2.numel() // K
-        out = x2.new_empty(M, N) if x.dim() == 2 else x2.new_empty((*x.shape[:-1], N))
-        z = x2.new_empty(M, N, dtype=torch.float32) if save and activation is not None else None
-        nb = _linear_bytes(False, M, K, N)
-        ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
-        _lib.check("mi355moe_linear_forward", _lib.lib().mi355moe_linear_forward(
-            x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw, _addr(b), bcode, ACTIVATIONS[activation], _addr(r), ldr,
-            out.data_ptr(), N, _addr(z), _addr(ws), max(nb, 0), _raw_stream(dev)))
+    (x2, ldx), (w2, ldw) = _linear_operand(x, K), _linear_operand(w, K)
+    b = None if bias is None else _packed(bias)
+    r, ldr = (residual, N) if residual is None or residual.is_contiguous() else _rows_any(residual)
+    M = x2.numel() // K
+    out = x2.new_empty(M, N) if x.dim() == 2 else x2.new_empty((*x.shape[:-1], N))
+    z = x2.new_empty(M, N, dtype=torch.float32) if save and activation is not None else None
+    nb = _linear_bytes(False, M, K, N)
+    ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
+    rc = _lib.lib().mi355moe_linear_forward(
+        x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw, _addr(b), bcode, ACTIVATIONS[activation], _addr(r), ldr, out.data_ptr(), N,
+        _addr(z), _addr(ws), max(nb, 0), _raw_stream(dev))
+    if rc:
+        _lib.check("mi355moe_linear_forward", rc)
     return (out, z) if save else out
 
 
@@ -238,23 +242,28 @@ def linear_backward(dout: torch.Tensor, z: torch.Tensor | None, x: torch.Tensor,
 
 
 def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw):
-    """linear_backward of arguments that have been looked at."""
+    """linear_backward of arguments that have been looked at. (It runs on autograd's own thread, where a helper's frame costs some us.)"""
     dev, code, _ = kinds
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw)
     N, K = w.shape
-    with _on_device(dev):
-        (x2, ldx), (w2, ldw), (d2, ldd) = _linear_operand(x, K), _linear_operand(w, K), _rows_any(dout)
-        M = x2.numel() // K
-        dx = _empty_like(x) if need_dx else None
-        dw = _empty_like(w) if need_dw else None
-        db = x2.new_empty(N, dtype=bias_dtype) if bias_dtype is not None else None
-        if M == 0 or (dx is None and dw is None and db is None):
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-        nb = _linear_bytes(True, M, K, N)
-        ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
-        _lib.check("mi355moe_linear_backward", _lib.lib().mi355moe_linear_backward(
-            d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw,
-            ACTIVATIONS[activation], _addr(dx), _addr(dw), _addr(db), _lib.F32 if db is None else weight_dtype_code(bias_dtype),
-            ws.data_ptr(), max(nb, 0), _raw_stream(dev)))
+    M = x.numel() // K
+    dx = _empty_like(x) if need_dx else None
+    dw = _empty_like(w) if need_dw else None
+    db = None if bias_dtype is None else x.new_empty(N, dtype=bias_dtype)
+    if M == 0 or (dx is None and dw is None and db is None):
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    (x2, ldx), (w2, ldw) = _linear_operand(x, K), _linear_operand(w, K)
+    d2, ldd = (dout, N) if dout.is_contiguous() else _rows_any(dout)
+    nb = _linear_bytes(True, M, K, N)
+    ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
+    rc = _lib.lib().mi355moe_linear_backward(
+        d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw,
+        ACTIVATIONS[activation], _addr(dx), _addr(dw), _addr(db), _lib.F32 if db is None else weight_dtype_code(bias_dtype), ws.data_ptr(),
+        max(nb, 0), _raw_stream(dev))
+    if rc:
+        _lib.check("mi355moe_linear_backward", rc)
     return dx, dw, db
 
 
@@ -269,7 +278,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dout):
-        if _capturing(dout.device):
+        if _capturing(ctx.rest[0][0]):
             raise RuntimeError("mi355moe: the backward pass of an eagerly recorded ffn.linear cannot be captured; capture "
                                "ffn.linear_forward(save=True) and ffn.linear_backward")
         x, w, z = ctx.saved_tensors

@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from .ops import (_addr, _capturing, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any,
+from .ops import (_addr, _capturing, _current_device, _empty_like, _need_cuda, _no_tangents, _once, _packed, _raw_stream, _rows_any,
                   weight_dtype_code)
 
 _NONE, _CHANNEL, _TOKEN, _FULL = 0, 1, 2, 3
@@ -63,30 +63,31 @@ def _check(branch, residual, post, gate, pre):
     return dev, code, wcode, _gate_kind(shape, gate.shape), weight_dtype_code(gate.dtype)
 
 
-def _rows(t: torch.Tensor | None, H: int) -> tuple[torch.Tensor | None, int]:
-    return (None, H) if t is None else _rows_any(t)
-
-
-def _flat(t: torch.Tensor | None) -> torch.Tensor | None:
-    return None if t is None else _packed(t)
+# The two functions below run once a step, the second on autograd's own thread, where what the first thread touched last is far
+# away: a helper's frame there costs some us. So what is there already is looked at in place, and helpers take the rest.
 
 
 def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, need_stats):
     dev, code, wcode, kind, gcode = kinds
     if pre is None and not need_s:
         raise ValueError("neither s nor y is asked for")
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, need_stats)
     H = branch.shape[-1]
-    with _on_device(dev):
-        (b, ldb), (r, ldr) = _rows_any(branch), _rows(residual, H)
-        n = b.numel() // H
-        post, pre, gate = _flat(post), _flat(pre), _flat(gate)
-        s = _empty_like(branch) if need_s else None
-        y = _empty_like(branch) if pre is not None else None
-        stats = b.new_empty(n, 2, dtype=torch.float32) if need_stats else None
-        if n:
-            _lib.check("mi355moe_norm_forward", _lib.lib().mi355moe_norm_forward(
-                b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode, kind, eps, scale,
-                residual_scale, _addr(s), _addr(y), _addr(stats), _raw_stream(dev)))
+    n = branch.numel() // H
+    s = _empty_like(branch) if need_s else None
+    y = _empty_like(branch) if pre is not None else None
+    stats = branch.new_empty(n, 2, dtype=torch.float32) if need_stats else None
+    if n:
+        b, ldb = (branch, H) if branch.is_contiguous() else _rows_any(branch)
+        r, ldr = (residual, H) if residual is None or residual.is_contiguous() else _rows_any(residual)
+        post, pre, gate = (None if t is None else _packed(t) for t in (post, pre, gate))
+        rc = _lib.lib().mi355moe_norm_forward(
+            b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode, kind, eps, scale,
+            residual_scale, _addr(s), _addr(y), _addr(stats), _raw_stream(dev))
+        if rc:
+            _lib.check("mi355moe_norm_forward", rc)
     return s, y, stats
 
 
@@ -122,29 +123,36 @@ def join_backward(ds: torch.Tensor | None, dy: torch.Tensor | None, stats: torch
 def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, residual_scale, need):
     """join_backward of arguments that have been looked at (kinds: what _check said of them)."""
     dev, code, wcode, kind, gcode = kinds
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, residual_scale, need)
     H = branch.shape[-1]
-    with _on_device(dev):
-        (b, ldb), (r, ldr), (ds, lds), (dy, ldy) = _rows_any(branch), _rows(residual, H), _rows(ds, H), _rows(dy, H)
-        n = b.numel() // H
-        nothing = n == 0 or (ds is None and dy is None)
-
-        def like(t, wanted):
-            return None if t is None or not wanted else t.new_zeros(t.shape) if nothing else _empty_like(t)
-
-        db, dr, dpost, dgate = like(branch, need[0]), like(residual, need[1]), like(post, need[2]), like(gate, need[3])
-        dpre = like(pre, need[4])
-        if nothing:
-            return db, dr, dpost, dgate, dpre
-        if dy is None and dpre is not None:
-            dpre.zero_()
-        post, pre, gate = _flat(post), _flat(pre), _flat(gate)
-        join = dpost is not None or (dpre is not None and dy is not None) or (dgate is not None and kind == _CHANNEL)
-        nb = _backward_bytes(n, H) if join else 0
-        ws = b.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
-        _lib.check("mi355moe_norm_backward", _lib.lib().mi355moe_norm_backward(
-            _addr(ds), lds, _addr(dy), ldy, b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode,
-            _addr(gate), gcode, kind, scale, residual_scale, stats.data_ptr(), _addr(db), _addr(dr), _addr(dpost),
-            None if dy is None else _addr(dpre), _addr(dgate), _addr(ws), max(nb, 0), _raw_stream(dev)))
+    n = branch.numel() // H
+    db = _empty_like(branch) if need[0] else None
+    dr = _empty_like(residual) if need[1] and residual is not None else None
+    dpost = _empty_like(post) if need[2] and post is not None else None
+    dgate = _empty_like(gate) if need[3] and gate is not None else None
+    dpre = _empty_like(pre) if need[4] and pre is not None else None
+    if n == 0 or (ds is None and dy is None):
+        return tuple(None if t is None else t.zero_() for t in (db, dr, dpost, dgate, dpre))
+    if dy is None and dpre is not None:
+        dpre.zero_()
+    b, ldb = (branch, H) if branch.is_contiguous() else _rows_any(branch)
+    r, ldr = (residual, H) if residual is None or residual.is_contiguous() else _rows_any(residual)
+    s, lds = (ds, H) if ds is None or ds.is_contiguous() else _rows_any(ds)
+    y, ldy = (dy, H) if dy is None or dy.is_contiguous() else _rows_any(dy)
+    post, pre, gate = (None if t is None else _packed(t) for t in (post, pre, gate))
+    wpre = None if dy is None else dpre
+    nb, ws = 0, None
+    if dpost is not None or wpre is not None or (dgate is not None and kind == _CHANNEL):
+        nb = _backward_bytes(n, H)
+        ws = b.new_empty(max(nb, 0), dtype=torch.uint8)
+    rc = _lib.lib().mi355moe_norm_backward(
+        _addr(s), lds, _addr(y), ldy, b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode,
+        kind, scale, residual_scale, stats.data_ptr(), _addr(db), _addr(dr), _addr(dpost), _addr(wpre), _addr(dgate), _addr(ws), max(nb, 0),
+        _raw_stream(dev))
+    if rc:
+        _lib.check("mi355moe_norm_backward", rc)
     return db, dr, dpost, dgate, dpre
 
 
@@ -161,7 +169,7 @@ class _Join(torch.autograd.Function):
     @_once
     def backward(ctx, *grads):
         branch, residual, post, gate, pre, stats = ctx.saved_tensors
-        if _capturing(branch.device):
+        if _capturing(ctx.rest[0][0]):
             raise RuntimeError("mi355moe: the backward pass of an eagerly recorded norm cannot be captured; capture "
                                "norm.join_forward and norm.join_backward")
         kinds, scale, residual_scale, has_s, has_y = ctx.rest

@@ -31,7 +31,10 @@ _HERE = contextlib.nullcontext()
 
 def _on_device(dev: torch.device):
     """A context in which `dev` is the current device (kernels are launched on the current one)."""
-    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+    return _HERE if dev.index == _current_device() else torch.cuda.device(dev)
+
+
+_current_device = torch._C._cuda_getDevice
 
 
 def _raw_stream(dev: torch.device) -> int:
@@ -141,7 +144,7 @@ def ids_dtype_code(dt: torch.dtype) -> int:
 
 def _capturing(dev: torch.device) -> bool:
     """True while the current stream of a GPU device is being captured into a graph."""
-    return dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    return dev.type == "cuda" and torch._C._cuda_isCurrentStreamCapturing()
 
 
 def workspace(dev: torch.device, nbytes: int) -> torch.Tensor:

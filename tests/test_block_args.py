@@ -159,9 +159,9 @@ def test_backward_is_refused_during_capture(monkeypatch):
     t = torch.zeros(2, 16)
     six = types.SimpleNamespace(saved_tensors=(t,) * 6, rest=((t.device, 0, 0, 0, 0), 1.0, 1.0, True, True), needs_input_grad=(True,) * 10)
     three = types.SimpleNamespace(saved_tensors=(t,) * 3, rest=((t.device, 0, 0), None, None), needs_input_grad=(True, True, False, False, False, False))
-    two = types.SimpleNamespace(saved_tensors=(t, t), plan=None, needs_input_grad=(True, True, False, False))
+    two = types.SimpleNamespace(saved_tensors=(t, t), rest=(t.device, 0, None), needs_input_grad=(True, True, False, False))
     for mod, fn, inner, ctx, grads in ((norm, norm._Join, "_backward", six, (t, t)), (ffn, ffn._Linear, "_linear_grads", three, (t,)),
-                                       (dispatch, dispatch._From, "_from_grads", two, (t,)), (dispatch, dispatch._To, "_from_experts", two, (t,))):
+                                       (dispatch, dispatch._From, "_from_grads", two, (t,)), (dispatch, dispatch._To, "_gather", two, (t,))):
         monkeypatch.setattr(mod, inner, launched)
         monkeypatch.setattr(mod, "_capturing", lambda dev: True)
         for enabled in (False, True):
