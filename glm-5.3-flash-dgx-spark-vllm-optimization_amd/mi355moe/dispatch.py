@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from .ops import (_addr, _capturing, _current_device, _need_cuda, _no_tangents, _on_device, _once, _packed, _raw_stream, _rows_any,
-                  ids_dtype_code, weight_dtype_code)
+                  _stream_at, ids_dtype_code, weight_dtype_code)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -112,7 +112,8 @@ def _scatter(dev, code, x, plan):
     T, topk, H = plan.tokens, plan.topk, x.shape[1]
     x, ldx = (x, H) if x.is_contiguous() else _rows_any(x)
     rows = x.new_empty(T * topk, H)
-    rc = _lib.lib().mi355moe_rows_to_experts(x.data_ptr(), code, T, H, ldx, plan._words.data_ptr(), topk, rows.data_ptr(), _raw_stream(dev))
+    rc = _lib.lib().mi355moe_rows_to_experts(x.data_ptr(), code, T, H, ldx, plan._words.data_ptr(), topk, rows.data_ptr(),
+                                               _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_rows_to_experts", rc)
     return rows
@@ -140,13 +141,13 @@ def _gather(dev, code, rows, weights, plan, shared):
             return _gather(dev, code, rows, weights, plan, shared)
     wcode = _lib.F32 if weights is None else weight_dtype_code(weights.dtype)
     T, H = plan.tokens, rows.shape[1]
-    rows = _packed(rows)
-    weights = None if weights is None else _packed(weights)
+    rows = rows if rows.is_contiguous() else _packed(rows)
+    weights = weights if weights is None or weights.is_contiguous() else _packed(weights)
     shared, lds = (shared, H) if shared is None or shared.is_contiguous() else _rows_any(shared)
     out = rows.new_empty(T, H)
     rc = _lib.lib().mi355moe_rows_from_experts(
-        rows.data_ptr(), code, T, H, plan._words.data_ptr(), plan.topk, _addr(weights), wcode, _addr(shared), lds, out.data_ptr(), H,
-        _raw_stream(dev))
+        rows.data_ptr(), code, T, H, plan._words.data_ptr(), plan.topk, weights if weights is None else weights.data_ptr(), wcode,
+        shared if shared is None else shared.data_ptr(), lds, out.data_ptr(), H, _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_rows_from_experts", rc)
     return out
@@ -172,12 +173,13 @@ def _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights):
             return _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights)
     H = rows.shape[1]
     dout, ldd = (dout, H) if dout.is_contiguous() else _rows_any(dout)
-    rows, weights = _packed(rows), _packed(weights)
+    rows = rows if rows.is_contiguous() else _packed(rows)
+    weights = weights if weights.is_contiguous() else _packed(weights)
     drows = torch.empty_like(rows) if need_rows else None
     dw = torch.empty_like(weights) if need_weights else None
     rc = _lib.lib().mi355moe_rows_from_experts_backward(
         dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(), weight_dtype_code(weights.dtype),
-        rows.data_ptr(), _addr(drows), _addr(dw), _raw_stream(dev))
+        rows.data_ptr(), drows if drows is None else drows.data_ptr(), dw if dw is None else dw.data_ptr(), _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_rows_from_experts_backward", rc)
     return drows, dw

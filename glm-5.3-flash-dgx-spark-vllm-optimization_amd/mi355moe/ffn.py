@@ -30,7 +30,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .ops import (_addr, _capturing, _current_device, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain,
-                  _raw_stream, _row_stride, _rows_any, act_dtype_code, weight_dtype_code)
+                  _raw_stream, _row_stride, _rows_any, _stream_at, act_dtype_code, weight_dtype_code)
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -217,7 +217,7 @@ def _linear(kinds, x, w, bias, activation, residual, save):
     ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
     rc = _lib.lib().mi355moe_linear_forward(
         x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw, _addr(b), bcode, ACTIVATIONS[activation], _addr(r), ldr, out.data_ptr(), N,
-        _addr(z), _addr(ws), max(nb, 0), _raw_stream(dev))
+        _addr(z), _addr(ws), max(nb, 0), _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_linear_forward", rc)
     return (out, z) if save else out
@@ -249,8 +249,11 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
             return _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw)
     N, K = w.shape
     M = x.numel() // K
-    dx = _empty_like(x) if need_dx else None
-    dw = _empty_like(w) if need_dw else None
+    dx = dw = None
+    if need_dx:
+        dx = torch.empty_like(x) if x.is_contiguous() else _empty_like(x)
+    if need_dw:
+        dw = torch.empty_like(w) if w.is_contiguous() else _empty_like(w)
     db = None if bias_dtype is None else x.new_empty(N, dtype=bias_dtype)
     if M == 0 or (dx is None and dw is None and db is None):
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
@@ -260,8 +263,9 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
     ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
     rc = _lib.lib().mi355moe_linear_backward(
         d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw,
-        ACTIVATIONS[activation], _addr(dx), _addr(dw), _addr(db), _lib.F32 if db is None else weight_dtype_code(bias_dtype), ws.data_ptr(),
-        max(nb, 0), _raw_stream(dev))
+        ACTIVATIONS[activation], dx if dx is None else dx.data_ptr(), dw if dw is None else dw.data_ptr(),
+        db if db is None else db.data_ptr(), _lib.F32 if db is None else weight_dtype_code(bias_dtype), ws.data_ptr(), nb if nb > 0 else 0,
+        _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_linear_backward", rc)
     return dx, dw, db

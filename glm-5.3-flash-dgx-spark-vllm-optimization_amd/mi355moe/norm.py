@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from .ops import (_addr, _capturing, _current_device, _empty_like, _need_cuda, _no_tangents, _once, _packed, _raw_stream, _rows_any,
+from .ops import (_capturing, _current_device, _empty_like, _need_cuda, _no_tangents, _once, _packed, _rows_any, _stream_at,
                   weight_dtype_code)
 
 _NONE, _CHANNEL, _TOKEN, _FULL = 0, 1, 2, 3
@@ -82,10 +82,14 @@ def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scal
     if n:
         b, ldb = (branch, H) if branch.is_contiguous() else _rows_any(branch)
         r, ldr = (residual, H) if residual is None or residual.is_contiguous() else _rows_any(residual)
-        post, pre, gate = (None if t is None else _packed(t) for t in (post, pre, gate))
+        post = post if post is None or post.is_contiguous() else _packed(post)
+        pre = pre if pre is None or pre.is_contiguous() else _packed(pre)
+        gate = gate if gate is None or gate.is_contiguous() else _packed(gate)
         rc = _lib.lib().mi355moe_norm_forward(
-            b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode, kind, eps, scale,
-            residual_scale, _addr(s), _addr(y), _addr(stats), _raw_stream(dev))
+            b.data_ptr(), code, n, H, ldb, r if r is None else r.data_ptr(), ldr, post if post is None else post.data_ptr(),
+            pre if pre is None else pre.data_ptr(), wcode, gate if gate is None else gate.data_ptr(), gcode, kind, eps, scale,
+            residual_scale, s if s is None else s.data_ptr(), y if y is None else y.data_ptr(), stats if stats is None else stats.data_ptr(),
+            _stream_at(dev.index))
         if rc:
             _lib.check("mi355moe_norm_forward", rc)
     return s, y, stats
@@ -128,11 +132,17 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
             return _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, residual_scale, need)
     H = branch.shape[-1]
     n = branch.numel() // H
-    db = _empty_like(branch) if need[0] else None
-    dr = _empty_like(residual) if need[1] and residual is not None else None
-    dpost = _empty_like(post) if need[2] and post is not None else None
-    dgate = _empty_like(gate) if need[3] and gate is not None else None
-    dpre = _empty_like(pre) if need[4] and pre is not None else None
+    db = dr = dpost = dgate = dpre = None
+    if need[0]:
+        db = torch.empty_like(branch) if branch.is_contiguous() else _empty_like(branch)
+    if need[1] and residual is not None:
+        dr = torch.empty_like(residual) if residual.is_contiguous() else _empty_like(residual)
+    if need[2] and post is not None:
+        dpost = torch.empty_like(post) if post.is_contiguous() else _empty_like(post)
+    if need[3] and gate is not None:
+        dgate = torch.empty_like(gate) if gate.is_contiguous() else _empty_like(gate)
+    if need[4] and pre is not None:
+        dpre = torch.empty_like(pre) if pre.is_contiguous() else _empty_like(pre)
     if n == 0 or (ds is None and dy is None):
         return tuple(None if t is None else t.zero_() for t in (db, dr, dpost, dgate, dpre))
     if dy is None and dpre is not None:
@@ -141,16 +151,20 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
     r, ldr = (residual, H) if residual is None or residual.is_contiguous() else _rows_any(residual)
     s, lds = (ds, H) if ds is None or ds.is_contiguous() else _rows_any(ds)
     y, ldy = (dy, H) if dy is None or dy.is_contiguous() else _rows_any(dy)
-    post, pre, gate = (None if t is None else _packed(t) for t in (post, pre, gate))
+    post = post if post is None or post.is_contiguous() else _packed(post)
+    pre = pre if pre is None or pre.is_contiguous() else _packed(pre)
+    gate = gate if gate is None or gate.is_contiguous() else _packed(gate)
     wpre = None if dy is None else dpre
     nb, ws = 0, None
     if dpost is not None or wpre is not None or (dgate is not None and kind == _CHANNEL):
         nb = _backward_bytes(n, H)
         ws = b.new_empty(max(nb, 0), dtype=torch.uint8)
     rc = _lib.lib().mi355moe_norm_backward(
-        _addr(s), lds, _addr(y), ldy, b.data_ptr(), code, n, H, ldb, _addr(r), ldr, _addr(post), _addr(pre), wcode, _addr(gate), gcode,
-        kind, scale, residual_scale, stats.data_ptr(), _addr(db), _addr(dr), _addr(dpost), _addr(wpre), _addr(dgate), _addr(ws), max(nb, 0),
-        _raw_stream(dev))
+        s if s is None else s.data_ptr(), lds, y if y is None else y.data_ptr(), ldy, b.data_ptr(), code, n, H, ldb,
+        r if r is None else r.data_ptr(), ldr, post if post is None else post.data_ptr(), pre if pre is None else pre.data_ptr(), wcode,
+        gate if gate is None else gate.data_ptr(), gcode, kind, scale, residual_scale, stats.data_ptr(),
+        db if db is None else db.data_ptr(), dr if dr is None else dr.data_ptr(), dpost if dpost is None else dpost.data_ptr(), wpre if wpre is None else wpre.data_ptr(),
+        dgate if dgate is None else dgate.data_ptr(), ws if ws is None else ws.data_ptr(), nb if nb > 0 else 0, _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_norm_backward", rc)
     return db, dr, dpost, dgate, dpre

@@ -35,6 +35,7 @@ def _on_device(dev: torch.device):
 
 
 _current_device = torch._C._cuda_getDevice
+_stream_at = torch._C._cuda_getCurrentRawStream      # by a device's index
 
 
 def _raw_stream(dev: torch.device) -> int:
