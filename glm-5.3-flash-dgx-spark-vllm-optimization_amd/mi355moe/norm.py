@@ -88,8 +88,8 @@ def _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scal
         rc = _lib.lib().mi355moe_norm_forward(
             b.data_ptr(), code, n, H, ldb, r if r is None else r.data_ptr(), ldr, post if post is None else post.data_ptr(),
             pre if pre is None else pre.data_ptr(), wcode, gate if gate is None else gate.data_ptr(), gcode, kind, eps, scale,
-            residual_scale, s if s is None else s.data_ptr(), y if y is None else y.data_ptr(), stats if stats is None else stats.data_ptr(),
-            _stream_at(dev.index))
+            residual_scale, s if s is None else s.data_ptr(), y if y is None else y.data_ptr(),
+            stats if stats is None else stats.data_ptr(), _stream_at(dev.index))
         if rc:
             _lib.check("mi355moe_norm_forward", rc)
     return s, y, stats
@@ -163,8 +163,9 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
         s if s is None else s.data_ptr(), lds, y if y is None else y.data_ptr(), ldy, b.data_ptr(), code, n, H, ldb,
         r if r is None else r.data_ptr(), ldr, post if post is None else post.data_ptr(), pre if pre is None else pre.data_ptr(), wcode,
         gate if gate is None else gate.data_ptr(), gcode, kind, scale, residual_scale, stats.data_ptr(),
-        db if db is None else db.data_ptr(), dr if dr is None else dr.data_ptr(), dpost if dpost is None else dpost.data_ptr(), wpre if wpre is None else wpre.data_ptr(),
-        dgate if dgate is None else dgate.data_ptr(), ws if ws is None else ws.data_ptr(), nb if nb > 0 else 0, _stream_at(dev.index))
+        db if db is None else db.data_ptr(), dr if dr is None else dr.data_ptr(), dpost if dpost is None else dpost.data_ptr(),
+        wpre if wpre is None else wpre.data_ptr(), dgate if dgate is None else dgate.data_ptr(),
+        ws if ws is None else ws.data_ptr(), nb if nb > 0 else 0, _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_norm_backward", rc)
     return db, dr, dpost, dgate, dpre
