@@ -34,8 +34,9 @@ def _on_device(dev: torch.device):
     return _HERE if dev.index == _current_device() else torch.cuda.device(dev)
 
 
-_current_device = torch._C._cuda_getDevice
-_stream_at = torch._C._cuda_getCurrentRawStream      # by a device's index
+# (a torch without GPU bindings has neither; there every call is refused before it asks, since no tensor is on a GPU)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_stream_at = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # by a device's index
 
 
 def _raw_stream(dev: torch.device) -> int:
