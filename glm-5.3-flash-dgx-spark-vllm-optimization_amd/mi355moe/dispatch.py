@@ -156,7 +156,8 @@ def _gather(dev, code, rows, weights, plan, shared):
 def from_experts_backward(dout: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, plan: SortedTokens, need_rows: bool = True,
                           need_weights: bool = True):
     """(drows, dweights), None where not needed, of from_experts(rows, weights, plan) from dout [T, H]: drows in rows' dtype, zero
-    behind offsets[n]; dweights in weights' dtype, zero for the pairs that no local expert takes. shared's gradient is dout."""
+    behind offsets[n]; dweights in weights' dtype, zero for the pairs that no local expert takes. shared's gradient is dout. rows'
+    values are read for dweights only."""
     dev, code = _check_back(rows, weights, plan, None)
     _need_cuda(rows, dout)
     _no_tangents("from_experts_backward", dout, rows, weights)
@@ -167,19 +168,23 @@ def from_experts_backward(dout: torch.Tensor, rows: torch.Tensor, weights: torch
 
 
 def _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights):
-    """from_experts_backward of arguments that have been looked at."""
+    """from_experts_backward of arguments that have been looked at. rows may be None where dweights is not needed."""
     if dev.index != _current_device():
         with torch.cuda.device(dev):
             return _from_grads(dev, code, dout, rows, weights, plan, need_rows, need_weights)
-    H = rows.shape[1]
+    H = dout.shape[1]
     dout, ldd = (dout, H) if dout.is_contiguous() else _rows_any(dout)
-    rows = rows if rows.is_contiguous() else _packed(rows)
     weights = weights if weights.is_contiguous() else _packed(weights)
-    drows = torch.empty_like(rows) if need_rows else None
-    dw = torch.empty_like(weights) if need_weights else None
+    drows = dw = None
+    if need_rows:
+        drows = torch.empty_like(rows) if rows is not None and rows.is_contiguous() else dout.new_empty(plan.tokens * plan.topk, H)
+    if need_weights:
+        dw = torch.empty_like(weights)
+        rows = rows if rows.is_contiguous() else _packed(rows)
     rc = _lib.lib().mi355moe_rows_from_experts_backward(
         dout.data_ptr(), code, plan.tokens, H, ldd, plan._words.data_ptr(), plan.topk, weights.data_ptr(), weight_dtype_code(weights.dtype),
-        rows.data_ptr(), drows if drows is None else drows.data_ptr(), dw if dw is None else dw.data_ptr(), _stream_at(dev.index))
+        rows.data_ptr() if need_weights else None, drows if drows is None else drows.data_ptr(), dw if dw is None else dw.data_ptr(),
+        _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_rows_from_experts_backward", rc)
     return drows, dw
@@ -211,7 +216,9 @@ class _From(torch.autograd.Function):
     def forward(ctx, rows, weights, plan, shared):
         dev, code = _check_back(rows, weights, plan, shared)
         ctx.rest = dev, code, plan
-        ctx.save_for_backward(rows, weights)
+        # (rows are read for the weights' gradient only: kept for nothing else, [T * topk, H] would stay until the backward pass)
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(rows if need[1] else None, weights if need[0] or need[1] else None)
         return _gather(dev, code, rows, weights, plan, shared)
 
     @staticmethod
