@@ -157,7 +157,9 @@ def from_experts_backward(dout: torch.Tensor, rows: torch.Tensor, weights: torch
                           need_weights: bool = True):
     """(drows, dweights), None where not needed, of from_experts(rows, weights, plan) from dout [T, H]: drows in rows' dtype, zero
     behind offsets[n]; dweights in weights' dtype, zero for the pairs that no local expert takes. shared's gradient is dout. rows'
-    values are read for dweights only."""
+    values are read for dweights only. (Without weights, rows' gradient is to_experts(dout, plan).)"""
+    if weights is None:
+        raise ValueError("from_experts_backward needs weights; without them the gradient of rows is to_experts(dout, plan)")
     dev, code = _check_back(rows, weights, plan, None)
     _need_cuda(rows, dout)
     _no_tangents("from_experts_backward", dout, rows, weights)
