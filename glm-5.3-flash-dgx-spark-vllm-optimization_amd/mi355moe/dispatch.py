@@ -68,8 +68,9 @@ def sort_tokens(topk_ids: torch.Tensor, n: int, expert_map: torch.Tensor | None 
     if topk_ids.dim() != 2 or topk_ids.shape[1] == 0:
         raise ValueError(f"topk_ids must be [T, topk], got {tuple(topk_ids.shape)}")
     if expert_map is not None:
-        if expert_map.dim() != 1 or expert_map.dtype.is_floating_point or expert_map.dtype == torch.bool:
-            raise ValueError(f"expert_map must be a vector of whole numbers, got {expert_map.dtype} {tuple(expert_map.shape)}")
+        kind = expert_map.dtype
+        if expert_map.dim() != 1 or kind.is_floating_point or kind.is_complex or kind == torch.bool:
+            raise ValueError(f"expert_map must be a vector of whole numbers, got {kind} {tuple(expert_map.shape)}")
     T, topk = topk_ids.shape
     n, P = int(n), T * topk
     nb = _sort_bytes(T, topk, n)

@@ -11,3 +11,12 @@ def test_gradients_of_rows_back_need_weights():
     for need in ((True, True), (True, False), (False, True)):
         with pytest.raises(ValueError, match="needs weights"):
             dispatch.from_experts_backward(torch.zeros(2, 8), torch.zeros(4, 8), None, plan, *need)
+
+
+@pytest.mark.gpu
+def test_maps_of_complex_numbers(cuda):
+    from mi355moe import dispatch
+    ids = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    for dt in (torch.complex64, torch.complex128):
+        with pytest.raises(ValueError, match="whole numbers"):
+            dispatch.sort_tokens(ids, 4, expert_map=torch.zeros(4, dtype=dt, device="cuda"))
