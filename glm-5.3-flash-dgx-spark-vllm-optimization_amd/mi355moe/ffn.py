@@ -257,13 +257,15 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
     db = None if bias_dtype is None else x.new_empty(N, dtype=bias_dtype)
     if M == 0 or (dx is None and dw is None and db is None):
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
-    (x2, ldx), (w2, ldw) = _linear_operand(x, K), _linear_operand(w, K)
+    # (x is read for dw, w for dx: what is not read is not copied to where it could be)
+    x2, ldx = _linear_operand(x, K) if need_dw else (None, (K + 7) & ~7)
+    w2, ldw = _linear_operand(w, K) if need_dx else (None, (K + 7) & ~7)
     d2, ldd = (dout, N) if dout.is_contiguous() else _rows_any(dout)
     nb = _linear_bytes(True, M, K, N)
-    ws = x2.new_empty(max(nb, 0), dtype=torch.uint8)
+    ws = dout.new_empty(max(nb, 0), dtype=torch.uint8)
     rc = _lib.lib().mi355moe_linear_backward(
-        d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw,
-        ACTIVATIONS[activation], dx if dx is None else dx.data_ptr(), dw if dw is None else dw.data_ptr(),
+        d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2 if x2 is None else x2.data_ptr(), code, M, K, ldx,
+        w2 if w2 is None else w2.data_ptr(), N, ldw, ACTIVATIONS[activation], dx if dx is None else dx.data_ptr(), dw if dw is None else dw.data_ptr(),
         db if db is None else db.data_ptr(), _lib.F32 if db is None else weight_dtype_code(bias_dtype), ws.data_ptr(), nb if nb > 0 else 0,
         _stream_at(dev.index))
     if rc:

@@ -78,3 +78,17 @@ def test_rows_backward_reads_rows_for_the_weights_only(cuda):
     assert bytes_ < T * k * H * 2 + MB
     drows, dw = dispatch.from_experts_backward(d, rows, w, plan, need_rows=False)
     assert drows is None and torch.equal(dw, both[1])
+
+
+def test_linear_gradients_copy_only_what_they_read(cuda):
+    """An operand that the kernels cannot read where it lies is copied for the product that reads it, and for no other."""
+    from mi355moe import ffn
+    M, K, N = 2048, 1024, 1024
+    x, w, d = (torch.randn(*s, device="cuda").bfloat16() for s in ((M, K), (N, K), (M, N)))
+    odd = lambda t: torch.cat([t[:, :1], t], 1)[:, 1:]  # noqa: E731
+    want = ffn.linear_backward(d, None, x, w)
+    for need, bad in (((True, False), (odd(x), w)), ((False, True), (x, odd(w)))):
+        plain, _ = _peak(lambda: ffn.linear_backward(d, None, x, w, None, None, *need))
+        moved, got = _peak(lambda: ffn.linear_backward(d, None, *bad, None, None, *need))
+        assert moved == plain, (need, moved, plain)
+        assert all(p is None or torch.equal(p, q) for p, q in zip(got, want))
