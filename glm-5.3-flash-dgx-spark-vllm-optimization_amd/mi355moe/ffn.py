@@ -29,7 +29,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import (_addr, _capturing, _current_device, _empty_like, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain,
+from .ops import (_addr, _capturing, _current_device, _need_cuda, _no_tangents, _on_device, _once, _packed, _plain,
                   _raw_stream, _row_stride, _rows_any, _stream_at, act_dtype_code, weight_dtype_code)
 
 
@@ -242,19 +242,21 @@ def linear_backward(dout: torch.Tensor, z: torch.Tensor | None, x: torch.Tensor,
 
 
 def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw):
-    """linear_backward of arguments that have been looked at. (It runs on autograd's own thread, where a helper's frame costs some us.)"""
+    """linear_backward of arguments that have been looked at; x may be None without dw, w without dx, z without any of the three. (It
+    runs on autograd's own thread, where a helper's frame costs some us.)"""
     dev, code, _ = kinds
     if dev.index != _current_device():
         with torch.cuda.device(dev):
             return _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw)
-    N, K = w.shape
-    M = x.numel() // K
+    N = dout.shape[-1]
+    K = w.shape[1] if w is not None else 1 if x is None else x.shape[-1]         # (the bias' gradient alone: any K)
+    M = dout.numel() // N
     dx = dw = None
     if need_dx:
-        dx = torch.empty_like(x) if x.is_contiguous() else _empty_like(x)
+        dx = torch.empty_like(x) if x is not None and x.is_contiguous() else dout.new_empty((*dout.shape[:-1], K))
     if need_dw:
-        dw = torch.empty_like(w) if w.is_contiguous() else _empty_like(w)
-    db = None if bias_dtype is None else x.new_empty(N, dtype=bias_dtype)
+        dw = torch.empty_like(w) if w is not None and w.is_contiguous() else dout.new_empty(N, K)
+    db = None if bias_dtype is None else dout.new_empty(N, dtype=bias_dtype)
     if M == 0 or (dx is None and dw is None and db is None):
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     # (x is read for dw, w for dx: what is not read is not copied to where it could be)
@@ -276,8 +278,12 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, kinds, activation):
-        out, z = _linear(kinds, x, w, bias, activation, residual, True)
-        ctx.save_for_backward(x, w, z)
+        # what the gradients that are asked for read: x for w's, w for x's, z for these and the bias', nothing for the residual's
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_z = need_x or need_w or need_b
+        out = _linear(kinds, x, w, bias, activation, residual, need_z)
+        out, z = out if need_z else (out, None)
+        ctx.save_for_backward(x if need_w else None, w if need_x else None, z)
         ctx.rest = kinds, activation, None if bias is None else bias.dtype
         return out
 
@@ -290,7 +296,9 @@ class _Linear(torch.autograd.Function):
         x, w, z = ctx.saved_tensors
         kinds, activation, bias_dtype = ctx.rest
         need = ctx.needs_input_grad
-        dx, dw, db = _linear_grads(kinds, dout, z, x, w, activation, bias_dtype if need[2] else None, need[0], need[1])
+        dx = dw = db = None
+        if need[0] or need[1] or need[2]:
+            dx, dw, db = _linear_grads(kinds, dout, z, x, w, activation, bias_dtype if need[2] else None, need[0], need[1])
         return dx, dw, db, dout if need[3] else None, None, None
 
 

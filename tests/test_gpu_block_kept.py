@@ -20,6 +20,13 @@ def _peak(f):
     return torch.cuda.max_memory_allocated() - before, out
 
 
+def _held(f):
+    """(f's results, the bytes that stay allocated with them)."""
+    before = torch.cuda.memory_allocated()
+    out = f()
+    return out, torch.cuda.memory_allocated() - before
+
+
 def _order(T, k, n):
     from mi355moe import dispatch
     return dispatch.sort_tokens(torch.randint(0, n + 2, (T, k), generator=torch.Generator().manual_seed(1)).cuda(), n)
@@ -92,3 +99,54 @@ def test_linear_gradients_copy_only_what_they_read(cuda):
         moved, got = _peak(lambda: ffn.linear_backward(d, None, *bad, None, None, *need))
         assert moved == plain, (need, moved, plain)
         assert all(p is None or torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_linear_keeps_what_its_gradients_read(cuda):
+    """x for w's gradient, w for x's, z for x's, w's and the bias' where there is an activation."""
+    from mi355moe import ffn
+    M, K, N = 1024, 512, 1024
+    g = torch.Generator(device="cuda").manual_seed(3)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    base = {"x": new(M, K).bfloat16(), "w": (new(N, K) / 16).bfloat16(), "bias": new(N), "residual": new(M, N).bfloat16()}
+    d = new(M, N).bfloat16()
+    for act in (None, "silu"):
+        out, z = ffn.linear_forward(*(base[k] for k in ("x", "w", "bias")), act, base["residual"], save=True)
+        grads = ffn.linear_backward(d, z, base["x"], base["w"], act, torch.float32)
+        want = dict(zip(("x", "w", "bias"), grads), residual=d)
+        for asked in (("x",), ("w",), ("bias",), ("residual",), ("x", "residual"), ("bias", "residual"), ("x", "w"), ("w", "bias"), tuple(base)):
+            # what is asked for is not a leaf, so that it may be changed in place
+            leaf = {k: base[k].clone().requires_grad_(k in asked) for k in base}
+            used = {k: leaf[k] * 1.0 for k in base}
+
+            def call():
+                return ffn.linear(used["x"], used["w"], used["bias"], act, used["residual"])
+
+            y, held = _held(call)
+            assert torch.equal(y, out)
+            kept_z = act is not None and any(k in asked for k in ("x", "w", "bias"))
+            assert (held >= M * N * 6) == kept_z, (act, asked, held)
+            read = [k for k, by in (("x", "w"), ("w", "x")) if by in asked]
+            with torch.no_grad():
+                for k in base:
+                    if k not in read:
+                        used[k].mul_(2.0)
+            y.backward(d, retain_graph=True)
+            for k in base:
+                assert (leaf[k].grad is None) == (k not in asked)
+                assert k not in asked or torch.equal(leaf[k].grad, want[k]), (act, asked, k)
+            if read:
+                with torch.no_grad():
+                    used[read[0]].mul_(2.0)
+                with pytest.raises(RuntimeError, match="modified by an inplace"):
+                    y.backward(d)
+    # no gradient of three dimensions, or of no rows, needs the other operand either
+    x3 = base["x"].reshape(4, M // 4, K).clone().requires_grad_()
+    y = ffn.linear(x3, base["w"])
+    y.backward(d.reshape(4, M // 4, N))
+    assert torch.equal(x3.grad.reshape(M, K), ffn.linear_backward(d, None, base["x"], base["w"])[0])
+    w = base["w"].clone().requires_grad_()
+    ffn.linear(base["x"][:0], w).sum().backward()
+    assert w.grad.shape == (N, K) and not w.grad.any()
+    x0 = base["x"][:0].clone().requires_grad_()
+    ffn.linear(x0, base["w"]).sum().backward()
+    assert x0.grad.shape == (0, K)
