@@ -2297,6 +2297,12 @@ int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N
     return linear_backward_bytes(M, N, K);
 }
 
+int64_t mi355moe_linear_backward_call_bytes(int64_t M, int64_t K, int64_t N, int dtype, int activation, int dy_aligned, int want_dx,
+                                            int want_dw, int want_dbias) {
+    if (linear_ok(dtype, M, K, N, activation)) return -1;
+    return linear_backward_call_bytes(dt_act(dtype), activation, M, N, K, dy_aligned != 0, want_dx != 0, want_dw != 0, want_dbias != 0);
+}
+
 int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, const void* x, int dtype, int64_t M, int64_t K,
                              int64_t x_stride, const void* w, int64_t N, int64_t w_stride, int activation, void* dx, void* dw,
                              void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -2305,11 +2311,12 @@ int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, 
     if (dy_stride < N) return MI355MOE_ESHAPE;
     if (!dx && !dw && !dbias) return 0;
     if (M == 0) return dw || dbias ? MI355MOE_ESHAPE : 0;
-    if (!dy || !workspace || (activation != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return MI355MOE_EINVAL;
+    const int64_t need = linear_backward_call_bytes(dt_act(dtype), activation, M, N, K, linear_dy_aligned(dy, dy_stride), dx, dw, dbias);
+    if (!dy || (need > 0 && !workspace) || (activation != ACT_NONE && !z) || (dx && !w) || (dw && !x)) return MI355MOE_EINVAL;
     if (!at_ok(dy, dtype) || !at_ok(z, MI355MOE_F32) || !at_ok(dx, dtype) || !at_ok(dw, dtype) || !at_ok(dbias, bias_dtype)) return MI355MOE_EINVAL;
     if (int r = linear_operands(dw ? x : nullptr, dw ? x_stride : (K + 7) / 8 * 8, dx ? w : nullptr, dx ? w_stride : (K + 7) / 8 * 8, K)) return r;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return MI355MOE_EINVAL;
-    if ((int64_t)workspace_bytes < linear_backward_bytes(M, N, K)) return MI355MOE_EWORKSPACE;
+    if ((int64_t)workspace_bytes < need) return MI355MOE_EWORKSPACE;
     LinearArgs a{};
     a.dt = dt_act(dtype);
     a.M = M;

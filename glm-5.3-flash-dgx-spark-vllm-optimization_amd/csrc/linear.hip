@@ -667,37 +667,56 @@ int launch_linear(const LinearArgs& a, void* ws, hipStream_t st) {
     return a.dt == DT_BF16 ? linear_forward<DT_BF16>(a, static_cast<char*>(ws), st) : linear_forward<DT_F16>(a, static_cast<char*>(ws), st);
 }
 
-// Whether the products can take dy as it is (its rows then lie as an operand's do).
-static bool dz_is_dy(const LinearArgs& a) {
-    return a.act == ACT_NONE && a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dy) & 15) == 0 && a.dy_stride % 8 == 0 && a.dy_stride <= (1 << 22);
+// What a gradient's call puts in its workspace: dz unless dy serves as it is, its largest values (tops), the copies and parts of
+// the products that are asked for, the sums of dbias.
+struct LinearUse {
+    bool dz, tops, dx, dw, dbias;
+};
+// Whether the products can take dy as it is (its rows then lie as an operand's do: aligned).
+static bool dz_is_dy(int act, int64_t N, bool aligned) { return act == ACT_NONE && N % 8 == 0 && aligned; }
+static LinearUse linear_use(int dt, int act, int64_t N, bool aligned, bool dx, bool dw, bool dbias) {
+    const bool dz = (dx || dw) && !dz_is_dy(act, N, aligned);
+    return {dz, dz && dt == DT_F16 && act != ACT_NONE && act != ACT_RELU, dx, dw, dbias};
 }
-static LinearSpace backward_space(int64_t M, int64_t N, int64_t K) {
+static LinearSpace backward_space(int64_t M, int64_t N, int64_t K, const LinearUse& u) {
     LinearSpace s;
-    s.dz = s.take(M * up8(N) * 2);
-    s.tops = s.take(4 * (LINEAR_TOPS + 1));
-    if (K % 8) s.x = s.take(M * up8(K) * 2), s.w = s.take(N * up8(K) * 2);
-    s.part = s.take(std::max({part_bytes(M, K, N), part_bytes(N, K, M), 4 * ((M + DZ_ROWS - 1) / DZ_ROWS) * up8(N)}));
+    if (u.dz) s.dz = s.take(M * up8(N) * 2);
+    if (u.tops) s.tops = s.take(4 * (LINEAR_TOPS + 1));
+    if (K % 8 && u.dw) s.x = s.take(M * up8(K) * 2);
+    if (K % 8 && u.dx) s.w = s.take(N * up8(K) * 2);
+    const int64_t part = std::max({u.dx ? part_bytes(M, K, N) : 0, u.dw ? part_bytes(N, K, M) : 0,
+                                   u.dbias ? 4 * ((M + DZ_ROWS - 1) / DZ_ROWS) * up8(N) : 0});
+    if (part) s.part = s.take(part);
     return s;
 }
-int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K) { return backward_space(M, N, K).bytes; }
+int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K) { return backward_space(M, N, K, {true, true, true, true, true}).bytes; }
+// A workspace of up to 1 MB for all gradients is laid out for all of them whatever is asked for: one size for a shape, and nothing
+// to gain (an allocator's own step is of that order).
+static LinearSpace call_space(int64_t M, int64_t N, int64_t K, const LinearUse& u) {
+    const LinearSpace all = backward_space(M, N, K, {true, true, true, true, true});
+    return all.bytes <= 1 << 20 ? all : backward_space(M, N, K, u);
+}
+int64_t linear_backward_call_bytes(int dt, int act, int64_t M, int64_t N, int64_t K, bool aligned, bool dx, bool dw, bool dbias) {
+    return call_space(M, N, K, linear_use(dt, act, N, aligned, dx, dw, dbias)).bytes;
+}
 
 template <int DT>
 static int linear_backward(const LinearArgs& a, char* ws, hipStream_t st) {
-    const LinearSpace s = backward_space(a.M, a.N, a.K);
+    const LinearUse use = linear_use(a.dt, a.act, a.N, linear_dy_aligned(a.dy, a.dy_stride), a.dx, a.dw, a.dbias);
+    const LinearSpace s = call_space(a.M, a.N, a.K, use);
     const int64_t N8 = up8(a.N), K8 = up8(a.K);
-    auto at = [&](int64_t o) { return reinterpret_cast<uint16_t*>(ws + o); };
-    const bool direct = dz_is_dy(a);
-    float* part = reinterpret_cast<float*>(ws + s.part);
+    auto at = [&](int64_t o) { return o < 0 ? nullptr : reinterpret_cast<uint16_t*>(ws + o); };
+    float* part = reinterpret_cast<float*>(at(s.part));
     SlopeArgs g{};
     g.a = a;
     g.part = part;
     g.part_stride = N8;
-    g.dz = (a.dx || a.dw) && !direct ? at(s.dz) : nullptr;
+    g.dz = use.dz ? at(s.dz) : nullptr;
     g.dz_stride = N8;
-    g.tops = reinterpret_cast<uint32_t*>(ws + s.tops);
-    g.unscale = reinterpret_cast<float*>(g.tops + LINEAR_TOPS);
     if constexpr (DT == DT_F16)
-        if (g.dz && a.act != ACT_NONE && a.act != ACT_RELU) {
+        if (use.tops) {
+            g.tops = reinterpret_cast<uint32_t*>(at(s.tops));
+            g.unscale = reinterpret_cast<float*>(g.tops + LINEAR_TOPS);
             g.ntops = (int)std::min<int64_t>((a.M * ((a.N + 7) / 8) + 255) / 256, LINEAR_TOPS);
             hipLaunchKernelGGL(linear_top_kernel<DT>, dim3(g.ntops), dim3(256), 0, st, g);
             if (hipGetLastError() != hipSuccess) return -1;
@@ -712,8 +731,8 @@ static int linear_backward(const LinearArgs& a, char* ws, hipStream_t st) {
         }
     }
     ProductArgs p{};
-    p.q = direct ? static_cast<const uint16_t*>(a.dy) : at(s.dz);
-    p.ldq = direct ? a.dy_stride : N8;
+    p.q = g.dz ? g.dz : static_cast<const uint16_t*>(a.dy);
+    p.ldq = g.dz ? N8 : a.dy_stride;
     p.qcols = (int)N8;
     p.pcols = (int)K8;
     p.N = a.K;
@@ -721,7 +740,7 @@ static int linear_backward(const LinearArgs& a, char* ws, hipStream_t st) {
     p.unscale = g.ntops ? g.unscale : nullptr;
     const uint16_t *x = a.x, *w = a.w;
     int64_t ldx = a.x_stride, ldw = a.w_stride;
-    if (s.x >= 0 && (a.dx || a.dw)) {
+    if (a.K % 8 && (a.dx || a.dw)) {
         const PadArgs pad{{a.x, a.w}, {ldx, ldw}, {a.dw ? a.M : 0, a.dx ? a.N : 0}, {at(s.x), at(s.w)}, a.K, (int)K8};
         if (int r = run_pad(pad, st)) return r;
         x = at(s.x), w = at(s.w), ldx = ldw = K8;

@@ -558,7 +558,12 @@ struct LinearArgs {
 };
 constexpr int LINEAR_TOPS = 1024;
 int64_t linear_forward_bytes(int64_t M, int64_t N, int64_t K);
-int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K);
+int64_t linear_backward_bytes(int64_t M, int64_t N, int64_t K);              // for any call of these sizes
+// For one call: which gradients it asks for, and whether dy's rows lie as an operand's.
+int64_t linear_backward_call_bytes(int dt, int act, int64_t M, int64_t N, int64_t K, bool aligned, bool dx, bool dw, bool dbias);
+inline bool linear_dy_aligned(const void* dy, int64_t stride) {
+    return (reinterpret_cast<uintptr_t>(dy) & 15) == 0 && stride % 8 == 0 && stride <= (1 << 22);
+}
 int launch_linear(const LinearArgs& a, void* workspace, hipStream_t st);
 int launch_linear_backward(const LinearArgs& a, void* workspace, hipStream_t st);
 

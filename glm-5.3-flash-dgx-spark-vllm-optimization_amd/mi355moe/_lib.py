@@ -150,6 +150,7 @@ _SIGS = {
     "mi355moe_linear_forward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _i64, _c_p, _int, _int, _c_p, _i64, _c_p, _i64,
                                        _c_p, _c_p, _sz, _c_p]),
     "mi355moe_linear_backward_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "mi355moe_linear_backward_call_bytes": (_i64, [_i64, _i64, _i64, _int, _int, _int, _int, _int, _int]),
     "mi355moe_linear_backward": (_int, [_c_p, _i64, _c_p, _c_p, _int, _i64, _i64, _i64, _c_p, _i64, _i64, _int, _c_p, _c_p, _c_p,
                                         _int, _c_p, _sz, _c_p]),
     "mi355moe_norm_forward": (_int, [_c_p, _int, _i64, _i64, _i64, _c_p, _i64, _c_p, _c_p, _int, _c_p, _int, _int, _f, _f, _f, _c_p,

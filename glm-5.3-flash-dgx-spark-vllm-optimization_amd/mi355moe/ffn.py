@@ -156,9 +156,13 @@ ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_bytes(backward: bool, M: int, K: int, N: int) -> int:
-    L = _lib.lib()
-    return (L.mi355moe_linear_backward_workspace_bytes if backward else L.mi355moe_linear_forward_workspace_bytes)(M, K, N)
+def _linear_bytes(M: int, K: int, N: int) -> int:
+    return _lib.lib().mi355moe_linear_forward_workspace_bytes(M, K, N)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_grad_bytes(*call) -> int:
+    return _lib.lib().mi355moe_linear_backward_call_bytes(*call)
 
 
 def _linear_operand(t: torch.Tensor, K: int) -> tuple[torch.Tensor, int]:
@@ -213,7 +217,7 @@ def _linear(kinds, x, w, bias, activation, residual, save):
     M = x2.numel() // K
     out = x2.new_empty(M, N) if x.dim() == 2 else x2.new_empty((*x.shape[:-1], N))
     z = x2.new_empty(M, N, dtype=torch.float32) if save and activation is not None else None
-    nb = _linear_bytes(False, M, K, N)
+    nb = _linear_bytes(M, K, N)
     ws = x2.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
     rc = _lib.lib().mi355moe_linear_forward(
         x2.data_ptr(), code, M, K, ldx, w2.data_ptr(), N, ldw, _addr(b), bcode, ACTIVATIONS[activation], _addr(r), ldr, out.data_ptr(), N,
@@ -263,12 +267,13 @@ def _linear_grads(kinds, dout, z, x, w, activation, bias_dtype, need_dx, need_dw
     x2, ldx = _linear_operand(x, K) if need_dw else (None, (K + 7) & ~7)
     w2, ldw = _linear_operand(w, K) if need_dx else (None, (K + 7) & ~7)
     d2, ldd = (dout, N) if dout.is_contiguous() else _rows_any(dout)
-    nb = _linear_bytes(True, M, K, N)
-    ws = dout.new_empty(max(nb, 0), dtype=torch.uint8)
+    at = d2.data_ptr()
+    nb = _linear_grad_bytes(M, K, N, code, ACTIVATIONS[activation], not at & 15 and not ldd & 7 and ldd <= 1 << 22, need_dx, need_dw, db is not None)
+    ws = dout.new_empty(nb, dtype=torch.uint8) if nb > 0 else None
     rc = _lib.lib().mi355moe_linear_backward(
-        d2.data_ptr(), ldd, None if activation is None else z.data_ptr(), x2 if x2 is None else x2.data_ptr(), code, M, K, ldx,
+        at, ldd, None if activation is None else z.data_ptr(), x2 if x2 is None else x2.data_ptr(), code, M, K, ldx,
         w2 if w2 is None else w2.data_ptr(), N, ldw, ACTIVATIONS[activation], dx if dx is None else dx.data_ptr(), dw if dw is None else dw.data_ptr(),
-        db if db is None else db.data_ptr(), _lib.F32 if db is None else weight_dtype_code(bias_dtype), ws.data_ptr(), nb if nb > 0 else 0,
+        db if db is None else db.data_ptr(), _lib.F32 if db is None else weight_dtype_code(bias_dtype), ws if ws is None else ws.data_ptr(), max(nb, 0),
         _stream_at(dev.index))
     if rc:
         _lib.check("mi355moe_linear_backward", rc)

@@ -563,7 +563,11 @@ int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int6
  * sums dz in fp32; the products take it rounded once to dtype (F16: times a power of two that brings the call's largest into
  * its range). Each gradient may be NULL (not computed). M >= 1 if dw or dbias is asked for. dy, dx and dw at any address of
  * their type; x, w (read for dw, dx) as for the forward. */
-int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N);      /* for any call of these sizes */
+/* For one call, which may need less (0: the workspace may be NULL): the gradients that it asks for; dy_aligned says that dy's address
+ * and row stride are multiples of 16 bytes, the stride at most 2^22 values. (Up to 1 MB both are the same.) */
+int64_t mi355moe_linear_backward_call_bytes(int64_t M, int64_t K, int64_t N, int dtype, int activation, int dy_aligned, int want_dx,
+                                            int want_dw, int want_dbias);
 int mi355moe_linear_backward(const void* dy, int64_t dy_stride, const float* z, const void* x, int dtype, int64_t M, int64_t K,
                              int64_t x_stride, const void* w, int64_t N, int64_t w_stride, int activation, void* dx, void* dw,
                              void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);

@@ -7,7 +7,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-MB = 1 << 20
+MB = 1 << 20          # (torch's allocator may count up to 1 MB more for a tensor: a block whose rest is smaller is not split)
 
 
 def _peak(f):
@@ -75,14 +75,14 @@ def test_rows_back_keep_rows_for_the_weights_only(cuda, weights):
 def test_rows_backward_reads_rows_for_the_weights_only(cuda):
     """Strided rows are copied where dweights reads them, and there alone."""
     from mi355moe import dispatch
-    T, k, H = 1024, 4, 1024
+    T, k, H = 1024, 4, 2048
     plan = _order(T, k, 6)
     wide = torch.randn(T * k, H + 8, device="cuda").bfloat16()
     rows, w, d = wide[:, :H], torch.rand(T, k, device="cuda"), torch.randn(T, H, device="cuda").bfloat16()
     both = dispatch.from_experts_backward(d, rows, w, plan)
     bytes_, (drows, dw) = _peak(lambda: dispatch.from_experts_backward(d, rows, w, plan, need_weights=False))
     assert dw is None and torch.equal(drows, both[0]) and drows.is_contiguous()
-    assert bytes_ < T * k * H * 2 + MB
+    assert bytes_ < T * k * H * 2 + 2 * MB
     drows, dw = dispatch.from_experts_backward(d, rows, w, plan, need_rows=False)
     assert drows is None and torch.equal(dw, both[1])
 
@@ -90,14 +90,14 @@ def test_rows_backward_reads_rows_for_the_weights_only(cuda):
 def test_linear_gradients_copy_only_what_they_read(cuda):
     """An operand that the kernels cannot read where it lies is copied for the product that reads it, and for no other."""
     from mi355moe import ffn
-    M, K, N = 2048, 1024, 1024
+    M, K, N = 4096, 2048, 4096
     x, w, d = (torch.randn(*s, device="cuda").bfloat16() for s in ((M, K), (N, K), (M, N)))
     odd = lambda t: torch.cat([t[:, :1], t], 1)[:, 1:]  # noqa: E731
     want = ffn.linear_backward(d, None, x, w)
     for need, bad in (((True, False), (odd(x), w)), ((False, True), (x, odd(w)))):
         plain, _ = _peak(lambda: ffn.linear_backward(d, None, x, w, None, None, *need))
         moved, got = _peak(lambda: ffn.linear_backward(d, None, *bad, None, None, *need))
-        assert moved == plain, (need, moved, plain)
+        assert abs(moved - plain) < 4 * MB, (need, moved, plain)     # (a copy has 16 MB)
         assert all(p is None or torch.equal(p, q) for p, q in zip(got, want))
 
 
@@ -150,3 +150,27 @@ def test_linear_keeps_what_its_gradients_read(cuda):
     x0 = base["x"][:0].clone().requires_grad_()
     ffn.linear(x0, base["w"]).sum().backward()
     assert x0.grad.shape == (0, K)
+
+
+def test_linear_gradients_take_the_scratch_they_use(cuda):
+    """Without an activation dout is an operand as it is, without a copy; copies of x and w (K no multiple of 8) are made for the
+    product that reads them. (Outputs of more than 512 tiles of 128 x 128: no product is cut into parts.)"""
+    from mi355moe import ffn
+    M, N, slack = 4096, 4096, 4 * MB
+    for K in (2560, 2563):
+        K8 = (K + 7) // 8 * 8
+        assert M * K > 512 * 128 * 128 and N * K > 512 * 128 * 128
+        cx, cw = (0, 0) if K == K8 else (2 * M * K8, 2 * N * K8)
+        x, w, d = (torch.randn(*s, device="cuda").bfloat16() for s in ((M, K), (N, K), (M, N)))
+        rows = 4 * (M // 64) * N                                 # the bias' sums
+        want = ffn.linear_backward(d, None, x, w, None, torch.float32)
+        for dx, dw, db in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1)):
+            peak, got = _peak(lambda: ffn.linear_backward(d, None, x, w, None, torch.float32 if db else None, bool(dx), bool(dw)))
+            assert peak < dx * (2 * M * K + cw) + dw * (2 * N * K + cx) + db * (rows + 4 * N) + slack, (K, dx, dw, db, peak)
+            assert all(p is None or torch.equal(p, q) for p, q in zip(got, want))
+        # an operand that is no 16-byte rows, and an activation's slope, take dz
+        z = torch.randn(M, N, device="cuda")
+        for dout, act in ((torch.cat([d[:, :1], d], 1)[:, 1:], None), (d, "silu")):
+            peak, got = _peak(lambda: ffn.linear_backward(dout, z, x, w, act, need_dw=False))
+            assert 2 * M * N <= peak - 2 * M * K - cw < 2 * M * N + slack
+            assert act is not None or torch.equal(got[0], want[0])
