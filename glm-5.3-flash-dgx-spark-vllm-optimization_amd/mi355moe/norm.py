@@ -121,11 +121,13 @@ def join_backward(ds: torch.Tensor | None, dy: torch.Tensor | None, stats: torch
     n = branch.numel() // branch.shape[-1]
     if stats.dtype != torch.float32 or tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
         raise ValueError(f"stats must be contiguous float32 {(n, 2)}, got {stats.dtype} {tuple(stats.shape)}")
+    need = (need[0], need[1] and residual is not None, *need[2:])
     return _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, float(scale), float(residual_scale), need)
 
 
 def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, residual_scale, need):
-    """join_backward of arguments that have been looked at (kinds: what _check said of them)."""
+    """join_backward of arguments that have been looked at (kinds: what _check said of them). residual's values are read with dy only;
+    without dy, need[1] alone says whether there is one."""
     dev, code, wcode, kind, gcode = kinds
     if dev.index != _current_device():
         with torch.cuda.device(dev):
@@ -135,8 +137,8 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
     db = dr = dpost = dgate = dpre = None
     if need[0]:
         db = torch.empty_like(branch) if branch.is_contiguous() else _empty_like(branch)
-    if need[1] and residual is not None:
-        dr = torch.empty_like(residual) if residual.is_contiguous() else _empty_like(residual)
+    if need[1]:
+        dr = torch.empty_like(branch) if branch.is_contiguous() else _empty_like(branch)      # (of branch's shape and type)
     if need[2] and post is not None:
         dpost = torch.empty_like(post) if post.is_contiguous() else _empty_like(post)
     if need[3] and gate is not None:
@@ -148,6 +150,8 @@ def _backward(kinds, ds, dy, stats, branch, residual, post, gate, pre, scale, re
     if dy is None and dpre is not None:
         dpre.zero_()
     b, ldb = (branch, H) if branch.is_contiguous() else _rows_any(branch)
+    if dy is None:
+        residual = None
     r, ldr = (residual, H) if residual is None or residual.is_contiguous() else _rows_any(residual)
     s, lds = (ds, H) if ds is None or ds.is_contiguous() else _rows_any(ds)
     y, ldy = (dy, H) if dy is None or dy.is_contiguous() else _rows_any(dy)
@@ -175,7 +179,8 @@ class _Join(torch.autograd.Function):
     @staticmethod
     def forward(ctx, branch, residual, post, gate, pre, kinds, eps, scale, residual_scale, need_s):
         s, y, stats = _forward(kinds, branch, residual, post, gate, pre, eps, scale, residual_scale, need_s, True)
-        ctx.save_for_backward(branch, residual, post, gate, pre, stats)
+        # (the residual is read for the gradient of the norm behind the sum; the residual stream of a sum alone may go on in place)
+        ctx.save_for_backward(branch, None if y is None else residual, post, gate, pre, stats)
         ctx.rest = kinds, scale, residual_scale, s is not None, y is not None
         ctx.set_materialize_grads(False)
         return (s, y) if s is not None and y is not None else s if y is None else y

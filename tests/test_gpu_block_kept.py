@@ -174,3 +174,28 @@ def test_linear_gradients_take_the_scratch_they_use(cuda):
             peak, got = _peak(lambda: ffn.linear_backward(dout, z, x, w, act, need_dw=False))
             assert 2 * M * N <= peak - 2 * M * K - cw < 2 * M * N + slack
             assert act is not None or torch.equal(got[0], want[0])
+
+
+def test_a_sum_without_a_norm_behind_it_keeps_no_residual(cuda):
+    from mi355moe import norm
+    g = torch.Generator(device="cuda").manual_seed(4)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    b, r, post, gate, ds = new(300, 520), new(300, 520), new(520), new(520), new(300, 520)
+    _, _, stats = norm.join_forward(b, r, post, gate, scale=0.5, residual_scale=1.5)
+    want = norm.join_backward(ds, None, stats, b, r, post, gate, None, 0.5, 1.5)
+    leaf = [t.clone().requires_grad_() for t in (b, r, post, gate)]
+    stream = leaf[1] * 1.0
+    s = norm.join(leaf[0], stream, post=leaf[2], gate=leaf[3], scale=0.5, residual_scale=1.5)
+    with torch.no_grad():
+        stream.add_(1.0)                                         # the residual stream goes on in place
+    s.backward(ds)
+    assert all(torch.equal(t.grad, v) for t, v in zip(leaf, want))
+    # the explicit form without dy reads no residual either, and gives its gradient where there is one
+    some = new(4096, 2048).t()
+    _, _, stats = norm.join_forward(some, some)
+    d = new(2048, 4096)
+    full, want = _peak(lambda: norm.join_backward(d, None, stats, some, some.contiguous(), residual_scale=1.5))
+    peak, got = _peak(lambda: norm.join_backward(d, None, stats, some, some, residual_scale=1.5))
+    assert all(p is q or torch.equal(p, q) for p, q in zip(got, want)) and torch.equal(got[1], 1.5 * d)
+    assert peak < full - 24 * MB, (peak, full)                   # (a copy has 32 MB)
+    assert norm.join_backward(d, None, stats, some, None)[1] is None
