@@ -230,7 +230,9 @@ def _linear(kinds, x, w, bias, activation, residual, save):
 def linear_backward(dout: torch.Tensor, z: torch.Tensor | None, x: torch.Tensor, w: torch.Tensor, activation: str | None = None,
                     bias_dtype: torch.dtype | None = None, need_dx: bool = True, need_dw: bool = True):
     """(dx, dw, dbias) from dout [..., N], the forward's z, x and w: fp32 sums, dx and dw in x's dtype, dbias in bias_dtype (None
-    where there is no bias or the gradient is not needed); the sums' order does not vary. residual's gradient is dout."""
+    where there is no bias or the gradient is not needed); the sums' order does not vary. With a curved activation dz = dout act'(z)
+    is rounded once to x's dtype for the two products (dbias sums it unrounded). x's values are read for dw, w's for dx. residual's
+    gradient is dout."""
     kinds = _check_linear(x, w, None, activation, None)
     _need_cuda(x, dout, z)
     _no_tangents("the dense product's backward", dout, z)
@@ -310,7 +312,8 @@ class _Linear(torch.autograd.Function):
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
            residual: torch.Tensor | None = None) -> torch.Tensor:
     """out [..., N] = act(x W^T + bias) + residual of x [..., K], w [N, K], bias [N] (any of fp32, fp16, bf16) and residual [..., N];
-    activation None, "relu", "silu", "gelu" or "gelu_tanh". Differentiable once in the four tensors by reverse mode
+    activation None, "relu", "silu", "gelu" or "gelu_tanh". Where K is a multiple of 8, an x or w whose rows lie at other than 16-byte
+    addresses is copied in every call: keep weights packed. Differentiable once in the four tensors by reverse mode
     (forward-mode derivatives are refused). While a graph is captured, a call that would record a gradient, and the backward
     pass of an eager one, are refused; capture linear_forward(save=True) and linear_backward instead."""
     kinds = _check_linear(x, w, bias, activation, residual)

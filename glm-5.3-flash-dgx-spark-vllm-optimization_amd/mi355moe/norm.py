@@ -10,8 +10,8 @@
 
 Everything is fp32 from the loads to one rounding of s and of y; y goes by s before its rounding. The gradients form s again
 from the inputs in fp32, and keep two fp32 numbers a row from the forward pass. Rows are fp32, fp16 or bf16. Values whose squares'
-mean passes fp32's range (magnitudes above 1e19) are outside the operator's range. Every call runs on the current stream of its
-tensors' device; outputs and scratch come from torch's caching allocator.
+mean leaves fp32's range (magnitudes above 1e19; with eps 0 also rows all below 1e-19) are outside the operator's range. Every call
+runs on the current stream of its tensors' device; outputs and scratch come from torch's caching allocator.
 """
 from __future__ import annotations
 

@@ -546,23 +546,26 @@ enum {
     MI355MOE_ACT_GELU = 3,      /* z * Phi(z) */
     MI355MOE_ACT_GELU_TANH = 4  /* z * (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
 };
+/* In fp32, small values within 2^-14 of themselves; a sigmoid or Phi below fp32's smallest normal number (silu: z < -87, gelu: z <
+ * -12.9, gelu_tanh: z < -10) may count as 0. */
 
-/* out [M][N] = act(x W^T + bias) + residual: fp32 sums and epilogue, rounded once. x [M][K] (row stride x_stride), w [N][K]
- * (row stride w_stride), residual [M][N] (optional) and out of one dtype, F16 or BF16; bias [N] (optional) F32, F16 or BF16. z
+/* out [M][N] = act(x W^T + bias) + residual: fp32 sums and epilogue, rounded once. x [M][K] (row stride x_stride), w [N][K] (row
+ * stride w_stride), residual [M][N] (optional) and out of one dtype, F16 or BF16; bias [N] (optional) F32, F16 or BF16. z
  * (optional, fp32 [M][N]) receives x W^T + bias for the backward pass. M <= 2^24, N <= 2^18, K <= 65536, any of them odd. K % 8 ==
- * 0: x and w at 16-byte addresses, their strides multiples of 8 and at most 2^22; other K: any address of their type, the call
- * lays padded copies out in the workspace. Outputs overlap no input. The workspace (may be NULL if the size query says 0) is 16-byte
- * aligned, uninitialised. */
+ * 0: x and w at 16-byte addresses, their strides multiples of 8 and at most 2^22; other K: any address of their type. Rows of such
+ * K are read where they lie, or for large products and the gradients' from padded copies that the call makes in the workspace.
+ * Outputs overlap no input. The workspace (may be NULL if the size query says 0) is 16-byte aligned, uninitialised. */
 int64_t mi355moe_linear_forward_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int mi355moe_linear_forward(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void* w, int64_t N,
                             int64_t w_stride, const void* bias, int bias_dtype, int activation, const void* residual,
                             int64_t residual_stride, void* out, int64_t out_stride, float* z, void* workspace,
                             size_t workspace_bytes, hipStream_t stream);
-/* Its gradients (the residual's is dy itself): dz = dy act'(z) from the forward's z (NULL without an activation); dx [M][K] =
- * dz W, dw [N][K] = dz^T x, dbias [N] (bias_dtype) = the sums of dz over the rows; fp32 sums rounded once, deterministic. dbias
- * sums dz in fp32; the products take it rounded once to dtype (F16: times a power of two that brings the call's largest into
- * its range). Each gradient may be NULL (not computed). M >= 1 if dw or dbias is asked for. dy, dx and dw at any address of
- * their type; x, w (read for dw, dx) as for the forward. */
+/* Its gradients (the residual's is dy itself): dz = dy act'(z) from the forward's z (NULL without an activation); dx [M][K] = dz W,
+ * dw [N][K] = dz^T x, dbias [N] (bias_dtype) = the sums of dz over the rows; fp32 sums rounded once, deterministic. dbias sums dz
+ * in fp32; the products take it rounded once to dtype, as the 16-bit matrix cores have to (F16: times a power of two that brings
+ * the call's largest into its range), which errs by as much again as the rounding of dx and dw themselves. Each gradient may be
+ * NULL (not computed). M >= 1 if dw or dbias is asked for. dy, dx and dw at any address of their type; x, w (read for dw, dx) as
+ * for the forward. */
 int64_t mi355moe_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N);      /* for any call of these sizes */
 /* For one call, which may need less (0: the workspace may be NULL): the gradients that it asks for; dy_aligned says that dy's address
  * and row stride are multiples of 16 bytes, the stride at most 2^22 values. (Up to 1 MB both are the same.) */
