@@ -175,9 +175,9 @@ __device__ __forceinline__ RowsPlace rows_place(int shift, int segs) {
     return {UNI ? (int64_t)__builtin_amdgcn_readfirstlane((int)t) : t, (int)(seg << shift) + (int)(threadIdx.x & ((1 << shift) - 1))};
 }
 
-// rows[row] = x[t] (live) or zero, 16 bytes a thread and store; ES: bytes of a value. x is read once, whatever topk: a thread keeps its 16
-// bytes and stores them to each row. Bound: HBM, its writes above all (bf16 rows of 4096, top 8: 4096 tokens 302 MB in 50 to 59 us,
-// 8192 in 107 to 115, 5.3 TB/s).
+// rows[row] = x[t] (live) or zero, 16 bytes a thread and store; ES: bytes of a value. x is read once, whatever topk: a thread keeps
+// its 16 bytes and stores them to each row. Bound: HBM, its writes above all (bf16 rows of 4096, top 8: 4096 tokens 302 MB in 50 to
+// 59 us, 8192 in 106 to 116, 5.3 TB/s; 4096 in fp32 604 MB in 106 to 117).
 template <int ES, bool UNI>
 __global__ __launch_bounds__(256) void rows_scatter_kernel(RowsArgs a, int shift, int segs) {
     const auto [t, u] = rows_place<UNI>(shift, segs);
@@ -224,9 +224,9 @@ __device__ __forceinline__ void add_rows(const RowsArgs& a, uint64_t& live, int 
 }
 
 // out[t] = shared[t] + the weighted rows of t, eight values a thread. A wave's lanes read the table entries of its token's slots
-// (at most 32), and the rows of up to eight slots are on their way at once; rows of fewer than 64 pieces share a wave, and each thread
-// reads the table itself. Bound: HBM (bf16 rows of 4096, top 8, 4096 tokens with shared: 336 MB in 58 to 70 us, 5.2 TB/s); a few
-// hundred tokens: latency (517 tokens of 2051, top 6, fp16: 5.3 us).
+// (at most 32), and the rows of up to eight slots are on their way at once; rows of fewer than 64 pieces share a wave, and each
+// thread reads the table itself. Bound: HBM (bf16 rows of 4096, top 8, 4096 tokens with shared: 336 MB in 58 to 70 us, 5.2 TB/s; in
+// fp32 671 MB in 128 to 145); a few hundred tokens: latency (517 tokens of 2051, top 6, fp16: 5.3 us).
 template <int DT, bool UNI, bool ONCE>
 __global__ __launch_bounds__(256) void rows_gather_kernel(RowsArgs a, int shift, int segs) {
     const auto [t, u] = rows_place<UNI>(shift, segs);
@@ -318,9 +318,9 @@ __device__ __forceinline__ void grad_rows(const RowsArgs& a, int64_t t, uint64_t
     __syncthreads();                                                 // (the sums have been read: the next slots write them)
 }
 
-// A workgroup a token: dout[t] is read once for eight slots, whose rows are on their way at once; at most four waves. The dots are sums
-// of a thread, a wave (by lane exchanges) and the waves in order. Bound: HBM (bf16 rows of 4096, top 8, 4096 tokens: 571 MB in 113 to
-// 118 us, 4.9 TB/s).
+// A workgroup a token: dout[t] is read once for eight slots, whose rows are on their way at once; at most four waves. The dots are
+// sums of a thread, a wave (by lane exchanges) and the waves in order. Bound: HBM (bf16 rows of 4096, top 8, 4096 tokens: 571 MB in
+// 113 to 118 us, 4.9 TB/s; in fp32 1142 MB in 234 to 240).
 template <int DT, bool ONCE>
 __global__ __launch_bounds__(256) void rows_grad_kernel(RowsArgs a) {
     __shared__ float red[8][4];

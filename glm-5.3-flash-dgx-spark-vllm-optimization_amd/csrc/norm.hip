@@ -55,8 +55,9 @@ __device__ __forceinline__ float inv_rms(float sum, int H, float eps) { return _
 // A row of up to 8 NV values a thread: by 2^shift lanes, as many rows a workgroup as fit (WG false), or by a workgroup of as many
 // threads as the row needs. Everything that the row reads is requested before the first sum, and stays in registers to the end: one
 // pass. Bound: HBM for many rows (16384 of 4096, bf16 with post, pre and residual: 537 MB in 80 to 86 us, 6.4 TB/s, what the caches
-// still hold among it; 32768 of 64: 7 us), latency for few (1 row 3.0 us, 1237 odd fp16 rows of 4099 15 us: their rows begin at any
-// 2-byte address, which costs 4 us over 1237 of 4096).
+// still hold among it; 32768 of 64: 7 us; 8192 fp32 rows of 4096: 537 MB in 107 to 113 us, 4.9 TB/s; 2048 rows of 16384: bf16 268
+// MB in 75 us, fp32 537 MB in 120), latency for few (1 row 3.0 us, 1237 odd fp16 rows of 4099 15 us: their rows begin at any 2-byte
+// address, which costs 4 us over 1237 of 4096).
 template <int DT, bool WG, int NV, bool ONCE>
 __global__ __launch_bounds__(WG ? 1024 : 256) void norm_kernel(NormArgs a, int shift) {
     __shared__ float red[2][16];
@@ -178,12 +179,12 @@ __device__ __forceinline__ void store_gate(const NormArgs& a, size_t at, int n, 
     else store8<DT_F16>(a.dgate, at, n, d);
 }
 
-// Gradients of rows blockIdx, blockIdx + gridDim, ... (WG false: of as many rows at once as 2^shift lanes each leave room for): those
-// of the weights and of a channel's gate stay in registers and go to this workgroup's part [2][H] at the end (norm_join_kernel adds
-// the parts in order): the sums of dy n_s, and of du n_b; a channel's gate takes its factors out of the second, sum of gs n_b,
-// which then gives dpost (times beta gate) and dgate (times beta post) both. A row's loads are requested while the row before it is
-// worked on. Bound: HBM with the two barriers of a row in its way (8192 rows of 4096, bf16, a channel's gate: 403 MB in 90 to 96 us,
-// 4.3 TB/s; 32768 rows of 64 11 us, of 512 43 us).
+// Gradients of rows blockIdx, blockIdx + gridDim, ... (WG false: of as many rows at once as 2^shift lanes each leave room for):
+// those of the weights and of a channel's gate stay in registers and go to this workgroup's part [2][H] at the end
+// (norm_join_kernel adds the parts in order): the sums of dy n_s, and of du n_b; a channel's gate takes its factors out of the
+// second, sum of gs n_b, which then gives dpost (times beta gate) and dgate (times beta post) both. A row's loads are requested
+// while the row before it is worked on. Bound: HBM with the two barriers of a row in its way (8192 rows of 4096, bf16, a channel's
+// gate: 403 MB in 90 to 96 us, 4.3 TB/s; in fp32 805 MB in 164 to 168, 4.8; 32768 rows of 64 11 us, of 512 43 us).
 template <int DT, bool WG>
 __global__ __launch_bounds__(WG ? 1024 : 256, WG ? 1 : DT == DT_F32 ? 3 : 4) void norm_grad_kernel(NormArgs a, int shift) {
     extern __shared__ __align__(16) f32x4 lds[];
@@ -331,8 +332,11 @@ __global__ __launch_bounds__(WG ? 1024 : 256, WG ? 1 : DT == DT_F32 ? 3 : 4) voi
 }
 
 // The same for rows of 8193 to 16384 values, sixteen a thread: held as floats they would not fit the registers of 1024 threads (the
-// kernel above with twice its values, which kept 360 to 500 bytes a lane in scratch: 2048 rows of 16384 284 us, this 176). So a row's
-// values stay as they were loaded and each pass makes them floats again, and the sums over the rows stay in LDS.
+// kernel above with twice its values, which kept 360 to 500 bytes a lane in scratch: 2048 rows of 16384 284 us). So a row's values
+// stay as they were loaded and each pass makes them floats again, and the sums over the rows stay in LDS. Four tensors' values over
+// two barriers pass 128 registers even so: 112 bytes a lane are in scratch for bf16 and fp16, 228 for fp32. Bound: that, and the
+// one workgroup that a CU holds, which waits at each row's barriers (2048 rows of 16384, a channel's gate: bf16 403 MB in 166 us,
+// 2.4 TB/s, fp16 177; fp32 805 MB in 325).
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormArgs a) {
     extern __shared__ __align__(16) f32x4 lds[];
