@@ -54,11 +54,11 @@ struct LinearKind {
 // ------------------------------------------------------------------------------------------------ activations
 
 __device__ __forceinline__ float sigmoid_rcp(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
-// Phi(z) from erfc(x) = t (a1 + t (a2 + ... + t a7)) e^(-x^2), t = 1 / (1 + 0.3625 x), x = |z| / sqrt(2). The coefficients (here halved)
-// and 0.3625 are a minimax fit made for this: up to x = 9.6, where e^(-x^2) leaves fp32, within 2^-18 of erfc itself and within
-// 4.2e-8 absolutely, so that the tail z Phi(z) at z << 0 keeps its own leading bits (in fp32: 8e-6 of itself at -12.5; a formula that
-// is good to 1.5e-7 absolutely alone, with five terms, is off by 0.4 % at -6, a bf16 half step, and by 3.6 % at -12.5). The
-// library's erfcf takes three times the instructions. e: e^(-z^2 / 2).
+// Phi(z) from erfc(x) = t (a1 + t (a2 + ... + t a7)) e^(-x^2), t = 1 / (1 + 0.3625 x), x = |z| / sqrt(2). The coefficients (here
+// halved) and 0.3625 are a minimax fit made for this: up to x = 9.6, where e^(-x^2) leaves fp32, within 2^-18 of erfc itself and
+// within 4.2e-8 absolutely, so that the tail z Phi(z) at z << 0 keeps its own leading bits (in fp32: 8e-6 of itself at -12.5; a
+// formula that is good to 1.5e-7 absolutely alone, with five terms, is off by 0.4 % at -6, a bf16 half step, and by 3.2 % at
+// -12.5). The library's erfcf takes three times the instructions. e: e^(-z^2 / 2).
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     e = __expf(-0.5f * z * z);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3625f * 0.70710678118654752f, fabsf(z), 1.0f));

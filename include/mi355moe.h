@@ -590,9 +590,10 @@ int mi355moe_norm_forward(const void* branch, int dtype, int64_t rows, int64_t H
                           int64_t residual_stride, const void* post, const void* pre, int weights_dtype, const void* gate,
                           int gate_dtype, int gate_kind, float eps, float scale, float residual_scale, void* s, void* y,
                           float* stats, hipStream_t stream);
-/* Its gradients from ds and dy (one may be NULL: zero) and the forward's inputs and stats: dbranch, dresidual [rows][H], dpost,
- * dpre [H] (weights_dtype), dgate (shaped and typed like gate); fp32, rounded once, deterministic. Each may be NULL. The
- * workspace is read where dpost, dpre or a CHANNEL gate's gradient is asked for (rows >= 1 then): 16-byte aligned, uninitialised. */
+/* Its gradients from ds and dy (one may be NULL: zero) and the forward's inputs and stats (residual is read with dy only): dbranch,
+ * dresidual [rows][H], dpost, dpre [H] (weights_dtype), dgate (shaped and typed like gate); fp32, rounded once, deterministic. Each
+ * may be NULL. The workspace is read where dpost, dpre or a CHANNEL gate's gradient is asked for (rows >= 1 then): 16-byte aligned,
+ * uninitialised. */
 int64_t mi355moe_norm_backward_workspace_bytes(int64_t rows, int64_t H);
 int mi355moe_norm_backward(const void* ds, int64_t ds_stride, const void* dy, int64_t dy_stride, const void* branch, int dtype,
                            int64_t rows, int64_t H, int64_t branch_stride, const void* residual, int64_t residual_stride,
